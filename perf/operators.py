@@ -316,7 +316,7 @@ def _plain_append(s):
     row = x.abs().amax(-1)
     amax.scatter_reduce_(0, run_of[:, None, None].expand_as(row), row, "amax")
     old = torch.where((first == 0)[:, None, None], 0.0, scale[pages])
-    grown = torch.maximum(torch.maximum(amax / 127, GROW_BY * old), torch.full_like(old, SCALE_MIN)).clamp(max=SCALE_MAX)
+    grown = torch.maximum(torch.maximum(amax / torch.full_like(amax, 127), GROW_BY * old), torch.full_like(old, SCALE_MIN)).clamp(max=SCALE_MAX)
     now = torch.where((amax > GROW_AT * old) | (old == 0), grown, old)
     scale[pages] = now
     before = kv[pages].float()
@@ -361,8 +361,9 @@ def _plain_attention(s):
 def _plain_matmul(s):
     x, w = s["x"].float(), s["w"][:, : s["case"]["k"]].float()
     amax = x.abs().amax(-1, keepdim=True)
-    inv = torch.where(amax > 0, (127 / amax).clamp(max=3.4028234663852886e38), 0.0)
-    y = (torch.round(x * inv) @ w.t()) * (amax / 127) * s["w_scale"]
+    most = torch.full_like(amax, 127)                                 # (a tensor: a number would be divided by approximately)
+    inv = torch.where(amax > 0, (most / amax).clamp(max=3.4028234663852886e38), 0.0)
+    y = (torch.round(x * inv) @ w.t()) * (amax / most) * s["w_scale"]
     if s["bias"] is not None:
         y = y + s["bias"]
     return {"y": y.to(s["x"].dtype)}
