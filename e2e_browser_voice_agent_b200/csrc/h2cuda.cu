@@ -2493,3 +2493,15 @@ extern "C" int h2c_selftest_math(int device, uint64_t* mismatches) {
   cudaFree(d);
   return c == cudaSuccess ? H2C_OK : H2C_ERR_CUDA;
 }
+
+// ---------------------------------------------------------------- the last error of the operators in other files
+
+namespace h2 {
+void set_last_error(const char* msg) noexcept {
+  try {
+    g_create_error = msg;
+  } catch (...) {  // (no memory for the message)
+    g_create_error.clear();
+  }
+}
+}  // namespace h2

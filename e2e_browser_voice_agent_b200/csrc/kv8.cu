@@ -1,0 +1,468 @@
+// The paged 8-bit KV cache: block tables and slot maps from request lengths (h2c_kv8_plan), K and V rows into pages
+// (h2c_kv8_append), and back out (h2c_kv8_read). The formulas are stated in include/h2cuda.h.
+#include "ops.cuh"
+
+#include <algorithm>
+#include <climits>
+
+namespace h2 {
+namespace {
+
+// ---------------------------------------------------------------- plan
+//
+// Three prefix sums over the requests (new tokens, pages taken, pages given back), then independent writes: one thread
+// per new token, per page taken and per page given back finds its request by a search in the sums. Nothing that one
+// thread writes is read by another (the tables' new entries are resolved through the ring, and the ring's new entries
+// lie behind its tail), so every CTA forms the sums for itself from the 8 bytes per request and no grid-wide step is
+// needed. Sums saturate at SUM_LIM, so that lengths without sense cannot wrap around to valid ones.
+// Bound: latency (launch, two dependent reads, the sums); the bytes are 8 per request, token and page.
+constexpr unsigned SUM_LIM = 0x3FFFFFFFu;
+constexpr int PLAN_THREADS = 512;
+
+__device__ __forceinline__ unsigned sat_add(unsigned a, unsigned b) { return min(a + b, SUM_LIM); }
+
+struct PlanArgs {
+  int n_req, page_log, table_cols, n_pages, max_tokens;
+  const int *cached, *total;
+  int *table, *ring;
+  const long long* state;
+  long long* state_out;
+  int *kv_len, *q_start, *slot, *position, *status;
+};
+
+// the request whose range [sum[r], sum[r + 1]) holds i (sum[0] = 0, i < sum[n])
+__device__ __forceinline__ int find_request(const unsigned* sum, int n, unsigned i) {
+  int lo = 0, hi = n;  // sum[lo] <= i < sum[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sum[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) k_kv8_plan(const PlanArgs a) {
+  extern __shared__ unsigned sums[];  // [3][n_req + 1]: new tokens, pages taken, pages given back
+  const int n = a.n_req, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  unsigned* s_new = sums;
+  unsigned* s_take = sums + n + 1;
+  unsigned* s_back = sums + 2 * (n + 1);
+  __shared__ unsigned part[3][PLAN_THREADS / 32];
+  __shared__ int any_bad;
+  if (tid == 0) {
+    any_bad = 0;
+    s_new[0] = s_take[0] = s_back[0] = 0;
+  }
+  const long long head = a.state[0], tail = a.state[1];
+  const long long room = (long long)a.table_cols << a.page_log;
+  const int round_up = (1 << a.page_log) - 1;
+  __syncthreads();
+  unsigned carry[3] = {0, 0, 0};
+  for (int base = 0; base < n; base += PLAN_THREADS) {
+    const int r = base + tid;
+    unsigned v[3] = {0, 0, 0};
+    if (r < n) {
+      const int c = a.cached[r], t = a.total[r];
+      if (c < 0 || t < 0 || c > room || t > room) {
+        any_bad = 1;
+      } else {
+        const int have = (int)(((long long)c + round_up) >> a.page_log), want = (int)(((long long)t + round_up) >> a.page_log);
+        v[0] = min((unsigned)max(t - c, 0), SUM_LIM);
+        v[1] = min((unsigned)max(want - have, 0), SUM_LIM);
+        v[2] = min((unsigned)max(have - want, 0), SUM_LIM);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned u = __shfl_up_sync(0xffffffffu, v[k], o);
+        if (lane >= o) v[k] = sat_add(v[k], u);
+      }
+      if (lane == 31) part[k][warp] = v[k];
+    }
+    __syncthreads();
+    if (warp < 3) {  // warp k sums the 16 warps' parts of sum k
+      unsigned u = lane < PLAN_THREADS / 32 ? part[warp][lane] : 0u;
+#pragma unroll
+      for (int o = 1; o < PLAN_THREADS / 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, u, o);
+        if (lane >= o) u = sat_add(u, x);
+      }
+      if (lane < PLAN_THREADS / 32) part[warp][lane] = u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      const unsigned before = sat_add(carry[k], warp ? part[k][warp - 1] : 0u);
+      if (r < n) sums[k * (n + 1) + r + 1] = sat_add(before, v[k]);
+      carry[k] = sat_add(carry[k], part[k][PLAN_THREADS / 32 - 1]);
+    }
+    __syncthreads();
+  }
+  const unsigned n_new = carry[0], n_take = carry[1], n_back = carry[2];
+  const long long avail = tail - head;
+  const bool bad = any_bad || n_new > (unsigned)a.max_tokens || head < 0 || avail < 0 || avail + n_back > a.n_pages;
+  const bool shortage = !bad && (long long)n_take > avail + n_back;
+  const bool ok = !bad && !shortage;
+  const int head_at = ok ? (int)(head % a.n_pages) : 0, tail_at = ok ? (int)(tail % a.n_pages) : 0;
+  const int stride = gridDim.x * PLAN_THREADS, first = blockIdx.x * PLAN_THREADS + tid;
+
+  auto pages_of = [&](int len) { return (int)(((long long)len + round_up) >> a.page_log); };
+  auto given_back = [&](unsigned i) {  // the i-th page given back
+    const int r = find_request(s_back, n, i);
+    return a.table[(size_t)r * a.table_cols + pages_of(a.total[r]) + (i - s_back[r])];
+  };
+  auto taken = [&](unsigned i) {  // the i-th page taken
+    if ((long long)i >= avail) return given_back(i - (unsigned)avail);
+    unsigned at = head_at + i;
+    if (at >= (unsigned)a.n_pages) at -= a.n_pages;
+    return a.ring[at];
+  };
+  for (int t = first; t < a.max_tokens; t += stride) {
+    int slot = -1, pos = -1;
+    if (ok && (unsigned)t < n_new) {
+      const int r = find_request(s_new, n, t), c = a.cached[r];
+      pos = c + (t - (int)s_new[r]);
+      const int have = pages_of(c), j = pos >> a.page_log;
+      const int page = j < have ? a.table[(size_t)r * a.table_cols + j] : taken(s_take[r] + (j - have));
+      slot = (page << a.page_log) + (pos & round_up);
+    }
+    a.slot[t] = slot;
+    a.position[t] = pos;
+  }
+  if (ok) {
+    for (unsigned i = first; i < n_take; i += stride) {
+      const int r = find_request(s_take, n, i);
+      a.table[(size_t)r * a.table_cols + pages_of(a.cached[r]) + (i - s_take[r])] = taken(i);
+    }
+    for (unsigned i = first; i < n_back; i += stride) {
+      unsigned at = tail_at + i;
+      if (at >= (unsigned)a.n_pages) at -= a.n_pages;
+      a.ring[at] = given_back(i);
+    }
+  }
+  for (int r = first; r <= n; r += stride) {
+    a.q_start[r] = ok ? (int)s_new[r] : 0;
+    if (r < n) {
+      const int c = a.cached[r];
+      a.kv_len[r] = ok ? a.total[r] : (c < 0 || c > room ? 0 : c);
+    }
+  }
+  if (first == 0) {
+    a.state_out[0] = head + (ok ? (long long)n_take : 0);
+    a.state_out[1] = tail + (ok ? (long long)n_back : 0);
+    a.status[0] = bad ? 2 : shortage ? 1 : 0;
+    a.status[1] = shortage ? (int)(n_take - (avail + n_back)) : 0;
+  }
+}
+
+// ---------------------------------------------------------------- append
+//
+// The rows that one call brings to one page form a run; its (K or V, head) part is quantized together because it shares
+// a scale. grid.x covers windows of 16 rows, grid.y K or V and the head: a CTA takes the runs that start in its window
+// (a run longer than the window reaches beyond it). Runs of up to SHORT rows (decode steps: one row) take a warp each,
+// longer ones the whole CTA. A thread holds its values in registers between the maximum and the codes, so each input
+// is read once. Bound: bandwidth for prompts, latency for single rows.
+constexpr int APP_THREADS = 256, APP_WIN = 16, APP_SHORT = 2;
+constexpr float SCALE_MIN = 0x1p-62f, SCALE_MAX = 0x1p63f;
+
+struct AppendArgs {
+  int8_t* kv;
+  float* scale;
+  int n_slots, page_log, kv_heads, rows;
+  const void *k, *v;
+  long long k_row, k_head, v_row, v_head;
+  const int* slot;
+};
+
+// the scale after a run: a the largest magnitude (NaN or infinity: the page is lost), s0 the scale so far
+__device__ __forceinline__ float grown_scale(float a, float s0, bool finite) {
+  if (!finite || s0 != s0) return __int_as_float(0x7fc00000);
+  if (s0 != 0.f && !(a > 127.5f * s0)) return s0;
+  return fminf(fmaxf(fmaxf(__fdiv_rn(a, 127.f), 1.25f * s0), SCALE_MIN), SCALE_MAX);
+}
+__device__ __forceinline__ int code_of(float x, float inv) {
+  return __float2int_rn(fminf(fmaxf(rintf(x * inv), -127.f), 127.f));
+}
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+  return (a & 255u) | ((b & 255u) << 8) | ((c & 255u) << 16) | ((uint32_t)d << 24);
+}
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+  int c[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) c[i] = __float2int_rn((float)(int8_t)(w >> (8 * i)) * ratio);
+  return pack4(c[0], c[1], c[2], c[3]);
+}
+
+// One run of one (K or V, head) by the threads i0 = 0 .. NT-1 of a warp (NT = 32) or of the CTA; reduce() combines the
+// largest magnitude bits over them. MAXU: units of 4 values that a thread keeps.
+template <class T, bool VEC, int HD, int NT, int MAXU, class R>
+__device__ __forceinline__ void append_run(const T* src, long long row_stride, int len, int8_t* page, int off,
+                                           float* scale, int i0, R reduce) {
+  constexpr int UPR = HD / 4;  // units per row
+  const int units = len * UPR;
+  const float s0 = off == 0 ? 0.f : *scale;
+  float v[MAXU][4];
+#pragma unroll
+  for (int k = 0; k < MAXU; k++) {
+    const int u = i0 + k * NT;
+    if (u < units) load4<VEC>(src + (u / UPR) * row_stride + (u % UPR) * 4, v[k]);
+  }
+  unsigned m = 0;  // magnitudes order as their bits do, infinities and NaN above every number
+#pragma unroll
+  for (int k = 0; k < MAXU; k++)
+    if (i0 + k * NT < units)
+#pragma unroll
+      for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(v[k][j]) & 0x7fffffffu);
+  for (int u = i0 + MAXU * NT; u < units; u += NT) {  // (what does not fit the registers is read again below)
+    float x[4];
+    load4<VEC>(src + (u / UPR) * row_stride + (u % UPR) * 4, x);
+#pragma unroll
+    for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+  }
+  m = reduce(m);
+  const bool finite = m < 0x7f800000u;
+  const float s = grown_scale(__uint_as_float(m), s0, finite);
+  const bool lost = s != s;
+  const float inv = lost ? 0.f : __fdiv_rn(1.f, s);
+  if (off && s != s0 && !lost) {
+    const float ratio = __fdiv_rn(s0, s);
+    for (int u = i0; u < off * UPR; u += NT) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(page) + u;
+      *w = rescale4(*w, ratio);
+    }
+  }
+  uint32_t* dst = reinterpret_cast<uint32_t*>(page + (size_t)off * HD);
+#pragma unroll
+  for (int k = 0; k < MAXU; k++) {
+    const int u = i0 + k * NT;
+    if (u < units)
+      dst[u] = lost ? 0u : pack4(code_of(v[k][0], inv), code_of(v[k][1], inv), code_of(v[k][2], inv), code_of(v[k][3], inv));
+  }
+  for (int u = i0 + MAXU * NT; u < units; u += NT) {
+    float x[4];
+    load4<VEC>(src + (u / UPR) * row_stride + (u % UPR) * 4, x);
+    dst[u] = lost ? 0u : pack4(code_of(x[0], inv), code_of(x[1], inv), code_of(x[2], inv), code_of(x[3], inv));
+  }
+  if (i0 == 0 && s != s0) *scale = s;  // (also when s is NaN; every thread has read s0: reduce() synchronises them)
+}
+
+template <class T, bool VEC, int HD>
+__global__ void __launch_bounds__(APP_THREADS) k_kv8_append(const AppendArgs a) {
+  __shared__ int run_row[APP_WIN], run_len[APP_WIN];
+  __shared__ int n_runs;
+  __shared__ unsigned red[APP_THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int P = 1 << a.page_log;
+  const int which = blockIdx.y / a.kv_heads, head = blockIdx.y % a.kv_heads;
+  const int w0 = blockIdx.x * APP_WIN;
+  if (warp == 0) {
+    // a row starts a run unless the row before it is at the offset before its own in the same page
+    const int t = w0 + lane;
+    bool lead = false;
+    if (lane < APP_WIN && t < a.rows) {
+      const int s = a.slot[t];
+      lead = s >= 0 && s < a.n_slots && ((s & (P - 1)) == 0 || t == 0 || a.slot[t - 1] != s - 1);
+    }
+    const unsigned b = __ballot_sync(0xffffffffu, lead);
+    if (lead) run_row[__popc(b & ((1u << lane) - 1))] = t;
+    if (lane == 0) n_runs = __popc(b);
+  }
+  __syncthreads();
+  const int runs = n_runs;
+  for (int i = warp; i < runs; i += APP_THREADS / 32) {  // run lengths, a warp per run
+    const int t = run_row[i], s = a.slot[t], most = min(P - (s & (P - 1)), a.rows - t);
+    int len = most;
+    for (int b = 0; b < most; b += 32) {
+      const bool in = b + lane < most && a.slot[t + b + lane] == s + b + lane;
+      const unsigned in_all = __ballot_sync(0xffffffffu, in);
+      if (in_all != 0xffffffffu) {
+        len = min(most, b + __ffs(~in_all) - 1);
+        break;
+      }
+    }
+    if (lane == 0) run_len[i] = len;
+  }
+  __syncthreads();
+  const T* src = static_cast<const T*>(which ? a.v : a.k) + head * (which ? a.v_head : a.k_head);
+  const long long row_stride = which ? a.v_row : a.k_row;
+  auto page_of = [&](int s) {
+    return a.kv + (((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head) * ((size_t)P * HD);
+  };
+  auto scale_of = [&](int s) { return a.scale + ((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head; };
+  for (int i = warp; i < runs; i += APP_THREADS / 32) {
+    if (run_len[i] > APP_SHORT) continue;
+    const int t = run_row[i], s = a.slot[t];
+    append_run<T, VEC, HD, 32, APP_SHORT * HD / 128>(src + t * row_stride, row_stride, run_len[i], page_of(s),
+                                                     s & (P - 1), scale_of(s), lane,
+                                                     [](unsigned m) {
+                                                       m = __reduce_max_sync(0xffffffffu, m);
+                                                       __syncwarp();  // (every lane has read the old scale)
+                                                       return m;
+                                                     });
+  }
+  for (int i = 0; i < runs; i++) {
+    if (run_len[i] <= APP_SHORT) continue;
+    const int t = run_row[i], s = a.slot[t];
+    append_run<T, VEC, HD, APP_THREADS, 8>(src + t * row_stride, row_stride, run_len[i], page_of(s), s & (P - 1),
+                                           scale_of(s), tid, [&](unsigned m) {
+                                             m = __reduce_max_sync(0xffffffffu, m);
+                                             __syncthreads();  // (the run before is done with red[])
+                                             if (lane == 0) red[warp] = m;
+                                             __syncthreads();
+                                             unsigned x = red[lane % (APP_THREADS / 32)];
+                                             return __reduce_max_sync(0xffffffffu, x);
+                                           });
+  }
+}
+
+// ---------------------------------------------------------------- read
+
+template <class T>
+__global__ void k_kv8_read(const int8_t* __restrict__ kv, const float* __restrict__ scale, int n_slots, int page_log,
+                           int kv_heads, int hd_log, const int* __restrict__ slot, long long units, T* __restrict__ k_out,
+                           T* __restrict__ v_out) {
+  // a unit is 16 codes; units of a row: K heads, then V heads
+  const int per_head_log = hd_log - 4, per_row = 2 * kv_heads << per_head_log;
+  for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (long long)gridDim.x * blockDim.x) {
+    const int t = (int)(u / per_row), w = (int)(u % per_row);
+    const int hh = w >> per_head_log, c = (w & ((1 << per_head_log) - 1)) * 16;  // (K or V, head), first dimension
+    const int which = hh >= kv_heads, head = hh - which * kv_heads;
+    const int s = slot[t];
+    alignas(16) T o[16];
+    if (s >= 0 && s < n_slots) {
+      const size_t ph = ((size_t)(s >> page_log) * 2 + which) * kv_heads + head;
+      const int4 q = *reinterpret_cast<const int4*>(kv + (((ph << page_log) + (s & ((1 << page_log) - 1))) << hd_log) + c);
+      const float f = scale[ph];
+      const int w4[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[i] = from_f<T>((float)(int8_t)(w4[i >> 2] >> (8 * (i & 3))) * f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[i] = from_f<T>(0.f);
+    }
+    int4* d = reinterpret_cast<int4*>((which ? v_out : k_out) + ((((size_t)t * kv_heads + head)) << hd_log) + c);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) * 16 / 16); i++) d[i] = reinterpret_cast<const int4*>(o)[i];
+  }
+}
+
+int log2_of(int x) {
+  int l = 0;
+  while ((1 << l) < x) l++;
+  return l;
+}
+
+int cache_ok(const char* who, const void* kv, const float* scale, int n_pages, int page_size, int kv_heads,
+             int head_dim) {
+  if (!kv || !scale) return op_error(H2C_ERR_INVALID, "%s: null cache", who);
+  if ((uintptr_t)kv & 15) return op_error(H2C_ERR_INVALID, "%s: the cache must be 16-byte aligned", who);
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+    return op_error(H2C_ERR_INVALID, "%s: page_size must be 16, 32, 64 or 128, not %d", who, page_size);
+  if (head_dim != 64 && head_dim != 128)
+    return op_error(H2C_ERR_INVALID, "%s: head_dim must be 64 or 128, not %d", who, head_dim);
+  if (n_pages < 1 || (long long)n_pages * page_size > INT_MAX)
+    return op_error(H2C_ERR_INVALID, "%s: n_pages %d out of range", who, n_pages);
+  if (kv_heads < 1 || kv_heads > 4096) return op_error(H2C_ERR_INVALID, "%s: kv_heads %d out of range", who, kv_heads);
+  return H2C_OK;
+}
+
+template <class T, bool VEC>
+void launch_append(const AppendArgs& a, int head_dim, cudaStream_t st) {
+  const dim3 grid((a.rows + APP_WIN - 1) / APP_WIN, 2 * a.kv_heads);
+  if (head_dim == 64) k_kv8_append<T, VEC, 64><<<grid, APP_THREADS, 0, st>>>(a);
+  else k_kv8_append<T, VEC, 128><<<grid, APP_THREADS, 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace h2
+
+using namespace h2;
+
+extern "C" {
+
+int h2c_kv8_plan(int32_t n_req, int32_t page_size, const int32_t* cached, const int32_t* total, int32_t* block_table,
+                 int32_t table_cols, int32_t* free_ring, int32_t n_pages, const int64_t* free_state,
+                 int64_t* free_state_out, int32_t* kv_len, int32_t* q_start, int32_t* slot, int32_t* position,
+                 int32_t max_tokens, int32_t* status, void* stream) {
+  const char* who = "h2c_kv8_plan";
+  if (n_req < 0 || n_req > H2C_KV8_MAX_REQUESTS)
+    return op_error(H2C_ERR_INVALID, "%s: n_req must be 0 to %d, not %d", who, H2C_KV8_MAX_REQUESTS, n_req);
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+    return op_error(H2C_ERR_INVALID, "%s: page_size must be 16, 32, 64 or 128, not %d", who, page_size);
+  if (!free_ring || !free_state || !free_state_out || !q_start || !status ||
+      (n_req && (!cached || !total || !block_table || !kv_len)) || (max_tokens && (!slot || !position)))
+    return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
+  if (free_state == free_state_out) return op_error(H2C_ERR_INVALID, "%s: free_state_out must not be free_state", who);
+  if (n_pages < 1 || n_pages >= (int)SUM_LIM || (long long)n_pages * page_size > INT_MAX)
+    return op_error(H2C_ERR_INVALID, "%s: n_pages %d out of range", who, n_pages);
+  if (table_cols < 0 || (n_req && table_cols < 1))
+    return op_error(H2C_ERR_INVALID, "%s: table_cols %d out of range", who, table_cols);
+  if (max_tokens < 0 || max_tokens >= (int)SUM_LIM)
+    return op_error(H2C_ERR_INVALID, "%s: max_tokens %d out of range", who, max_tokens);
+  static unsigned char done[OP_MAX_DEVICES];
+  const int smem_max = 3 * (H2C_KV8_MAX_REQUESTS + 1) * (int)sizeof(unsigned);
+  if (int rc = op_once(who, done, [&] {
+        return cudaFuncSetAttribute(k_kv8_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_max);
+      }))
+    return rc;
+  PlanArgs a{n_req, log2_of(page_size), table_cols, n_pages, max_tokens, cached, total, block_table, free_ring,
+             reinterpret_cast<const long long*>(free_state), reinterpret_cast<long long*>(free_state_out), kv_len, q_start,
+             slot, position, status};
+  const int work = std::max(max_tokens, n_req + 1);
+  const int ctas = std::min(148, (work + PLAN_THREADS - 1) / PLAN_THREADS);
+  k_kv8_plan<<<ctas, PLAN_THREADS, 3 * (n_req + 1) * sizeof(unsigned), (cudaStream_t)stream>>>(a);
+  return op_launched(who);
+}
+
+int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
+                   int32_t type, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                   int64_t v_head, int32_t rows, const int32_t* slot, void* stream) {
+  const char* who = "h2c_kv8_append";
+  if (int rc = cache_ok(who, kv, kv_scale, n_pages, page_size, kv_heads, head_dim)) return rc;
+  if (!op_type_ok(type)) return op_error(H2C_ERR_BAD_TYPE, "%s: element type %d", who, type);
+  if (rows < 0) return op_error(H2C_ERR_INVALID, "%s: rows %d", who, rows);
+  if (rows == 0) return H2C_OK;
+  if (!k || !v || !slot) return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
+  const size_t es = op_elem_size(type);
+  if (((uintptr_t)k | (uintptr_t)v) & (es - 1))
+    return op_error(H2C_ERR_INVALID, "%s: k and v must be aligned to their elements", who);
+  const AppendArgs a{static_cast<int8_t*>(kv), kv_scale, n_pages * page_size, log2_of(page_size), kv_heads, rows, k, v,
+                     k_row, k_head, v_row, v_head, slot};
+  // loads of four elements where every row and head starts at a multiple of four
+  const bool vec = !(((uintptr_t)k | (uintptr_t)v) & (4 * es - 1)) && !((k_row | k_head | v_row | v_head) & 3);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (type == H2C_TYPE_F32) vec ? launch_append<float, true>(a, head_dim, st) : launch_append<float, false>(a, head_dim, st);
+  else if (type == H2C_TYPE_F16) vec ? launch_append<__half, true>(a, head_dim, st) : launch_append<__half, false>(a, head_dim, st);
+  else vec ? launch_append<__nv_bfloat16, true>(a, head_dim, st) : launch_append<__nv_bfloat16, false>(a, head_dim, st);
+  return op_launched(who);
+}
+
+int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t page_size, int32_t kv_heads,
+                 int32_t head_dim, const int32_t* slot, int32_t rows, int32_t type, void* k_out, void* v_out,
+                 void* stream) {
+  const char* who = "h2c_kv8_read";
+  if (int rc = cache_ok(who, kv, kv_scale, n_pages, page_size, kv_heads, head_dim)) return rc;
+  if (!op_type_ok(type)) return op_error(H2C_ERR_BAD_TYPE, "%s: element type %d", who, type);
+  if (rows < 0) return op_error(H2C_ERR_INVALID, "%s: rows %d", who, rows);
+  if (rows == 0) return H2C_OK;
+  if (!slot || !k_out || !v_out) return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
+  if (((uintptr_t)k_out | (uintptr_t)v_out) & 15)
+    return op_error(H2C_ERR_INVALID, "%s: k_out and v_out must be 16-byte aligned", who);
+  const long long units = (long long)rows * 2 * kv_heads * (head_dim / 16);
+  const int ctas = (int)std::min<long long>((units + 255) / 256, 148 * 16);
+  const int8_t* c = static_cast<const int8_t*>(kv);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int n_slots = n_pages * page_size, pl = log2_of(page_size), hl = log2_of(head_dim);
+  if (type == H2C_TYPE_F32)
+    k_kv8_read<<<ctas, 256, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, units, (float*)k_out, (float*)v_out);
+  else if (type == H2C_TYPE_F16)
+    k_kv8_read<<<ctas, 256, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, units, (__half*)k_out, (__half*)v_out);
+  else
+    k_kv8_read<<<ctas, 256, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, units, (__nv_bfloat16*)k_out,
+                                     (__nv_bfloat16*)v_out);
+  return op_launched(who);
+}
+
+}  // extern "C"

@@ -1,0 +1,519 @@
+// Attention over the paged 8-bit cache (h2c_kv8_attention; the formula is stated in include/h2cuda.h).
+//
+// Few queries (k_att_rows). A CTA takes 8 rows (query, head of the kv head's group) of one request and kv head and one
+// span of its keys; 4 warps take blocks of 16 keys in turn, each with its own running maximum, sum and output, joined at
+// the end; spans are joined by k_att_join.
+// * Tensor cores (mma.sync m16n8k16, float16 in, float32 sums): codes are integers up to 127 and exact in float16. The
+//   16 rows of an operand tile hold 8 rows twice: a float16 term in rows 0-7 and the remainder in rows 8-15, for the
+//   queries (scaled by a power of two per row) and for the softmax weights, so the products carry 22 bits, whatever the
+//   element type, at the price of one. The group of 7 or fewer heads of a single token fills no more than 8 rows anyway.
+// * The cache is the traffic: each lane copies its own 16-byte pieces of a block with cp.async into a ring that only it
+//   reads, so the ring needs no barrier; the order of dimensions inside a product is free as long as both operands use
+//   it, which lets a lane take 16 consecutive bytes of a key (QK) or of 4 keys (PV) without a transpose.
+// * Bound: the cache's bytes for long histories; latency for short ones.
+#include "kv8_att.cuh"
+
+#include <algorithm>
+#include <climits>
+
+namespace h2 {
+namespace {
+
+constexpr int RW_WARPS = 4, RW_ROWS = 8, RW_BLK = 16, RW_STAGES = 4;
+constexpr float P_SHIFT = 8.f;     // weights are kept as 2^(y - m + P_SHIFT), so that small ones stay normal float16 numbers
+constexpr float M_SLACK = 6.f;     // the running maximum moves only when a score passes it by this much (2^14 < 65504)
+
+struct Span {  // the division of a row tile's keys (lo .. hi) into spans of `blocks` 16-key blocks
+  int first, n_blocks, used;
+};
+__device__ __forceinline__ Span spans_of(int lo, int hi, int splits, int blocks) {
+  Span s;
+  s.first = lo & ~(RW_BLK - 1);
+  s.n_blocks = hi > lo ? (hi - s.first + RW_BLK - 1) / RW_BLK : 0;
+  s.used = max(1, min(splits, (s.n_blocks + blocks - 1) / blocks));
+  return s;
+}
+
+struct RowArgs {
+  AttArgs a;
+  int splits, blocks, tiles;  // spans per row tile, blocks per span, row tiles per (request, kv head)
+  float* part;                // [request][kv head][tile][span][8][HD] sums, then the same without HD for m and l
+  float2* ml;
+};
+
+__device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <class T, int HD>
+__device__ __forceinline__ void store_row4(const AttArgs& a, T* dst, const float* v) {
+  if (a.out_vec) {
+    alignas(16) T o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = from_f<T>(v[i]);
+    if (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(o);
+    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) dst[i] = from_f<T>(v[i]);
+  }
+}
+
+template <int HD>
+struct RowSmem {
+  static constexpr int STAGE = RW_BLK * HD * 2;                       // a warp's block: K, then V
+  static constexpr int RING = RW_WARPS * RW_STAGES * STAGE;
+  static constexpr int JOIN = RW_WARPS * RW_ROWS * (HD + 2) * 4;      // (reuses the ring)
+  static constexpr int SCALES = RW_WARPS * RW_STAGES * 8;
+  static constexpr int BYTES = (RING > JOIN ? RING : JOIN) + SCALES;
+};
+
+template <class T, int HD>
+__global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
+  using S = RowSmem<HD>;
+  constexpr int KC = HD / 64;   // 16-byte pieces of a key per lane
+  constexpr int VB = HD / 8;    // bytes of a value row per lane (16 or 8)
+  constexpr int NT = HD / 8;    // output tiles of 8 dimensions
+  extern __shared__ __align__(16) uint8_t sm[];
+  const AttArgs& a = ra.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int split = blockIdx.x % ra.splits, th = blockIdx.x / ra.splits, head = th % a.kv_heads, tile = th / a.kv_heads;
+  const int r = blockIdx.y;
+  const Request R = request_of(a, r);
+  const int n_all = a.q_start[r + 1] - a.q_start[r];
+  const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group;
+  if (row0 >= n_rows) return;
+  int lo, hi;
+  key_range(a, R, n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
+  const Span sp = spans_of(lo, hi, ra.splits, ra.blocks);
+  if (split >= sp.used) return;
+  const int b_begin = split * ra.blocks, b_end = split == sp.used - 1 ? sp.n_blocks : b_begin + ra.blocks;
+
+  // ---- this lane's row: query dimensions 64j + 16c .. +15, as float16 terms
+  const int row = row0 + g;
+  const bool live = row < n_rows;
+  const int tok = live ? row / a.group : 0, hq = head * a.group + (live ? row % a.group : 0);
+  const int pos = R.len - n_all + tok;               // its position, and the keys it may see: [first_key, pos]
+  const int first_key = a.window > 0 ? pos + 1 - a.window : 0;
+  uint32_t qa[KC * 4][4];
+  float q_scale;  // what a product of codes is multiplied by: power of two of the row, softmax scale
+  {
+    float v[KC][16];
+    const T* src = static_cast<const T*>(a.q) + (long long)(R.first + tok) * a.q_row + hq * a.q_head + 16 * c;
+#pragma unroll
+    for (int j = 0; j < KC; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (live) {
+          if (a.q_vec) load4<true>(src + 64 * j + 4 * i, &v[j][4 * i]);
+          else load4<false>(src + 64 * j + 4 * i, &v[j][4 * i]);
+        } else {
+          v[j][4 * i] = v[j][4 * i + 1] = v[j][4 * i + 2] = v[j][4 * i + 3] = 0.f;
+        }
+      }
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < KC; j++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) m = max(m, __float_as_uint(v[j][i]) & 0x7fffffffu);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    // the largest magnitude to [2^13, 2^14): the remainders stay normal float16 numbers
+    const int e = (int)(m >> 23);
+    const int up = e == 255 || m == 0 ? 127 : min(253, 267 - e);
+    const float mul = __int_as_float(up << 23);
+    q_scale = __int_as_float((254 - up) << 23) * a.scale_log2;
+#pragma unroll
+    for (int j = 0; j < KC; j++)
+#pragma unroll
+      for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float x0 = v[j][4 * s + 2 * h] * mul, x1 = v[j][4 * s + 2 * h + 1] * mul;
+          const __half2 t = __floats2half2_rn(x0, x1);
+          qa[4 * j + s][2 * h] = *reinterpret_cast<const uint32_t*>(&t);
+          qa[4 * j + s][2 * h + 1] = pack_half2(x0 - __low2float(t), x1 - __high2float(t));
+        }
+  }
+
+  float o[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+
+  // ---- the warp's blocks: b_begin + warp + 4 it
+  const int n_it = max(0, (b_end - b_begin - warp + RW_WARPS - 1) / RW_WARPS);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * RW_STAGES * S::STAGE;
+  float2* scales = reinterpret_cast<float2*>(sm + S::BYTES - S::SCALES) + warp * RW_STAGES;
+  const int P = 1 << a.page_log;
+  const size_t head_bytes = (size_t)P * HD;
+  int i_page = 0;
+  float i_sk = 0.f, i_sv = 0.f;
+  auto issue = [&](int it) {
+    if (it < n_it) {
+      if ((it & 31) == 0) {  // pages and scales of the next 32 blocks, one per lane
+        const int b = b_begin + warp + RW_WARPS * (it + lane);
+        if (b < b_end) {
+          int pg = a.table[(size_t)r * a.table_cols + ((sp.first + b * RW_BLK) >> a.page_log)];
+          i_page = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
+          const float* s = a.kv_scale + (size_t)i_page * 2 * a.kv_heads + head;
+          i_sk = s[0];
+          i_sv = s[a.kv_heads];
+        }
+      }
+      const int page = __shfl_sync(0xffffffffu, i_page, it & 31);
+      const float sk = __shfl_sync(0xffffffffu, i_sk, it & 31), sv = __shfl_sync(0xffffffffu, i_sv, it & 31);
+      const int stage = it % RW_STAGES, b = b_begin + warp + RW_WARPS * it;
+      if (lane == 0) scales[stage] = make_float2(sk, sv);
+      const int8_t* kb = a.kv + ((size_t)page * 2 * a.kv_heads + head) * head_bytes + ((sp.first + b * RW_BLK) & (P - 1)) * HD;
+      const int8_t* vb = kb + a.kv_heads * head_bytes;
+      const uint32_t dst = ring + stage * S::STAGE + lane * 16;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int j = 0; j < KC; j++) copy_async<16>(dst + (t * KC + j) * 512, kb + (8 * t + g) * HD + 64 * j + 16 * c);
+      const uint32_t vd = ring + stage * S::STAGE + RW_BLK * HD + lane * VB;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        copy_async<VB>(vd + i * 32 * VB, vb + (2 * c + (i & 1) + 8 * (i >> 1)) * HD + VB * g);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int it = 0; it < RW_STAGES - 1; it++) issue(it);
+
+  for (int it = 0; it < n_it; it++) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(RW_STAGES - 2) : "memory");
+    __syncwarp();
+    const int stage = it % RW_STAGES;
+    const uint8_t* kst = sm + warp * RW_STAGES * S::STAGE + stage * S::STAGE + lane * 16;
+    const uint8_t* vst = sm + warp * RW_STAGES * S::STAGE + stage * S::STAGE + RW_BLK * HD + lane * VB;
+    const float2 sc = scales[stage];
+    const int key0 = sp.first + (b_begin + warp + RW_WARPS * it) * RW_BLK + 2 * c;
+    // scores of 8 rows x 16 keys: this lane has keys key0, key0 + 1 (tile 0), key0 + 8, key0 + 9 (tile 1) of its row
+    float y[4];
+    float e_v, mant, inv_pow;
+    split_scale(sc.y, &e_v, &mant, &inv_pow);
+    const float f = q_scale * sc.x;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KC; j++) {
+        const uint4 w4 = *reinterpret_cast<const uint4*>(kst + (t * KC + j) * 512);
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+          const uint32_t u = w[s] ^ 0x80808080u;
+          mma16816(d, qa[4 * j + s][0], qa[4 * j + s][1], qa[4 * j + s][2], qa[4 * j + s][3],
+                   half2_of(__byte_perm(u, 0x64646464u, 0x4140)), half2_of(__byte_perm(u, 0x64646464u, 0x4342)));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int key = key0 + 8 * t + i;
+        const float x = (d[i] + d[i + 2]) * f;
+        y[2 * t + i] = live && key <= pos && key >= first_key ? x + e_v : -INFINITY;
+      }
+    }
+    float mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    if (__any_sync(0xffffffffu, mx > m_run + M_SLACK)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float f_old = m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
+      m_run = m_new;
+      l_run *= f_old;
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        o[t][0] *= f_old; o[t][1] *= f_old; o[t][2] *= f_old; o[t][3] *= f_old;
+      }
+    }
+    const float m_use = (m_run == -INFINITY ? 0.f : m_run) - P_SHIFT;
+    float p[4], rest[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float w = exp2_fast(y[i] - m_use);
+      l_run += w * inv_pow;
+      p[i] = w * mant;
+    }
+    const uint32_t a0 = pack_half2(p[0], p[1]), a2 = pack_half2(p[2], p[3]);
+    {
+      const __half2 h0 = *reinterpret_cast<const __half2*>(&a0), h1 = *reinterpret_cast<const __half2*>(&a2);
+      rest[0] = p[0] - __low2float(h0); rest[1] = p[1] - __high2float(h0);
+      rest[2] = p[2] - __low2float(h1); rest[3] = p[3] - __high2float(h1);
+    }
+    const uint32_t a1 = pack_half2(rest[0], rest[1]), a3 = pack_half2(rest[2], rest[3]);
+    // values: 4 keys x VB consecutive dimensions; tile t of the output takes dimension VB * n + t at column n
+    uint32_t vw[4][VB / 4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (VB == 16) *reinterpret_cast<uint4*>(vw[i]) = *reinterpret_cast<const uint4*>(vst + i * 32 * VB);
+      else *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(vst + i * 32 * VB);
+    }
+#pragma unroll
+    for (int w = 0; w < VB / 4; w++) {
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) u[i] = vw[i][w] ^ 0x80808080u;
+#pragma unroll
+      for (int hpair = 0; hpair < 2; hpair++) {
+        const uint32_t k01 = __byte_perm(u[0], u[1], hpair ? 0x7362 : 0x5140);
+        const uint32_t k23 = __byte_perm(u[2], u[3], hpair ? 0x7362 : 0x5140);
+        mma16816(o[4 * w + 2 * hpair], a0, a1, a2, a3, half2_of(__byte_perm(k01, 0x64646464u, 0x4140)),
+                 half2_of(__byte_perm(k23, 0x64646464u, 0x4140)));
+        mma16816(o[4 * w + 2 * hpair + 1], a0, a1, a2, a3, half2_of(__byte_perm(k01, 0x64646464u, 0x4342)),
+                 half2_of(__byte_perm(k23, 0x64646464u, 0x4342)));
+      }
+    }
+    issue(it + RW_STAGES - 1);
+  }
+  l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+  l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+
+  // ---- join the warps: [warp][8][HD] sums, [warp][8] maxima, [warp][8] sums of weights
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float* js = reinterpret_cast<float*>(sm);
+  float* jm = js + RW_WARPS * RW_ROWS * HD;
+  float* jl = jm + RW_WARPS * RW_ROWS;
+  if (c == 0) {
+    jm[warp * RW_ROWS + g] = m_run;
+    jl[warp * RW_ROWS + g] = l_run;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int t = 0; t < NT; t += 4)
+      *reinterpret_cast<float4*>(js + (warp * RW_ROWS + g) * HD + VB * (2 * c + i) + t) =
+          make_float4(o[t][i] + o[t][i + 2], o[t + 1][i] + o[t + 1][i + 2], o[t + 2][i] + o[t + 2][i + 2],
+                      o[t + 3][i] + o[t + 3][i + 2]);
+  __syncthreads();
+  constexpr int TPR = RW_WARPS * 32 / RW_ROWS;  // threads per row
+  const int jr = threadIdx.x / TPR, jt = threadIdx.x % TPR, orow = row0 + jr;
+  if (orow >= n_rows) return;
+  float mm = -INFINITY, ll = 0.f, fw[RW_WARPS];
+#pragma unroll
+  for (int w = 0; w < RW_WARPS; w++) mm = fmaxf(mm, jm[w * RW_ROWS + jr]);
+#pragma unroll
+  for (int w = 0; w < RW_WARPS; w++) {
+    const float mw = jm[w * RW_ROWS + jr];
+    fw[w] = mw == -INFINITY ? 0.f : exp2_fast(mw - mm);
+    ll += fw[w] * jl[w * RW_ROWS + jr];
+  }
+  const size_t unit = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits + split;
+  const bool whole = sp.used == 1;
+  const float inv = whole && ll != 0.f ? 1.f / ll : 1.f;
+  const int otok = orow / a.group, oh = head * a.group + orow % a.group;
+#pragma unroll
+  for (int k = 0; k < HD / 4 / TPR; k++) {
+    const int d = (jt + k * TPR) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < RW_WARPS; w++) {
+      const float4 x = *reinterpret_cast<const float4*>(js + (w * RW_ROWS + jr) * HD + d);
+      v[0] += fw[w] * x.x; v[1] += fw[w] * x.y; v[2] += fw[w] * x.z; v[3] += fw[w] * x.w;
+    }
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] *= inv;
+      store_row4<T, HD>(a, static_cast<T*>(a.out) + (long long)(R.first + otok) * a.out_row + oh * a.out_head + d, v);
+    } else {
+      *reinterpret_cast<float4*>(ra.part + (unit * RW_ROWS + jr) * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+  if (jt == 0) {
+    if (!whole) ra.ml[unit * RW_ROWS + jr] = make_float2(mm, ll);
+    else if (a.lse)
+      a.lse[(size_t)(R.first + otok) * a.heads + oh] =
+          ll == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(ll) + mm - P_SHIFT);
+  }
+}
+
+// Joins the spans of one row: the weights of span s relative to the common maximum are 2^(m_s - m).
+template <class T, int HD>
+__global__ void __launch_bounds__(256) k_att_join(const RowArgs ra) {
+  constexpr int TPR = HD / 4, LANES = 256 / TPR;  // threads for a row's dimensions, spans in flight
+  const AttArgs& a = ra.a;
+  const int jr = blockIdx.x % RW_ROWS, th = blockIdx.x / RW_ROWS, head = th % a.kv_heads, tile = th / a.kv_heads;
+  const int r = blockIdx.y;
+  const Request R = request_of(a, r);
+  const int n_all = a.q_start[r + 1] - a.q_start[r];
+  const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group, orow = row0 + jr;
+  if (orow >= n_rows) return;
+  int lo, hi;
+  key_range(a, R, n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
+  const Span sp = spans_of(lo, hi, ra.splits, ra.blocks);
+  if (sp.used == 1) return;  // (written by its only span)
+  const size_t unit0 = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits;
+  const int d = (threadIdx.x % TPR) * 4, s0 = threadIdx.x / TPR;
+  __shared__ float red[8];
+  __shared__ float acc[LANES][HD + 1];
+  float m = -INFINITY;
+  for (int s = threadIdx.x; s < sp.used; s += 256) m = fmaxf(m, ra.ml[(unit0 + s) * RW_ROWS + jr].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; w++) m = fmaxf(m, red[w]);
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int s = s0; s < sp.used; s += LANES) {
+    const float2 ml = ra.ml[(unit0 + s) * RW_ROWS + jr];
+    const float4 x = *reinterpret_cast<const float4*>(ra.part + ((unit0 + s) * RW_ROWS + jr) * HD + d);
+    const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
+    l += f * ml.y;
+    v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) acc[s0][d + i] = v[i];
+  if (d == 0) acc[s0][HD] = l;
+  __syncthreads();
+  if (threadIdx.x >= TPR) return;
+  l = 0.f;
+  v[0] = v[1] = v[2] = v[3] = 0.f;
+#pragma unroll
+  for (int s = 0; s < LANES; s++) {
+    l += acc[s][HD];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] += acc[s][d + i];
+  }
+  const float inv = l != 0.f ? 1.f / l : 1.f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] *= inv;
+  const int tok = orow / a.group, hq = head * a.group + orow % a.group;
+  store_row4<T, HD>(a, static_cast<T*>(a.out) + (long long)(R.first + tok) * a.out_row + hq * a.out_head + d, v);
+  if (d == 0 && a.lse)
+    a.lse[(size_t)(R.first + tok) * a.heads + hq] =
+        l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
+}
+
+// ---------------------------------------------------------------- host
+
+struct RowPlan {
+  int splits, blocks, tiles;
+  size_t units, bytes;
+};
+// Spans: enough CTAs for two waves of three per SM, but no span under 256 keys (4 blocks per warp), below which its start-up
+// costs more than it shares out.
+RowPlan plan_rows(const h2c_kv8_attention_args* g) {
+  RowPlan p;
+  const int group = g->heads / g->kv_heads;
+  p.tiles = (int)(((long long)g->max_q * group + RW_ROWS - 1) / RW_ROWS);
+  long long keys = g->max_kv;
+  if (g->window > 0) keys = std::min(keys, (long long)g->window + g->max_q);
+  const int n_blocks = (int)((keys + RW_BLK - 1) / RW_BLK) + (g->window > 0 ? 1 : 0);
+  const long long groups = (long long)g->n_req * g->kv_heads * p.tiles;
+  const long long want = (888 + groups - 1) / groups;
+  const int most = std::max(1, n_blocks / 16);
+  p.splits = (int)std::max(1LL, std::min<long long>(want, most));
+  p.blocks = std::max(RW_WARPS, ((n_blocks + p.splits - 1) / p.splits + RW_WARPS - 1) / RW_WARPS * RW_WARPS);
+  p.splits = std::max(1, (n_blocks + p.blocks - 1) / p.blocks);
+  p.units = p.splits > 1 ? (size_t)groups * p.splits : 0;
+  p.bytes = p.units * RW_ROWS * ((size_t)g->head_dim * 4 + 8);
+  return p;
+}
+
+template <class T, int HD>
+int launch_rows(const char* who, const RowArgs& ra, cudaStream_t st) {
+  static unsigned char done[OP_MAX_DEVICES];
+  constexpr int smem = RowSmem<HD>::BYTES;
+  if (int rc = op_once(who, done, [] {
+        return cudaFuncSetAttribute(k_att_rows<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      }))
+    return rc;
+  const dim3 grid((unsigned)(ra.splits * ra.a.kv_heads) * ra.tiles, ra.a.n_req);
+  k_att_rows<T, HD><<<grid, RW_WARPS * 32, smem, st>>>(ra);
+  if (ra.splits > 1) {
+    const dim3 jgrid((unsigned)(RW_ROWS * ra.a.kv_heads) * ra.tiles, ra.a.n_req);
+    k_att_join<T, HD><<<jgrid, 256, 0, st>>>(ra);
+  }
+  return op_launched(who);
+}
+
+template <class T>
+int launch_typed(const char* who, int head_dim, const RowArgs& ra, cudaStream_t st) {
+  return head_dim == 64 ? launch_rows<T, 64>(who, ra, st) : launch_rows<T, 128>(who, ra, st);
+}
+
+int check_args(const char* who, const h2c_kv8_attention_args* g) {
+  if (!g) return op_error(H2C_ERR_INVALID, "%s: null arguments", who);
+  if (g->page_size != 16 && g->page_size != 32 && g->page_size != 64 && g->page_size != 128)
+    return op_error(H2C_ERR_INVALID, "%s: page_size must be 16, 32, 64 or 128, not %d", who, g->page_size);
+  if (g->head_dim != 64 && g->head_dim != 128)
+    return op_error(H2C_ERR_INVALID, "%s: head_dim must be 64 or 128, not %d", who, g->head_dim);
+  if (g->n_pages < 1 || (long long)g->n_pages * g->page_size > INT_MAX)
+    return op_error(H2C_ERR_INVALID, "%s: n_pages %d out of range", who, g->n_pages);
+  if (g->kv_heads < 1 || g->kv_heads > 4096 || g->heads < g->kv_heads || g->heads > 65536 || g->heads % g->kv_heads)
+    return op_error(H2C_ERR_INVALID, "%s: heads (%d) must be a multiple of kv_heads (%d)", who, g->heads, g->kv_heads);
+  if (!op_type_ok(g->type)) return op_error(H2C_ERR_BAD_TYPE, "%s: element type %d", who, g->type);
+  if (g->n_req < 0 || g->n_req > H2C_KV8_MAX_REQUESTS)
+    return op_error(H2C_ERR_INVALID, "%s: n_req must be 0 to %d, not %d", who, H2C_KV8_MAX_REQUESTS, g->n_req);
+  if (g->rows < 0 || g->max_q < 0 || g->max_kv < 0 || g->window < 0 || g->table_cols < 0)
+    return op_error(H2C_ERR_INVALID, "%s: a size is negative", who);
+  if ((long long)g->max_q * (g->heads / g->kv_heads) > INT_MAX / 2)
+    return op_error(H2C_ERR_INVALID, "%s: max_q %d out of range", who, g->max_q);
+  return H2C_OK;
+}
+
+bool nothing_to_do(const h2c_kv8_attention_args* g) { return g->n_req == 0 || g->rows == 0 || g->max_q == 0; }
+
+}  // namespace
+}  // namespace h2
+
+using namespace h2;
+
+extern "C" {
+
+uint64_t h2c_kv8_attention_workspace(const h2c_kv8_attention_args* g) {
+  if (check_args("h2c_kv8_attention_workspace", g) || nothing_to_do(g)) return 0;
+  return plan_rows(g).bytes;
+}
+
+int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
+  const char* who = "h2c_kv8_attention";
+  if (int rc = check_args(who, g)) return rc;
+  if (nothing_to_do(g)) return H2C_OK;
+  if (!g->q || !g->out || !g->kv || !g->kv_scale || !g->q_start || !g->kv_len || (g->table_cols && !g->block_table))
+    return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
+  const size_t es = op_elem_size(g->type);
+  if ((uintptr_t)g->kv & 15) return op_error(H2C_ERR_INVALID, "%s: the cache must be 16-byte aligned", who);
+  if (((uintptr_t)g->q | (uintptr_t)g->out) & (es - 1))
+    return op_error(H2C_ERR_INVALID, "%s: q and out must be aligned to their elements", who);
+  const RowPlan p = plan_rows(g);
+  if (p.bytes && (!g->workspace || g->workspace_bytes < p.bytes || ((uintptr_t)g->workspace & 15)))
+    return op_error(H2C_ERR_INVALID, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
+                    (unsigned long long)p.bytes, (unsigned long long)(g->workspace ? g->workspace_bytes : 0));
+  if ((long long)p.splits * g->kv_heads * p.tiles > INT_MAX / RW_ROWS)
+    return op_error(H2C_ERR_INVALID, "%s: max_q %d out of range", who, g->max_q);
+  RowArgs ra;
+  AttArgs& a = ra.a;
+  a.q = g->q; a.q_row = g->q_row; a.q_head = g->q_head;
+  a.out = g->out; a.out_row = g->out_row; a.out_head = g->out_head;
+  a.lse = g->lse;
+  a.kv = static_cast<const int8_t*>(g->kv); a.kv_scale = g->kv_scale;
+  a.table = g->block_table; a.q_start = g->q_start; a.kv_len = g->kv_len;
+  a.n_pages = g->n_pages; a.kv_heads = g->kv_heads; a.heads = g->heads; a.group = g->heads / g->kv_heads;
+  a.page_log = g->page_size == 16 ? 4 : g->page_size == 32 ? 5 : g->page_size == 64 ? 6 : 7;
+  a.table_cols = g->table_cols; a.n_req = g->n_req; a.rows = g->rows; a.max_q = g->max_q; a.window = g->window;
+  a.q_vec = !((uintptr_t)g->q & (4 * es - 1)) && !((g->q_row | g->q_head) & 3);
+  a.out_vec = !((uintptr_t)g->out & (4 * es - 1)) && !((g->out_row | g->out_head) & 3);
+  a.scale_log2 = g->scale * 1.4426950408889634f;
+  ra.splits = p.splits; ra.blocks = p.blocks; ra.tiles = p.tiles;
+  ra.part = static_cast<float*>(g->workspace);
+  ra.ml = reinterpret_cast<float2*>(ra.part + p.units * RW_ROWS * g->head_dim);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (g->type == H2C_TYPE_F32) return launch_typed<float>(who, g->head_dim, ra, st);
+  if (g->type == H2C_TYPE_F16) return launch_typed<__half>(who, g->head_dim, ra, st);
+  return launch_typed<__nv_bfloat16>(who, g->head_dim, ra, st);
+}
+
+}  // extern "C"

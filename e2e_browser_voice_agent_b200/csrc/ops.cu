@@ -1,0 +1,62 @@
+// Host side shared by the stand-alone 8-bit serving operators (ops.cuh).
+#include "ops.cuh"
+
+#include <cstdarg>
+#include <cstdio>
+#include <mutex>
+
+namespace h2 {
+
+void set_last_error(const char* msg) noexcept;  // h2cuda.cu: the message of h2c_last_error(NULL)
+
+int op_error(int code, const char* fmt, ...) noexcept {
+  char buf[400];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  set_last_error(buf);
+  return code;
+}
+
+int op_launched(const char* who) noexcept {
+  const cudaError_t c = cudaGetLastError();
+  return c == cudaSuccess ? H2C_OK : op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
+}
+
+namespace {
+__device__ int g_op_err[4];
+int* g_op_err_ptr[OP_MAX_DEVICES];
+}  // namespace
+
+int* op_err_words() noexcept {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= OP_MAX_DEVICES) return nullptr;
+  int* p = __atomic_load_n(&g_op_err_ptr[dev], __ATOMIC_ACQUIRE);
+  if (!p) {
+    void* q = nullptr;
+    if (cudaGetSymbolAddress(&q, g_op_err) != cudaSuccess) return nullptr;
+    p = static_cast<int*>(q);
+    __atomic_store_n(&g_op_err_ptr[dev], p, __ATOMIC_RELEASE);
+  }
+  return p;
+}
+
+}  // namespace h2
+
+extern "C" int h2c_ops_check(void* stream) {
+  using namespace h2;
+  int* d = op_err_words();
+  if (!d) return op_error(H2C_ERR_CUDA, "h2c_ops_check: no device");
+  int w[4] = {0, 0, 0, 0};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t c = cudaMemcpyAsync(w, d, sizeof w, cudaMemcpyDeviceToHost, st);
+  if (c == cudaSuccess) c = cudaStreamSynchronize(st);
+  if (c == cudaSuccess && w[0]) {
+    c = cudaMemsetAsync(d, 0, sizeof w, st);
+    if (c == cudaSuccess) c = cudaStreamSynchronize(st);
+  }
+  if (c != cudaSuccess) return op_error(H2C_ERR_CUDA, "h2c_ops_check: %s", cudaGetErrorString(c));
+  if (w[0]) return op_error(H2C_ERR_TIMEOUT, "a wait inside an operator expired (CTA %d, role %d): its output is not valid", w[1], w[2]);
+  return H2C_OK;
+}

@@ -1,0 +1,79 @@
+// What the stand-alone 8-bit serving operators (kv8.cu, kv8_att.cu, i8mm.cu) share: error reporting at the C entries,
+// once-per-device kernel attributes, the record of expired waits, and loads and stores of activations of any type.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/h2cuda.h"
+
+namespace h2 {
+
+// Record the message of a failed call (h2c_last_error(NULL)) and return `code`. Never throws.
+int op_error(int code, const char* fmt, ...) noexcept __attribute__((format(printf, 2, 3)));
+// H2C_OK, or H2C_ERR_CUDA with "<who>: launch failed: ..." when the last launch of this thread failed.
+int op_launched(const char* who) noexcept;
+// Four device words of the current device in which a kernel whose bounded wait expired leaves {1, CTA, role, 0}
+// (read by h2c_ops_check); nullptr when the device cannot be queried.
+int* op_err_words() noexcept;
+
+constexpr int OP_MAX_DEVICES = 64;
+// Run fn() once per device (kernel attributes); its status, or H2C_OK when it has already run on this device.
+template <class F>
+int op_once(const char* who, unsigned char* done, F fn) noexcept {
+  int dev = -1;
+  cudaError_t c = cudaGetDevice(&dev);
+  if (c != cudaSuccess || dev < 0 || dev >= OP_MAX_DEVICES)
+    return op_error(H2C_ERR_CUDA, "%s: cudaGetDevice: %s", who,
+                    c != cudaSuccess ? cudaGetErrorString(c) : "device index out of range");
+  if (__atomic_load_n(done + dev, __ATOMIC_ACQUIRE)) return H2C_OK;
+  c = fn();  // idempotent: two threads that get here together both set the same attributes
+  if (c != cudaSuccess) return op_error(H2C_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", who, cudaGetErrorString(c));
+  __atomic_store_n(done + dev, 1, __ATOMIC_RELEASE);
+  return H2C_OK;
+}
+
+inline size_t op_elem_size(int type) { return type == H2C_TYPE_F32 ? 4 : 2; }
+inline bool op_type_ok(int type) { return type == H2C_TYPE_F32 || type == H2C_TYPE_F16 || type == H2C_TYPE_BF16; }
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// four consecutive values; VEC: the address is aligned to four of them
+template <bool VEC>
+__device__ __forceinline__ void load4(const float* p, float* v) {
+  if (VEC) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = p[i];
+  }
+}
+template <bool VEC, class T>
+__device__ __forceinline__ void load4(const T* p, float* v) {
+  static_assert(sizeof(T) == 2, "16-bit types");
+  if (VEC) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    const T* h = reinterpret_cast<const T*>(&a);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = to_f(h[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = to_f(p[i]);
+  }
+}
+#endif
+
+}  // namespace h2

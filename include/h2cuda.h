@@ -243,6 +243,104 @@ int h2c_q4_matvec(const void* w, int32_t n_rows, int32_t k, const float* x, int3
 int h2c_q4_matvec_noalloc(const void* w, int32_t n_rows, int32_t k, const float* x, int32_t m, float* y,
                           int32_t op, const float* bias, void* stream);
 
+/* ---- 8-bit serving operators: a paged 8-bit KV cache and matrix products in 8-bit integers. Stand-alone device
+ * operations (no engine): every pointer is a DEVICE pointer unless said otherwise, `stream` is a cudaStream_t of the
+ * current device (0 = default) and a call only enqueues work on it, nothing is allocated, and a call whose arguments
+ * do not fit returns a status with a message in h2c_last_error(NULL) before anything is enqueued. Sizes of zero
+ * (requests, rows) are valid and do nothing. Results do not depend on the stream, the launch or other calls.
+ *
+ * The cache: `kv` holds int8 codes [n_pages][2][kv_heads][page_size][head_dim] (index 0 of the second axis: K, 1: V;
+ * 16-byte aligned), `kv_scale` float32 [n_pages][2][kv_heads]; a cached value is code * scale. page_size is 16, 32, 64 or
+ * 128, head_dim 64 or 128, n_pages * page_size < 2^31. A slot is page * page_size + offset. A request's position p lies
+ * in page block_table[request][p / page_size] at offset p % page_size; no page belongs to two requests. ---- */
+
+/* element types of activations */
+#define H2C_TYPE_F32 0
+#define H2C_TYPE_F16 1
+#define H2C_TYPE_BF16 2
+
+#define H2C_KV8_MAX_REQUESTS 8192
+
+/* H2C_OK, or H2C_ERR_TIMEOUT when a bounded wait inside one of these operators' kernels expired on the current device
+ * since the last check (its output is then not valid; this never happens in normal operation). Waits for `stream`. */
+int h2c_ops_check(void* stream);
+
+/* Block tables and slot maps from request lengths, on the device. Request r holds cached[r] tokens and will hold total[r]
+ * after the step: more (its new tokens are cached[r] .. total[r]-1, pages are taken for them), as many, or fewer (it is
+ * cut back, or ends at 0, and the pages beyond are given back).
+ *   cached, total    int32 [n_req], n_req <= H2C_KV8_MAX_REQUESTS
+ *   block_table      int32 [n_req][table_cols], in place: the entries of the pages taken are written; entries past a
+ *                    request's length keep what they held and mean nothing
+ *   free_ring        int32 [n_pages], in place: a ring of free page numbers; free_state int64 [2] = {head, tail}
+ *                    (both only grow): the free pages are free_ring[head % n_pages] .. free_ring[(tail - 1) % n_pages].
+ *                    Pages are taken at the head in request order, those given back are appended at the tail in
+ *                    request order, and can be taken in the same call once the older ones are used up
+ *   free_state_out   int64 [2], the ring after the step (not the same memory as free_state: a call with the same
+ *                    inputs again gives the same results)
+ *   kv_len           int32 [n_req]: total[r];  q_start int32 [n_req + 1]: prefix sums of the new tokens
+ *   slot, position   int32 [max_tokens]: slot and position of each new token, in request order; -1 beyond the last
+ *   status           int32 [2]: {0, 0}; {1, missing} when the free pages do not suffice; {2, 0} when a length is negative
+ *                    or above table_cols * page_size, the new tokens are more than max_tokens, or the ring's state is
+ *                    not that of n_pages pages. With a non-zero status nothing is taken or given back: kv_len is
+ *                    cached (0 where that is invalid), q_start all 0, slot and position all -1, free_state_out =
+ *                    free_state. */
+int h2c_kv8_plan(int32_t n_req, int32_t page_size, const int32_t* cached, const int32_t* total, int32_t* block_table,
+                 int32_t table_cols, int32_t* free_ring, int32_t n_pages, const int64_t* free_state,
+                 int64_t* free_state_out, int32_t* kv_len, int32_t* q_start, int32_t* slot, int32_t* position,
+                 int32_t max_tokens, int32_t* status, void* stream);
+
+/* Append rows of K and V (element type `type`, row t of head h at k + t * k_row + h * k_head elements, head_dim values
+ * each, likewise v) to the cache at slot[t]; rows whose slot is not in the cache (-1) are skipped. The rows of one page
+ * must be consecutive rows at consecutive offsets, as h2c_kv8_plan orders them. Per (page, K or V, head), with a the
+ * largest magnitude of the rows that go there and s0 the scale so far (0 when they start at offset 0, which makes the
+ * page new whatever it held): if a > 127.5 s0 the scale becomes s = max(a / 127, 1.25 s0), within [2^-62, 2^63], and the
+ * codes at earlier offsets become round(code * (s0 / s)); else s = s0. The new codes are round(x * (1 / s)), within
+ * [-127, 127] (float32 operations, halves to even). A code is re-rounded only when the scale grows, which it does by at
+ * least 1.25 each time, so a cached value is off by at most 2.5 final steps. A row with an infinity or NaN makes its
+ * page's scale NaN until the page is new again: every read of that page and head gives NaN. */
+int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
+                   int32_t type, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                   int64_t v_head, int32_t rows, const int32_t* slot, void* stream);
+
+/* The cached values at slot[t], t < rows: k_out and v_out [rows][kv_heads][head_dim] of element type `type` (16-byte
+ * aligned); zeros where the slot is not in the cache. To move a session elsewhere, or to look at what the cache holds. */
+int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t page_size, int32_t kv_heads,
+                 int32_t head_dim, const int32_t* slot, int32_t rows, int32_t type, void* k_out, void* v_out,
+                 void* stream);
+
+/* Grouped-query attention of a ragged batch over the cache. Request r's queries are rows q_start[r] .. q_start[r + 1]-1 of
+ * q, its last query at position kv_len[r] - 1: query i of n sits at position p = kv_len[r] - n + i and attends to the cached
+ * positions 0 .. p, or p - window + 1 .. p with window > 0. Head h reads kv head h / (heads / kv_heads).
+ *   x = scale * (q . k),  out = sum softmax(x) v  (rounded once to `type`),  lse = log sum exp x  (natural logarithm)
+ * A query with no position to attend to (p < 0) gives zeros and lse = -infinity. Rows of q that belong to no request are
+ * not touched. Scores, softmax statistics and sums are float32; codes and float16 / bfloat16 queries enter the tensor
+ * cores exactly, float32 queries as two float16 terms (22 bits). */
+typedef struct h2c_kv8_attention_args {
+  const void* q;          /* row t of head h at t * q_row + h * q_head elements, head_dim values */
+  int64_t q_row, q_head;
+  void* out;              /* the same with out_row, out_head */
+  int64_t out_row, out_head;
+  float* lse;             /* [rows][heads], or NULL */
+  const void* kv;
+  const float* kv_scale;
+  int32_t n_pages, page_size, kv_heads, head_dim;
+  int32_t heads, type;    /* heads a multiple of kv_heads; element type of q and out */
+  const int32_t* block_table; /* [n_req][table_cols] */
+  int32_t table_cols, n_req;
+  const int32_t* q_start; /* [n_req + 1] */
+  const int32_t* kv_len;  /* [n_req] */
+  int32_t rows;           /* rows of q and out */
+  int32_t max_q, max_kv;  /* bounds of the requests' query counts and kv_len, for the division of the work: a request with
+                             more than max_q queries has only its first max_q computed; kv_len above max_kv costs time */
+  int32_t window;         /* 0: none */
+  float scale;
+  void* workspace;        /* h2c_kv8_attention_workspace(args) bytes, 16-byte aligned; NULL when that is 0 */
+  uint64_t workspace_bytes;
+} h2c_kv8_attention_args;
+/* Bytes of device workspace a call with these sizes needs (pointers are not looked at). Host only. */
+uint64_t h2c_kv8_attention_workspace(const h2c_kv8_attention_args* args);
+int h2c_kv8_attention(const h2c_kv8_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
