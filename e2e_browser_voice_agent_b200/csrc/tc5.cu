@@ -33,6 +33,7 @@
 // Every wait is bounded (%globaltimer, 1 s) and watches a CTA abort flag: on expiry the CTA records the failure in
 // `err`, drains its copies and MMAs, frees its TMEM and returns.
 #include "tc5.cuh"
+#include "tc5_ptx.cuh"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -41,13 +42,26 @@
 #include <mutex>
 
 namespace h2 {
+
+PFN_cuTensorMapEncodeTiled_v12000 tma_encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
 namespace {
 
 constexpr int CB = 4;         // Q4_0 blocks per chunk (128 activation bytes per token: one 128-byte swizzle row)
 constexpr int NA = 16;        // A-tile slots (4 chunks)
 constexpr int ATILE = 4096;   // one A tile: 128 rows x 32 bytes, no swizzle (core matrices 8 rows x 16 B)
 constexpr uint32_t FMAGIC = 0x4B400000u;
-constexpr unsigned long long TIMEOUT_NS = 1000000000ull;
 
 // Every hand-off between the roles is per chunk of 4 blocks (one mbarrier wait per role per chunk: a wait costs
 // about 0.1 us even when the phase has completed, which per block was the pipeline's whole budget), and the rings are
@@ -69,121 +83,6 @@ struct Cfg {
   static_assert(COLS <= 512 && SMEM <= 227 * 1024, "TMEM or shared memory budget");
 };
 
-__device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint64_t* b, unsigned n) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n));
-}
-__device__ __forceinline__ void bar_expect(uint64_t* b, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
-}
-// (with a suspend-time hint: a waiting thread sleeps in hardware until the phase completes, or at most ~20 us,
-// instead of polling; polling warps crowd the shared-memory pipe that the working warps need)
-__device__ __forceinline__ bool bar_try(uint64_t* b, unsigned parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(su32(b)), "r"(parity), "r"(20000u)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-
-struct Abort {
-  volatile int* flag;  // shared: any role of the CTA raised it
-  int* err;            // global: {code, CTA, role, 0}
-};
-__device__ __noinline__ void raise_abort(const Abort& a, int role) {
-  if (atomicCAS(a.err, 0, 1) == 0) {
-    a.err[1] = blockIdx.x;
-    a.err[2] = role;
-  }
-  *a.flag = 1;
-}
-// bounded wait for the completion of the phase with this parity; false (abort raised) on expiry or abort
-__device__ __forceinline__ bool wait_phase(uint64_t* b, unsigned parity, const Abort& a, int role) {
-  if (bar_try(b, parity)) return true;
-  const unsigned long long t0 = now_ns();
-  for (unsigned it = 0;; it++) {
-    if (bar_try(b, parity)) return true;
-    if ((it & 3) == 3) {
-      if (*a.flag) return false;
-      if (now_ns() - t0 > TIMEOUT_NS) {
-        raise_abort(a, role);
-        return false;
-      }
-    }
-  }
-}
-// the same for a whole warp: lane 0 polls (32 lanes polling one mbarrier serialize on it) and the warp follows;
-// false on every lane if it failed
-__device__ __forceinline__ bool wait_phase_warp(uint64_t* b, unsigned parity, const Abort& a, int role) {
-  int ok = 1;
-  if ((threadIdx.x & 31) == 0) ok = wait_phase(b, parity, a, role);
-  ok = __shfl_sync(0xffffffffu, ok, 0);
-  __syncwarp();
-  return ok != 0;
-}
-// the same, ignoring the abort flag (teardown: copies or MMAs that were issued must complete)
-__device__ __forceinline__ void drain_phase(uint64_t* b, unsigned parity) {
-  const unsigned long long t0 = now_ns();
-  while (!bar_try(b, parity))
-    if (now_ns() - t0 > TIMEOUT_NS) return;
-}
-
-__device__ __forceinline__ void tma2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          su32(dst)),
-      "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(su32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void bulk1d(void* dst, const void* src, unsigned bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(su32(dst)),
-               "l"(src), "r"(bytes), "r"(su32(bar))
-               : "memory");
-}
-
-// shared-memory matrix descriptors (tcgen05): start address, leading / stride byte offsets (16-byte units), version 1
-__device__ __forceinline__ uint64_t desc_plain(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);
-}
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) |
-         (2ull << 61);
-}
-
-__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
-}
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// 32 lanes x 16 columns of 32-bit words (lane = the thread's TMEM lane) into v[0..16)
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-}
 // every one of the NW columns of the warp's 32 lanes set to w
 template <int NW>
 __device__ __forceinline__ void tmem_fill(uint32_t taddr, uint32_t w);
@@ -469,19 +368,6 @@ __global__ void __launch_bounds__(128 + 128 * EW, EW * NW <= 16 ? 2 : 1)
 
 // ---------------------------------------------------------------- host side
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
-
 // The tensor maps of one launch, cached by their arguments (the engine's buffers repeat from call to call).
 struct MapKey {
   const void* ptr;
@@ -507,7 +393,7 @@ bool make_map(CUtensorMap* out, int kind, const void* ptr, uint64_t d0, uint64_t
       *out = e.m;
       return true;
     }
-  auto fn = encode_fn();
+  auto fn = tma_encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[2] = {d0, d1};
   const cuuint64_t strides[1] = {stride};

@@ -341,6 +341,30 @@ typedef struct h2c_kv8_attention_args {
 uint64_t h2c_kv8_attention_workspace(const h2c_kv8_attention_args* args);
 int h2c_kv8_attention(const h2c_kv8_attention_args* args, void* stream);
 
+/* Matrix products in 8-bit integers, with a scale for each token and each output channel. */
+#define H2C_TYPE_I8 3         /* codes, where an entry says so */
+#define H2C_I8_MAX_K 131072   /* (sums of k products of two codes stay within 32 bits) */
+
+/* Rows of x (element type `type`, row r at x + r * x_row elements, k values) as codes q[r][0 .. k) and scale[r]: with a the
+ * row's largest magnitude, scale = a / 127 and q = round(x * min(127 / a, FLT_MAX)) (float32 operations, halves to even;
+ * a row of zeros gives zeros). Rows of q start q_row bytes apart (a multiple of 16, at least k, q 16-byte aligned); the
+ * bytes from k to the next multiple of 16 become 0. A row with NaN has the scale NaN, one with an infinity the scale
+ * infinity, and every product with it is NaN. For weights (rows = output channels), once, and for activations that
+ * several products share. */
+int h2c_i8_quantize(int32_t type, const void* x, int64_t x_row, int32_t rows, int32_t k, void* q, int64_t q_row,
+                    float* scale, void* stream);
+
+/* y[i][j] = (sum over k of xq[i][k] * w[j][k]) * xs[i] * w_scale[j] + bias[j], i < m, j < n, rounded to y_type; the integer
+ * sum is exact. xq and xs are the codes and scales of h2c_i8_quantize for row i of x: x_type F32, F16 or BF16 makes them
+ * in the workspace (x_scale is not looked at), x_type H2C_TYPE_I8 takes x as codes (x_row bytes apart) with x_scale.
+ * w: int8 [n] rows w_row bytes apart. Codes and w are 16-byte aligned with rows a multiple of 16 bytes apart, at least k;
+ * what lies beyond k is not looked at. y: row i at y + i * y_row elements. bias: float32 [n] or NULL. workspace:
+ * h2c_i8_matmul_workspace bytes, 16-byte aligned (NULL when that is 0). m = 0 or n = 0 does nothing. */
+uint64_t h2c_i8_matmul_workspace(int32_t x_type, int32_t m, int32_t k);
+int h2c_i8_matmul(int32_t x_type, const void* x, int64_t x_row, const float* x_scale, const void* w, int64_t w_row,
+                  const float* w_scale, int32_t m, int32_t n, int32_t k, int32_t y_type, void* y, int64_t y_row,
+                  const float* bias, void* workspace, uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,3 +90,32 @@ def test_attention_of_nothing_and_its_workspace(lib):
     assert 0 < need < 1 << 24
     a = attention_args(max_kv=4000, workspace=X, workspace_bytes=need - 1)
     assert lib.h2c_kv8_attention(C.byref(a), None) == _lib.ERR_INVALID and str(need) in message(lib)
+
+
+MATMUL = dict(x_type=0, x=X, x_row=64, x_scale=None, w=X, w_row=64, w_scale=X, m=2, n=3, k=50, y_type=0, y=X, y_row=3, bias=None,
+              workspace=X, workspace_bytes=1 << 20, stream=None)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(m=-1), "sizes"), (dict(k=0), "sizes"), (dict(k=131073, w_row=131088), "sizes"), (dict(w=None), "null"),
+    (dict(w_scale=None), "null"), (dict(x_type=3, x_scale=None), "null"), (dict(w=X + 8), "w must"), (dict(w_row=56), "w must"),
+    (dict(w_row=48), "w must"), (dict(x_type=3, x_scale=X, x_row=50), "codes must"), (dict(x=X + 2), "x must"),
+    (dict(y=X + 2), "y must"), (dict(workspace=None), "workspace"), (dict(workspace_bytes=10), "workspace"),
+    (dict(workspace=X + 8), "workspace"),
+])
+def test_matmul_refuses(lib, change, word):
+    assert lib.h2c_i8_matmul(*{**MATMUL, **change}.values()) == _lib.ERR_INVALID
+    assert message(lib).startswith("h2c_i8_matmul:") and word in message(lib)
+
+
+def test_matmul_types_sizes_of_zero_and_quantize(lib):
+    assert lib.h2c_i8_matmul(*{**MATMUL, "x_type": 4}.values()) == _lib.ERR_BAD_TYPE
+    assert lib.h2c_i8_matmul(*{**MATMUL, "y_type": 3}.values()) == _lib.ERR_BAD_TYPE
+    assert lib.h2c_i8_matmul(*{**MATMUL, "m": 0, "x": None}.values()) == _lib.OK
+    assert lib.h2c_i8_matmul(*{**MATMUL, "n": 0, "y": None}.values()) == _lib.OK
+    assert lib.h2c_i8_matmul_workspace(0, 2, 50) >= 2 * 64 + 8 and lib.h2c_i8_matmul_workspace(3, 2, 50) == 0
+    q = dict(type=0, x=X, x_row=50, rows=2, k=50, q=X, q_row=64, scale=X, stream=None)
+    for change in (dict(k=0), dict(rows=-1), dict(x=None), dict(q=X + 4), dict(q_row=48), dict(q_row=60), dict(x=X + 1)):
+        assert lib.h2c_i8_quantize(*{**q, **change}.values()) == _lib.ERR_INVALID
+    assert lib.h2c_i8_quantize(*{**q, "type": 3}.values()) == _lib.ERR_BAD_TYPE
+    assert lib.h2c_i8_quantize(*{**q, "rows": 0, "x": None}.values()) == _lib.OK
