@@ -1,8 +1,8 @@
 // Attention over the paged 8-bit cache (h2c_kv8_attention; the formula is stated in include/h2cuda.h).
 //
-// Few queries (k_att_rows). A CTA takes 8 rows (query, head of the kv head's group) of one request and kv head and one
+// Many queries (k_att_prompt): kv8_prompt.cuh. Few queries (k_att_rows): a CTA takes 8 rows (query, head of the kv head's group) of one request and kv head and one
 // span of its keys; 4 warps take blocks of 16 keys in turn, each with its own running maximum, sum and output, joined at
-// the end; spans are joined by k_att_join.
+// the end; spans are joined by a kernel of their own.
 // * Tensor cores (mma.sync m16n8k16, float16 in, float32 sums): codes are integers up to 127 and exact in float16. The
 //   16 rows of an operand tile hold 8 rows twice: a float16 term in rows 0-7 and the remainder in rows 8-15, for the
 //   queries (scaled by a power of two per row) and for the softmax weights, so the products carry 22 bits, whatever the
@@ -12,6 +12,7 @@
 //   it, which lets a lane take 16 consecutive bytes of a key (QK) or of 4 keys (PV) without a transpose.
 // * Bound: the cache's bytes for long histories; latency for short ones.
 #include "kv8_att.cuh"
+#include "kv8_prompt.cuh"
 
 #include <algorithm>
 #include <climits>
@@ -20,23 +21,10 @@ namespace h2 {
 namespace {
 
 constexpr int RW_WARPS = 4, RW_ROWS = 8, RW_BLK = 16, RW_STAGES = 4;
-constexpr float P_SHIFT = 8.f;     // weights are kept as 2^(y - m + P_SHIFT), so that small ones stay normal float16 numbers
-constexpr float M_SLACK = 6.f;     // the running maximum moves only when a score passes it by this much (2^14 < 65504)
-
-struct Span {  // the division of a row tile's keys (lo .. hi) into spans of `blocks` 16-key blocks
-  int first, n_blocks, used;
-};
-__device__ __forceinline__ Span spans_of(int lo, int hi, int splits, int blocks) {
-  Span s;
-  s.first = lo & ~(RW_BLK - 1);
-  s.n_blocks = hi > lo ? (hi - s.first + RW_BLK - 1) / RW_BLK : 0;
-  s.used = max(1, min(splits, (s.n_blocks + blocks - 1) / blocks));
-  return s;
-}
-
 struct RowArgs {
   AttArgs a;
   int splits, blocks, tiles;  // spans per row tile, blocks per span, row tiles per (request, kv head)
+  int max_rows;               // requests of more rows are k_att_prompt's
   float* part;                // [request][kv head][tile][span][8][HD] sums, then the same without HD for m and l
   float2* ml;
 };
@@ -51,20 +39,6 @@ template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-
-template <class T, int HD>
-__device__ __forceinline__ void store_row4(const AttArgs& a, T* dst, const float* v) {
-  if (a.out_vec) {
-    alignas(16) T o[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = from_f<T>(v[i]);
-    if (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(o);
-    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) dst[i] = from_f<T>(v[i]);
-  }
 }
 
 template <int HD>
@@ -90,10 +64,10 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   const Request R = request_of(a, r);
   const int n_all = a.q_start[r + 1] - a.q_start[r];
   const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group;
-  if (row0 >= n_rows) return;
+  if (row0 >= n_rows || n_rows > ra.max_rows) return;
   int lo, hi;
   key_range(a, R, n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-  const Span sp = spans_of(lo, hi, ra.splits, ra.blocks);
+  const Span sp = spans_of(lo, hi, ra.splits, ra.blocks, RW_BLK);
   if (split >= sp.used) return;
   const int b_begin = split * ra.blocks, b_end = split == sp.used - 1 ? sp.n_blocks : b_begin + ra.blocks;
 
@@ -228,8 +202,8 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     if (__any_sync(0xffffffffu, mx > m_run + M_SLACK)) {
-      const float m_new = fmaxf(m_run, mx);
-      const float f_old = m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
+      const float m_new = mx > m_run + M_SLACK ? mx : m_run;  // (a row's result does not depend on its neighbours)
+      const float f_old = m_new == m_run ? 1.f : m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
       m_run = m_new;
       l_run *= f_old;
 #pragma unroll
@@ -338,27 +312,17 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   }
 }
 
-// Joins the spans of one row: the weights of span s relative to the common maximum are 2^(m_s - m).
+// Joins the spans of one row: the weights of span s relative to the common maximum are 2^(m_s - m). Span s of the row has
+// its sums at part + s * part_step and its (m, l) at ml + s * ml_step.
 template <class T, int HD>
-__global__ void __launch_bounds__(256) k_att_join(const RowArgs ra) {
+__device__ __forceinline__ void join_row(const AttArgs& a, const float* part, size_t part_step, const float2* ml, size_t ml_step,
+                                         int used, int tok, int hq) {
   constexpr int TPR = HD / 4, LANES = 256 / TPR;  // threads for a row's dimensions, spans in flight
-  const AttArgs& a = ra.a;
-  const int jr = blockIdx.x % RW_ROWS, th = blockIdx.x / RW_ROWS, head = th % a.kv_heads, tile = th / a.kv_heads;
-  const int r = blockIdx.y;
-  const Request R = request_of(a, r);
-  const int n_all = a.q_start[r + 1] - a.q_start[r];
-  const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group, orow = row0 + jr;
-  if (orow >= n_rows) return;
-  int lo, hi;
-  key_range(a, R, n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-  const Span sp = spans_of(lo, hi, ra.splits, ra.blocks);
-  if (sp.used == 1) return;  // (written by its only span)
-  const size_t unit0 = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits;
   const int d = (threadIdx.x % TPR) * 4, s0 = threadIdx.x / TPR;
   __shared__ float red[8];
   __shared__ float acc[LANES][HD + 1];
   float m = -INFINITY;
-  for (int s = threadIdx.x; s < sp.used; s += 256) m = fmaxf(m, ra.ml[(unit0 + s) * RW_ROWS + jr].x);
+  for (int s = threadIdx.x; s < used; s += 256) m = fmaxf(m, ml[s * ml_step].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
@@ -366,12 +330,12 @@ __global__ void __launch_bounds__(256) k_att_join(const RowArgs ra) {
 #pragma unroll
   for (int w = 0; w < 8; w++) m = fmaxf(m, red[w]);
   float v[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  for (int s = s0; s < sp.used; s += LANES) {
-    const float2 ml = ra.ml[(unit0 + s) * RW_ROWS + jr];
-    const float4 x = *reinterpret_cast<const float4*>(ra.part + ((unit0 + s) * RW_ROWS + jr) * HD + d);
-    const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
-    l += f * ml.y;
-    v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+  for (int s = s0; s < used; s += LANES) {
+    const float2 x = ml[s * ml_step];
+    const float4 o = *reinterpret_cast<const float4*>(part + s * part_step + d);
+    const float f = x.x == -INFINITY ? 0.f : exp2_fast(x.x - m);
+    l += f * x.y;
+    v[0] += f * o.x; v[1] += f * o.y; v[2] += f * o.z; v[3] += f * o.w;
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) acc[s0][d + i] = v[i];
@@ -389,59 +353,137 @@ __global__ void __launch_bounds__(256) k_att_join(const RowArgs ra) {
   const float inv = l != 0.f ? 1.f / l : 1.f;
 #pragma unroll
   for (int i = 0; i < 4; i++) v[i] *= inv;
-  const int tok = orow / a.group, hq = head * a.group + orow % a.group;
-  store_row4<T, HD>(a, static_cast<T*>(a.out) + (long long)(R.first + tok) * a.out_row + hq * a.out_head + d, v);
+  store_row4<T, HD>(a, static_cast<T*>(a.out) + (long long)tok * a.out_row + hq * a.out_head + d, v);
   if (d == 0 && a.lse)
-    a.lse[(size_t)(R.first + tok) * a.heads + hq] =
-        l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
+    a.lse[(size_t)tok * a.heads + hq] = l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
+}
+
+template <class T, int HD>
+__global__ void __launch_bounds__(256) k_att_join_rows(const RowArgs ra) {
+  const AttArgs& a = ra.a;
+  const int jr = blockIdx.x % RW_ROWS, th = blockIdx.x / RW_ROWS, head = th % a.kv_heads, tile = th / a.kv_heads;
+  const int r = blockIdx.y;
+  const Request R = request_of(a, r);
+  const int n_all = a.q_start[r + 1] - a.q_start[r];
+  const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group, row = row0 + jr;
+  if (row >= n_rows || n_rows > ra.max_rows) return;
+  int lo, hi;
+  key_range(a, R, n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
+  const Span sp = spans_of(lo, hi, ra.splits, ra.blocks, RW_BLK);
+  if (sp.used == 1) return;  // (written by its only span)
+  const size_t at = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits * RW_ROWS + jr;
+  join_row<T, HD>(a, ra.part + at * HD, (size_t)RW_ROWS * HD, ra.ml + at, RW_ROWS, sp.used, R.first + row / a.group,
+                  head * a.group + row % a.group);
+}
+
+template <class T, int HD>
+__global__ void __launch_bounds__(256) k_att_join_prompt(const PromptArgs pa) {
+  const AttArgs& a = pa.a;
+  const int jr = blockIdx.x % PR_ROWS, th = blockIdx.x / PR_ROWS, head = th % a.kv_heads, idx = th / a.kv_heads;
+  const TileAt at = tile_at(pa, idx);
+  if (at.r < 0) return;
+  const Request R = request_of(a, at.r);
+  const int n_all = a.q_start[at.r + 1] - a.q_start[at.r], n_rows = R.n_q * a.group, row = at.row0 + jr;
+  if (row >= n_rows) return;
+  int lo, hi;
+  key_range(a, R, n_all, at.row0 / a.group, min(at.row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
+  const Span sp = spans_of(lo, hi, pa.splits, pa.blocks, PR_KEYS);
+  if (sp.used == 1) return;
+  const size_t u = ((size_t)idx * a.kv_heads + head) * pa.splits * PR_ROWS + jr;
+  join_row<T, HD>(a, pa.part + u * HD, (size_t)PR_ROWS * HD, pa.ml + u, PR_ROWS, sp.used, R.first + row / a.group,
+                  head * a.group + row % a.group);
 }
 
 // ---------------------------------------------------------------- host
 
-struct RowPlan {
-  int splits, blocks, tiles;
-  size_t units, bytes;
+// Requests of up to RW_MAX rows take k_att_rows, others k_att_prompt, each CTA looking at its request's count on the device;
+// the host knows only max_q, and launches the one kernel or both. (A single request takes the one its max_q asks for.)
+constexpr int RW_MAX = 64;
+struct WorkPlan {
+  bool rows, prompt;
+  int max_rows, splits, blocks, tiles;         // k_att_rows
+  int min_rows, p_splits, p_blocks, p_tiles;   // k_att_prompt
+  size_t units, p_units;                       // row tiles x spans in the workspace
+  size_t bytes;
 };
-// Spans: enough CTAs for two waves of three per SM, but no span under 256 keys (4 blocks per warp), below which its start-up
-// costs more than it shares out.
-RowPlan plan_rows(const h2c_kv8_attention_args* g) {
-  RowPlan p;
-  const int group = g->heads / g->kv_heads;
-  p.tiles = (int)(((long long)g->max_q * group + RW_ROWS - 1) / RW_ROWS);
+WorkPlan plan_work(const h2c_kv8_attention_args* g) {
+  WorkPlan p = {};
+  const long long group = g->heads / g->kv_heads, most_rows = g->max_q * group;
+  p.prompt = most_rows > RW_MAX;
+  p.rows = !p.prompt || g->n_req > 1;
   long long keys = g->max_kv;
   if (g->window > 0) keys = std::min(keys, (long long)g->window + g->max_q);
-  const int n_blocks = (int)((keys + RW_BLK - 1) / RW_BLK) + (g->window > 0 ? 1 : 0);
-  const long long groups = (long long)g->n_req * g->kv_heads * p.tiles;
-  const long long want = (888 + groups - 1) / groups;
-  const int most = std::max(1, n_blocks / 16);
-  p.splits = (int)std::max(1LL, std::min<long long>(want, most));
-  p.blocks = std::max(RW_WARPS, ((n_blocks + p.splits - 1) / p.splits + RW_WARPS - 1) / RW_WARPS * RW_WARPS);
-  p.splits = std::max(1, (n_blocks + p.blocks - 1) / p.blocks);
-  p.units = p.splits > 1 ? (size_t)groups * p.splits : 0;
-  p.bytes = p.units * RW_ROWS * ((size_t)g->head_dim * 4 + 8);
+  if (p.rows) {
+    p.max_rows = p.prompt ? RW_MAX : INT_MAX;
+    p.tiles = (int)((std::min<long long>(most_rows, p.max_rows) + RW_ROWS - 1) / RW_ROWS);
+    // spans: enough CTAs for two waves of three per SM, but no span under 256 keys (4 blocks per warp), below which its
+    // start-up costs more than it shares out
+    const long long groups = (long long)g->n_req * g->kv_heads * p.tiles;
+    const int n_blocks = (int)((keys + RW_BLK - 1) / RW_BLK) + (g->window > 0 ? 1 : 0);
+    p.splits = (int)std::max(1LL, std::min<long long>((888 + groups - 1) / groups, n_blocks / 16));
+    p.blocks = std::max(RW_WARPS, ((n_blocks + p.splits - 1) / p.splits + RW_WARPS - 1) / RW_WARPS * RW_WARPS);
+    p.splits = std::max(1, (n_blocks + p.blocks - 1) / p.blocks);
+    p.units = p.splits > 1 ? (size_t)groups * p.splits : 0;
+  }
+  if (p.prompt) {
+    p.min_rows = p.rows ? RW_MAX + 1 : 0;
+    p.p_tiles = (int)std::min((long long)g->n_req * ((most_rows + PR_ROWS - 1) / PR_ROWS),
+                              (long long)g->rows * group / PR_ROWS + g->n_req);
+    // spans: as many as fill the SMs once (one CTA each), of at least 256 keys
+    const long long groups = (long long)g->kv_heads * p.p_tiles;
+    const int n_blocks = (int)((keys + PR_KEYS - 1) / PR_KEYS) + (g->window > 0 ? 1 : 0);
+    p.p_splits = (int)std::max(1LL, std::min<long long>(148 / groups, n_blocks / 4));
+    p.p_blocks = std::max(1, (n_blocks + p.p_splits - 1) / p.p_splits);
+    p.p_splits = std::max(1, (n_blocks + p.p_blocks - 1) / p.p_blocks);
+    p.p_units = p.p_splits > 1 ? (size_t)groups * p.p_splits : 0;
+  }
+  p.bytes = (p.units * RW_ROWS + p.p_units * PR_ROWS) * ((size_t)g->head_dim * 4 + 8);
   return p;
 }
 
 template <class T, int HD>
-int launch_rows(const char* who, const RowArgs& ra, cudaStream_t st) {
-  static unsigned char done[OP_MAX_DEVICES];
-  constexpr int smem = RowSmem<HD>::BYTES;
-  if (int rc = op_once(who, done, [] {
-        return cudaFuncSetAttribute(k_att_rows<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      }))
-    return rc;
-  const dim3 grid((unsigned)(ra.splits * ra.a.kv_heads) * ra.tiles, ra.a.n_req);
-  k_att_rows<T, HD><<<grid, RW_WARPS * 32, smem, st>>>(ra);
-  if (ra.splits > 1) {
-    const dim3 jgrid((unsigned)(RW_ROWS * ra.a.kv_heads) * ra.tiles, ra.a.n_req);
-    k_att_join<T, HD><<<jgrid, 256, 0, st>>>(ra);
+int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaStream_t st) {
+  float* part = static_cast<float*>(workspace);
+  float* p_part = part + p.units * RW_ROWS * HD;
+  float2* ml = reinterpret_cast<float2*>(p_part + p.p_units * PR_ROWS * HD);
+  if (p.prompt) {
+    static unsigned char done[OP_MAX_DEVICES];
+    constexpr int smem = PromptCfg<T, HD>::SMEM;
+    if (int rc = op_once(who, done, [] {
+          return cudaFuncSetAttribute(k_att_prompt<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        }))
+      return rc;
+    int* err = op_err_words();
+    if (!err) return op_error(H2C_ERR_CUDA, "%s: no device", who);
+    const PromptArgs pa{a, p.min_rows, p.p_tiles, p.p_splits, p.p_blocks, p_part, ml + p.units * RW_ROWS, err};
+    k_att_prompt<T, HD><<<(unsigned)p.p_tiles * p.p_splits * a.kv_heads, PR_THREADS, smem, st>>>(pa);
+    if (int rc = op_launched(who)) return rc;
+    if (p.p_splits > 1) {
+      k_att_join_prompt<T, HD><<<(unsigned)p.p_tiles * a.kv_heads * PR_ROWS, 256, 0, st>>>(pa);
+      if (int rc = op_launched(who)) return rc;
+    }
   }
-  return op_launched(who);
+  if (p.rows) {
+    static unsigned char done[OP_MAX_DEVICES];
+    constexpr int smem = RowSmem<HD>::BYTES;
+    if (int rc = op_once(who, done, [] {
+          return cudaFuncSetAttribute(k_att_rows<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        }))
+      return rc;
+    const RowArgs ra{a, p.splits, p.blocks, p.tiles, p.max_rows, part, ml};
+    k_att_rows<T, HD><<<dim3((unsigned)p.splits * a.kv_heads * p.tiles, a.n_req), RW_WARPS * 32, smem, st>>>(ra);
+    if (int rc = op_launched(who)) return rc;
+    if (p.splits > 1) {
+      k_att_join_rows<T, HD><<<dim3((unsigned)RW_ROWS * a.kv_heads * p.tiles, a.n_req), 256, 0, st>>>(ra);
+      return op_launched(who);
+    }
+  }
+  return H2C_OK;
 }
 
 template <class T>
-int launch_typed(const char* who, int head_dim, const RowArgs& ra, cudaStream_t st) {
-  return head_dim == 64 ? launch_rows<T, 64>(who, ra, st) : launch_rows<T, 128>(who, ra, st);
+int launch_typed(const char* who, int head_dim, const WorkPlan& p, const AttArgs& a, void* workspace, cudaStream_t st) {
+  return head_dim == 64 ? launch<T, 64>(who, p, a, workspace, st) : launch<T, 128>(who, p, a, workspace, st);
 }
 
 int check_args(const char* who, const h2c_kv8_attention_args* g) {
@@ -475,7 +517,7 @@ extern "C" {
 
 uint64_t h2c_kv8_attention_workspace(const h2c_kv8_attention_args* g) {
   if (check_args("h2c_kv8_attention_workspace", g) || nothing_to_do(g)) return 0;
-  return plan_rows(g).bytes;
+  return plan_work(g).bytes;
 }
 
 int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
@@ -488,14 +530,13 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
   if ((uintptr_t)g->kv & 15) return op_error(H2C_ERR_INVALID, "%s: the cache must be 16-byte aligned", who);
   if (((uintptr_t)g->q | (uintptr_t)g->out) & (es - 1))
     return op_error(H2C_ERR_INVALID, "%s: q and out must be aligned to their elements", who);
-  const RowPlan p = plan_rows(g);
+  const WorkPlan p = plan_work(g);
   if (p.bytes && (!g->workspace || g->workspace_bytes < p.bytes || ((uintptr_t)g->workspace & 15)))
     return op_error(H2C_ERR_INVALID, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
                     (unsigned long long)p.bytes, (unsigned long long)(g->workspace ? g->workspace_bytes : 0));
-  if ((long long)p.splits * g->kv_heads * p.tiles > INT_MAX / RW_ROWS)
-    return op_error(H2C_ERR_INVALID, "%s: max_q %d out of range", who, g->max_q);
-  RowArgs ra;
-  AttArgs& a = ra.a;
+  const long long most = std::max((long long)p.splits * p.tiles * RW_ROWS, (long long)p.p_splits * p.p_tiles * PR_ROWS);
+  if (most * g->kv_heads > INT_MAX) return op_error(H2C_ERR_INVALID, "%s: too many rows for one call", who);
+  AttArgs a;
   a.q = g->q; a.q_row = g->q_row; a.q_head = g->q_head;
   a.out = g->out; a.out_row = g->out_row; a.out_head = g->out_head;
   a.lse = g->lse;
@@ -507,13 +548,10 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
   a.q_vec = !((uintptr_t)g->q & (4 * es - 1)) && !((g->q_row | g->q_head) & 3);
   a.out_vec = !((uintptr_t)g->out & (4 * es - 1)) && !((g->out_row | g->out_head) & 3);
   a.scale_log2 = g->scale * 1.4426950408889634f;
-  ra.splits = p.splits; ra.blocks = p.blocks; ra.tiles = p.tiles;
-  ra.part = static_cast<float*>(g->workspace);
-  ra.ml = reinterpret_cast<float2*>(ra.part + p.units * RW_ROWS * g->head_dim);
   cudaStream_t st = (cudaStream_t)stream;
-  if (g->type == H2C_TYPE_F32) return launch_typed<float>(who, g->head_dim, ra, st);
-  if (g->type == H2C_TYPE_F16) return launch_typed<__half>(who, g->head_dim, ra, st);
-  return launch_typed<__nv_bfloat16>(who, g->head_dim, ra, st);
+  if (g->type == H2C_TYPE_F32) return launch_typed<float>(who, g->head_dim, p, a, g->workspace, st);
+  if (g->type == H2C_TYPE_F16) return launch_typed<__half>(who, g->head_dim, p, a, g->workspace, st);
+  return launch_typed<__nv_bfloat16>(who, g->head_dim, p, a, g->workspace, st);
 }
 
 }  // extern "C"

@@ -22,6 +22,22 @@ struct AttArgs {
 
 #ifdef __CUDACC__
 
+namespace {
+
+constexpr float P_SHIFT = 8.f;     // weights are kept as 2^(y - m + P_SHIFT), so that small ones stay normal float16 numbers
+constexpr float M_SLACK = 6.f;     // the running maximum moves only when a score passes it by this much (2^14 < 65504)
+
+struct Span {  // the division of a row tile's keys (lo .. hi) into spans of `blocks` blocks of `keys` keys, from a multiple of 16
+  int first, n_blocks, used;
+};
+__device__ __forceinline__ Span spans_of(int lo, int hi, int splits, int blocks, int keys) {
+  Span s;
+  s.first = lo & ~15;
+  s.n_blocks = hi > lo ? (hi - s.first + keys - 1) / keys : 0;
+  s.used = max(1, min(splits, (s.n_blocks + blocks - 1) / blocks));
+  return s;
+}
+
 // A request's queries and keys, clamped to what the arrays hold.
 struct Request {
   int first, n_q, len;  // first row of q, queries, cached positions
@@ -62,6 +78,11 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 // weights that enter the tensor cores never leave float16's range however the pages' scales differ; the mantissa
 // multiplies the weight. e is bounded so that 2^-e stays a normal number.
 __device__ __forceinline__ void split_scale(float s, float* e, float* mant, float* inv_pow) {
+  if (!(fabsf(s) < INFINITY)) {  // a lost page: NaN through the exponent, so that keys a row does not see stay without effect
+    *e = __int_as_float(0x7fc00000);
+    *mant = *inv_pow = 1.f;
+    return;
+  }
   const int x = max(-62, min(63, (int)((__float_as_uint(s) >> 23) & 255u) - 127));
   const float inv = __int_as_float((127 - x) << 23);
   *e = (float)x;
@@ -69,5 +90,20 @@ __device__ __forceinline__ void split_scale(float s, float* e, float* mant, floa
   *mant = s * inv;
 }
 
+template <class T, int HD>
+__device__ __forceinline__ void store_row4(const AttArgs& a, T* dst, const float* v) {
+  if (a.out_vec) {
+    alignas(16) T o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = from_f<T>(v[i]);
+    if (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(o);
+    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) dst[i] = from_f<T>(v[i]);
+  }
+}
+
+}  // namespace
 #endif
 }  // namespace h2

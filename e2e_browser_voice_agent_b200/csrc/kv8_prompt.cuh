@@ -1,0 +1,506 @@
+// Attention over the paged 8-bit cache for many queries (prompts, long continuations): the tensor-core kernel of
+// h2c_kv8_attention. Included by kv8_att.cu.
+//
+// A CTA takes 256 rows (query, head of the kv head's group) of one request and kv head, as two tiles of 128, and one span of
+// its keys, 64 keys at a time:
+//   warps 8-11  converters: 8-bit codes from their pages to float16 tiles of K and V in shared memory (exact: codes are
+//               integers up to 127), next tile's loads in flight meanwhile; both row tiles use them
+//   warp 12     tcgen05.mma (kind::f16): S = Q K^T into TMEM, O += P V with P read from TMEM
+//   warps 0-3, 4-7   softmax of row tile 0, 1: a thread owns a row; S from TMEM, P back into S's columns as float16
+// TMEM per row tile: two S slots of 64 columns (P takes its S slot's place) and O. S of the next keys is issued before O's
+// update with the present ones, so the tensor cores work while the softmax does.
+// * A page's scale of K multiplies its scores; its scale of V joins the exponent (see split_scale), so a row's weights
+//   are powers of two relative to one running maximum, which moves only when a score passes it by M_SLACK: only then is
+//   O rescaled (by the softmax warps, in TMEM).
+// * float32 queries and weights are two float16 terms each (22 bits), one tcgen05.mma per term.
+// * V lies in shared memory as its rows come, [key][dimension]: the second product's B operand in MN-major form.
+// Bound: exponentials (256 x 64 per tile at 16 a cycle: 1,024 cycles) and tensor cores (about 1,280: the S products'
+// operands of 64 keys take 1.5 times their multiply time to read from shared memory) at about the same level.
+#pragma once
+#include "kv8_att.cuh"
+#include "tc5_ptx.cuh"
+
+namespace h2 {
+namespace {
+
+constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 13 * 32, PR_STAGES = 2, PR_INFO = 4;
+enum { PR_CONVERT = 21, PR_MMA = 22, PR_SOFTMAX = 23 };
+
+struct PromptArgs {
+  AttArgs a;
+  int min_rows;              // requests of fewer rows are k_att_rows'
+  int tiles, splits, blocks; // bound of the row tiles of all requests, spans per row tile, 64-key tiles per span
+  float* part;
+  float2* ml;
+  int* err;
+};
+
+// The idx-th row tile over all requests: its request and first row; r = -1 beyond the last. Called by whole warps.
+struct TileAt {
+  int r, row0;
+};
+__device__ __forceinline__ TileAt tile_at(const PromptArgs& pa, int idx) {
+  const AttArgs& a = pa.a;
+  const int lane = threadIdx.x & 31;
+  TileAt t{-1, 0};
+  int before = 0;
+  for (int base = 0; base < a.n_req; base += 32) {
+    const int r = base + lane;
+    int n = 0;
+    if (r < a.n_req) {
+      const int rows = request_of(a, r).n_q * a.group;
+      if (rows >= pa.min_rows) n = (rows + PR_ROWS - 1) / PR_ROWS;
+    }
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += u;
+    }
+    const int at = idx - before;  // among this round's tiles
+    const unsigned in = __ballot_sync(0xffffffffu, at >= sum - n && at < sum);
+    if (in) {
+      const int l = __ffs(in) - 1;
+      t.r = base + l;
+      t.row0 = (at - (__shfl_sync(0xffffffffu, sum, l) - __shfl_sync(0xffffffffu, n, l))) * PR_ROWS;
+      return t;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return t;
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
+      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
+      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+      : "memory");
+}
+// D (TMEM, float32) (+)= A B with float16 operands: both in shared memory, or A in TMEM
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+// a 128-byte-swizzled tile of 64-element (128-byte) rows: byte address of the 16-byte piece c of row r
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+template <class T, int HD>
+struct PromptCfg {
+  static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // float16 terms of queries and weights
+  static constexpr int BLKS = HD / 64;                   // 64-dimension blocks of a row
+  static constexpr int Q_TILE = 128 * HD * 2;            // one row tile, one term
+  static constexpr int KV_TILE = PR_KEYS * HD * 2;
+  static constexpr int OFF_K = 2 * TERMS * Q_TILE;
+  static constexpr int OFF_V = OFF_K + PR_STAGES * KV_TILE;
+  static constexpr int SMEM = OFF_V + PR_STAGES * KV_TILE + 1024;
+  static_assert(SMEM <= 226 * 1024, "shared memory budget");
+};
+
+// what the softmax needs of 16 keys: scale of K, the term of V's scale in the exponent, its factor (TERMS = 2), and what
+// turns a weight back into the softmax's
+struct KeyInfo {
+  float k, e, mant, inv;
+};
+
+template <class T, int HD>
+__global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs pa) {
+  using C = PromptCfg<T, HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u);
+  __shared__ uint64_t k_full[PR_STAGES], k_empty[PR_STAGES], v_full[PR_STAGES], v_empty[PR_STAGES], i_full[PR_INFO];
+  __shared__ uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full, mma_end;  // ([row tile][tile of keys & 1])
+  __shared__ KeyInfo info[PR_INFO][PR_KEYS / 16];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_s;
+  const AttArgs& a = pa.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x % pa.splits, head = (blockIdx.x / pa.splits) % a.kv_heads;
+  // the last tiles of a causal prompt have the most keys and go first
+  const int idx = pa.tiles - 1 - blockIdx.x / (pa.splits * a.kv_heads);
+  const TileAt at = tile_at(pa, idx);
+  if (at.r < 0) return;
+  const Request R = request_of(a, at.r);
+  const int n_all = a.q_start[at.r + 1] - a.q_start[at.r], n_rows = R.n_q * a.group;
+  int lo, hi;
+  key_range(a, R, n_all, at.row0 / a.group, min(at.row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
+  const Span sp = spans_of(lo, hi, pa.splits, pa.blocks, PR_KEYS);
+  if (split >= sp.used) return;
+  const int t_begin = split * pa.blocks, t_end = split == sp.used - 1 ? sp.n_blocks : t_begin + pa.blocks;
+  const int n_tiles = t_end - t_begin, key_begin = sp.first + t_begin * PR_KEYS;
+  const int n_q_tiles = n_rows - at.row0 > 128 ? 2 : 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PR_STAGES; s++) {
+      bar_init(k_full + s, 4);
+      bar_init(k_empty + s, 1);
+      bar_init(v_full + s, 4);
+      bar_init(v_empty + s, 1);
+    }
+    for (int s = 0; s < PR_INFO; s++) bar_init(i_full + s, 1);
+    for (int q = 0; q < 2; q++) {
+      bar_init(&s_full[q][0], 1);
+      bar_init(&s_full[q][1], 1);
+      for (int i = 0; i < 2; i++) {  // (two: a warp may be one tile of keys ahead of another, or of O's update)
+        bar_init(&p_full[q][i], 4);
+        bar_init(&pv_done[q][i], 1);
+      }
+    }
+    bar_init(&q_full, 4 * n_q_tiles);
+    bar_init(&mma_end, 1);
+    abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const Abort ab{&abort_s, pa.err};
+
+  if (warp >= 8 && warp < 12) {  // ---------------- converters
+    constexpr int CPR = HD / 16;             // 16-code pieces of a row
+    constexpr int RPI = 128 / CPR;           // rows that the 128 threads take at once
+    constexpr int NI = PR_KEYS / RPI;
+    const int tid = threadIdx.x - 256, piece = tid % CPR, row = tid / CPR;
+    const size_t head_bytes = (size_t)HD << a.page_log;
+    const int* table = a.table + (size_t)at.r * a.table_cols;
+    uint4 kr[NI], vr[NI];
+    KeyInfo ki = {0.f, 0.f, 1.f, 1.f};
+    auto load = [&](int j) {
+      const int key0 = key_begin + j * PR_KEYS;
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int key = key0 + row + RPI * i;
+        kr[i] = vr[i] = make_uint4(0, 0, 0, 0);  // (keys past the last page: code 0)
+        if ((key & ~15) < hi) {
+          int pg = table[key >> a.page_log];
+          pg = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
+          const int8_t* kb = a.kv + ((size_t)pg * 2 * a.kv_heads + head) * head_bytes +
+                             (size_t)(key & ((1 << a.page_log) - 1)) * HD + piece * 16;
+          kr[i] = *reinterpret_cast<const uint4*>(kb);
+          vr[i] = *reinterpret_cast<const uint4*>(kb + a.kv_heads * head_bytes);
+        }
+      }
+      if (tid < PR_KEYS / 16) {
+        const int key = key0 + 16 * tid;
+        ki = {0.f, 0.f, 1.f, 1.f};
+        if (key < hi) {
+          int pg = table[key >> a.page_log];
+          pg = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
+          const float* s = a.kv_scale + (size_t)pg * 2 * a.kv_heads + head;
+          ki.k = s[0];
+          split_scale(s[a.kv_heads], &ki.e, &ki.mant, &ki.inv);
+          if (C::TERMS == 1) {  // the whole scale goes into the exponent (its logarithm is off by 2^-22 of the result)
+            const float mant = fmaxf(ki.mant, 1.f);  // (a scale below 2^-62, or 0, counts as 2^-62)
+            ki.e += log2f(mant);
+            ki.inv /= mant;
+          }
+        }
+      }
+    };
+    auto convert = [&](uint8_t* tile, const uint4* r) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t u = w[k] ^ 0x80808080u;
+          h[2 * k] = half2_of(__byte_perm(u, 0x64646464u, 0x4140));
+          h[2 * k + 1] = half2_of(__byte_perm(u, 0x64646464u, 0x4342));
+        }
+        uint8_t* blk = tile + (piece >> 2) * (PR_KEYS * 128);
+        const int rr = row + RPI * i, c = (piece & 3) * 2;
+        *reinterpret_cast<uint4*>(blk + sw128(rr, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(blk + sw128(rr, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+      }
+    };
+    if (n_tiles > 0) load(0);
+    for (int j = 0; j < n_tiles; j++) {
+      const int s = j % PR_STAGES;
+      uint4 kc[NI], vc[NI];
+#pragma unroll
+      for (int i = 0; i < NI; i++) kc[i] = kr[i], vc[i] = vr[i];
+      const KeyInfo kic = ki;
+      if (j + 1 < n_tiles) load(j + 1);
+      if (!wait_phase_warp(k_empty + s, ((j / PR_STAGES) & 1) ^ 1, ab, PR_CONVERT)) break;
+      if (warp == 8) {
+        if (tid < PR_KEYS / 16) info[j % PR_INFO][tid] = kic;
+        __syncwarp();
+        if (lane == 0) bar_arrive(i_full + j % PR_INFO);
+      }
+      convert(sm + C::OFF_K + s * C::KV_TILE, kc);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(k_full + s);
+      if (!wait_phase_warp(v_empty + s, ((j / PR_STAGES) & 1) ^ 1, ab, PR_CONVERT)) break;
+      convert(sm + C::OFF_V + s * C::KV_TILE, vc);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(v_full + s);
+    }
+  } else if (warp == 12) {  // ---------------- products
+    if (lane == 0) {
+      const uint32_t id_s = (1u << 4) | ((uint32_t)(PR_KEYS >> 3) << 17) | (8u << 24);
+      const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B in MN-major form
+      auto scores = [&](int j) {
+        const int s = j % PR_STAGES;
+        if (!wait_phase(k_full + s, (j / PR_STAGES) & 1, ab, PR_MMA)) return false;
+        tc_fence_after();
+        const uint32_t kb = su32(sm + C::OFF_K + s * C::KV_TILE);
+        for (int q = 0; q < n_q_tiles; q++) {
+#pragma unroll
+          for (int t = 0; t < C::TERMS; t++) {
+            const uint32_t qb = su32(sm + (q * C::TERMS + t) * C::Q_TILE);
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++)
+              mma_f16(tmem + q * 256 + (j & 1) * PR_KEYS,
+                      desc_sw128(qb + (k >> 2) * (128 * 128) + (k & 3) * 32, 1024),
+                      desc_sw128(kb + (k >> 2) * (PR_KEYS * 128) + (k & 3) * 32, 1024), id_s, t > 0 || k > 0);
+          }
+          mma_commit(&s_full[q][j & 1]);
+        }
+        mma_commit(k_empty + s);
+        return true;
+      };
+      bool ok = n_tiles == 0 || (wait_phase(&q_full, 0, ab, PR_MMA) && scores(0));
+      for (int j = 0; ok && j < n_tiles; j++) {
+        if (j + 1 < n_tiles && !scores(j + 1)) break;
+        const int s = j % PR_STAGES;
+        if (!wait_phase(v_full + s, (j / PR_STAGES) & 1, ab, PR_MMA)) break;
+        const uint32_t vb = su32(sm + C::OFF_V + s * C::KV_TILE);
+        for (int q = 0; q < n_q_tiles; q++) {
+          if (!wait_phase(&p_full[q][j & 1], (j >> 1) & 1, ab, PR_MMA)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int t = 0; t < C::TERMS; t++)
+#pragma unroll
+            for (int k = 0; k < PR_KEYS / 16; k++)
+              mma_f16_ts(tmem + q * 256 + 128, tmem + q * 256 + (j & 1) * PR_KEYS + t * (PR_KEYS / 2) + 8 * k,
+                         desc_sw128(vb + k * 2048, 1024) - (1ull << 16) + ((uint64_t)((PR_KEYS * 128) >> 4) << 16), id_o,
+                         j > 0 || t > 0 || k > 0);
+          mma_commit(&pv_done[q][j & 1]);
+        }
+        mma_commit(v_empty + s);
+      }
+      mma_commit(&mma_end);
+      drain_phase(&mma_end, 0);
+    }
+  } else if (warp < 8 && (warp >> 2) < n_q_tiles) {  // ---------------- softmax: one thread, one row
+    const int q = warp >> 2, w4 = warp & 3;
+    const int trow = 32 * w4 + lane, row = at.row0 + q * 128 + trow;
+    const bool live = row < n_rows;
+    const int rr = live ? row : n_rows - 1;  // (rows past the last compute what the last one does, on zeros)
+    const int tok = rr / a.group, hq = head * a.group + rr % a.group;
+    const int pos = R.len - n_all + tok, first_key = a.window > 0 ? pos + 1 - a.window : 0;
+    float f_row;
+    {  // the row's query: largest magnitude to [2^13, 2^14) by a power of two, then one or two float16 terms
+      const T* src = static_cast<const T*>(a.q) + (long long)(R.first + tok) * a.q_row + hq * a.q_head;
+      unsigned m = 0;
+      for (int d = 0; d < HD; d += 4) {
+        float v[4];
+        if (a.q_vec) load4<true>(src + d, v);
+        else load4<false>(src + d, v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+      }
+      const int e = (int)(m >> 23);
+      const int up = e == 255 || m == 0 ? 127 : min(253, 267 - e);
+      // (the sign of the softmax scale goes into the query, so that larger products are larger scores)
+      const float mul = live ? copysignf(__int_as_float(up << 23), a.scale_log2) : 0.f;
+      f_row = __int_as_float((254 - up) << 23) * fabsf(a.scale_log2);
+      for (int d = 0; d < HD; d += 8) {
+        float v[8];
+        if (a.q_vec) load4<true>(src + d, v), load4<true>(src + d + 4, v + 4);
+        else load4<false>(src + d, v), load4<false>(src + d + 4, v + 4);
+        uint32_t h[4], r[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float x0 = live ? v[2 * i] * mul : 0.f, x1 = live ? v[2 * i + 1] * mul : 0.f;
+          const __half2 t = __floats2half2_rn(x0, x1);
+          h[i] = *reinterpret_cast<const uint32_t*>(&t);
+          r[i] = pack_half2(x0 - __low2float(t), x1 - __high2float(t));
+        }
+        const uint32_t o = (d >> 6) * (128 * 128) + sw128(trow, (d & 63) >> 3);
+        uint8_t* qt = sm + q * C::TERMS * C::Q_TILE;
+        *reinterpret_cast<uint4*>(qt + o) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (C::TERMS == 2) *reinterpret_cast<uint4*>(qt + C::Q_TILE + o) = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(&q_full);
+    }
+    const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + q * 256, to = tl + 128;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n_tiles; j++) {
+      if (!wait_phase_warp(i_full + j % PR_INFO, (j / PR_INFO) & 1, ab, PR_SOFTMAX) ||
+          !wait_phase_warp(&s_full[q][j & 1], (j >> 1) & 1, ab, PR_SOFTMAX)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float s[PR_KEYS];
+      const uint32_t ts = tl + (j & 1) * PR_KEYS;
+      tmem_ld32(ts, s);
+      tmem_ld32(ts + 32, s + 32);
+      tc_wait_ld();
+      const KeyInfo* in = info[j % PR_INFO];
+      const int key0 = key_begin + j * PR_KEYS;
+      // scores in place: y = s f + e, -infinity where the row does not see the key
+      float mx = -INFINITY;
+      const bool edge = __any_sync(0xffffffffu, key0 + PR_KEYS - 1 > pos || key0 < first_key);
+      if (edge) {
+#pragma unroll
+        for (int g = 0; g < PR_KEYS / 16; g++) {
+          const float f = f_row * in[g].k, e = in[g].e;
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int key = key0 + 16 * g + i;
+            s[16 * g + i] = key <= pos && key >= first_key ? fmaf(s[16 * g + i], f, e) : -INFINITY;
+            mx = fmaxf(mx, s[16 * g + i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < PR_KEYS / 16; g++) {
+          float top = s[16 * g];
+#pragma unroll
+          for (int i = 1; i < 16; i++) top = fmaxf(top, s[16 * g + i]);
+          mx = fmaxf(mx, fmaf(top, f_row * in[g].k, in[g].e));
+        }
+      }
+      if (__any_sync(0xffffffffu, mx > m_run + M_SLACK)) {
+        const float m_new = mx > m_run + M_SLACK ? mx : m_run;  // (a row's result does not depend on its neighbours)
+        const float f_old = m_new == m_run ? 1.f : m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
+        m_run = m_new;
+        l_run *= f_old;
+        if (j > 0) {
+          if (!wait_phase_warp(&pv_done[q][(j - 1) & 1], ((j - 1) >> 1) & 1, ab, PR_SOFTMAX)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            float o[32];
+            tmem_ld32(to + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] *= f_old;
+            tmem_st32(to + c, reinterpret_cast<const uint32_t*>(o));
+          }
+          tc_wait_st();
+        }
+      }
+      const float base = P_SHIFT - (m_run == -INFINITY ? 0.f : m_run);
+      uint32_t p[PR_KEYS / 2], rest[C::TERMS == 2 ? PR_KEYS / 2 : 1];
+#pragma unroll
+      for (int g = 0; g < PR_KEYS / 16; g++) {
+        const float f = f_row * in[g].k, e = in[g].e + base, mant = in[g].mant;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float w0 = exp2_fast(edge ? s[16 * g + i] + base : fmaf(s[16 * g + i], f, e));
+          float w1 = exp2_fast(edge ? s[16 * g + i + 1] + base : fmaf(s[16 * g + i + 1], f, e));
+          sum += w0 + w1;
+          if (C::TERMS == 2) {
+            w0 *= mant;
+            w1 *= mant;
+            const __half2 t = __floats2half2_rn(w0, w1);
+            p[8 * g + i / 2] = *reinterpret_cast<const uint32_t*>(&t);
+            rest[8 * g + i / 2] = pack_half2(w0 - __low2float(t), w1 - __high2float(t));
+          } else {
+            p[8 * g + i / 2] = pack_half2(w0, w1);
+          }
+        }
+        l_run = fmaf(sum, in[g].inv, l_run);
+      }
+      tmem_st32(ts, p);
+      if (C::TERMS == 2) tmem_st32(ts + 32, rest);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&p_full[q][j & 1]);
+    }
+    // ---- the row's output
+    if (ok && n_tiles > 0) {
+      ok = wait_phase_warp(&pv_done[q][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, ab, PR_SOFTMAX);
+      tc_fence_after();
+    }
+    if (ok) {
+      const bool whole = sp.used == 1;
+      const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
+      const size_t unit = ((size_t)idx * a.kv_heads + head) * pa.splits + split;
+      T* dst = static_cast<T*>(a.out) + (long long)(R.first + tok) * a.out_row + hq * a.out_head;
+      float* part = pa.part + (unit * PR_ROWS + q * 128 + trow) * HD;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        float o[32];
+        if (n_tiles > 0) {
+          tmem_ld32(to + c, o);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i++) o[i] = 0.f;
+        }
+        if (live) {
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+#pragma unroll
+              for (int k = 0; k < 4; k++) o[i + k] *= inv;
+              store_row4<T, HD>(a, dst + c + i, o + i);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+      }
+      if (live) {
+        if (!whole) pa.ml[unit * PR_ROWS + q * 128 + trow] = make_float2(m_run, l_run);
+        else if (a.lse)
+          a.lse[(size_t)(R.first + tok) * a.heads + hq] =
+              l_run == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l_run) + m_run - P_SHIFT);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+}  // namespace
+}  // namespace h2

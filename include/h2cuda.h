@@ -250,7 +250,7 @@ int h2c_q4_matvec_noalloc(const void* w, int32_t n_rows, int32_t k, const float*
  * (requests, rows) are valid and do nothing. Results do not depend on the stream, the launch or other calls.
  *
  * The cache: `kv` holds int8 codes [n_pages][2][kv_heads][page_size][head_dim] (index 0 of the second axis: K, 1: V;
- * 16-byte aligned), `kv_scale` float32 [n_pages][2][kv_heads]; a cached value is code * scale. page_size is 16, 32, 64 or
+ * 16-byte aligned), `kv_scale` float32 [n_pages][2][kv_heads], not negative; a cached value is code * scale. page_size is 16, 32, 64 or
  * 128, head_dim 64 or 128, n_pages * page_size < 2^31. A slot is page * page_size + offset. A request's position p lies
  * in page block_table[request][p / page_size] at offset p % page_size; no page belongs to two requests. ---- */
 
