@@ -23,7 +23,7 @@
 namespace h2 {
 namespace {
 
-constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 13 * 32, PR_STAGES = 2, PR_INFO = 4;
+constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 13 * 32, PR_INFO = 8;
 enum { PR_CONVERT = 21, PR_MMA = 22, PR_SOFTMAX = 23 };
 
 struct PromptArgs {
@@ -91,6 +91,25 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* u) {
       "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
       : "memory");
 }
+// packed pairs of float32
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(unsigned long long v, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // D (TMEM, float32) (+)= A B with float16 operands: both in shared memory, or A in TMEM
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -112,9 +131,11 @@ struct PromptCfg {
   static constexpr int Q_TILE = 128 * HD * 2;            // one row tile, one term
   static constexpr int KV_TILE = PR_KEYS * HD * 2;
   static constexpr int OFF_K = 2 * TERMS * Q_TILE;
-  static constexpr int OFF_V = OFF_K + PR_STAGES * KV_TILE;
-  static constexpr int SMEM = OFF_V + PR_STAGES * KV_TILE + 1024;
-  static_assert(SMEM <= 226 * 1024, "shared memory budget");
+  static constexpr int STAGES = TERMS * HD > 128 ? 2 : 3;   // K and V tiles each
+  static constexpr int OFF_V = OFF_K + STAGES * KV_TILE;
+  static constexpr int SMEM = OFF_V + STAGES * KV_TILE + 1024;
+  static constexpr int OUT_LD = 36;                      // floats per row of a warp's output staging (32 columns)
+  static_assert(8 * 32 * OUT_LD * 4 <= OFF_V && SMEM <= 226 * 1024, "shared memory budget");
 };
 
 // what the softmax needs of 16 keys: scale of K, the term of V's scale in the exponent, its factor (TERMS = 2), and what
@@ -123,14 +144,54 @@ struct KeyInfo {
   float k, e, mant, inv;
 };
 
+// The weights of one tile of keys for one row: scores s (products of codes) to p = 2^(s f + e - m), packed as float16 (and the
+// remainders when two terms are kept); the sum of the softmax's weights is added to l. base = P_SHIFT - m.
+template <int TERMS, bool EDGE>
+__device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float f_row, float base, int key0, int first_key,
+                                        int pos, uint32_t* p, uint32_t* rest, float* l) {
+#pragma unroll
+  for (int g = 0; g < PR_KEYS / 16; g++) {
+    const float f = f_row * in[g].k, e = in[g].e + base;
+    const unsigned long long ff = pair(f, f), ee = pair(e, e);
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      float w0, w1;
+      unpair(fma2(pair(s[16 * g + i], s[16 * g + i + 1]), ff, ee), &w0, &w1);
+      if (EDGE) {
+        const int key = key0 + 16 * g + i;
+        w0 = key <= pos && key >= first_key ? w0 : -INFINITY;
+        w1 = key + 1 <= pos && key + 1 >= first_key ? w1 : -INFINITY;
+      }
+      w0 = exp2_fast(w0);
+      w1 = exp2_fast(w1);
+      sum = add2(sum, pair(w0, w1));
+      if (TERMS == 2) {
+        w0 *= in[g].mant;
+        w1 *= in[g].mant;
+        const __half2 t = __floats2half2_rn(w0, w1);
+        p[8 * g + i / 2] = *reinterpret_cast<const uint32_t*>(&t);
+        rest[8 * g + i / 2] = pack_half2(w0 - __low2float(t), w1 - __high2float(t));
+      } else {
+        p[8 * g + i / 2] = pack_half2(w0, w1);
+      }
+    }
+    float s0, s1;
+    unpair(sum, &s0, &s1);
+    *l = fmaf(s0 + s1, in[g].inv, *l);
+  }
+}
+
 template <class T, int HD>
 __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs pa) {
   using C = PromptCfg<T, HD>;
+  constexpr int STG = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t k_full[PR_STAGES], k_empty[PR_STAGES], v_full[PR_STAGES], v_empty[PR_STAGES], i_full[PR_INFO];
+  __shared__ uint64_t k_full[STG], k_empty[STG], v_full[STG], v_empty[STG], i_full[PR_INFO];
   __shared__ uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full, mma_end;  // ([row tile][tile of keys & 1])
   __shared__ KeyInfo info[PR_INFO][PR_KEYS / 16];
+  __shared__ float row_scale[PR_ROWS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s;
   const AttArgs& a = pa.a;
@@ -151,7 +212,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   const int n_q_tiles = n_rows - at.row0 > 128 ? 2 : 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < PR_STAGES; s++) {
+    for (int s = 0; s < STG; s++) {
       bar_init(k_full + s, 4);
       bar_init(k_empty + s, 1);
       bar_init(v_full + s, 4);
@@ -187,26 +248,36 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     constexpr int NI = PR_KEYS / RPI;
     const int tid = threadIdx.x - 256, piece = tid % CPR, row = tid / CPR;
     const size_t head_bytes = (size_t)HD << a.page_log;
+    const int page_mask = (1 << a.page_log) - 1;
     const int* table = a.table + (size_t)at.r * a.table_cols;
+    // K and V of a tile are read one tile before they are converted, their page numbers another tile before that
     uint4 kr[NI], vr[NI];
+    int id_k[NI], id_v[NI], id_next[NI];
     KeyInfo ki = {0.f, 0.f, 1.f, 1.f};
-    auto load = [&](int j) {
-      const int key0 = key_begin + j * PR_KEYS;
+    auto pages_of = [&](int j, int* id) {  // -1: past the last key (code 0)
 #pragma unroll
       for (int i = 0; i < NI; i++) {
-        const int key = key0 + row + RPI * i;
-        kr[i] = vr[i] = make_uint4(0, 0, 0, 0);  // (keys past the last page: code 0)
-        if ((key & ~15) < hi) {
-          int pg = table[key >> a.page_log];
-          pg = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
-          const int8_t* kb = a.kv + ((size_t)pg * 2 * a.kv_heads + head) * head_bytes +
-                             (size_t)(key & ((1 << a.page_log) - 1)) * HD + piece * 16;
-          kr[i] = *reinterpret_cast<const uint4*>(kb);
-          vr[i] = *reinterpret_cast<const uint4*>(kb + a.kv_heads * head_bytes);
+        const int key = key_begin + j * PR_KEYS + row + RPI * i;
+        id[i] = -1;
+        if (j < n_tiles && (key & ~15) < hi) {
+          const int pg = table[key >> a.page_log];
+          id[i] = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
         }
       }
+    };
+    auto load = [&](int j, const int* id, int which, uint4* r) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int key = key_begin + j * PR_KEYS + row + RPI * i;
+        r[i] = make_uint4(0, 0, 0, 0);
+        if (id[i] >= 0)
+          r[i] = *reinterpret_cast<const uint4*>(a.kv + (((size_t)id[i] * 2 + which) * a.kv_heads + head) * head_bytes +
+                                                 (size_t)(key & page_mask) * HD + piece * 16);
+      }
+    };
+    auto load_info = [&](int j) {
       if (tid < PR_KEYS / 16) {
-        const int key = key0 + 16 * tid;
+        const int key = key_begin + j * PR_KEYS + 16 * tid;
         ki = {0.f, 0.f, 1.f, 1.f};
         if (key < hi) {
           int pg = table[key >> a.page_log];
@@ -222,7 +293,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         }
       }
     };
-    auto convert = [&](uint8_t* tile, const uint4* r) {
+    auto convert = [&](uint8_t* tile, const uint4* r, uint64_t* full) {
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
@@ -238,50 +309,67 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         *reinterpret_cast<uint4*>(blk + sw128(rr, c)) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(blk + sw128(rr, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(full);
     };
-    if (n_tiles > 0) load(0);
-    for (int j = 0; j < n_tiles; j++) {
-      const int s = j % PR_STAGES;
-      uint4 kc[NI], vc[NI];
-#pragma unroll
-      for (int i = 0; i < NI; i++) kc[i] = kr[i], vc[i] = vr[i];
-      const KeyInfo kic = ki;
-      if (j + 1 < n_tiles) load(j + 1);
-      if (!wait_phase_warp(k_empty + s, ((j / PR_STAGES) & 1) ^ 1, ab, PR_CONVERT)) break;
+    // K of tile j: wait for its stage, hand over the scales and the tile, and read ahead
+    auto put_k = [&](int j) {
+      const int s = j % STG;
+      if (!wait_phase_warp(k_empty + s, ((j / STG) & 1) ^ 1, ab, PR_CONVERT)) return false;
       if (warp == 8) {
-        if (tid < PR_KEYS / 16) info[j % PR_INFO][tid] = kic;
+        if (tid < PR_KEYS / 16) info[j % PR_INFO][tid] = ki;
         __syncwarp();
         if (lane == 0) bar_arrive(i_full + j % PR_INFO);
       }
-      convert(sm + C::OFF_K + s * C::KV_TILE, kc);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) bar_arrive(k_full + s);
-      if (!wait_phase_warp(v_empty + s, ((j / PR_STAGES) & 1) ^ 1, ab, PR_CONVERT)) break;
-      convert(sm + C::OFF_V + s * C::KV_TILE, vc);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) bar_arrive(v_full + s);
+      convert(sm + C::OFF_K + s * C::KV_TILE, kr, k_full + s);
+      if (j + 1 < n_tiles) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) id_k[i] = id_next[i];
+        load(j + 1, id_k, 0, kr);
+        load_info(j + 1);
+        pages_of(j + 2, id_next);
+      }
+      return true;
+    };
+    if (n_tiles > 0) {
+      pages_of(0, id_k);
+      load(0, id_k, 0, kr);
+      load(0, id_k, 1, vr);
+      load_info(0);
+      pages_of(1, id_next);
+      bool ok = put_k(0);
+      for (int j = 0; ok && j < n_tiles; j++) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) id_v[i] = id_k[i];  // (those of tile j + 1 by now)
+        if (j + 1 < n_tiles && !put_k(j + 1)) break;
+        const int s = j % STG;
+        if (!wait_phase_warp(v_empty + s, ((j / STG) & 1) ^ 1, ab, PR_CONVERT)) break;
+        convert(sm + C::OFF_V + s * C::KV_TILE, vr, v_full + s);
+        if (j + 1 < n_tiles) load(j + 1, id_v, 1, vr);
+      }
     }
   } else if (warp == 12) {  // ---------------- products
     if (lane == 0) {
       const uint32_t id_s = (1u << 4) | ((uint32_t)(PR_KEYS >> 3) << 17) | (8u << 24);
       const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B in MN-major form
+      const uint64_t q_desc = desc_sw128(su32(sm), 1024), k_desc = desc_sw128(su32(sm + C::OFF_K), 1024);
+      // (V's blocks of 64 dimensions lie PR_KEYS rows apart)
+      const uint64_t v_desc = desc_sw128(su32(sm + C::OFF_V), 1024) + ((uint64_t)(((PR_KEYS * 128) >> 4) - 1) << 16);
       auto scores = [&](int j) {
-        const int s = j % PR_STAGES;
-        if (!wait_phase(k_full + s, (j / PR_STAGES) & 1, ab, PR_MMA)) return false;
+        const int s = j % STG;
+        if (!wait_phase(k_full + s, (j / STG) & 1, ab, PR_MMA)) return false;
         tc_fence_after();
-        const uint32_t kb = su32(sm + C::OFF_K + s * C::KV_TILE);
+        const uint64_t kd = k_desc + s * (C::KV_TILE >> 4);
         for (int q = 0; q < n_q_tiles; q++) {
+          const uint64_t qd = q_desc + q * ((C::TERMS * C::Q_TILE) >> 4);
+          const uint32_t d = tmem + q * 256 + (j & 1) * PR_KEYS;
 #pragma unroll
-          for (int t = 0; t < C::TERMS; t++) {
-            const uint32_t qb = su32(sm + (q * C::TERMS + t) * C::Q_TILE);
+          for (int t = 0; t < C::TERMS; t++)
 #pragma unroll
             for (int k = 0; k < HD / 16; k++)
-              mma_f16(tmem + q * 256 + (j & 1) * PR_KEYS,
-                      desc_sw128(qb + (k >> 2) * (128 * 128) + (k & 3) * 32, 1024),
-                      desc_sw128(kb + (k >> 2) * (PR_KEYS * 128) + (k & 3) * 32, 1024), id_s, t > 0 || k > 0);
-          }
+              mma_f16(d, qd + ((t * C::Q_TILE + (k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
+                      kd + (((k >> 2) * (PR_KEYS * 128) + (k & 3) * 32) >> 4), id_s, t > 0 || k > 0);
           mma_commit(&s_full[q][j & 1]);
         }
         mma_commit(k_empty + s);
@@ -290,21 +378,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       bool ok = n_tiles == 0 || (wait_phase(&q_full, 0, ab, PR_MMA) && scores(0));
       for (int j = 0; ok && j < n_tiles; j++) {
         if (j + 1 < n_tiles && !scores(j + 1)) break;
-        const int s = j % PR_STAGES;
-        if (!wait_phase(v_full + s, (j / PR_STAGES) & 1, ab, PR_MMA)) break;
-        const uint32_t vb = su32(sm + C::OFF_V + s * C::KV_TILE);
+        const int s = j % STG;
+        if (!wait_phase(v_full + s, (j / STG) & 1, ab, PR_MMA)) break;
+        const uint64_t vd = v_desc + s * (C::KV_TILE >> 4);
         for (int q = 0; q < n_q_tiles; q++) {
           if (!wait_phase(&p_full[q][j & 1], (j >> 1) & 1, ab, PR_MMA)) {
             ok = false;
             break;
           }
           tc_fence_after();
+          const uint32_t p = tmem + q * 256 + (j & 1) * PR_KEYS;
 #pragma unroll
           for (int t = 0; t < C::TERMS; t++)
 #pragma unroll
             for (int k = 0; k < PR_KEYS / 16; k++)
-              mma_f16_ts(tmem + q * 256 + 128, tmem + q * 256 + (j & 1) * PR_KEYS + t * (PR_KEYS / 2) + 8 * k,
-                         desc_sw128(vb + k * 2048, 1024) - (1ull << 16) + ((uint64_t)((PR_KEYS * 128) >> 4) << 16), id_o,
+              mma_f16_ts(tmem + q * 256 + 128, p + t * (PR_KEYS / 2) + 8 * k, vd + k * (2048 >> 4), id_o,
                          j > 0 || t > 0 || k > 0);
           mma_commit(&pv_done[q][j & 1]);
         }
@@ -317,46 +405,56 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     const int q = warp >> 2, w4 = warp & 3;
     const int trow = 32 * w4 + lane, row = at.row0 + q * 128 + trow;
     const bool live = row < n_rows;
-    const int rr = live ? row : n_rows - 1;  // (rows past the last compute what the last one does, on zeros)
+    const int rr = live ? row : n_rows - 1;  // (rows past the last compute on zeros and are not stored)
     const int tok = rr / a.group, hq = head * a.group + rr % a.group;
     const int pos = R.len - n_all + tok, first_key = a.window > 0 ? pos + 1 - a.window : 0;
-    float f_row;
-    {  // the row's query: largest magnitude to [2^13, 2^14) by a power of two, then one or two float16 terms
-      const T* src = static_cast<const T*>(a.q) + (long long)(R.first + tok) * a.q_row + hq * a.q_head;
-      unsigned m = 0;
-      for (int d = 0; d < HD; d += 4) {
-        float v[4];
-        if (a.q_vec) load4<true>(src + d, v);
-        else load4<false>(src + d, v);
+    {  // the warp's 32 queries, HD / 8 lanes each: largest magnitude to [2^13, 2^14) by a power of two, one or two terms
+      constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, BATCH = 4;
+      const long long src = (long long)(R.first + tok) * a.q_row + hq * a.q_head;
+      const int sub = lane / LPR, piece = lane % LPR;
+      uint8_t* qt = sm + q * C::TERMS * C::Q_TILE;
+#pragma unroll 1
+      for (int p0 = 0; p0 < PASSES; p0 += BATCH) {
+        float v[BATCH][8];
 #pragma unroll
-        for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-      }
-      const int e = (int)(m >> 23);
-      const int up = e == 255 || m == 0 ? 127 : min(253, 267 - e);
-      // (the sign of the softmax scale goes into the query, so that larger products are larger scores)
-      const float mul = live ? copysignf(__int_as_float(up << 23), a.scale_log2) : 0.f;
-      f_row = __int_as_float((254 - up) << 23) * fabsf(a.scale_log2);
-      for (int d = 0; d < HD; d += 8) {
-        float v[8];
-        if (a.q_vec) load4<true>(src + d, v), load4<true>(src + d + 4, v + 4);
-        else load4<false>(src + d, v), load4<false>(src + d + 4, v + 4);
-        uint32_t h[4], r[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float x0 = live ? v[2 * i] * mul : 0.f, x1 = live ? v[2 * i + 1] * mul : 0.f;
-          const __half2 t = __floats2half2_rn(x0, x1);
-          h[i] = *reinterpret_cast<const uint32_t*>(&t);
-          r[i] = pack_half2(x0 - __low2float(t), x1 - __high2float(t));
+        for (int b = 0; b < BATCH; b++) {
+          const int r = (p0 + b) * RPP + sub;  // row of the warp
+          const T* x = static_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, src, r) + 8 * piece;
+          if (a.q_vec) load4<true>(x, v[b]), load4<true>(x + 4, v[b] + 4);
+          else load4<false>(x, v[b]), load4<false>(x + 4, v[b] + 4);
         }
-        const uint32_t o = (d >> 6) * (128 * 128) + sw128(trow, (d & 63) >> 3);
-        uint8_t* qt = sm + q * C::TERMS * C::Q_TILE;
-        *reinterpret_cast<uint4*>(qt + o) = make_uint4(h[0], h[1], h[2], h[3]);
-        if (C::TERMS == 2) *reinterpret_cast<uint4*>(qt + C::Q_TILE + o) = make_uint4(r[0], r[1], r[2], r[3]);
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+          const int r = (p0 + b) * RPP + sub;
+          unsigned m = 0;
+#pragma unroll
+          for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[b][i]) & 0x7fffffffu);
+#pragma unroll
+          for (int o = 1; o < LPR; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const int e = (int)(m >> 23);
+          const int up = e == 255 || m == 0 ? 127 : min(253, 267 - e);
+          // (the sign of the softmax scale goes into the query, so that larger products are larger scores)
+          const float mul = copysignf(__int_as_float(up << 23), a.scale_log2);
+          if (piece == 0) row_scale[q * 128 + 32 * w4 + r] = __int_as_float((254 - up) << 23) * fabsf(a.scale_log2);
+          const bool row_live = at.row0 + q * 128 + 32 * w4 + r < n_rows;
+          uint32_t h[4], rest[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float x0 = row_live ? v[b][2 * i] * mul : 0.f, x1 = row_live ? v[b][2 * i + 1] * mul : 0.f;
+            const __half2 t = __floats2half2_rn(x0, x1);
+            h[i] = *reinterpret_cast<const uint32_t*>(&t);
+            rest[i] = pack_half2(x0 - __low2float(t), x1 - __high2float(t));
+          }
+          const uint32_t o = (piece >> 3) * (128 * 128) + sw128(32 * w4 + r, piece & 7);
+          *reinterpret_cast<uint4*>(qt + o) = make_uint4(h[0], h[1], h[2], h[3]);
+          if (C::TERMS == 2) *reinterpret_cast<uint4*>(qt + C::Q_TILE + o) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) bar_arrive(&q_full);
     }
+    const float f_row = row_scale[q * 128 + trow];
     const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + q * 256, to = tl + 128;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
@@ -374,28 +472,24 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       tc_wait_ld();
       const KeyInfo* in = info[j % PR_INFO];
       const int key0 = key_begin + j * PR_KEYS;
-      // scores in place: y = s f + e, -infinity where the row does not see the key
+      // the largest score among the keys the row sees
       float mx = -INFINITY;
       const bool edge = __any_sync(0xffffffffu, key0 + PR_KEYS - 1 > pos || key0 < first_key);
-      if (edge) {
 #pragma unroll
-        for (int g = 0; g < PR_KEYS / 16; g++) {
-          const float f = f_row * in[g].k, e = in[g].e;
+      for (int g = 0; g < PR_KEYS / 16; g++) {
+        float top = -INFINITY;
+        if (edge) {
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             const int key = key0 + 16 * g + i;
-            s[16 * g + i] = key <= pos && key >= first_key ? fmaf(s[16 * g + i], f, e) : -INFINITY;
-            mx = fmaxf(mx, s[16 * g + i]);
+            top = fmaxf(top, key <= pos && key >= first_key ? s[16 * g + i] : -INFINITY);
           }
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int g = 0; g < PR_KEYS / 16; g++) {
-          float top = s[16 * g];
-#pragma unroll
-          for (int i = 1; i < 16; i++) top = fmaxf(top, s[16 * g + i]);
-          mx = fmaxf(mx, fmaf(top, f_row * in[g].k, in[g].e));
+          for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, s[16 * g + i]), s[16 * g + i + 1]);
         }
+        // (no key seen: stays -infinity whatever the page's scale is)
+        mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, f_row * in[g].k, in[g].e));
       }
       if (__any_sync(0xffffffffu, mx > m_run + M_SLACK)) {
         const float m_new = mx > m_run + M_SLACK ? mx : m_run;  // (a row's result does not depend on its neighbours)
@@ -422,27 +516,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       }
       const float base = P_SHIFT - (m_run == -INFINITY ? 0.f : m_run);
       uint32_t p[PR_KEYS / 2], rest[C::TERMS == 2 ? PR_KEYS / 2 : 1];
-#pragma unroll
-      for (int g = 0; g < PR_KEYS / 16; g++) {
-        const float f = f_row * in[g].k, e = in[g].e + base, mant = in[g].mant;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          float w0 = exp2_fast(edge ? s[16 * g + i] + base : fmaf(s[16 * g + i], f, e));
-          float w1 = exp2_fast(edge ? s[16 * g + i + 1] + base : fmaf(s[16 * g + i + 1], f, e));
-          sum += w0 + w1;
-          if (C::TERMS == 2) {
-            w0 *= mant;
-            w1 *= mant;
-            const __half2 t = __floats2half2_rn(w0, w1);
-            p[8 * g + i / 2] = *reinterpret_cast<const uint32_t*>(&t);
-            rest[8 * g + i / 2] = pack_half2(w0 - __low2float(t), w1 - __high2float(t));
-          } else {
-            p[8 * g + i / 2] = pack_half2(w0, w1);
-          }
-        }
-        l_run = fmaf(sum, in[g].inv, l_run);
-      }
+      if (edge) weights<C::TERMS, true>(s, in, f_row, base, key0, first_key, pos, p, rest, &l_run);
+      else weights<C::TERMS, false>(s, in, f_row, base, key0, first_key, pos, p, rest, &l_run);
       tmem_st32(ts, p);
       if (C::TERMS == 2) tmem_st32(ts + 32, rest);
       tc_wait_st();
@@ -450,7 +525,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       __syncwarp();
       if (lane == 0) bar_arrive(&p_full[q][j & 1]);
     }
-    // ---- the row's output
+    // ---- the rows' output: 32 columns at a time through shared memory, so that 8 lanes write 32 consecutive values of a
+    // row. The staging takes the place of Q and K: every product of scores was issued before the last update of O, whose
+    // completion is waited for.
     if (ok && n_tiles > 0) {
       ok = wait_phase_warp(&pv_done[q][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, ab, PR_SOFTMAX);
       tc_fence_after();
@@ -459,8 +536,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       const bool whole = sp.used == 1;
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
       const size_t unit = ((size_t)idx * a.kv_heads + head) * pa.splits + split;
-      T* dst = static_cast<T*>(a.out) + (long long)(R.first + tok) * a.out_row + hq * a.out_head;
-      float* part = pa.part + (unit * PR_ROWS + q * 128 + trow) * HD;
+      const long long dst = (long long)(R.first + tok) * a.out_row + hq * a.out_head;
+      float* stage = reinterpret_cast<float*>(sm) + warp * 32 * C::OUT_LD;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
@@ -471,18 +548,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
 #pragma unroll
           for (int i = 0; i < 32; i++) o[i] = 0.f;
         }
-        if (live) {
-          if (whole) {
+        __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<float4*>(stage + lane * C::OUT_LD + i) =
+              make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+        __syncwarp();
 #pragma unroll
-              for (int k = 0; k < 4; k++) o[i + k] *= inv;
-              store_row4<T, HD>(a, dst + c + i, o + i);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        for (int k = 0; k < 8; k++) {
+          const int r = 4 * k + (lane >> 3), i = 4 * (lane & 7);
+          const long long to_row = __shfl_sync(0xffffffffu, dst, r);
+          const float4 x = *reinterpret_cast<const float4*>(stage + r * C::OUT_LD + i);
+          if (at.row0 + q * 128 + 32 * w4 + r < n_rows) {
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            if (whole) store_row4<T, HD>(a, static_cast<T*>(a.out) + to_row + c + i, v);
+            else *reinterpret_cast<float4*>(pa.part + (unit * PR_ROWS + q * 128 + 32 * w4 + r) * HD + c + i) = x;
           }
         }
       }
