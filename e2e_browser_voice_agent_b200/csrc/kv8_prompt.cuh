@@ -213,9 +213,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STG; s++) {
-      bar_init(k_full + s, 4);
+      bar_init(k_full + s, 2);
       bar_init(k_empty + s, 1);
-      bar_init(v_full + s, 4);
+      bar_init(v_full + s, 2);
       bar_init(v_empty + s, 1);
     }
     for (int s = 0; s < PR_INFO; s++) bar_init(i_full + s, 1);
@@ -242,61 +242,91 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   const uint32_t tmem = tmem_slot;
   const Abort ab{&abort_s, pa.err};
 
-  if (warp >= 8 && warp < 12) {  // ---------------- converters
+  if (warp >= 8 && warp < 12) {  // ---------------- converters: warps 8, 9 for K, warps 10, 11 for V
     constexpr int CPR = HD / 16;             // 16-code pieces of a row
-    constexpr int RPI = 128 / CPR;           // rows that the 128 threads take at once
+    constexpr int RPI = 64 / CPR;            // rows that 64 threads take at once
     constexpr int NI = PR_KEYS / RPI;
-    const int tid = threadIdx.x - 256, piece = tid % CPR, row = tid / CPR;
+    const int which = (warp - 8) >> 1, tid = threadIdx.x & 63, piece = tid % CPR, row = tid / CPR;
     const size_t head_bytes = (size_t)HD << a.page_log;
     const int page_mask = (1 << a.page_log) - 1;
     const int* table = a.table + (size_t)at.r * a.table_cols;
-    // K and V of a tile are read one tile before they are converted, their page numbers another tile before that
-    uint4 kr[NI], vr[NI];
-    int id_k[NI], id_v[NI], id_next[NI];
-    KeyInfo ki = {0.f, 0.f, 1.f, 1.f};
-    auto pages_of = [&](int j, int* id) {  // -1: past the last key (code 0)
+    const int8_t* src = a.kv + ((size_t)which * a.kv_heads + head) * head_bytes + piece * 16;
+    const size_t page_bytes = 2 * a.kv_heads * head_bytes;
+    uint64_t* full = which ? v_full : k_full;
+    uint64_t* empty = which ? v_empty : k_empty;
+    uint8_t* tiles = sm + (which ? C::OFF_V : C::OFF_K) + (piece >> 2) * (PR_KEYS * 128);
+    // a tile is read while the one before it is converted, its page numbers another tile before that
+    uint4 raw[NI];
+    int id[NI];
+    auto pages_of = [&](int j) {
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         const int key = key_begin + j * PR_KEYS + row + RPI * i;
-        id[i] = -1;
+        id[i] = -1;  // past the last key: code 0
         if (j < n_tiles && (key & ~15) < hi) {
           const int pg = table[key >> a.page_log];
           id[i] = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
         }
       }
     };
-    auto load = [&](int j, const int* id, int which, uint4* r) {
+    auto load = [&](int j) {
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         const int key = key_begin + j * PR_KEYS + row + RPI * i;
-        r[i] = make_uint4(0, 0, 0, 0);
-        if (id[i] >= 0)
-          r[i] = *reinterpret_cast<const uint4*>(a.kv + (((size_t)id[i] * 2 + which) * a.kv_heads + head) * head_bytes +
-                                                 (size_t)(key & page_mask) * HD + piece * 16);
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (id[i] >= 0) raw[i] = *reinterpret_cast<const uint4*>(src + id[i] * page_bytes + (size_t)(key & page_mask) * HD);
       }
     };
-    auto load_info = [&](int j) {
-      if (tid < PR_KEYS / 16) {
-        const int key = key_begin + j * PR_KEYS + 16 * tid;
-        ki = {0.f, 0.f, 1.f, 1.f};
-        if (key < hi) {
-          int pg = table[key >> a.page_log];
-          pg = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
-          const float* s = a.kv_scale + (size_t)pg * 2 * a.kv_heads + head;
-          ki.k = s[0];
-          split_scale(s[a.kv_heads], &ki.e, &ki.mant, &ki.inv);
-          if (C::TERMS == 1) {  // the whole scale goes into the exponent (its logarithm is off by 2^-22 of the result)
-            const float mant = fmaxf(ki.mant, 1.f);  // (a scale below 2^-62, or 0, counts as 2^-62)
-            ki.e += log2f(mant);
-            ki.inv /= mant;
-          }
-        }
+    // (warp 8) the scales of a tile's four 16-key groups, one per lane, read ahead likewise
+    int info_id = -1;
+    float sk = 0.f, sv = 0.f;
+    auto info_page_of = [&](int j) {
+      const int key = key_begin + j * PR_KEYS + 16 * lane;
+      info_id = -1;
+      if (lane < PR_KEYS / 16 && j < n_tiles && key < hi) {
+        const int pg = table[key >> a.page_log];
+        info_id = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
       }
     };
-    auto convert = [&](uint8_t* tile, const uint4* r, uint64_t* full) {
+    auto load_info = [&] {
+      sk = sv = 0.f;
+      if (info_id >= 0) {
+        const float* s = a.kv_scale + (size_t)info_id * 2 * a.kv_heads + head;
+        sk = s[0];
+        sv = s[a.kv_heads];
+      }
+    };
+    auto publish_info = [&](int j) {
+      KeyInfo ki;
+      ki.k = sk;
+      split_scale(sv, &ki.e, &ki.mant, &ki.inv);
+      if (C::TERMS == 1) {  // the whole scale goes into the exponent (its logarithm is off by 2^-22 of the result)
+        const float mant = fmaxf(ki.mant, 1.f);  // (a scale below 2^-62, or 0, counts as 2^-62)
+        ki.e += __log2f(mant);
+        ki.inv = __fdividef(ki.inv, mant);
+      }
+      if (lane < PR_KEYS / 16) info[j % PR_INFO][lane] = ki;
+      __syncwarp();
+      if (lane == 0) bar_arrive(i_full + j % PR_INFO);
+    };
+    if (n_tiles > 0) {
+      pages_of(0);
+      load(0);
+      pages_of(1);
+      if (warp == 8) {
+        info_page_of(0);
+        load_info();
+        info_page_of(1);
+      }
+    }
+    for (int j = 0; j < n_tiles; j++) {
+      const int s = j % STG;
+      if (!wait_phase_warp(empty + s, ((j / STG) & 1) ^ 1, ab, PR_CONVERT)) break;
+      if (warp == 8) publish_info(j);
+      uint8_t* tile = tiles + s * C::KV_TILE;
 #pragma unroll
       for (int i = 0; i < NI; i++) {
-        const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         uint32_t h[8];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -304,49 +334,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
           h[2 * k] = half2_of(__byte_perm(u, 0x64646464u, 0x4140));
           h[2 * k + 1] = half2_of(__byte_perm(u, 0x64646464u, 0x4342));
         }
-        uint8_t* blk = tile + (piece >> 2) * (PR_KEYS * 128);
         const int rr = row + RPI * i, c = (piece & 3) * 2;
-        *reinterpret_cast<uint4*>(blk + sw128(rr, c)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(blk + sw128(rr, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+        *reinterpret_cast<uint4*>(tile + sw128(rr, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(tile + sw128(rr, c + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) bar_arrive(full);
-    };
-    // K of tile j: wait for its stage, hand over the scales and the tile, and read ahead
-    auto put_k = [&](int j) {
-      const int s = j % STG;
-      if (!wait_phase_warp(k_empty + s, ((j / STG) & 1) ^ 1, ab, PR_CONVERT)) return false;
-      if (warp == 8) {
-        if (tid < PR_KEYS / 16) info[j % PR_INFO][tid] = ki;
-        __syncwarp();
-        if (lane == 0) bar_arrive(i_full + j % PR_INFO);
-      }
-      convert(sm + C::OFF_K + s * C::KV_TILE, kr, k_full + s);
+      if (lane == 0) bar_arrive(full + s);
       if (j + 1 < n_tiles) {
-#pragma unroll
-        for (int i = 0; i < NI; i++) id_k[i] = id_next[i];
-        load(j + 1, id_k, 0, kr);
-        load_info(j + 1);
-        pages_of(j + 2, id_next);
-      }
-      return true;
-    };
-    if (n_tiles > 0) {
-      pages_of(0, id_k);
-      load(0, id_k, 0, kr);
-      load(0, id_k, 1, vr);
-      load_info(0);
-      pages_of(1, id_next);
-      bool ok = put_k(0);
-      for (int j = 0; ok && j < n_tiles; j++) {
-#pragma unroll
-        for (int i = 0; i < NI; i++) id_v[i] = id_k[i];  // (those of tile j + 1 by now)
-        if (j + 1 < n_tiles && !put_k(j + 1)) break;
-        const int s = j % STG;
-        if (!wait_phase_warp(v_empty + s, ((j / STG) & 1) ^ 1, ab, PR_CONVERT)) break;
-        convert(sm + C::OFF_V + s * C::KV_TILE, vr, v_full + s);
-        if (j + 1 < n_tiles) load(j + 1, id_v, 1, vr);
+        load(j + 1);
+        if (warp == 8) {
+          load_info();
+          info_page_of(j + 2);
+        }
+        pages_of(j + 2);
       }
     }
   } else if (warp == 12) {  // ---------------- products
