@@ -3,10 +3,12 @@
 //
 // A CTA takes 256 rows (query, head of the kv head's group) of one request and kv head, as two tiles of 128, and one span of
 // its keys, 64 keys at a time:
-//   warps 8-11  converters: 8-bit codes from their pages to float16 tiles of K and V in shared memory (exact: codes are
-//               integers up to 127), next tile's loads in flight meanwhile; both row tiles use them
-//   warp 12     tcgen05.mma (kind::f16): S = Q K^T into TMEM, O += P V with P read from TMEM
-//   warps 0-3, 4-7   softmax of row tile 0, 1: a thread owns a row; S from TMEM, P back into S's columns as float16
+//   warps 0-3, 4-7     softmax of row tile 0, 1: a thread owns a row; S from TMEM, P back into S's columns as float16
+//   warps 8-11, 12-15  converters of K and of V: 8-bit codes from their pages to float16 tiles in shared memory (exact:
+//                      codes are integers up to 127), the next tile's loads in flight meanwhile; both row tiles use them
+//   warp 16            tcgen05.mma (kind::f16): S = Q K^T into TMEM, O += P V with P read from TMEM
+// The block starts with 96 registers a thread (20 warps); the softmax warps take 136, the converters 64, the last four 40:
+// 8 x 136 + 8 x 64 + 4 x 40 = 1,760 of 20 x 96 = 1,920.
 // TMEM per row tile: two S slots of 64 columns (P takes its S slot's place) and O. S of the next keys is issued before O's
 // update with the present ones, so the tensor cores work while the softmax does.
 // * A page's scale of K multiplies its scores; its scale of V joins the exponent (see split_scale), so a row's weights
@@ -23,7 +25,7 @@
 namespace h2 {
 namespace {
 
-constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 13 * 32, PR_INFO = 8;
+constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 5 * 128, PR_INFO = 8;
 enum { PR_CONVERT = 21, PR_MMA = 22, PR_SOFTMAX = 23 };
 
 struct PromptArgs {
@@ -213,9 +215,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STG; s++) {
-      bar_init(k_full + s, 2);
+      bar_init(k_full + s, 4);
       bar_init(k_empty + s, 1);
-      bar_init(v_full + s, 2);
+      bar_init(v_full + s, 4);
       bar_init(v_empty + s, 1);
     }
     for (int s = 0; s < PR_INFO; s++) bar_init(i_full + s, 1);
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -242,11 +244,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   const uint32_t tmem = tmem_slot;
   const Abort ab{&abort_s, pa.err};
 
-  if (warp >= 8 && warp < 12) {  // ---------------- converters: warps 8, 9 for K, warps 10, 11 for V
+  if (warp >= 8 && warp < 16) {  // ---------------- converters: warps 8-11 for K, warps 12-15 for V
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     constexpr int CPR = HD / 16;             // 16-code pieces of a row
-    constexpr int RPI = 64 / CPR;            // rows that 64 threads take at once
+    constexpr int RPI = 128 / CPR;           // rows that 128 threads take at once
     constexpr int NI = PR_KEYS / RPI;
-    const int which = (warp - 8) >> 1, tid = threadIdx.x & 63, piece = tid % CPR, row = tid / CPR;
+    const int which = (warp - 8) >> 2, tid = threadIdx.x & 127, piece = tid % CPR, row = tid / CPR;
     const size_t head_bytes = (size_t)HD << a.page_log;
     const int page_mask = (1 << a.page_log) - 1;
     const int* table = a.table + (size_t)at.r * a.table_cols;
@@ -350,8 +353,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         pages_of(j + 2);
       }
     }
-  } else if (warp == 12) {  // ---------------- products
-    if (lane == 0) {
+  } else if (warp >= 16) {  // ---------------- products
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 16 && lane == 0) {
       const uint32_t id_s = (1u << 4) | ((uint32_t)(PR_KEYS >> 3) << 17) | (8u << 24);
       const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B in MN-major form
       const uint64_t q_desc = desc_sw128(su32(sm), 1024), k_desc = desc_sw128(su32(sm + C::OFF_K), 1024);
@@ -402,14 +406,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       mma_commit(&mma_end);
       drain_phase(&mma_end, 0);
     }
-  } else if (warp < 8 && (warp >> 2) < n_q_tiles) {  // ---------------- softmax: one thread, one row
+  } else if ((warp >> 2) < n_q_tiles) {  // ---------------- softmax: one thread, one row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     const int q = warp >> 2, w4 = warp & 3;
     const int trow = 32 * w4 + lane, row = at.row0 + q * 128 + trow;
     const bool live = row < n_rows;
     const int rr = live ? row : n_rows - 1;  // (rows past the last compute on zeros and are not stored)
     const int tok = rr / a.group, hq = head * a.group + rr % a.group;
     const int pos = R.len - n_all + tok, first_key = a.window > 0 ? pos + 1 - a.window : 0;
-    {  // the warp's 32 queries, HD / 8 lanes each: largest magnitude to [2^13, 2^14) by a power of two, one or two terms
+    if (n_tiles > 0) {  // the warp's 32 queries, HD / 8 lanes each: largest magnitude to [2^13, 2^14) by a power of two, one or two terms
       constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, BATCH = 4;
       const long long src = (long long)(R.first + tok) * a.q_row + hq * a.q_head;
       const int sub = lane / LPR, piece = lane % LPR;
@@ -455,7 +460,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       __syncwarp();
       if (lane == 0) bar_arrive(&q_full);
     }
-    const float f_row = row_scale[q * 128 + trow];
+    const float f_row = n_tiles > 0 ? row_scale[q * 128 + trow] : 0.f;
     const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + q * 256, to = tl + 128;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
@@ -528,7 +533,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     }
     // ---- the rows' output: 32 columns at a time through shared memory, so that 8 lanes write 32 consecutive values of a
     // row. The staging takes the place of Q and K: every product of scores was issued before the last update of O, whose
-    // completion is waited for.
+    // completion is waited for (and without keys neither was written).
     if (ok && n_tiles > 0) {
       ok = wait_phase_warp(&pv_done[q][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, ab, PR_SOFTMAX);
       tc_fence_after();
@@ -577,7 +582,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
