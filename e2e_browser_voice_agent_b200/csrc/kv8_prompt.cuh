@@ -7,8 +7,8 @@
 //   warps 8-11, 12-15  converters of K and of V: 8-bit codes from their pages to float16 tiles in shared memory (exact:
 //                      codes are integers up to 127), the next tile's loads in flight meanwhile; both row tiles use them
 //   warp 16            tcgen05.mma (kind::f16): S = Q K^T into TMEM, O += P V with P read from TMEM
-// The block starts with 96 registers a thread (20 warps); the softmax warps take 136, the converters 64, the last four 40:
-// 8 x 136 + 8 x 64 + 4 x 40 = 1,760 of 20 x 96 = 1,920.
+// The block starts with 96 registers a thread (20 warps); the softmax warps take 136, the converters 64, the last four 56:
+// 8 x 136 + 8 x 64 + 4 x 56 = 1,824 of 20 x 96 = 1,920.
 // TMEM per row tile: two S slots of 64 columns (P takes its S slot's place) and O. S of the next keys is issued before O's
 // update with the present ones, so the tensor cores work while the softmax does.
 // * A page's scale of K multiplies its scores; its scale of V joins the exponent (see split_scale), so a row's weights
@@ -184,6 +184,33 @@ __device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float
   }
 }
 
+// The largest score of one tile of keys among those the row sees, with the exponent of V's scale.
+template <bool EDGE>
+__device__ __forceinline__ float tile_max(const float* s, const KeyInfo* in, float f_row, int key0, int first_key, int pos) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < PR_KEYS / 16; g++) {
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float x0 = s[16 * g + i + 2 * h], x1 = s[16 * g + i + 2 * h + 1];
+        if (EDGE) {
+          const int key = key0 + 16 * g + i + 2 * h;
+          x0 = key <= pos && key >= first_key ? x0 : -INFINITY;
+          x1 = key + 1 <= pos && key + 1 >= first_key ? x1 : -INFINITY;
+        }
+        top[h] = fmaxf(fmaxf(x0, x1), top[h]);
+      }
+    }
+    const float x = fmaxf(top[0], top[1]);
+    // (no key seen: stays -infinity whatever the page's scale is)
+    mx = fmaxf(mx, x == -INFINITY ? x : fmaf(x, f_row * in[g].k, in[g].e));
+  }
+  return mx;
+}
+
 template <class T, int HD>
 __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs pa) {
   using C = PromptCfg<T, HD>;
@@ -354,7 +381,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       }
     }
   } else if (warp >= 16) {  // ---------------- products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 16 && lane == 0) {
       const uint32_t id_s = (1u << 4) | ((uint32_t)(PR_KEYS >> 3) << 17) | (8u << 24);
       const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B in MN-major form
@@ -478,25 +505,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       tc_wait_ld();
       const KeyInfo* in = info[j % PR_INFO];
       const int key0 = key_begin + j * PR_KEYS;
-      // the largest score among the keys the row sees
-      float mx = -INFINITY;
       const bool edge = __any_sync(0xffffffffu, key0 + PR_KEYS - 1 > pos || key0 < first_key);
-#pragma unroll
-      for (int g = 0; g < PR_KEYS / 16; g++) {
-        float top = -INFINITY;
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int key = key0 + 16 * g + i;
-            top = fmaxf(top, key <= pos && key >= first_key ? s[16 * g + i] : -INFINITY);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, s[16 * g + i]), s[16 * g + i + 1]);
-        }
-        // (no key seen: stays -infinity whatever the page's scale is)
-        mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, f_row * in[g].k, in[g].e));
-      }
+      float mx;
+      if (edge) mx = tile_max<true>(s, in, f_row, key0, first_key, pos);
+      else mx = tile_max<false>(s, in, f_row, key0, first_key, pos);
       if (__any_sync(0xffffffffu, mx > m_run + M_SLACK)) {
         const float m_new = mx > m_run + M_SLACK ? mx : m_run;  // (a row's result does not depend on its neighbours)
         const float f_old = m_new == m_run ? 1.f : m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
