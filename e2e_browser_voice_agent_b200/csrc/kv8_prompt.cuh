@@ -6,7 +6,8 @@
 //   warps 0-3, 4-7     softmax of row tile 0, 1: a thread owns a row; S from TMEM, P back into S's columns as float16
 //   warps 8-11, 12-15  converters of K and of V: 8-bit codes from their pages to float16 tiles in shared memory (exact:
 //                      codes are integers up to 127), the next tile's loads in flight meanwhile; both row tiles use them
-//   warp 16            tcgen05.mma (kind::f16): S = Q K^T into TMEM, O += P V with P read from TMEM
+//   warps 16, 17       tcgen05.mma (kind::f16): S = Q K^T of row tile 0, 1 into TMEM
+//   warps 18, 19       O += P V of row tile 0, 1, with P read from TMEM
 // The block starts with 96 registers a thread (20 warps); the softmax warps take 136, the converters 64, the last four 56:
 // 8 x 136 + 8 x 64 + 4 x 56 = 1,824 of 20 x 96 = 1,920.
 // TMEM per row tile: two S slots of 64 columns (P takes its S slot's place) and O. S of the next keys is issued before O's
@@ -25,7 +26,7 @@
 namespace h2 {
 namespace {
 
-constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 5 * 128, PR_INFO = 8;
+constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 5 * 128, PR_INFO = 32;
 enum { PR_CONVERT = 21, PR_MMA = 22, PR_SOFTMAX = 23 };
 
 struct PromptArgs {
@@ -123,6 +124,28 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(acc));
 }
+// A wait of a warpgroup: its first thread polls (many pollers slow every barrier operation of the SM down: measured 250
+// cycles per completed wait with 17 warps polling), the others stand at a named barrier. `go` holds the outcome for two waits
+// in turn, so that every thread of the group takes the same way; false when the wait expired.
+__device__ __forceinline__ bool wait_group(uint64_t* b, unsigned parity, const Abort& a, int role, int id, volatile int* go, int j) {
+  if ((threadIdx.x & 127) == 0) go[j & 1] = wait_phase(b, parity, a, role);
+  asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+  return go[j & 1] != 0;
+}
+// whether the phase has completed, without waiting
+__device__ __forceinline__ bool bar_test(uint64_t* b, unsigned parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(ok)
+               : "r"(su32(b)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
+// both phases (their tests in flight together: a test takes over 100 cycles)
+__device__ __forceinline__ bool wait_two(uint64_t* b0, unsigned p0, uint64_t* b1, unsigned p1, const Abort& a, int role) {
+  const bool d0 = bar_test(b0, p0), d1 = bar_test(b1, p1);
+  return (d0 || wait_phase(b0, p0, a, role)) && (d1 || wait_phase(b1, p1, a, role));
+}
 // a 128-byte-swizzled tile of 64-element (128-byte) rows: byte address of the 16-byte piece c of row r
 __device__ __forceinline__ uint32_t sw128(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
@@ -132,28 +155,30 @@ struct PromptCfg {
   static constexpr int BLKS = HD / 64;                   // 64-dimension blocks of a row
   static constexpr int Q_TILE = 128 * HD * 2;            // one row tile, one term
   static constexpr int KV_TILE = PR_KEYS * HD * 2;
-  static constexpr int OFF_K = 2 * TERMS * Q_TILE;
+  static constexpr int OUT_LD = 36;                      // floats per row of a warp's output staging (32 columns)
+  // a row tile's queries, later the staging of its output
+  static constexpr int Q_AREA = TERMS * Q_TILE > 4 * 32 * OUT_LD * 4 ? TERMS * Q_TILE : 4 * 32 * OUT_LD * 4;
+  static constexpr int OFF_K = 2 * Q_AREA;
   static constexpr int STAGES = TERMS * HD > 128 ? 2 : 3;   // K and V tiles each
   static constexpr int OFF_V = OFF_K + STAGES * KV_TILE;
   static constexpr int SMEM = OFF_V + STAGES * KV_TILE + 1024;
-  static constexpr int OUT_LD = 36;                      // floats per row of a warp's output staging (32 columns)
-  static_assert(8 * 32 * OUT_LD * 4 <= OFF_V && SMEM <= 226 * 1024, "shared memory budget");
+  static_assert(Q_AREA % 1024 == 0 && SMEM <= 226 * 1024, "shared memory budget");
 };
 
 // what the softmax needs of 16 keys: scale of K, the term of V's scale in the exponent, its factor (TERMS = 2), and what
 // turns a weight back into the softmax's
-struct KeyInfo {
+struct __align__(16) KeyInfo {
   float k, e, mant, inv;
 };
 
 // The weights of one tile of keys for one row: scores s (products of codes) to p = 2^(s f + e - m), packed as float16 (and the
 // remainders when two terms are kept); the sum of the softmax's weights is added to l. base = P_SHIFT - m.
 template <int TERMS, bool EDGE>
-__device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float f_row, float base, int key0, int first_key,
+__device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float base, int key0, int first_key,
                                         int pos, uint32_t* p, uint32_t* rest, float* l) {
 #pragma unroll
   for (int g = 0; g < PR_KEYS / 16; g++) {
-    const float f = f_row * in[g].k, e = in[g].e + base;
+    const float f = in[g].k, e = in[g].e + base;
     const unsigned long long ff = pair(f, f), ee = pair(e, e);
     unsigned long long sum = 0;
 #pragma unroll
@@ -186,7 +211,7 @@ __device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float
 
 // The largest score of one tile of keys among those the row sees, with the exponent of V's scale.
 template <bool EDGE>
-__device__ __forceinline__ float tile_max(const float* s, const KeyInfo* in, float f_row, int key0, int first_key, int pos) {
+__device__ __forceinline__ float tile_max(const float* s, const KeyInfo* in, int key0, int first_key, int pos) {
   float mx = -INFINITY;
 #pragma unroll
   for (int g = 0; g < PR_KEYS / 16; g++) {
@@ -206,7 +231,7 @@ __device__ __forceinline__ float tile_max(const float* s, const KeyInfo* in, flo
     }
     const float x = fmaxf(top[0], top[1]);
     // (no key seen: stays -infinity whatever the page's scale is)
-    mx = fmaxf(mx, x == -INFINITY ? x : fmaf(x, f_row * in[g].k, in[g].e));
+    mx = fmaxf(mx, x == -INFINITY ? x : fmaf(x, in[g].k, in[g].e));
   }
   return mx;
 }
@@ -217,9 +242,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   constexpr int STG = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t k_full[STG], k_empty[STG], v_full[STG], v_empty[STG], i_full[PR_INFO];
-  __shared__ uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full, mma_end;  // ([row tile][tile of keys & 1])
-  __shared__ KeyInfo info[PR_INFO][PR_KEYS / 16];
+  __shared__ uint64_t k_full[STG], k_empty[STG], v_full[STG], v_empty[STG], i_full[2];
+  __shared__ uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], q_full[2], mma_end[4];  // ([row tile][tile of keys & 1])
+  __shared__ KeyInfo info[2][PR_INFO][PR_KEYS / 16];  // of two batches of PR_INFO tiles in turn
+  __shared__ int go[2][2];
   __shared__ float row_scale[PR_ROWS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s;
@@ -243,12 +269,16 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   if (threadIdx.x == 0) {
     for (int s = 0; s < STG; s++) {
       bar_init(k_full + s, 4);
-      bar_init(k_empty + s, 1);
+      bar_init(k_empty + s, n_q_tiles);
       bar_init(v_full + s, 4);
-      bar_init(v_empty + s, 1);
+      bar_init(v_empty + s, n_q_tiles);
     }
-    for (int s = 0; s < PR_INFO; s++) bar_init(i_full + s, 1);
+    bar_init(i_full, 1);
+    bar_init(i_full + 1, 1);
     for (int q = 0; q < 2; q++) {
+      bar_init(q_full + q, 4);
+      bar_init(mma_end + q, 1);
+      bar_init(mma_end + 2 + q, 1);
       bar_init(&s_full[q][0], 1);
       bar_init(&s_full[q][1], 1);
       for (int i = 0; i < 2; i++) {  // (two: a warp may be one tile of keys ahead of another, or of O's update)
@@ -256,8 +286,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         bar_init(&pv_done[q][i], 1);
       }
     }
-    bar_init(&q_full, 4 * n_q_tiles);
-    bar_init(&mma_end, 1);
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -307,52 +335,48 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         if (id[i] >= 0) raw[i] = *reinterpret_cast<const uint4*>(src + id[i] * page_bytes + (size_t)(key & page_mask) * HD);
       }
     };
-    // (warp 8) the scales of a tile's four 16-key groups, one per lane, read ahead likewise
-    int info_id = -1;
-    float sk = 0.f, sv = 0.f;
-    auto info_page_of = [&](int j) {
-      const int key = key_begin + j * PR_KEYS + 16 * lane;
-      info_id = -1;
-      if (lane < PR_KEYS / 16 && j < n_tiles && key < hi) {
-        const int pg = table[key >> a.page_log];
-        info_id = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
+    // (warp 8) the scales of the 16-key groups of PR_INFO tiles, the batch-th such. Its place held batch - 2: this is called
+    // 16 tiles before the batch begins, and a tile of K is not converted before the softmax is done with the tile five before
+    auto publish_info = [&](int batch) {
+      const int g0 = batch * PR_INFO * (PR_KEYS / 16);
+      float sk[4], sv[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int key = key_begin + 16 * (g0 + lane + 32 * i);
+        sk[i] = sv[i] = 0.f;
+        if (key < min(hi, key_begin + n_tiles * PR_KEYS)) {
+          int pg = table[key >> a.page_log];
+          pg = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
+          const float* s = a.kv_scale + (size_t)pg * 2 * a.kv_heads + head;
+          sk[i] = s[0];
+          sv[i] = s[a.kv_heads];
+        }
       }
-    };
-    auto load_info = [&] {
-      sk = sv = 0.f;
-      if (info_id >= 0) {
-        const float* s = a.kv_scale + (size_t)info_id * 2 * a.kv_heads + head;
-        sk = s[0];
-        sv = s[a.kv_heads];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        KeyInfo ki;
+        ki.k = sk[i];
+        split_scale(sv[i], &ki.e, &ki.mant, &ki.inv);
+        if (C::TERMS == 1) {  // the whole scale goes into the exponent (its logarithm is off by 2^-22 of the result)
+          const float mant = fmaxf(ki.mant, 1.f);  // (a scale below 2^-62, or 0, counts as 2^-62)
+          ki.e += __log2f(mant);
+          ki.inv = __fdividef(ki.inv, mant);
+        }
+        info[batch & 1][(lane + 32 * i) / (PR_KEYS / 16)][lane % (PR_KEYS / 16)] = ki;
       }
-    };
-    auto publish_info = [&](int j) {
-      KeyInfo ki;
-      ki.k = sk;
-      split_scale(sv, &ki.e, &ki.mant, &ki.inv);
-      if (C::TERMS == 1) {  // the whole scale goes into the exponent (its logarithm is off by 2^-22 of the result)
-        const float mant = fmaxf(ki.mant, 1.f);  // (a scale below 2^-62, or 0, counts as 2^-62)
-        ki.e += __log2f(mant);
-        ki.inv = __fdividef(ki.inv, mant);
-      }
-      if (lane < PR_KEYS / 16) info[j % PR_INFO][lane] = ki;
       __syncwarp();
-      if (lane == 0) bar_arrive(i_full + j % PR_INFO);
+      if (lane == 0) bar_arrive(i_full + (batch & 1));
     };
     if (n_tiles > 0) {
       pages_of(0);
       load(0);
       pages_of(1);
-      if (warp == 8) {
-        info_page_of(0);
-        load_info();
-        info_page_of(1);
-      }
+      if (warp == 8) publish_info(0);
     }
     for (int j = 0; j < n_tiles; j++) {
       const int s = j % STG;
-      if (!wait_phase_warp(empty + s, ((j / STG) & 1) ^ 1, ab, PR_CONVERT)) break;
-      if (warp == 8) publish_info(j);
+      if (!wait_group(empty + s, ((j / STG) & 1) ^ 1, ab, PR_CONVERT, 1 + which, go[which], j)) break;
+      if (warp == 8 && j % PR_INFO == PR_INFO - 16 && j + 16 < n_tiles) publish_info(j / PR_INFO + 1);
       uint8_t* tile = tiles + s * C::KV_TILE;
 #pragma unroll
       for (int i = 0; i < NI; i++) {
@@ -373,65 +397,55 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       if (lane == 0) bar_arrive(full + s);
       if (j + 1 < n_tiles) {
         load(j + 1);
-        if (warp == 8) {
-          load_info();
-          info_page_of(j + 2);
-        }
         pages_of(j + 2);
       }
     }
   } else if (warp >= 16) {  // ---------------- products
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 16 && lane == 0) {
-      const uint32_t id_s = (1u << 4) | ((uint32_t)(PR_KEYS >> 3) << 17) | (8u << 24);
-      const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B in MN-major form
-      const uint64_t q_desc = desc_sw128(su32(sm), 1024), k_desc = desc_sw128(su32(sm + C::OFF_K), 1024);
-      // (V's blocks of 64 dimensions lie PR_KEYS rows apart)
-      const uint64_t v_desc = desc_sw128(su32(sm + C::OFF_V), 1024) + ((uint64_t)(((PR_KEYS * 128) >> 4) - 1) << 16);
-      auto scores = [&](int j) {
-        const int s = j % STG;
-        if (!wait_phase(k_full + s, (j / STG) & 1, ab, PR_MMA)) return false;
-        tc_fence_after();
-        const uint64_t kd = k_desc + s * (C::KV_TILE >> 4);
-        for (int q = 0; q < n_q_tiles; q++) {
-          const uint64_t qd = q_desc + q * ((C::TERMS * C::Q_TILE) >> 4);
-          const uint32_t d = tmem + q * 256 + (j & 1) * PR_KEYS;
+    const int q = (warp - 16) & 1, what = (warp - 16) >> 1;  // row tile; scores, or O's update
+    if (q < n_q_tiles && lane == 0) {
+      const uint32_t base = tmem + q * 256;
+      if (what == 0) {
+        const uint32_t id_s = (1u << 4) | ((uint32_t)(PR_KEYS >> 3) << 17) | (8u << 24);
+        const uint64_t q_desc = desc_sw128(su32(sm + q * C::Q_AREA), 1024);
+        const uint64_t k_desc = desc_sw128(su32(sm + C::OFF_K), 1024);
+        if (n_tiles == 0 || wait_phase(q_full + q, 0, ab, PR_MMA))
+          for (int j = 0; j < n_tiles; j++) {
+            // the slot held the weights of tile j - 2
+            const int s = j % STG;
+            if (!wait_two(k_full + s, (j / STG) & 1, &pv_done[q][j & 1], ((j >> 1) & 1) ^ 1, ab, PR_MMA)) break;
+            tc_fence_after();
+            const uint64_t kd = k_desc + s * (C::KV_TILE >> 4);
 #pragma unroll
-          for (int t = 0; t < C::TERMS; t++)
+            for (int t = 0; t < C::TERMS; t++)
 #pragma unroll
-            for (int k = 0; k < HD / 16; k++)
-              mma_f16(d, qd + ((t * C::Q_TILE + (k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
-                      kd + (((k >> 2) * (PR_KEYS * 128) + (k & 3) * 32) >> 4), id_s, t > 0 || k > 0);
-          mma_commit(&s_full[q][j & 1]);
-        }
-        mma_commit(k_empty + s);
-        return true;
-      };
-      bool ok = n_tiles == 0 || (wait_phase(&q_full, 0, ab, PR_MMA) && scores(0));
-      for (int j = 0; ok && j < n_tiles; j++) {
-        if (j + 1 < n_tiles && !scores(j + 1)) break;
-        const int s = j % STG;
-        if (!wait_phase(v_full + s, (j / STG) & 1, ab, PR_MMA)) break;
-        const uint64_t vd = v_desc + s * (C::KV_TILE >> 4);
-        for (int q = 0; q < n_q_tiles; q++) {
-          if (!wait_phase(&p_full[q][j & 1], (j >> 1) & 1, ab, PR_MMA)) {
-            ok = false;
-            break;
+              for (int k = 0; k < HD / 16; k++)
+                mma_f16(base + (j & 1) * PR_KEYS, q_desc + ((t * C::Q_TILE + (k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
+                        kd + (((k >> 2) * (PR_KEYS * 128) + (k & 3) * 32) >> 4), id_s, t > 0 || k > 0);
+            mma_commit(&s_full[q][j & 1]);
+            mma_commit(k_empty + s);
           }
+      } else {
+        const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B in MN-major form
+        // (V's blocks of 64 dimensions lie PR_KEYS rows apart)
+        const uint64_t v_desc = desc_sw128(su32(sm + C::OFF_V), 1024) + ((uint64_t)(((PR_KEYS * 128) >> 4) - 1) << 16);
+        for (int j = 0; j < n_tiles; j++) {
+          const int s = j % STG;
+          if (!wait_two(v_full + s, (j / STG) & 1, &p_full[q][j & 1], (j >> 1) & 1, ab, PR_MMA)) break;
           tc_fence_after();
-          const uint32_t p = tmem + q * 256 + (j & 1) * PR_KEYS;
+          const uint64_t vd = v_desc + s * (C::KV_TILE >> 4);
 #pragma unroll
           for (int t = 0; t < C::TERMS; t++)
 #pragma unroll
             for (int k = 0; k < PR_KEYS / 16; k++)
-              mma_f16_ts(tmem + q * 256 + 128, p + t * (PR_KEYS / 2) + 8 * k, vd + k * (2048 >> 4), id_o,
+              mma_f16_ts(base + 128, base + (j & 1) * PR_KEYS + t * (PR_KEYS / 2) + 8 * k, vd + k * (2048 >> 4), id_o,
                          j > 0 || t > 0 || k > 0);
           mma_commit(&pv_done[q][j & 1]);
+          mma_commit(v_empty + s);
         }
-        mma_commit(v_empty + s);
       }
-      mma_commit(&mma_end);
-      drain_phase(&mma_end, 0);
+      mma_commit(mma_end + 2 * what + q);
+      drain_phase(mma_end + 2 * what + q, 0);
     }
   } else if ((warp >> 2) < n_q_tiles) {  // ---------------- softmax: one thread, one row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
@@ -442,10 +456,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     const int tok = rr / a.group, hq = head * a.group + rr % a.group;
     const int pos = R.len - n_all + tok, first_key = a.window > 0 ? pos + 1 - a.window : 0;
     if (n_tiles > 0) {  // the warp's 32 queries, HD / 8 lanes each: largest magnitude to [2^13, 2^14) by a power of two, one or two terms
-      constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, BATCH = 4;
+      constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, BATCH = 8;
       const long long src = (long long)(R.first + tok) * a.q_row + hq * a.q_head;
       const int sub = lane / LPR, piece = lane % LPR;
-      uint8_t* qt = sm + q * C::TERMS * C::Q_TILE;
+      uint8_t* qt = sm + q * C::Q_AREA;
 #pragma unroll 1
       for (int p0 = 0; p0 < PASSES; p0 += BATCH) {
         float v[BATCH][8];
@@ -485,40 +499,40 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) bar_arrive(&q_full);
+      if (lane == 0) bar_arrive(q_full + q);
     }
     const float f_row = n_tiles > 0 ? row_scale[q * 128 + trow] : 0.f;
     const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + q * 256, to = tl + 128;
     float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true;
+    bool ok = true, ready = false;
     for (int j = 0; j < n_tiles; j++) {
-      if (!wait_phase_warp(i_full + j % PR_INFO, (j / PR_INFO) & 1, ab, PR_SOFTMAX) ||
-          !wait_phase_warp(&s_full[q][j & 1], (j >> 1) & 1, ab, PR_SOFTMAX)) {
-        ok = false;
-        break;
+      if (j % PR_INFO == 0 && !wait_phase_warp(i_full + (j / PR_INFO & 1), (j / PR_INFO >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
+      KeyInfo in[PR_KEYS / 16];
+#pragma unroll
+      for (int g = 0; g < PR_KEYS / 16; g++) {
+        const float4 x = *reinterpret_cast<const float4*>(&info[j / PR_INFO & 1][j % PR_INFO][g]);
+        in[g] = {x.x * f_row, x.y, x.z, x.w};
       }
+      if (!ready && !wait_phase_warp(&s_full[q][j & 1], (j >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
+      if (!ok) break;
       tc_fence_after();
       float s[PR_KEYS];
       const uint32_t ts = tl + (j & 1) * PR_KEYS;
       tmem_ld32(ts, s);
       tmem_ld32(ts + 32, s + 32);
       tc_wait_ld();
-      const KeyInfo* in = info[j % PR_INFO];
       const int key0 = key_begin + j * PR_KEYS;
       const bool edge = __any_sync(0xffffffffu, key0 + PR_KEYS - 1 > pos || key0 < first_key);
       float mx;
-      if (edge) mx = tile_max<true>(s, in, f_row, key0, first_key, pos);
-      else mx = tile_max<false>(s, in, f_row, key0, first_key, pos);
+      if (edge) mx = tile_max<true>(s, in, key0, first_key, pos);
+      else mx = tile_max<false>(s, in, key0, first_key, pos);
       if (__any_sync(0xffffffffu, mx > m_run + M_SLACK)) {
         const float m_new = mx > m_run + M_SLACK ? mx : m_run;  // (a row's result does not depend on its neighbours)
         const float f_old = m_new == m_run ? 1.f : m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
         m_run = m_new;
         l_run *= f_old;
         if (j > 0) {
-          if (!wait_phase_warp(&pv_done[q][(j - 1) & 1], ((j - 1) >> 1) & 1, ab, PR_SOFTMAX)) {
-            ok = false;
-            break;
-          }
+          if (!wait_phase_warp(&pv_done[q][(j - 1) & 1], ((j - 1) >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
@@ -534,18 +548,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       }
       const float base = P_SHIFT - (m_run == -INFINITY ? 0.f : m_run);
       uint32_t p[PR_KEYS / 2], rest[C::TERMS == 2 ? PR_KEYS / 2 : 1];
-      if (edge) weights<C::TERMS, true>(s, in, f_row, base, key0, first_key, pos, p, rest, &l_run);
-      else weights<C::TERMS, false>(s, in, f_row, base, key0, first_key, pos, p, rest, &l_run);
+      if (edge) weights<C::TERMS, true>(s, in, base, key0, first_key, pos, p, rest, &l_run);
+      else weights<C::TERMS, false>(s, in, base, key0, first_key, pos, p, rest, &l_run);
       tmem_st32(ts, p);
       if (C::TERMS == 2) tmem_st32(ts + 32, rest);
+      // (the next scores are most often there: their test is under way while the stores are)
+      ready = __all_sync(0xffffffffu, bar_test(&s_full[q][(j + 1) & 1], ((j + 1) >> 1) & 1));
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&p_full[q][j & 1]);
     }
     // ---- the rows' output: 32 columns at a time through shared memory, so that 8 lanes write 32 consecutive values of a
-    // row. The staging takes the place of Q and K: every product of scores was issued before the last update of O, whose
-    // completion is waited for (and without keys neither was written).
+    // row. The staging takes the place of the row tile's queries: their last product was issued before the last update of O,
+    // whose completion is waited for (and without keys they were not written).
     if (ok && n_tiles > 0) {
       ok = wait_phase_warp(&pv_done[q][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, ab, PR_SOFTMAX);
       tc_fence_after();
@@ -555,7 +571,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
       const size_t unit = ((size_t)idx * a.kv_heads + head) * pa.splits + split;
       const long long dst = (long long)(R.first + tok) * a.out_row + hq * a.out_head;
-      float* stage = reinterpret_cast<float*>(sm) + warp * 32 * C::OUT_LD;
+      float* stage = reinterpret_cast<float*>(sm + q * C::Q_AREA) + w4 * 32 * C::OUT_LD;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
