@@ -61,8 +61,8 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x % ra.splits, th = blockIdx.x / ra.splits, head = th % a.kv_heads, tile = th / a.kv_heads;
   const int r = blockIdx.y;
-  const Request R = request_of(a, r);
-  const int n_all = a.q_start[r + 1] - a.q_start[r];
+  int n_all;
+  const Request R = request_of(a, r, &n_all);
   const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group;
   if (row0 >= n_rows || n_rows > ra.max_rows) return;
   int lo, hi;
@@ -74,7 +74,9 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   // ---- this lane's row: query dimensions 64j + 16c .. +15, as float16 terms
   const int row = row0 + g;
   const bool live = row < n_rows;
-  const int tok = live ? row / a.group : 0, hq = head * a.group + (live ? row % a.group : 0);
+  int hq;
+  const int tok = token_of(a, live ? row : row0, &hq);
+  hq += head * a.group;
   const int pos = R.len - n_all + tok;               // its position, and the keys it may see: [first_key, pos]
   const int first_key = a.window > 0 ? pos + 1 - a.window : 0;
   uint32_t qa[KC * 4][4];
@@ -286,7 +288,9 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   const size_t unit = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits + split;
   const bool whole = sp.used == 1;
   const float inv = whole && ll != 0.f ? 1.f / ll : 1.f;
-  const int otok = orow / a.group, oh = head * a.group + orow % a.group;
+  int oh;
+  const int otok = token_of(a, orow, &oh);
+  oh += head * a.group;
 #pragma unroll
   for (int k = 0; k < HD / 4 / TPR; k++) {
     const int d = (jt + k * TPR) * 4;
@@ -299,7 +303,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
     if (whole) {
 #pragma unroll
       for (int i = 0; i < 4; i++) v[i] *= inv;
-      store_row4<T, HD>(a, static_cast<T*>(a.out) + (long long)(R.first + otok) * a.out_row + oh * a.out_head + d, v);
+      store4(static_cast<T*>(a.out) + (long long)(R.first + otok) * a.out_row + oh * a.out_head + d, v, a.out_vec);
     } else {
       *reinterpret_cast<float4*>(ra.part + (unit * RW_ROWS + jr) * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
     }
@@ -353,7 +357,7 @@ __device__ __forceinline__ void join_row(const AttArgs& a, const float* part, si
   const float inv = l != 0.f ? 1.f / l : 1.f;
 #pragma unroll
   for (int i = 0; i < 4; i++) v[i] *= inv;
-  store_row4<T, HD>(a, static_cast<T*>(a.out) + (long long)tok * a.out_row + hq * a.out_head + d, v);
+  store4(static_cast<T*>(a.out) + (long long)tok * a.out_row + hq * a.out_head + d, v, a.out_vec);
   if (d == 0 && a.lse)
     a.lse[(size_t)tok * a.heads + hq] = l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
 }
@@ -363,8 +367,8 @@ __global__ void __launch_bounds__(256) k_att_join_rows(const RowArgs ra) {
   const AttArgs& a = ra.a;
   const int jr = blockIdx.x % RW_ROWS, th = blockIdx.x / RW_ROWS, head = th % a.kv_heads, tile = th / a.kv_heads;
   const int r = blockIdx.y;
-  const Request R = request_of(a, r);
-  const int n_all = a.q_start[r + 1] - a.q_start[r];
+  int n_all;
+  const Request R = request_of(a, r, &n_all);
   const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group, row = row0 + jr;
   if (row >= n_rows || n_rows > ra.max_rows) return;
   int lo, hi;
@@ -382,8 +386,8 @@ __global__ void __launch_bounds__(256) k_att_join_prompt(const PromptArgs pa) {
   const int jr = blockIdx.x % PR_ROWS, th = blockIdx.x / PR_ROWS, head = th % a.kv_heads, idx = th / a.kv_heads;
   const TileAt at = tile_at(pa, idx);
   if (at.r < 0) return;
-  const Request R = request_of(a, at.r);
-  const int n_all = a.q_start[at.r + 1] - a.q_start[at.r], n_rows = R.n_q * a.group, row = at.row0 + jr;
+  const Request R = at.R;
+  const int n_all = at.n_all, n_rows = R.n_q * a.group, row = at.row0 + jr;
   if (row >= n_rows) return;
   int lo, hi;
   key_range(a, R, n_all, at.row0 / a.group, min(at.row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
@@ -543,6 +547,7 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
   a.kv = static_cast<const int8_t*>(g->kv); a.kv_scale = g->kv_scale;
   a.table = g->block_table; a.q_start = g->q_start; a.kv_len = g->kv_len;
   a.n_pages = g->n_pages; a.kv_heads = g->kv_heads; a.heads = g->heads; a.group = g->heads / g->kv_heads;
+  a.group_magic = 0xffffffffu / (unsigned)a.group;
   a.page_log = g->page_size == 16 ? 4 : g->page_size == 32 ? 5 : g->page_size == 64 ? 6 : 7;
   a.table_cols = g->table_cols; a.n_req = g->n_req; a.rows = g->rows; a.max_q = g->max_q; a.window = g->window;
   a.q_vec = !((uintptr_t)g->q & (4 * es - 1)) && !((g->q_row | g->q_head) & 3);

@@ -16,6 +16,7 @@ struct AttArgs {
   const int *q_start, *kv_len;
   int n_pages, page_log, kv_heads, heads, group;  // group = heads / kv_heads
   int table_cols, n_req, rows, max_q, window;
+  unsigned group_magic;   // see token_of
   int q_vec, out_vec;     // four-element loads of q, stores of out are aligned
   float scale_log2;       // scale * log2(e): scores are kept in powers of two
 };
@@ -42,9 +43,10 @@ __device__ __forceinline__ Span spans_of(int lo, int hi, int splits, int blocks,
 struct Request {
   int first, n_q, len;  // first row of q, queries, cached positions
 };
-__device__ __forceinline__ Request request_of(const AttArgs& a, int r) {
+__device__ __forceinline__ Request request_of(const AttArgs& a, int r, int* n_all) {  // n_all: the queries, max_q or not
   Request R;
   const int s0 = a.q_start[r], s1 = a.q_start[r + 1];
+  *n_all = s1 - s0;
   R.first = max(s0, 0);
   R.n_q = min(min(s1, a.rows) - R.first, a.max_q);
   const long long room = (long long)a.table_cols << a.page_log;
@@ -90,9 +92,9 @@ __device__ __forceinline__ void split_scale(float s, float* e, float* mant, floa
   *mant = s * inv;
 }
 
-template <class T, int HD>
-__device__ __forceinline__ void store_row4(const AttArgs& a, T* dst, const float* v) {
-  if (a.out_vec) {
+template <class T>
+__device__ __forceinline__ void store4(T* dst, const float* v, bool vec) {
+  if (vec) {
     alignas(16) T o[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = from_f<T>(v[i]);
@@ -102,6 +104,16 @@ __device__ __forceinline__ void store_row4(const AttArgs& a, T* dst, const float
 #pragma unroll
     for (int i = 0; i < 4; i++) dst[i] = from_f<T>(v[i]);
   }
+}
+
+// row / group, and the head of the group, by a multiplication: group_magic = 2^32 / group, so the quotient is off by at most one
+// for rows below 2^31
+__device__ __forceinline__ int token_of(const AttArgs& a, int row, int* head) {
+  int t = (int)__umulhi((unsigned)row, a.group_magic), r = row - t * a.group;
+  if (r >= a.group) t++, r -= a.group;
+  if (r < 0) t--, r += a.group;
+  *head = r;
+  return t;
 }
 
 }  // namespace

@@ -38,20 +38,24 @@ struct PromptArgs {
   int* err;
 };
 
-// The idx-th row tile over all requests: its request and first row; r = -1 beyond the last. Called by whole warps.
+// The idx-th row tile over all requests: its request (r = -1 beyond the last), what it holds, and the tile's first row. Called
+// by whole warps.
 struct TileAt {
-  int r, row0;
+  int r, row0, n_all;  // n_all: the request's queries, max_q or not
+  Request R;
 };
 __device__ __forceinline__ TileAt tile_at(const PromptArgs& pa, int idx) {
   const AttArgs& a = pa.a;
   const int lane = threadIdx.x & 31;
-  TileAt t{-1, 0};
+  TileAt t{-1, 0, 0, {0, 0, 0}};
   int before = 0;
   for (int base = 0; base < a.n_req; base += 32) {
     const int r = base + lane;
-    int n = 0;
+    int n = 0, n_all = 0;
+    Request R{0, 0, 0};
     if (r < a.n_req) {
-      const int rows = request_of(a, r).n_q * a.group;
+      R = request_of(a, r, &n_all);
+      const int rows = R.n_q * a.group;
       if (rows >= pa.min_rows) n = (rows + PR_ROWS - 1) / PR_ROWS;
     }
     int sum = n;
@@ -65,7 +69,11 @@ __device__ __forceinline__ TileAt tile_at(const PromptArgs& pa, int idx) {
     if (in) {
       const int l = __ffs(in) - 1;
       t.r = base + l;
-      t.row0 = (at - (__shfl_sync(0xffffffffu, sum, l) - __shfl_sync(0xffffffffu, n, l))) * PR_ROWS;
+      t.row0 = (at - __shfl_sync(0xffffffffu, sum - n, l)) * PR_ROWS;
+      t.n_all = __shfl_sync(0xffffffffu, n_all, l);
+      t.R.first = __shfl_sync(0xffffffffu, R.first, l);
+      t.R.n_q = __shfl_sync(0xffffffffu, R.n_q, l);
+      t.R.len = __shfl_sync(0xffffffffu, R.len, l);
       return t;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
@@ -209,6 +217,103 @@ __device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float
   }
 }
 
+// Eight consecutive values as they lie in memory, and as float32.
+template <class T>
+struct Raw8 {
+  uint32_t w[2 * sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); i++) {
+        const uint2 x = reinterpret_cast<const uint2*>(p)[i];
+        w[2 * i] = x.x;
+        w[2 * i + 1] = x.y;
+      }
+    } else {
+      T v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = p[i];
+#pragma unroll
+      for (int i = 0; i < 2 * (int)sizeof(T); i++) w[i] = reinterpret_cast<const uint32_t*>(v)[i];
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return to_f(reinterpret_cast<const T*>(w)[i]); }
+  // the largest magnitude's bits as a float32 (infinities and NaN above every number)
+  __device__ __forceinline__ unsigned largest() const {
+    if (sizeof(T) == 4) {
+      unsigned m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    }
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    const unsigned short u = (unsigned short)m;
+    return __float_as_uint(to_f(*reinterpret_cast<const T*>(&u)));
+  }
+};
+
+// A warp's 32 rows of a row tile's queries (from row r0 of the tile, which begins at row tile0 of the request): HD / 8 lanes a
+// row; lane i has the place of row i in q (row_at). A row is scaled by a power of two so that its largest magnitude lies in
+// [2^13, 2^14) and split into one or two float16 terms; what undoes the scaling, times the softmax scale, goes to row_scale.
+template <class T, int HD>
+__device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, int n_rows, int tile0, int r0, uint8_t* qt,
+                                            float* row_scale) {
+  using C = PromptCfg<T, HD>;
+  constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP;
+  constexpr int MOST = sizeof(T) == 4 ? 8 : 16, NB = MOST < PASSES ? MOST : PASSES;  // passes whose loads are in flight together
+  const int lane = threadIdx.x & 31, sub = lane / LPR, piece = lane % LPR;
+  const T* q = static_cast<const T*>(a.q) + 8 * piece;
+#pragma unroll 1
+  for (int p0 = 0; p0 < PASSES; p0 += NB) {
+    Raw8<T> v[NB];
+    long long at[NB];
+    unsigned m[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) at[b] = __shfl_sync(0xffffffffu, row_at, (p0 + b) * RPP + sub);
+    if (a.q_vec) {
+#pragma unroll
+      for (int b = 0; b < NB; b++) v[b].load(q + at[b], true);
+    } else {
+#pragma unroll
+      for (int b = 0; b < NB; b++) v[b].load(q + at[b], false);
+    }
+    // (each step for all passes, so that their latencies overlap)
+#pragma unroll
+    for (int b = 0; b < NB; b++) m[b] = v[b].largest();
+#pragma unroll
+    for (int o = 1; o < LPR; o <<= 1)
+#pragma unroll
+      for (int b = 0; b < NB; b++) m[b] = max(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const int r = r0 + (p0 + b) * RPP + sub;
+      const int e = (int)(m[b] >> 23);
+      const int up = e == 255 || m[b] == 0 ? 127 : min(253, 267 - e);
+      // (the sign of the softmax scale goes into the query, so that larger products are larger scores; rows past the last
+      // are zeros)
+      const bool live = tile0 + r < n_rows;
+      const float mul = copysignf(__int_as_float(up << 23), a.scale_log2);
+      if (piece == 0) row_scale[r] = __int_as_float((254 - up) << 23) * fabsf(a.scale_log2);
+      uint32_t h[4], rest[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float x0 = v[b].at(2 * i) * mul, x1 = v[b].at(2 * i + 1) * mul;
+        const __half2 t = __floats2half2_rn(x0, x1);
+        h[i] = live ? *reinterpret_cast<const uint32_t*>(&t) : 0u;
+        if (C::TERMS == 2) rest[i] = live ? pack_half2(x0 - __low2float(t), x1 - __high2float(t)) : 0u;
+      }
+      const uint32_t o = (piece >> 3) * (128 * 128) + sw128(r, piece & 7);
+      *reinterpret_cast<uint4*>(qt + o) = make_uint4(h[0], h[1], h[2], h[3]);
+      if (C::TERMS == 2) *reinterpret_cast<uint4*>(qt + C::Q_TILE + o) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
 // The largest score of one tile of keys among those the row sees, with the exponent of V's scale.
 template <bool EDGE>
 __device__ __forceinline__ float tile_max(const float* s, const KeyInfo* in, int key0, int first_key, int pos) {
@@ -256,8 +361,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   const int idx = pa.tiles - 1 - blockIdx.x / (pa.splits * a.kv_heads);
   const TileAt at = tile_at(pa, idx);
   if (at.r < 0) return;
-  const Request R = request_of(a, at.r);
-  const int n_all = a.q_start[at.r + 1] - a.q_start[at.r], n_rows = R.n_q * a.group;
+  const Request R = at.R;
+  const int n_all = at.n_all, n_rows = R.n_q * a.group;
   int lo, hi;
   key_range(a, R, n_all, at.row0 / a.group, min(at.row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
   const Span sp = spans_of(lo, hi, pa.splits, pa.blocks, PR_KEYS);
@@ -453,58 +558,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     const int trow = 32 * w4 + lane, row = at.row0 + q * 128 + trow;
     const bool live = row < n_rows;
     const int rr = live ? row : n_rows - 1;  // (rows past the last compute on zeros and are not stored)
-    const int tok = rr / a.group, hq = head * a.group + rr % a.group;
+    int hq;
+    const int tok = token_of(a, rr, &hq);
+    hq += head * a.group;
     const int pos = R.len - n_all + tok, first_key = a.window > 0 ? pos + 1 - a.window : 0;
-    if (n_tiles > 0) {  // the warp's 32 queries, HD / 8 lanes each: largest magnitude to [2^13, 2^14) by a power of two, one or two terms
-      constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, BATCH = 8;
-      const long long src = (long long)(R.first + tok) * a.q_row + hq * a.q_head;
-      const int sub = lane / LPR, piece = lane % LPR;
-      uint8_t* qt = sm + q * C::Q_AREA;
-#pragma unroll 1
-      for (int p0 = 0; p0 < PASSES; p0 += BATCH) {
-        float v[BATCH][8];
-#pragma unroll
-        for (int b = 0; b < BATCH; b++) {
-          const int r = (p0 + b) * RPP + sub;  // row of the warp
-          const T* x = static_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, src, r) + 8 * piece;
-          if (a.q_vec) load4<true>(x, v[b]), load4<true>(x + 4, v[b] + 4);
-          else load4<false>(x, v[b]), load4<false>(x + 4, v[b] + 4);
-        }
-#pragma unroll
-        for (int b = 0; b < BATCH; b++) {
-          const int r = (p0 + b) * RPP + sub;
-          unsigned m = 0;
-#pragma unroll
-          for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[b][i]) & 0x7fffffffu);
-#pragma unroll
-          for (int o = 1; o < LPR; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const int e = (int)(m >> 23);
-          const int up = e == 255 || m == 0 ? 127 : min(253, 267 - e);
-          // (the sign of the softmax scale goes into the query, so that larger products are larger scores)
-          const float mul = copysignf(__int_as_float(up << 23), a.scale_log2);
-          if (piece == 0) row_scale[q * 128 + 32 * w4 + r] = __int_as_float((254 - up) << 23) * fabsf(a.scale_log2);
-          const bool row_live = at.row0 + q * 128 + 32 * w4 + r < n_rows;
-          uint32_t h[4], rest[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float x0 = row_live ? v[b][2 * i] * mul : 0.f, x1 = row_live ? v[b][2 * i + 1] * mul : 0.f;
-            const __half2 t = __floats2half2_rn(x0, x1);
-            h[i] = *reinterpret_cast<const uint32_t*>(&t);
-            rest[i] = pack_half2(x0 - __low2float(t), x1 - __high2float(t));
-          }
-          const uint32_t o = (piece >> 3) * (128 * 128) + sw128(32 * w4 + r, piece & 7);
-          *reinterpret_cast<uint4*>(qt + o) = make_uint4(h[0], h[1], h[2], h[3]);
-          if (C::TERMS == 2) *reinterpret_cast<uint4*>(qt + C::Q_TILE + o) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
+    bool ok = true;
+    if (n_tiles > 0) {
+      put_queries<T, HD>(a, (long long)(R.first + tok) * a.q_row + hq * a.q_head, n_rows, at.row0 + q * 128, 32 * w4,
+                         sm + q * C::Q_AREA, row_scale + q * 128);
       if (lane == 0) bar_arrive(q_full + q);
     }
     const float f_row = n_tiles > 0 ? row_scale[q * 128 + trow] : 0.f;
     const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + q * 256, to = tl + 128;
     float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true, ready = false;
+    bool ready = false;
     for (int j = 0; j < n_tiles; j++) {
       if (j % PR_INFO == 0 && !wait_phase_warp(i_full + (j / PR_INFO & 1), (j / PR_INFO >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
       KeyInfo in[PR_KEYS / 16];
@@ -588,16 +655,30 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
           *reinterpret_cast<float4*>(stage + lane * C::OUT_LD + i) =
               make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
         __syncwarp();
+        // 8 lanes a row, 4 rows at a time
+        float4 x[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const int r = 4 * k + (lane >> 3), i = 4 * (lane & 7);
-          const long long to_row = __shfl_sync(0xffffffffu, dst, r);
-          const float4 x = *reinterpret_cast<const float4*>(stage + r * C::OUT_LD + i);
-          if (at.row0 + q * 128 + 32 * w4 + r < n_rows) {
-            const float v[4] = {x.x, x.y, x.z, x.w};
-            if (whole) store_row4<T, HD>(a, static_cast<T*>(a.out) + to_row + c + i, v);
-            else *reinterpret_cast<float4*>(pa.part + (unit * PR_ROWS + q * 128 + 32 * w4 + r) * HD + c + i) = x;
-          }
+        for (int k = 0; k < 8; k++)
+          x[k] = *reinterpret_cast<const float4*>(stage + (4 * k + (lane >> 3)) * C::OUT_LD + 4 * (lane & 7));
+        const int col = c + 4 * (lane & 7), rows_left = n_rows - (at.row0 + q * 128 + 32 * w4) - (lane >> 3);
+        if (whole) {
+          T* d[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) d[k] = static_cast<T*>(a.out) + __shfl_sync(0xffffffffu, dst, 4 * k + (lane >> 3)) + col;
+          auto store = [&](bool vec) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+              const float v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+              if (4 * k < rows_left) store4(d[k], v, vec);
+            }
+          };
+          if (a.out_vec) store(true);
+          else store(false);
+        } else {
+          float* d = pa.part + (unit * PR_ROWS + q * 128 + 32 * w4 + (lane >> 3)) * HD + col;
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (4 * k < rows_left) *reinterpret_cast<float4*>(d + 4 * k * HD) = x[k];
         }
       }
       if (live) {
