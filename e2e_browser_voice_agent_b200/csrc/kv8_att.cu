@@ -552,6 +552,8 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
   a.table_cols = g->table_cols; a.n_req = g->n_req; a.rows = g->rows; a.max_q = g->max_q; a.window = g->window;
   a.q_vec = !((uintptr_t)g->q & (4 * es - 1)) && !((g->q_row | g->q_head) & 3);
   a.out_vec = !((uintptr_t)g->out & (4 * es - 1)) && !((g->out_row | g->out_head) & 3);
+  a.q_vec16 = !((uintptr_t)g->q & 15) && !((g->q_row * es | g->q_head * es) & 15);
+  a.out_vec16 = !((uintptr_t)g->out & 15) && !((g->out_row * es | g->out_head * es) & 15);
   a.scale_log2 = g->scale * 1.4426950408889634f;
   cudaStream_t st = (cudaStream_t)stream;
   if (g->type == H2C_TYPE_F32) return launch_typed<float>(who, g->head_dim, p, a, g->workspace, st);

@@ -18,6 +18,7 @@ struct AttArgs {
   int table_cols, n_req, rows, max_q, window;
   unsigned group_magic;   // see token_of
   int q_vec, out_vec;     // four-element loads of q, stores of out are aligned
+  int q_vec16, out_vec16; // rows of q, of out begin at multiples of 16 bytes
   float scale_log2;       // scale * log2(e): scores are kept in powers of two
 };
 

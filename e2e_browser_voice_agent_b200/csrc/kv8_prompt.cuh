@@ -163,9 +163,9 @@ struct PromptCfg {
   static constexpr int BLKS = HD / 64;                   // 64-dimension blocks of a row
   static constexpr int Q_TILE = 128 * HD * 2;            // one row tile, one term
   static constexpr int KV_TILE = PR_KEYS * HD * 2;
-  static constexpr int OUT_LD = 36;                      // floats per row of a warp's output staging (32 columns)
+  static constexpr int OUT_LD = 256 + 16;                // bytes per row of a row tile's output staging: up to 256 of the row
   // a row tile's queries, later the staging of its output
-  static constexpr int Q_AREA = TERMS * Q_TILE > 4 * 32 * OUT_LD * 4 ? TERMS * Q_TILE : 4 * 32 * OUT_LD * 4;
+  static constexpr int Q_AREA = TERMS * Q_TILE > 128 * OUT_LD ? TERMS * Q_TILE : 128 * OUT_LD;
   static constexpr int OFF_K = 2 * Q_AREA;
   static constexpr int STAGES = TERMS * HD > 128 ? 2 : 3;   // K and V tiles each
   static constexpr int OFF_V = OFF_K + STAGES * KV_TILE;
@@ -217,36 +217,19 @@ __device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float
   }
 }
 
-// Eight consecutive values as they lie in memory, and as float32.
+// Eight values as they lie in memory, and as float32.
 template <class T>
 struct Raw8 {
   uint32_t w[2 * sizeof(T)];
-  __device__ __forceinline__ void load(const T* p, bool vec) {
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T); i++) {
-        const uint2 x = reinterpret_cast<const uint2*>(p)[i];
-        w[2 * i] = x.x;
-        w[2 * i + 1] = x.y;
-      }
-    } else {
-      T v[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = p[i];
-#pragma unroll
-      for (int i = 0; i < 2 * (int)sizeof(T); i++) w[i] = reinterpret_cast<const uint32_t*>(v)[i];
-    }
-  }
   __device__ __forceinline__ float at(int i) const { return to_f(reinterpret_cast<const T*>(w)[i]); }
   // the largest magnitude's bits as a float32 (infinities and NaN above every number)
   __device__ __forceinline__ unsigned largest() const {
+    unsigned m = 0;
     if (sizeof(T) == 4) {
-      unsigned m = 0;
 #pragma unroll
       for (int i = 0; i < 8; i++) m = max(m, w[i] & 0x7fffffffu);
       return m;
     }
-    unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
     m = max(m & 0xffffu, m >> 16);
@@ -258,29 +241,50 @@ struct Raw8 {
 // A warp's 32 rows of a row tile's queries (from row r0 of the tile, which begins at row tile0 of the request): HD / 8 lanes a
 // row; lane i has the place of row i in q (row_at). A row is scaled by a power of two so that its largest magnitude lies in
 // [2^13, 2^14) and split into one or two float16 terms; what undoes the scaling, times the softmax scale, goes to row_scale.
+// The raw values are copied to where their terms will lie (8 of them take as many bytes as their terms do) and replaced
+// there by the same lane. Rolled loops: code that runs once waits for its own fetching.
 template <class T, int HD>
 __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, int n_rows, int tile0, int r0, uint8_t* qt,
                                             float* row_scale) {
   using C = PromptCfg<T, HD>;
-  constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP;
-  constexpr int MOST = sizeof(T) == 4 ? 8 : 16, NB = MOST < PASSES ? MOST : PASSES;  // passes whose loads are in flight together
+  constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP, NB = 4;
   const int lane = threadIdx.x & 31, sub = lane / LPR, piece = lane % LPR;
   const T* q = static_cast<const T*>(a.q) + 8 * piece;
+  uint8_t* blk = qt + (piece >> 3) * (128 * 128);
+  if (a.q_vec16) {
+#pragma unroll 2
+    for (int p = 0; p < PASSES; p++) {
+      const T* src = q + __shfl_sync(0xffffffffu, row_at, p * RPP + sub);
+      const uint32_t dst = su32(blk + sw128(r0 + p * RPP + sub, piece & 7));
+#pragma unroll
+      for (int t = 0; t < C::TERMS; t++)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + t * C::Q_TILE), "l"(src + t * 4) : "memory");
+    }
+    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+  } else {
+#pragma unroll 1
+    for (int p = 0; p < PASSES; p++) {
+      const T* src = q + __shfl_sync(0xffffffffu, row_at, p * RPP + sub);
+      uint8_t* dst = blk + sw128(r0 + p * RPP + sub, piece & 7);
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        *reinterpret_cast<T*>(dst + (i * (int)sizeof(T) >> 4) * C::Q_TILE + (i * (int)sizeof(T) & 15)) = src[i];
+    }
+  }
 #pragma unroll 1
   for (int p0 = 0; p0 < PASSES; p0 += NB) {
     Raw8<T> v[NB];
-    long long at[NB];
     unsigned m[NB];
-#pragma unroll
-    for (int b = 0; b < NB; b++) at[b] = __shfl_sync(0xffffffffu, row_at, (p0 + b) * RPP + sub);
-    if (a.q_vec) {
-#pragma unroll
-      for (int b = 0; b < NB; b++) v[b].load(q + at[b], true);
-    } else {
-#pragma unroll
-      for (int b = 0; b < NB; b++) v[b].load(q + at[b], false);
-    }
     // (each step for all passes, so that their latencies overlap)
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const uint8_t* at = blk + sw128(r0 + (p0 + b) * RPP + sub, piece & 7);
+#pragma unroll
+      for (int t = 0; t < C::TERMS; t++) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at + t * C::Q_TILE);
+        v[b].w[4 * t] = x.x, v[b].w[4 * t + 1] = x.y, v[b].w[4 * t + 2] = x.z, v[b].w[4 * t + 3] = x.w;
+      }
+    }
 #pragma unroll
     for (int b = 0; b < NB; b++) m[b] = v[b].largest();
 #pragma unroll
@@ -305,13 +309,52 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
         h[i] = live ? *reinterpret_cast<const uint32_t*>(&t) : 0u;
         if (C::TERMS == 2) rest[i] = live ? pack_half2(x0 - __low2float(t), x1 - __high2float(t)) : 0u;
       }
-      const uint32_t o = (piece >> 3) * (128 * 128) + sw128(r, piece & 7);
-      *reinterpret_cast<uint4*>(qt + o) = make_uint4(h[0], h[1], h[2], h[3]);
-      if (C::TERMS == 2) *reinterpret_cast<uint4*>(qt + C::Q_TILE + o) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+      uint8_t* at = blk + sw128(r, piece & 7);
+      *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+      if (C::TERMS == 2) *reinterpret_cast<uint4*>(at + C::Q_TILE) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
+}
+
+// A thread's row of O, scaled, as NC values of type U at dst (a row of the warp's staging; columns col .. col + NC of the row).
+template <class U, int NC>
+__device__ __forceinline__ void stage_row(uint8_t* dst, uint32_t o_at, bool any, float inv) {
+#pragma unroll 1
+  for (int c = 0; c < NC; c += 32) {
+    float o[32];
+    if (any) {
+      tmem_ld32(o_at + c, o);
+      tc_wait_ld();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++) o[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 16 / (int)sizeof(U)) {
+      alignas(16) U x[16 / sizeof(U)];
+#pragma unroll
+      for (int k = 0; k < 16 / (int)sizeof(U); k++) x[k] = from_f<U>(o[i + k] * inv);
+      *reinterpret_cast<uint4*>(dst + (c + i) * sizeof(U)) = *reinterpret_cast<const uint4*>(x);
+    }
+  }
+}
+// The staged NC values to global memory, where `store` says so: one bulk copy when both sides are 16-byte aligned. On return
+// the staging can be written again.
+template <class U, int NC>
+__device__ __forceinline__ void copy_row(U* dst, const uint8_t* src, bool store, bool bulk) {
+  if (bulk) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (store)
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(__cvta_generic_to_global(dst)),
+                   "r"(su32(src)), "r"(NC * (int)sizeof(U))
+                   : "memory");
+    asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group.read 0;" ::: "memory");
+  } else if (store) {
+#pragma unroll 1
+    for (int i = 0; i < NC; i++) dst[i] = reinterpret_cast<const U*>(src)[i];
+  }
 }
 
 // The largest score of one tile of keys among those the row sees, with the exponent of V's scale.
@@ -440,8 +483,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         if (id[i] >= 0) raw[i] = *reinterpret_cast<const uint4*>(src + id[i] * page_bytes + (size_t)(key & page_mask) * HD);
       }
     };
-    // (warp 8) the scales of the 16-key groups of PR_INFO tiles, the batch-th such. Its place held batch - 2: this is called
-    // 16 tiles before the batch begins, and a tile of K is not converted before the softmax is done with the tile five before
+    // (warp 12) the scales of the 16-key groups of PR_INFO tiles, the batch-th such. Its place held batch - 2: this is called
+    // 16 tiles before the batch begins, and a tile of V is not converted before the softmax is done with the tile STG before
     auto publish_info = [&](int batch) {
       const int g0 = batch * PR_INFO * (PR_KEYS / 16);
       float sk[4], sv[4];
@@ -476,12 +519,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       pages_of(0);
       load(0);
       pages_of(1);
-      if (warp == 8) publish_info(0);
+      if (warp == 12) publish_info(0);
     }
     for (int j = 0; j < n_tiles; j++) {
       const int s = j % STG;
       if (!wait_group(empty + s, ((j / STG) & 1) ^ 1, ab, PR_CONVERT, 1 + which, go[which], j)) break;
-      if (warp == 8 && j % PR_INFO == PR_INFO - 16 && j + 16 < n_tiles) publish_info(j / PR_INFO + 1);
+      if (warp == 12 && j % PR_INFO == PR_INFO - 16 && j + 16 < n_tiles) publish_info(j / PR_INFO + 1);
       uint8_t* tile = tiles + s * C::KV_TILE;
 #pragma unroll
       for (int i = 0; i < NI; i++) {
@@ -626,9 +669,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       __syncwarp();
       if (lane == 0) bar_arrive(&p_full[q][j & 1]);
     }
-    // ---- the rows' output: 32 columns at a time through shared memory, so that 8 lanes write 32 consecutive values of a
-    // row. The staging takes the place of the row tile's queries: their last product was issued before the last update of O,
-    // whose completion is waited for (and without keys they were not written).
+    // ---- the rows' output: each thread stages its row in the place of the row tile's queries (their last product was issued
+    // before the last update of O, whose completion is waited for; without keys they were not written) and copies it out
     if (ok && n_tiles > 0) {
       ok = wait_phase_warp(&pv_done[q][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, ab, PR_SOFTMAX);
       tc_fence_after();
@@ -637,48 +679,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       const bool whole = sp.used == 1;
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
       const size_t unit = ((size_t)idx * a.kv_heads + head) * pa.splits + split;
-      const long long dst = (long long)(R.first + tok) * a.out_row + hq * a.out_head;
-      float* stage = reinterpret_cast<float*>(sm + q * C::Q_AREA) + w4 * 32 * C::OUT_LD;
+      uint8_t* stage = sm + q * C::Q_AREA + trow * C::OUT_LD;
+      if (whole) {
+        constexpr int NC = 256 / (int)sizeof(T) < HD ? 256 / (int)sizeof(T) : HD;
+        T* dst = static_cast<T*>(a.out) + (long long)(R.first + tok) * a.out_row + hq * a.out_head;
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 32) {
-        float o[32];
-        if (n_tiles > 0) {
-          tmem_ld32(to + c, o);
-          tc_wait_ld();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i++) o[i] = 0.f;
+        for (int c = 0; c < HD; c += NC) {
+          stage_row<T, NC>(stage, to + c, n_tiles > 0, inv);
+          copy_row<T, NC>(dst + c, stage, live, a.out_vec16);
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4*>(stage + lane * C::OUT_LD + i) =
-              make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
-        __syncwarp();
-        // 8 lanes a row, 4 rows at a time
-        float4 x[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-          x[k] = *reinterpret_cast<const float4*>(stage + (4 * k + (lane >> 3)) * C::OUT_LD + 4 * (lane & 7));
-        const int col = c + 4 * (lane & 7), rows_left = n_rows - (at.row0 + q * 128 + 32 * w4) - (lane >> 3);
-        if (whole) {
-          T* d[8];
-#pragma unroll
-          for (int k = 0; k < 8; k++) d[k] = static_cast<T*>(a.out) + __shfl_sync(0xffffffffu, dst, 4 * k + (lane >> 3)) + col;
-          auto store = [&](bool vec) {
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-              const float v[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-              if (4 * k < rows_left) store4(d[k], v, vec);
-            }
-          };
-          if (a.out_vec) store(true);
-          else store(false);
-        } else {
-          float* d = pa.part + (unit * PR_ROWS + q * 128 + 32 * w4 + (lane >> 3)) * HD + col;
-#pragma unroll
-          for (int k = 0; k < 8; k++)
-            if (4 * k < rows_left) *reinterpret_cast<float4*>(d + 4 * k * HD) = x[k];
+      } else {
+        float* dst = pa.part + (unit * PR_ROWS + q * 128 + trow) * HD;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 64) {
+          stage_row<float, 64>(stage, to + c, n_tiles > 0, 1.f);
+          copy_row<float, 64>(dst + c, stage, live, true);
         }
       }
       if (live) {
