@@ -13,7 +13,6 @@ that do not fit raise ValueError or TypeError here, or H2CError from the library
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -33,61 +32,67 @@ class Plan(NamedTuple):
     status: torch.Tensor      # int32 [2]
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# The current device and its current stream, without the Stream object that torch.cuda.current_stream makes of it (which
+# costs as much as a launch).
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
 
 
-class _On:
-    """The device of `t` as the current one, for the time of a call (most often it is already)."""
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, stream) with device `index` current, on its current stream."""
+    if index < 0:
+        raise ValueError("CUDA tensors are wanted")
+    before = _device()
+    if index == before:
+        rc = fn(*args, _stream(index))
+    else:
+        torch.cuda.set_device(index)
+        try:
+            rc = fn(*args, _stream(index))
+        finally:
+            torch.cuda.set_device(before)
+    if rc:
+        _lib.check(rc)
 
-    def __init__(self, t: torch.Tensor):
-        if not t.is_cuda:
-            raise ValueError("a CUDA tensor is wanted")
-        self.device, self.before = t.device, torch.cuda.current_device()
 
-    def __enter__(self):
-        if self.device.index != self.before:
-            torch.cuda.set_device(self.device)
-        return _stream(self.device)
-
-    def __exit__(self, *_):
-        if self.device.index != self.before:
-            torch.cuda.set_device(self.before)
-
-
-def _want(name: str, t: torch.Tensor, dtype: torch.dtype, device: torch.device, shape: Optional[Tuple] = None) -> int:
-    """The address of a contiguous tensor of this type and shape on this device."""
+def _want(name: str, t: torch.Tensor, dtype: torch.dtype, index: int, shape: Optional[Tuple] = None) -> int:
+    """The address of a contiguous tensor of this type and shape on device `index`."""
+    if t.dtype is dtype and t.get_device() == index and t.is_contiguous() and (shape is None or t.shape == shape):
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{name}: {dtype} is wanted, not {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, not {device}")
-    if shape is not None and tuple(t.shape) != shape:
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on {t.device}, not cuda:{index}")
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name}: shape {shape} is wanted, not {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{name}: must be contiguous")
 
 
 def _cache(kv: torch.Tensor, kv_scale: torch.Tensor):
-    if kv.dim() != 5 or kv.shape[1] != 2:
-        raise ValueError(f"kv: [pages, 2, kv heads, page size, head dim] is wanted, not {tuple(kv.shape)}")
-    n_pages, _, kv_heads, page, head_dim = kv.shape
-    return (_want("kv", kv, torch.int8, kv.device),
-            _want("kv_scale", kv_scale, torch.float32, kv.device, (n_pages, 2, kv_heads)), n_pages, page, kv_heads, head_dim)
+    """(device, address, address of the scales, pages, page size, kv heads, head dimension)"""
+    shape = kv.shape
+    if len(shape) != 5 or shape[1] != 2:
+        raise ValueError(f"kv: [pages, 2, kv heads, page size, head dim] is wanted, not {tuple(shape)}")
+    n_pages, _, kv_heads, page, head_dim = shape
+    index = kv.get_device()
+    return (index, _want("kv", kv, torch.int8, index),
+            _want("kv_scale", kv_scale, torch.float32, index, (n_pages, 2, kv_heads)), n_pages, page, kv_heads, head_dim)
 
 
-def _rows(name: str, t: torch.Tensor, device: torch.device, heads: int, head_dim: int) -> Tuple[int, int, int, int]:
+def _rows(name: str, t: torch.Tensor, index: int, heads: int, head_dim: int) -> Tuple[int, int, int, int]:
     """(address, element type, row stride, head stride) of [rows, heads, head_dim] values, the last axis dense."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
-        raise ValueError(f"{name}: [rows, {heads}, {head_dim}] is wanted, not {tuple(t.shape)}")
-    if t.dtype not in _TYPES:
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"{name}: [rows, {heads}, {head_dim}] is wanted, not {tuple(shape)}")
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
         raise TypeError(f"{name}: float32, float16 or bfloat16 is wanted, not {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, not {device}")
-    s = t.stride()
-    if s[2] != 1:
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on {t.device}, not cuda:{index}")
+    row, head, dense = t.stride()
+    if dense != 1:
         raise ValueError(f"{name}: the head dimension must be dense")
-    return t.data_ptr(), _TYPES[t.dtype], s[0], s[1]
+    return t.data_ptr(), kind, row, head
 
 
 def allocate(n_pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
@@ -107,66 +112,62 @@ def plan(cached: torch.Tensor, total: torch.Tensor, block_table: torch.Tensor, f
     """Take and give back pages so that request r goes from cached[r] to total[r] tokens, and map the new tokens to
     slots (h2c_kv8_plan). block_table (int32 [requests, columns]) and free_pages (int32 [pages], a ring) change in place.
     out: a Plan of an earlier call of the same sizes, whose tensors are written again."""
-    dev = cached.device
-    n = cached.shape[0] if cached.dim() == 1 else -1
-    if n < 0:
+    if cached.dim() != 1:
         raise ValueError(f"cached: one length per request is wanted, not {tuple(cached.shape)}")
+    index, n = cached.get_device(), cached.shape[0]
     if block_table.dim() != 2 or block_table.shape[0] != n:
         raise ValueError(f"block_table: [{n}, columns] is wanted, not {tuple(block_table.shape)}")
     if free_pages.dim() != 1:
         raise ValueError(f"free_pages: one number per page is wanted, not {tuple(free_pages.shape)}")
     if max_tokens < 0:
         raise ValueError(f"max_tokens: {max_tokens}")
-    with _On(cached) as stream:
-        i32, i64 = torch.int32, torch.int64
-        if out is None:
-            # one allocation; the 64-bit state first
-            buf = torch.empty(4 + 2 + n + (n + 1) + 2 * max_tokens, dtype=i32, device=dev)
-            state, status, kv_len, q_start, slot, position = buf.split([4, 2, n, n + 1, max_tokens, max_tokens])
-            out = Plan(kv_len, q_start, slot, position, state.view(i64), status)
-        p = (_want("cached", cached, i32, dev), _want("total", total, i32, dev, (n,)),
-             _want("block_table", block_table, i32, dev))
-        _lib.check(_lib.load().h2c_kv8_plan(
-            n, page_size, *p, block_table.shape[1], _want("free_pages", free_pages, i32, dev), free_pages.shape[0],
-            _want("free_state", free_state, i64, dev, (2,)), _want("out.free_state", out.free_state, i64, dev, (2,)),
-            _want("out.kv_len", out.kv_len, i32, dev, (n,)), _want("out.q_start", out.q_start, i32, dev, (n + 1,)),
-            _want("out.slot", out.slot, i32, dev, (max_tokens,)),
-            _want("out.position", out.position, i32, dev, (max_tokens,)), max_tokens,
-            _want("out.status", out.status, i32, dev, (2,)), stream))
+    i32, i64 = torch.int32, torch.int64
+    args = (n, page_size, _want("cached", cached, i32, index), _want("total", total, i32, index, (n,)),
+            _want("block_table", block_table, i32, index), block_table.shape[1],
+            _want("free_pages", free_pages, i32, index), free_pages.shape[0], _want("free_state", free_state, i64, index, (2,)))
+    if out is None:
+        # one allocation; the 64-bit state first
+        buf = torch.empty(4 + 2 + n + (n + 1) + 2 * max_tokens, dtype=i32, device=cached.device)
+        state, status, kv_len, q_start, slot, position = buf.split((4, 2, n, n + 1, max_tokens, max_tokens))
+        out = Plan(kv_len, q_start, slot, position, state.view(i64), status)
+        at = buf.data_ptr()
+        places = (at, at + 24, at + 24 + 4 * n, at + 28 + 8 * n, at + 28 + 8 * n + 4 * max_tokens, max_tokens, at + 16)
+    else:
+        places = (_want("out.free_state", out.free_state, i64, index, (2,)), _want("out.kv_len", out.kv_len, i32, index, (n,)),
+                  _want("out.q_start", out.q_start, i32, index, (n + 1,)), _want("out.slot", out.slot, i32, index, (max_tokens,)),
+                  _want("out.position", out.position, i32, index, (max_tokens,)), max_tokens,
+                  _want("out.status", out.status, i32, index, (2,)))
+    _call(index, _lib.load().h2c_kv8_plan, *args, *places)
     return out
 
 
 def append(kv: torch.Tensor, kv_scale: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor) -> None:
     """Quantize rows of K and V ([rows, kv heads, head dim], any row and head stride) into the cache at slot
     (h2c_kv8_append); slot may hold more entries than there are rows."""
-    pkv, ps, n_pages, page, kvh, hd = _cache(kv, kv_scale)
-    dev = kv.device
-    pk, tk, k_row, k_head = _rows("k", k, dev, kvh, hd)
-    pv, tv, v_row, v_head = _rows("v", v, dev, kvh, hd)
+    index, *cache = _cache(kv, kv_scale)
+    pk, tk, k_row, k_head = _rows("k", k, index, cache[4], cache[5])
+    pv, tv, v_row, v_head = _rows("v", v, index, cache[4], cache[5])
     rows = k.shape[0]
     if v.shape[0] != rows or tv != tk:
         raise ValueError("k and v must have as many rows and the same type")
     if slot.dim() != 1 or slot.shape[0] < rows:
         raise ValueError(f"slot: at least {rows} entries are wanted, not {tuple(slot.shape)}")
-    with _On(kv) as stream:
-        _lib.check(_lib.load().h2c_kv8_append(pkv, ps, n_pages, page, kvh, hd, tk, pk, k_row, k_head, pv, v_row, v_head,
-                                              rows, _want("slot", slot, torch.int32, dev), stream))
+    _call(index, _lib.load().h2c_kv8_append, *cache, tk, pk, k_row, k_head, pv, v_row, v_head, rows,
+          _want("slot", slot, torch.int32, index))
 
 
 def read(kv: torch.Tensor, kv_scale: torch.Tensor, slot: torch.Tensor,
          dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
     """The cached K and V at slot, [slots, kv heads, head dim] each (h2c_kv8_read)."""
-    pkv, ps, n_pages, page, kvh, hd = _cache(kv, kv_scale)
+    index, *cache = _cache(kv, kv_scale)
     if dtype not in _TYPES:
         raise TypeError(f"dtype: float32, float16 or bfloat16 is wanted, not {dtype}")
     if slot.dim() != 1:
         raise ValueError(f"slot: one entry per row is wanted, not {tuple(slot.shape)}")
     rows = slot.shape[0]
-    with _On(kv) as stream:
-        k, v = torch.empty(2, rows, kvh, hd, dtype=dtype, device=kv.device).unbind(0)
-        _lib.check(_lib.load().h2c_kv8_read(pkv, ps, n_pages, page, kvh, hd,
-                                            _want("slot", slot, torch.int32, kv.device), rows, _TYPES[dtype],
-                                            k.data_ptr(), v.data_ptr(), stream))
+    k, v = (torch.empty(rows, cache[4], cache[5], dtype=dtype, device=kv.device) for _ in range(2))
+    _call(index, _lib.load().h2c_kv8_read, *cache, _want("slot", slot, torch.int32, index), rows, _TYPES[dtype], k.data_ptr(),
+          v.data_ptr())
     return k, v
 
 
@@ -177,32 +178,31 @@ def attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, block_t
     with any row and head stride; scale defaults to head_dim ** -0.5; window > 0 limits each query to that many positions.
     max_q and max_kv bound the requests' query counts and lengths. Returns out ([rows, heads, head dim], q's type), or
     (out, lse) with lse float32 [rows, heads]; rows that belong to no request keep what out held."""
-    pkv, ps, n_pages, page, kvh, hd = _cache(kv, kv_scale)
-    dev = kv.device
+    index, pkv, ps, n_pages, page, kvh, hd = _cache(kv, kv_scale)
     if q.dim() != 3:
         raise ValueError(f"q: [rows, heads, {hd}] is wanted, not {tuple(q.shape)}")
-    rows, heads = q.shape[0], q.shape[1]
-    pq, tq, q_row, q_head = _rows("q", q, dev, heads, hd)
+    rows, heads, _ = q.shape
+    pq, tq, q_row, q_head = _rows("q", q, index, heads, hd)
     n = kv_len.shape[0]
     if block_table.dim() != 2 or block_table.shape[0] != n:
         raise ValueError(f"block_table: [{n}, columns] is wanted, not {tuple(block_table.shape)}")
-    i32 = torch.int32
-    with _On(kv) as stream:
-        if out is None:
-            out = torch.empty(rows, heads, hd, dtype=q.dtype, device=dev)
-        po, to, o_row, o_head = _rows("out", out, dev, heads, hd)
+    i32, dev = torch.int32, kv.device
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        po, o_row, o_head = out.data_ptr(), heads * hd, hd
+    else:
+        po, to, o_row, o_head = _rows("out", out, index, heads, hd)
         if to != tq or out.shape[0] != rows:
             raise ValueError("out must have q's rows and type")
-        lse = torch.empty(rows, heads, dtype=torch.float32, device=dev) if return_lse else None
-        a = _lib.Kv8AttentionArgs(pq, q_row, q_head, po, o_row, o_head, lse.data_ptr() if return_lse else None, pkv, ps,
-                                  n_pages, page, kvh, hd, heads, tq, _want("block_table", block_table, i32, dev),
-                                  block_table.shape[1], n, _want("q_start", q_start, i32, dev, (n + 1,)),
-                                  _want("kv_len", kv_len, i32, dev, (n,)), rows, max_q, max_kv, window,
-                                  hd ** -0.5 if scale is None else scale, None, 0)
-        L = _lib.load()
-        need = L.h2c_kv8_attention_workspace(a)
-        if need:
-            work = torch.empty(need, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = work.data_ptr(), need
-        _lib.check(L.h2c_kv8_attention(a, stream))
+    lse = torch.empty(rows, heads, dtype=torch.float32, device=dev) if return_lse else None
+    a = _lib.Kv8AttentionArgs(pq, q_row, q_head, po, o_row, o_head, lse.data_ptr() if return_lse else None, pkv, ps, n_pages,
+                              page, kvh, hd, heads, tq, _want("block_table", block_table, i32, index), block_table.shape[1], n,
+                              _want("q_start", q_start, i32, index, (n + 1,)), _want("kv_len", kv_len, i32, index, (n,)), rows,
+                              max_q, max_kv, window, hd ** -0.5 if scale is None else scale, None, 0)
+    L = _lib.load()
+    need = L.h2c_kv8_attention_workspace(a)
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
+    _call(index, L.h2c_kv8_attention, a)
     return (out, lse) if return_lse else out
