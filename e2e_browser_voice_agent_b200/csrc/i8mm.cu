@@ -51,10 +51,9 @@ __global__ void __launch_bounds__(1024) k_i8_quantize(const T* __restrict__ x, l
   __syncthreads();
   m = __reduce_max_sync(0xffffffffu, lane < (int)(blockDim.x >> 5) ? red[lane] : 0u);
   const float a = __uint_as_float(m);
-  // 127 / a overflows for denormal rows, whose largest code is then below 127; infinities and NaN make the scale carry them
+  // 127 / a overflows for denormal rows, whose largest code is then below 127; infinities and NaN make the scale NaN
   const float inv = a > 0.f ? fminf(__fdiv_rn(127.f, a), 3.4028234663852886e38f) : 0.f;
-  if (threadIdx.x == 0) scale[blockIdx.x] = m > 0x7f800000u ? __int_as_float(0x7fc00000) : __fdiv_rn(a, 127.f);
-  auto code = [&](float v) { return __float2int_rn(rintf(v * inv)) & 255u; };  // (NaN: 0)
+  if (threadIdx.x == 0) scale[blockIdx.x] = m >= 0x7f800000u ? __int_as_float(0x7fc00000) : __fdiv_rn(a, 127.f);
   uint32_t* dst = reinterpret_cast<uint32_t*>(q + (long long)blockIdx.x * q_row);
   for (int u = threadIdx.x; u < k_pad >> 2; u += blockDim.x) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -64,7 +63,7 @@ __global__ void __launch_bounds__(1024) k_i8_quantize(const T* __restrict__ x, l
       for (int i = 0; i < 4; i++)
         if (4 * u + i < k) v[i] = to_f(src[4 * u + i]);
     }
-    dst[u] = code(v[0]) | code(v[1]) << 8 | code(v[2]) << 16 | code(v[3]) << 24;
+    dst[u] = round_bytes(__fmul_rn(v[0], inv), __fmul_rn(v[1], inv), __fmul_rn(v[2], inv), __fmul_rn(v[3], inv));
   }
 }
 

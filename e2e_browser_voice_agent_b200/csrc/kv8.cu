@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv8_plan(const PlanArgs a) {
 // ---------------------------------------------------------------- append
 //
 // The rows that one call brings to one page form a run; its (K or V, head) part is quantized together because it shares
-// a scale. grid.x covers windows of 16 rows, grid.y K or V and the head: a CTA takes the runs that start in its window
+// a scale. grid.x covers windows of 16 rows, grid.y K and V and the heads: a CTA takes the runs that start in its window
 // (a run longer than the window reaches beyond it). Runs of up to SHORT rows (decode steps: one row) take a warp each,
 // longer ones the whole CTA. A thread holds its values in registers between the maximum and the codes, so each input
 // is read once. Bound: bandwidth for prompts, latency for single rows.
@@ -170,7 +170,7 @@ constexpr float SCALE_MIN = 0x1p-62f, SCALE_MAX = 0x1p63f;
 struct AppendArgs {
   int8_t* kv;
   float* scale;
-  int n_slots, page_log, kv_heads, rows;
+  int n_slots, page_log, kv_heads, rows, heads_per_cta;
   const void *k, *v;
   long long k_row, k_head, v_row, v_head;
   const int* slot;
@@ -182,17 +182,17 @@ __device__ __forceinline__ float grown_scale(float a, float s0, bool finite) {
   if (s0 != 0.f && !(a > 127.5f * s0)) return s0;
   return fminf(fmaxf(fmaxf(__fdiv_rn(a, 127.f), 1.25f * s0), SCALE_MIN), SCALE_MAX);
 }
-__device__ __forceinline__ int code_of(float x, float inv) {
-  return __float2int_rn(fminf(fmaxf(rintf(x * inv), -127.f), 127.f));
-}
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-  return (a & 255u) | ((b & 255u) << 8) | ((c & 255u) << 16) | ((uint32_t)d << 24);
+__device__ __forceinline__ uint32_t codes_of(const float* x, float inv) {
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = fminf(fmaxf(__fmul_rn(x[i], inv), -127.f), 127.f);
+  return round_bytes(v[0], v[1], v[2], v[3]);
 }
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
-  int c[4];
+  float v[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) c[i] = __float2int_rn((float)(int8_t)(w >> (8 * i)) * ratio);
-  return pack4(c[0], c[1], c[2], c[3]);
+  for (int i = 0; i < 4; i++) v[i] = __fmul_rn((float)(int8_t)(w >> (8 * i)), ratio);
+  return round_bytes(v[0], v[1], v[2], v[3]);
 }
 
 // One run of one (K or V, head) by the threads i0 = 0 .. NT-1 of a warp (NT = 32) or of the CTA; reduce() combines the
@@ -238,12 +238,12 @@ __device__ __forceinline__ void append_run(const T* src, long long row_stride, i
   for (int k = 0; k < MAXU; k++) {
     const int u = i0 + k * NT;
     if (u < units)
-      dst[u] = lost ? 0u : pack4(code_of(v[k][0], inv), code_of(v[k][1], inv), code_of(v[k][2], inv), code_of(v[k][3], inv));
+      dst[u] = lost ? 0u : codes_of(v[k], inv);
   }
   for (int u = i0 + MAXU * NT; u < units; u += NT) {
     float x[4];
     load4<VEC>(src + (u / UPR) * row_stride + (u % UPR) * 4, x);
-    dst[u] = lost ? 0u : pack4(code_of(x[0], inv), code_of(x[1], inv), code_of(x[2], inv), code_of(x[3], inv));
+    dst[u] = lost ? 0u : codes_of(x, inv);
   }
   if (i0 == 0 && s != s0) *scale = s;  // (also when s is NaN; every thread has read s0: reduce() synchronises them)
 }
@@ -251,31 +251,34 @@ __device__ __forceinline__ void append_run(const T* src, long long row_stride, i
 template <class T, bool VEC, int HD>
 __global__ void __launch_bounds__(APP_THREADS) k_kv8_append(const AppendArgs a) {
   __shared__ int run_row[APP_WIN], run_len[APP_WIN];
+  __shared__ int slots[APP_WIN + 128];  // of the window and of the rows that its last run may reach
   __shared__ int n_runs;
   __shared__ unsigned red[APP_THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int P = 1 << a.page_log;
-  const int which = blockIdx.y / a.kv_heads, head = blockIdx.y % a.kv_heads;
   const int w0 = blockIdx.x * APP_WIN;
+  if (tid < APP_WIN + 128) slots[tid] = w0 + tid < a.rows ? a.slot[w0 + tid] : -1;
+  const int before = w0 > 0 && tid == 0 ? a.slot[w0 - 1] : -2;
+  __syncthreads();
   if (warp == 0) {
     // a row starts a run unless the row before it is at the offset before its own in the same page
-    const int t = w0 + lane;
+    const int last = __shfl_sync(0xffffffffu, before, 0);
     bool lead = false;
-    if (lane < APP_WIN && t < a.rows) {
-      const int s = a.slot[t];
-      lead = s >= 0 && s < a.n_slots && ((s & (P - 1)) == 0 || t == 0 || a.slot[t - 1] != s - 1);
+    if (lane < APP_WIN) {
+      const int s = slots[lane];
+      lead = s >= 0 && s < a.n_slots && ((s & (P - 1)) == 0 || (lane ? slots[lane - 1] : last) != s - 1);
     }
     const unsigned b = __ballot_sync(0xffffffffu, lead);
-    if (lead) run_row[__popc(b & ((1u << lane) - 1))] = t;
+    if (lead) run_row[__popc(b & ((1u << lane) - 1))] = lane;
     if (lane == 0) n_runs = __popc(b);
   }
   __syncthreads();
   const int runs = n_runs;
   for (int i = warp; i < runs; i += APP_THREADS / 32) {  // run lengths, a warp per run
-    const int t = run_row[i], s = a.slot[t], most = min(P - (s & (P - 1)), a.rows - t);
+    const int t = run_row[i], s = slots[t], most = P - (s & (P - 1));
     int len = most;
     for (int b = 0; b < most; b += 32) {
-      const bool in = b + lane < most && a.slot[t + b + lane] == s + b + lane;
+      const bool in = b + lane < most && slots[t + b + lane] == s + b + lane;
       const unsigned in_all = __ballot_sync(0xffffffffu, in);
       if (in_all != 0xffffffffu) {
         len = min(most, b + __ffs(~in_all) - 1);
@@ -285,66 +288,86 @@ __global__ void __launch_bounds__(APP_THREADS) k_kv8_append(const AppendArgs a) 
     if (lane == 0) run_len[i] = len;
   }
   __syncthreads();
-  const T* src = static_cast<const T*>(which ? a.v : a.k) + head * (which ? a.v_head : a.k_head);
-  const long long row_stride = which ? a.v_row : a.k_row;
-  auto page_of = [&](int s) {
-    return a.kv + (((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head) * ((size_t)P * HD);
-  };
-  auto scale_of = [&](int s) { return a.scale + ((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head; };
-  for (int i = warp; i < runs; i += APP_THREADS / 32) {
-    if (run_len[i] > APP_SHORT) continue;
-    const int t = run_row[i], s = a.slot[t];
-    append_run<T, VEC, HD, 32, APP_SHORT * HD / 128>(src + t * row_stride, row_stride, run_len[i], page_of(s),
-                                                     s & (P - 1), scale_of(s), lane,
-                                                     [](unsigned m) {
-                                                       m = __reduce_max_sync(0xffffffffu, m);
-                                                       __syncwarp();  // (every lane has read the old scale)
-                                                       return m;
-                                                     });
-  }
-  for (int i = 0; i < runs; i++) {
-    if (run_len[i] <= APP_SHORT) continue;
-    const int t = run_row[i], s = a.slot[t];
-    append_run<T, VEC, HD, APP_THREADS, 8>(src + t * row_stride, row_stride, run_len[i], page_of(s), s & (P - 1),
-                                           scale_of(s), tid, [&](unsigned m) {
-                                             m = __reduce_max_sync(0xffffffffu, m);
-                                             __syncthreads();  // (the run before is done with red[])
-                                             if (lane == 0) red[warp] = m;
-                                             __syncthreads();
-                                             unsigned x = red[lane % (APP_THREADS / 32)];
-                                             return __reduce_max_sync(0xffffffffu, x);
-                                           });
+  for (int hh = blockIdx.y * a.heads_per_cta; hh < (int)(blockIdx.y + 1) * a.heads_per_cta; hh++) {
+    const int which = hh / a.kv_heads, head = hh - which * a.kv_heads;
+    const T* src = static_cast<const T*>(which ? a.v : a.k) + head * (which ? a.v_head : a.k_head);
+    const long long row_stride = which ? a.v_row : a.k_row;
+    auto page_of = [&](int s) {
+      return a.kv + (((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head) * ((size_t)P * HD);
+    };
+    auto scale_of = [&](int s) { return a.scale + ((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head; };
+    for (int i = warp; i < runs; i += APP_THREADS / 32) {
+      if (run_len[i] > APP_SHORT) continue;
+      const int t = w0 + run_row[i], s = slots[run_row[i]];
+      append_run<T, VEC, HD, 32, APP_SHORT * HD / 128>(src + t * row_stride, row_stride, run_len[i], page_of(s),
+                                                       s & (P - 1), scale_of(s), lane, [](unsigned m) {
+                                                         m = __reduce_max_sync(0xffffffffu, m);
+                                                         __syncwarp();  // (every lane has read the old scale)
+                                                         return m;
+                                                       });
+    }
+    for (int i = 0; i < runs; i++) {
+      if (run_len[i] <= APP_SHORT) continue;
+      const int t = w0 + run_row[i], s = slots[run_row[i]];
+      append_run<T, VEC, HD, APP_THREADS, 8>(src + t * row_stride, row_stride, run_len[i], page_of(s), s & (P - 1),
+                                             scale_of(s), tid, [&](unsigned m) {
+                                               m = __reduce_max_sync(0xffffffffu, m);
+                                               __syncthreads();  // (the run before is done with red[])
+                                               if (lane == 0) red[warp] = m;
+                                               __syncthreads();
+                                               unsigned x = red[lane % (APP_THREADS / 32)];
+                                               return __reduce_max_sync(0xffffffffu, x);
+                                             });
+    }
   }
 }
 
 // ---------------------------------------------------------------- read
 
+// A thread takes four consecutive codes of a row (blockDim.x threads across the row's K heads, then V heads) and goes from row to
+// row: its 16 or 8 bytes of output join its neighbours'. Four rows in flight. Bound: bandwidth.
 template <class T>
-__global__ void k_kv8_read(const int8_t* __restrict__ kv, const float* __restrict__ scale, int n_slots, int page_log,
-                           int kv_heads, int hd_log, const int* __restrict__ slot, long long units, T* __restrict__ k_out,
-                           T* __restrict__ v_out) {
-  // a unit is 16 codes; units of a row: K heads, then V heads
-  const int per_head_log = hd_log - 4, per_row = 2 * kv_heads << per_head_log;
-  for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (long long)gridDim.x * blockDim.x) {
-    const int t = (int)(u / per_row), w = (int)(u % per_row);
-    const int hh = w >> per_head_log, c = (w & ((1 << per_head_log) - 1)) * 16;  // (K or V, head), first dimension
-    const int which = hh >= kv_heads, head = hh - which * kv_heads;
-    const int s = slot[t];
-    alignas(16) T o[16];
-    if (s >= 0 && s < n_slots) {
-      const size_t ph = ((size_t)(s >> page_log) * 2 + which) * kv_heads + head;
-      const int4 q = *reinterpret_cast<const int4*>(kv + (((ph << page_log) + (s & ((1 << page_log) - 1))) << hd_log) + c);
-      const float f = scale[ph];
-      const int w4[4] = {q.x, q.y, q.z, q.w};
+__global__ void __launch_bounds__(256) k_kv8_read(const int8_t* __restrict__ kv, const float* __restrict__ scale, int n_slots,
+                                                  int page_log, int kv_heads, int hd_log, const int* __restrict__ slot, int rows,
+                                                  T* __restrict__ k_out, T* __restrict__ v_out) {
+  constexpr int NR = 4;
+  const int half = kv_heads << (hd_log - 2);  // units of four in a row's K
+  const int page_mask = (1 << page_log) - 1, step = gridDim.x * blockDim.y;
+  for (int u = threadIdx.x; u < 2 * half; u += blockDim.x) {
+    const int which = u >= half, w = u - which * half;
+    const int head = w >> (hd_log - 2), d = (w & ((1 << (hd_log - 2)) - 1)) * 4;
+    T* out = (which ? v_out : k_out) + (head << hd_log) + d;
+    const size_t row_len = (size_t)kv_heads << hd_log;
+    for (int t0 = blockIdx.x * blockDim.y + threadIdx.y; t0 < rows; t0 += NR * step) {
+      int sl[NR];
+      uint32_t q[NR];
+      float f[NR];
 #pragma unroll
-      for (int i = 0; i < 16; i++) o[i] = from_f<T>((float)(int8_t)(w4[i >> 2] >> (8 * (i & 3))) * f);
-    } else {
+      for (int i = 0; i < NR; i++) {
+        const int t = t0 + i * step;
+        sl[i] = t < rows ? slot[t] : -1;
+      }
 #pragma unroll
-      for (int i = 0; i < 16; i++) o[i] = from_f<T>(0.f);
+      for (int i = 0; i < NR; i++) {
+        q[i] = 0;
+        f[i] = 0.f;
+        if (sl[i] >= 0 && sl[i] < n_slots) {
+          const size_t ph = ((size_t)(sl[i] >> page_log) * 2 + which) * kv_heads + head;
+          q[i] = *reinterpret_cast<const uint32_t*>(kv + (((ph << page_log) + (sl[i] & page_mask)) << hd_log) + d);
+          f[i] = scale[ph];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NR; i++) {
+        const int t = t0 + i * step;
+        if (t >= rows) break;
+        alignas(16) T o[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[k] = from_f<T>((float)(int8_t)(q[i] >> (8 * k)) * f[i]);
+        if (sizeof(T) == 4) *reinterpret_cast<uint4*>(out + t * row_len) = *reinterpret_cast<const uint4*>(o);
+        else *reinterpret_cast<uint2*>(out + t * row_len) = *reinterpret_cast<const uint2*>(o);
+      }
     }
-    int4* d = reinterpret_cast<int4*>((which ? v_out : k_out) + ((((size_t)t * kv_heads + head)) << hd_log) + c);
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) * 16 / 16); i++) d[i] = reinterpret_cast<const int4*>(o)[i];
   }
 }
 
@@ -370,7 +393,7 @@ int cache_ok(const char* who, const void* kv, const float* scale, int n_pages, i
 
 template <class T, bool VEC>
 void launch_append(const AppendArgs& a, int head_dim, cudaStream_t st) {
-  const dim3 grid((a.rows + APP_WIN - 1) / APP_WIN, 2 * a.kv_heads);
+  const dim3 grid((a.rows + APP_WIN - 1) / APP_WIN, 2 * a.kv_heads / a.heads_per_cta);
   if (head_dim == 64) k_kv8_append<T, VEC, 64><<<grid, APP_THREADS, 0, st>>>(a);
   else k_kv8_append<T, VEC, 128><<<grid, APP_THREADS, 0, st>>>(a);
 }
@@ -428,7 +451,10 @@ int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size
   const size_t es = op_elem_size(type);
   if (((uintptr_t)k | (uintptr_t)v) & (es - 1))
     return op_error(H2C_ERR_INVALID, "%s: k and v must be aligned to their elements", who);
-  const AppendArgs a{static_cast<int8_t*>(kv), kv_scale, n_pages * page_size, log2_of(page_size), kv_heads, rows, k, v,
+  // few rows: a CTA for each (K or V, head), so that nothing waits in line; many: one for K and one for V, since most windows of
+  // a prompt begin no run and a CTA that finds none costs as much as its launch (16k rows: 41 us with one per head, 19 us so)
+  const int heads_per_cta = (long long)(rows + APP_WIN - 1) / APP_WIN * 2 * kv_heads > 1184 ? kv_heads : 1;
+  const AppendArgs a{static_cast<int8_t*>(kv), kv_scale, n_pages * page_size, log2_of(page_size), kv_heads, rows, heads_per_cta, k, v,
                      k_row, k_head, v_row, v_head, slot};
   // loads of four elements where every row and head starts at a multiple of four
   const bool vec = !(((uintptr_t)k | (uintptr_t)v) & (4 * es - 1)) && !((k_row | k_head | v_row | v_head) & 3);
@@ -450,18 +476,19 @@ int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t
   if (!slot || !k_out || !v_out) return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15)
     return op_error(H2C_ERR_INVALID, "%s: k_out and v_out must be 16-byte aligned", who);
-  const long long units = (long long)rows * 2 * kv_heads * (head_dim / 16);
-  const int ctas = (int)std::min<long long>((units + 255) / 256, 148 * 16);
+  const int across = std::min(256, (2 * kv_heads * (head_dim / 4) + 31) / 32 * 32);
+  const dim3 block(across, 256 / across);
+  const int ctas = std::min((rows + (int)block.y - 1) / (int)block.y, 148 * 8);
   const int8_t* c = static_cast<const int8_t*>(kv);
   cudaStream_t st = (cudaStream_t)stream;
   const int n_slots = n_pages * page_size, pl = log2_of(page_size), hl = log2_of(head_dim);
   if (type == H2C_TYPE_F32)
-    k_kv8_read<<<ctas, 256, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, units, (float*)k_out, (float*)v_out);
+    k_kv8_read<<<ctas, block, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, rows, (float*)k_out, (float*)v_out);
   else if (type == H2C_TYPE_F16)
-    k_kv8_read<<<ctas, 256, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, units, (__half*)k_out, (__half*)v_out);
+    k_kv8_read<<<ctas, block, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, rows, (__half*)k_out, (__half*)v_out);
   else
-    k_kv8_read<<<ctas, 256, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, units, (__nv_bfloat16*)k_out,
-                                     (__nv_bfloat16*)v_out);
+    k_kv8_read<<<ctas, block, 0, st>>>(c, kv_scale, n_slots, pl, kv_heads, hl, slot, rows, (__nv_bfloat16*)k_out,
+                                       (__nv_bfloat16*)v_out);
   return op_launched(who);
 }
 

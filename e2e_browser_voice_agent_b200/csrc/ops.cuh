@@ -50,6 +50,14 @@ __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Four values with |v| < 2^22, rounded to integers (halves to even), as the low bytes of their two's complements: adding 1.5 x 2^23
+// leaves the integer in the low bits of the sum. (Conversions to integers run at a quarter of the rate of additions.)
+__device__ __forceinline__ uint32_t round_bytes(float a, float b, float c, float d) {
+  const uint32_t x = __float_as_uint(__fadd_rn(a, 12582912.f)), y = __float_as_uint(__fadd_rn(b, 12582912.f)),
+                 z = __float_as_uint(__fadd_rn(c, 12582912.f)), w = __float_as_uint(__fadd_rn(d, 12582912.f));
+  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+
 // four consecutive values; VEC: the address is aligned to four of them
 template <bool VEC>
 __device__ __forceinline__ void load4(const float* p, float* v) {

@@ -348,8 +348,8 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* args, void* stream);
 /* Rows of x (element type `type`, row r at x + r * x_row elements, k values) as codes q[r][0 .. k) and scale[r]: with a the
  * row's largest magnitude, scale = a / 127 and q = round(x * min(127 / a, FLT_MAX)) (float32 operations, halves to even;
  * a row of zeros gives zeros). Rows of q start q_row bytes apart (a multiple of 16, at least k, q 16-byte aligned); the
- * bytes from k to the next multiple of 16 become 0. A row with NaN has the scale NaN, one with an infinity the scale
- * infinity, and every product with it is NaN. For weights (rows = output channels), once, and for activations that
+ * bytes from k to the next multiple of 16 become 0. A row with an infinity or NaN has the scale NaN (and codes without
+ * meaning): every product with it is NaN. For weights (rows = output channels), once, and for activations that
  * several products share. */
 int h2c_i8_quantize(int32_t type, const void* x, int64_t x_row, int32_t rows, int32_t k, void* q, int64_t q_row,
                     float* scale, void* stream);
