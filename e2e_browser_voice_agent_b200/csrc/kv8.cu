@@ -182,10 +182,13 @@ __device__ __forceinline__ float grown_scale(float a, float s0, bool finite) {
   if (s0 != 0.f && !(a > 127.5f * s0)) return s0;
   return fminf(fmaxf(fmaxf(__fdiv_rn(a, 127.f), 1.25f * s0), SCALE_MIN), SCALE_MAX);
 }
-__device__ __forceinline__ uint32_t codes_of(const float* x, float inv) {
+__device__ __forceinline__ uint32_t codes_of(const float* x, float inv, bool clip) {
   float v[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = fminf(fmaxf(__fmul_rn(x[i], inv), -127.f), 127.f);
+  for (int i = 0; i < 4; i++) {
+    v[i] = __fmul_rn(x[i], inv);
+    if (clip) v[i] = fminf(fmaxf(v[i], -127.f), 127.f);
+  }
   return round_bytes(v[0], v[1], v[2], v[3]);
 }
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
@@ -195,33 +198,71 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   return round_bytes(v[0], v[1], v[2], v[3]);
 }
 
+// Four consecutive values as they lie in memory.
+template <class T, bool VEC>
+struct Raw4 {
+  uint32_t w[sizeof(T)];
+  __device__ __forceinline__ void load(const T* p) {
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); i += 2) {
+        const uint2 x = reinterpret_cast<const uint2*>(p)[i / 2];
+        w[i] = x.x, w[i + 1] = x.y;
+      }
+    } else {
+      T v[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = p[i];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); i++) w[i] = reinterpret_cast<const uint32_t*>(v)[i];
+    }
+  }
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = to_f(reinterpret_cast<const T*>(w)[i]);
+  }
+  // Magnitudes order as their bits do, infinities and NaN above every number: 16-bit ones two at a time. merge() joins the largest
+  // so far with these; bits() makes the bits of a float32 of it.
+  __device__ __forceinline__ unsigned merge(unsigned m) const {
+    if (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); i++) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    }
+    return __vmaxu2(m, __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu));
+  }
+  static __device__ __forceinline__ unsigned bits(unsigned m) {
+    if (sizeof(T) == 4) return m;
+    const unsigned short u = (unsigned short)max(m & 0xffffu, m >> 16);
+    return __float_as_uint(to_f(*reinterpret_cast<const T*>(&u)));
+  }
+};
+
 // One run of one (K or V, head) by the threads i0 = 0 .. NT-1 of a warp (NT = 32) or of the CTA; reduce() combines the
-// largest magnitude bits over them. MAXU: units of 4 values that a thread keeps.
+// largest magnitude bits over them. MAXU: units of 4 values that a thread keeps. A thread stays in one column of four.
 template <class T, bool VEC, int HD, int NT, int MAXU, class R>
 __device__ __forceinline__ void append_run(const T* src, long long row_stride, int len, int8_t* page, int off,
                                            float* scale, int i0, R reduce) {
-  constexpr int UPR = HD / 4;  // units per row
-  const int units = len * UPR;
+  constexpr int UPR = HD / 4, RPS = NT / UPR;  // units per row, rows per step of all threads
+  static_assert(NT % UPR == 0, "a thread's column must not change");
+  const int row0 = i0 / UPR, col = (i0 % UPR) * 4;
   const float s0 = off == 0 ? 0.f : *scale;
-  float v[MAXU][4];
-#pragma unroll
-  for (int k = 0; k < MAXU; k++) {
-    const int u = i0 + k * NT;
-    if (u < units) load4<VEC>(src + (u / UPR) * row_stride + (u % UPR) * 4, v[k]);
-  }
-  unsigned m = 0;  // magnitudes order as their bits do, infinities and NaN above every number
+  const T* p = src + row0 * row_stride + col;
+  const long long step = RPS * row_stride;
+  Raw4<T, VEC> v[MAXU];
 #pragma unroll
   for (int k = 0; k < MAXU; k++)
-    if (i0 + k * NT < units)
+    if (row0 + k * RPS < len) v[k].load(p + k * step);
+  unsigned m = 0;
 #pragma unroll
-      for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(v[k][j]) & 0x7fffffffu);
-  for (int u = i0 + MAXU * NT; u < units; u += NT) {  // (what does not fit the registers is read again below)
-    float x[4];
-    load4<VEC>(src + (u / UPR) * row_stride + (u % UPR) * 4, x);
-#pragma unroll
-    for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+  for (int k = 0; k < MAXU; k++)
+    if (row0 + k * RPS < len) m = v[k].merge(m);
+  for (int r = row0 + MAXU * RPS; r < len; r += RPS) {  // (what does not fit the registers is read again below)
+    Raw4<T, VEC> x;
+    x.load(src + r * row_stride + col);
+    m = x.merge(m);
   }
-  m = reduce(m);
+  m = reduce(Raw4<T, VEC>::bits(m));
   const bool finite = m < 0x7f800000u;
   const float s = grown_scale(__uint_as_float(m), s0, finite);
   const bool lost = s != s;
@@ -233,23 +274,31 @@ __device__ __forceinline__ void append_run(const T* src, long long row_stride, i
       *w = rescale4(*w, ratio);
     }
   }
-  uint32_t* dst = reinterpret_cast<uint32_t*>(page + (size_t)off * HD);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(page + (size_t)off * HD) + i0;
+  auto put = [&](bool clip) {
 #pragma unroll
-  for (int k = 0; k < MAXU; k++) {
-    const int u = i0 + k * NT;
-    if (u < units)
-      dst[u] = lost ? 0u : codes_of(v[k], inv);
-  }
-  for (int u = i0 + MAXU * NT; u < units; u += NT) {
-    float x[4];
-    load4<VEC>(src + (u / UPR) * row_stride + (u % UPR) * 4, x);
-    dst[u] = lost ? 0u : codes_of(x, inv);
-  }
+    for (int k = 0; k < MAXU; k++)
+      if (row0 + k * RPS < len) {
+        float x[4];
+        v[k].get(x);
+        dst[k * NT] = lost ? 0u : codes_of(x, inv, clip);
+      }
+    for (int r = row0 + MAXU * RPS; r < len; r += RPS) {
+      Raw4<T, VEC> y;
+      float x[4];
+      y.load(src + r * row_stride + col);
+      y.get(x);
+      dst[(r - row0) * UPR] = lost ? 0u : codes_of(x, inv, clip);
+    }
+  };
+  // (codes above 127 arise only where the largest magnitude is above 127 steps, and the scale did not grow for it)
+  if (!lost && __fmul_rn(__uint_as_float(m), inv) > 127.25f) put(true);
+  else put(false);
   if (i0 == 0 && s != s0) *scale = s;  // (also when s is NaN; every thread has read s0: reduce() synchronises them)
 }
 
 template <class T, bool VEC, int HD>
-__global__ void __launch_bounds__(APP_THREADS) k_kv8_append(const AppendArgs a) {
+__global__ void __launch_bounds__(APP_THREADS, VEC && sizeof(T) == 2 ? 4 : 2) k_kv8_append(const AppendArgs a) {
   __shared__ int run_row[APP_WIN], run_len[APP_WIN];
   __shared__ int slots[APP_WIN + 128];  // of the window and of the rows that its last run may reach
   __shared__ int n_runs;

@@ -2,7 +2,7 @@
 //
 // Many queries (k_att_prompt): kv8_prompt.cuh. Few queries (k_att_rows): a CTA takes 8 rows (query, head of the kv head's group) of one request and kv head and one
 // span of its keys; 4 warps take blocks of 16 keys in turn, each with its own running maximum, sum and output, joined at
-// the end; spans are joined by a kernel of their own.
+// the end; up to 8 spans are joined by their cluster, more by a second kernel.
 // * Tensor cores (mma.sync m16n8k16, float16 in, float32 sums): codes are integers up to 127 and exact in float16. The
 //   16 rows of an operand tile hold 8 rows twice: a float16 term in rows 0-7 and the remainder in rows 8-15, for the
 //   queries (scaled by a power of two per row) and for the softmax weights, so the products carry 22 bits, whatever the
@@ -20,12 +20,13 @@
 namespace h2 {
 namespace {
 
-constexpr int RW_WARPS = 4, RW_ROWS = 8, RW_BLK = 16, RW_STAGES = 4;
+constexpr int RW_WARPS = 4, RW_ROWS = 8, RW_BLK = 16, RW_STAGES = 4, RW_CLUSTER = 8;
 struct RowArgs {
   AttArgs a;
   int splits, blocks, tiles;  // spans per row tile, blocks per span, row tiles per (request, kv head)
   int max_rows;               // requests of more rows are k_att_prompt's
-  float* part;                // [request][kv head][tile][span][8][HD] sums, then the same without HD for m and l
+  int cluster;                // the spans of a row tile are a cluster, which joins them itself
+  float* part;                // (without clusters) [request][kv head][tile][span][8][HD] sums, then the same without HD for m and l
   float2* ml;
 };
 
@@ -45,7 +46,7 @@ template <int HD>
 struct RowSmem {
   static constexpr int STAGE = RW_BLK * HD * 2;                       // a warp's block: K, then V
   static constexpr int RING = RW_WARPS * RW_STAGES * STAGE;
-  static constexpr int JOIN = RW_WARPS * RW_ROWS * (HD + 2) * 4;      // (reuses the ring)
+  static constexpr int JOIN = (RW_WARPS + 1) * RW_ROWS * (HD + 2) * 4;  // (reuses the ring) the warps' parts, then the CTA's
   static constexpr int SCALES = RW_WARPS * RW_STAGES * 8;
   static constexpr int BYTES = (RING > JOIN ? RING : JOIN) + SCALES;
 };
@@ -68,8 +69,10 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   int lo, hi;
   key_range(a, R, n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
   const Span sp = spans_of(lo, hi, ra.splits, ra.blocks, RW_BLK);
-  if (split >= sp.used) return;
-  const int b_begin = split * ra.blocks, b_end = split == sp.used - 1 ? sp.n_blocks : b_begin + ra.blocks;
+  if (split >= sp.used && !ra.cluster) return;
+  // (in a cluster a span without keys has its part in the join)
+  const int b_begin = split * ra.blocks;
+  const int b_end = split >= sp.used ? b_begin : split == sp.used - 1 ? sp.n_blocks : b_begin + ra.blocks;
 
   // ---- this lane's row: query dimensions 64j + 16c .. +15, as float16 terms
   const int row = row0 + g;
@@ -275,7 +278,6 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   __syncthreads();
   constexpr int TPR = RW_WARPS * 32 / RW_ROWS;  // threads per row
   const int jr = threadIdx.x / TPR, jt = threadIdx.x % TPR, orow = row0 + jr;
-  if (orow >= n_rows) return;
   float mm = -INFINITY, ll = 0.f, fw[RW_WARPS];
 #pragma unroll
   for (int w = 0; w < RW_WARPS; w++) mm = fmaxf(mm, jm[w * RW_ROWS + jr]);
@@ -286,11 +288,12 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
     ll += fw[w] * jl[w * RW_ROWS + jr];
   }
   const size_t unit = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits + split;
-  const bool whole = sp.used == 1;
+  const bool whole = sp.used == 1 && !ra.cluster;
   const float inv = whole && ll != 0.f ? 1.f / ll : 1.f;
   int oh;
   const int otok = token_of(a, orow, &oh);
   oh += head * a.group;
+  float* cs = jl + RW_WARPS * RW_ROWS;  // (cluster) this CTA's rows: sums, then (m, l) pairs
 #pragma unroll
   for (int k = 0; k < HD / 4 / TPR; k++) {
     const int d = (jt + k * TPR) * 4;
@@ -300,7 +303,10 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
       const float4 x = *reinterpret_cast<const float4*>(js + (w * RW_ROWS + jr) * HD + d);
       v[0] += fw[w] * x.x; v[1] += fw[w] * x.y; v[2] += fw[w] * x.z; v[3] += fw[w] * x.w;
     }
-    if (whole) {
+    if (ra.cluster) {
+      *reinterpret_cast<float4*>(cs + jr * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (orow >= n_rows) {
+    } else if (whole) {
 #pragma unroll
       for (int i = 0; i < 4; i++) v[i] *= inv;
       store4(static_cast<T*>(a.out) + (long long)(R.first + otok) * a.out_row + oh * a.out_head + d, v, a.out_vec);
@@ -309,11 +315,61 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
     }
   }
   if (jt == 0) {
-    if (!whole) ra.ml[unit * RW_ROWS + jr] = make_float2(mm, ll);
+    if (ra.cluster) reinterpret_cast<float2*>(cs + RW_ROWS * HD)[jr] = make_float2(mm, ll);
+    else if (orow >= n_rows) {
+    } else if (!whole) ra.ml[unit * RW_ROWS + jr] = make_float2(mm, ll);
     else if (a.lse)
       a.lse[(size_t)(R.first + otok) * a.heads + oh] =
           ll == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(ll) + mm - P_SHIFT);
   }
+  if (!ra.cluster) return;
+
+  // ---- the cluster's spans, each CTA a share of the rows' pieces of four dimensions, through distributed shared memory
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const uint32_t c_at = (uint32_t)__cvta_generic_to_shared(cs);
+  for (int u = split * RW_WARPS * 32 + threadIdx.x; u < RW_ROWS * HD / 4; u += ra.splits * RW_WARPS * 32) {
+    const int cr = u / (HD / 4), d = (u % (HD / 4)) * 4, row_c = row0 + cr;
+    if (row_c >= n_rows) break;
+    float2 ml[RW_CLUSTER];
+    float4 x[RW_CLUSTER];
+#pragma unroll
+    for (int k = 0; k < RW_CLUSTER; k++)
+      if (k < ra.splits) {
+        uint32_t at;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(c_at), "r"(k));
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(ml[k].x), "=f"(ml[k].y)
+                     : "r"(at + RW_ROWS * HD * 4 + cr * 8)
+                     : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(x[k].x), "=f"(x[k].y), "=f"(x[k].z), "=f"(x[k].w)
+                     : "r"(at + (cr * HD + d) * 4)
+                     : "memory");
+      }
+    float m = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < RW_CLUSTER; k++)
+      if (k < ra.splits) m = fmaxf(m, ml[k].x);
+#pragma unroll
+    for (int k = 0; k < RW_CLUSTER; k++)
+      if (k < ra.splits) {
+        const float f = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - m);
+        l += f * ml[k].y;
+        v[0] += f * x[k].x; v[1] += f * x[k].y; v[2] += f * x[k].z; v[3] += f * x[k].w;
+      }
+    const float c_inv = l != 0.f ? 1.f / l : 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] *= c_inv;
+    int ch;
+    const int ctok = token_of(a, row_c, &ch);
+    ch += head * a.group;
+    store4(static_cast<T*>(a.out) + (long long)(R.first + ctok) * a.out_row + ch * a.out_head + d, v, a.out_vec);
+    if (d == 0 && a.lse)
+      a.lse[(size_t)(R.first + ctok) * a.heads + ch] = l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
+  }
+  __syncwarp();
+  // (the others may still read this CTA's part)
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Joins the spans of one row: the weights of span s relative to the common maximum are 2^(m_s - m). Span s of the row has
@@ -404,7 +460,7 @@ __global__ void __launch_bounds__(256) k_att_join_prompt(const PromptArgs pa) {
 // the host knows only max_q, and launches the one kernel or both. (A single request takes the one its max_q asks for.)
 constexpr int RW_MAX = 64;
 struct WorkPlan {
-  bool rows, prompt;
+  bool rows, prompt, cluster;
   int max_rows, splits, blocks, tiles;         // k_att_rows
   int min_rows, p_splits, p_blocks, p_tiles;   // k_att_prompt
   size_t units, p_units;                       // row tiles x spans in the workspace
@@ -420,14 +476,18 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g) {
   if (p.rows) {
     p.max_rows = p.prompt ? RW_MAX : INT_MAX;
     p.tiles = (int)((std::min<long long>(most_rows, p.max_rows) + RW_ROWS - 1) / RW_ROWS);
-    // spans: enough CTAs for two waves of three per SM, but no span under 256 keys (4 blocks per warp), below which its
-    // start-up costs more than it shares out
-    const long long groups = (long long)g->n_req * g->kv_heads * p.tiles;
+    // spans: enough CTAs for two waves of three per SM. Up to 8 are one cluster, whose join costs little: spans of 128 keys (2
+    // blocks per warp) or more. More of them, for few rows over long histories, leave their parts in the workspace for a
+    // second kernel: spans of 256 keys or more, below which a span's start-up costs more than it shares out
+    const long long groups = (long long)g->n_req * g->kv_heads * p.tiles, want = (888 + groups - 1) / groups;
     const int n_blocks = (int)((keys + RW_BLK - 1) / RW_BLK) + (g->window > 0 ? 1 : 0);
-    p.splits = (int)std::max(1LL, std::min<long long>((888 + groups - 1) / groups, n_blocks / 16));
+    p.cluster = groups * RW_CLUSTER <= 444 && n_blocks / 16 <= RW_CLUSTER;
+    p.splits = (int)std::max(1LL, p.cluster ? std::min<long long>({(long long)RW_CLUSTER, want, (n_blocks + 7LL) / 8})
+                                            : std::min<long long>(want, n_blocks / 16));
     p.blocks = std::max(RW_WARPS, ((n_blocks + p.splits - 1) / p.splits + RW_WARPS - 1) / RW_WARPS * RW_WARPS);
     p.splits = std::max(1, (n_blocks + p.blocks - 1) / p.blocks);
-    p.units = p.splits > 1 ? (size_t)groups * p.splits : 0;
+    p.cluster = p.cluster && p.splits > 1;
+    p.units = p.splits > 1 && !p.cluster ? (size_t)groups * p.splits : 0;
   }
   if (p.prompt) {
     p.min_rows = p.rows ? RW_MAX + 1 : 0;
@@ -474,10 +534,23 @@ int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaS
           return cudaFuncSetAttribute(k_att_rows<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         }))
       return rc;
-    const RowArgs ra{a, p.splits, p.blocks, p.tiles, p.max_rows, part, ml};
-    k_att_rows<T, HD><<<dim3((unsigned)p.splits * a.kv_heads * p.tiles, a.n_req), RW_WARPS * 32, smem, st>>>(ra);
-    if (int rc = op_launched(who)) return rc;
-    if (p.splits > 1) {
+    const RowArgs ra{a, p.splits, p.blocks, p.tiles, p.max_rows, p.cluster, part, ml};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.splits * a.kv_heads * p.tiles, a.n_req);
+    cfg.blockDim = dim3(RW_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)p.splits, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = p.cluster;
+    const cudaError_t c = cudaLaunchKernelEx(&cfg, k_att_rows<T, HD>, ra);
+    if (c != cudaSuccess) {
+      cudaGetLastError();
+      return op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
+    }
+    if (p.splits > 1 && !p.cluster) {
       k_att_join_rows<T, HD><<<dim3((unsigned)RW_ROWS * a.kv_heads * p.tiles, a.n_req), 256, 0, st>>>(ra);
       return op_launched(who);
     }
