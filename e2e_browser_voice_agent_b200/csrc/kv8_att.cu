@@ -47,7 +47,7 @@ struct RowSmem {
   static constexpr int STAGE = RW_BLK * HD * 2;                       // a warp's block: K, then V
   static constexpr int RING = RW_WARPS * RW_STAGES * STAGE;
   static constexpr int JOIN = (RW_WARPS + 1) * RW_ROWS * (HD + 2) * 4;  // (reuses the ring) the warps' parts, then the CTA's
-  static constexpr int SCALES = RW_WARPS * RW_STAGES * 8;
+  static constexpr int SCALES = RW_WARPS * 64 * 16;                   // KeyInfo of 64 blocks per warp
   static constexpr int BYTES = (RING > JOIN ? RING : JOIN) + SCALES;
 };
 
@@ -131,41 +131,45 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   // ---- the warp's blocks: b_begin + warp + 4 it
   const int n_it = max(0, (b_end - b_begin - warp + RW_WARPS - 1) / RW_WARPS);
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * RW_STAGES * S::STAGE;
-  float2* scales = reinterpret_cast<float2*>(sm + S::BYTES - S::SCALES) + warp * RW_STAGES;
+  KeyInfo* info = reinterpret_cast<KeyInfo*>(sm + S::BYTES - S::SCALES) + warp * 64;
   const int P = 1 << a.page_log;
   const size_t head_bytes = (size_t)P * HD;
-  int i_page = 0;
-  float i_sk = 0.f, i_sv = 0.f;
+  const size_t v_off = a.kv_heads * head_bytes;
+  const int8_t* k_lane = a.kv + head * head_bytes + g * HD + 16 * c;              // this lane's pieces of a block at offset 0
+  const int8_t* v_lane = a.kv + head * head_bytes + v_off + 2 * c * HD + VB * g;
+  const uint32_t k_dst = ring + lane * 16, v_dst = ring + RW_BLK * HD + lane * VB;
+  unsigned long long i_off = 0;
   auto issue = [&](int it) {
     if (it < n_it) {
-      if ((it & 31) == 0) {  // pages and scales of the next 32 blocks, one per lane
+      if ((it & 31) == 0) {  // places and scales of the next 32 blocks, one per lane
         const int b = b_begin + warp + RW_WARPS * (it + lane);
         if (b < b_end) {
-          int pg = a.table[(size_t)r * a.table_cols + ((sp.first + b * RW_BLK) >> a.page_log)];
-          i_page = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
-          const float* s = a.kv_scale + (size_t)i_page * 2 * a.kv_heads + head;
-          i_sk = s[0];
-          i_sv = s[a.kv_heads];
+          const int key = sp.first + b * RW_BLK;
+          int pg = a.table[(size_t)r * a.table_cols + (key >> a.page_log)];
+          pg = (unsigned)pg < (unsigned)a.n_pages ? pg : 0;
+          i_off = (size_t)pg * 2 * v_off + (key & (P - 1)) * HD;
+          const float* s = a.kv_scale + (size_t)pg * 2 * a.kv_heads + head;
+          KeyInfo ki;
+          ki.k = s[0];
+          split_scale(s[a.kv_heads], &ki.e, &ki.mant, &ki.inv);
+          info[(it + lane) & 63] = ki;  // (the block that was there 64 turns before is done with)
         }
       }
-      const int page = __shfl_sync(0xffffffffu, i_page, it & 31);
-      const float sk = __shfl_sync(0xffffffffu, i_sk, it & 31), sv = __shfl_sync(0xffffffffu, i_sv, it & 31);
-      const int stage = it % RW_STAGES, b = b_begin + warp + RW_WARPS * it;
-      if (lane == 0) scales[stage] = make_float2(sk, sv);
-      const int8_t* kb = a.kv + ((size_t)page * 2 * a.kv_heads + head) * head_bytes + ((sp.first + b * RW_BLK) & (P - 1)) * HD;
-      const int8_t* vb = kb + a.kv_heads * head_bytes;
-      const uint32_t dst = ring + stage * S::STAGE + lane * 16;
+      const size_t off = __shfl_sync(0xffffffffu, i_off, it & 31);
+      const uint32_t st = (it % RW_STAGES) * S::STAGE;
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int j = 0; j < KC; j++) copy_async<16>(dst + (t * KC + j) * 512, kb + (8 * t + g) * HD + 64 * j + 16 * c);
-      const uint32_t vd = ring + stage * S::STAGE + RW_BLK * HD + lane * VB;
+        for (int j = 0; j < KC; j++) copy_async<16>(k_dst + st + (t * KC + j) * 512, k_lane + off + 8 * t * HD + 64 * j);
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        copy_async<VB>(vd + i * 32 * VB, vb + (2 * c + (i & 1) + 8 * (i >> 1)) * HD + VB * g);
+        copy_async<VB>(v_dst + st + i * 32 * VB, v_lane + off + ((i & 1) + 8 * (i >> 1)) * HD);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // blocks that every row of the tile sees whole need no masks
+  const int clear_from = __reduce_max_sync(0xffffffffu, live ? first_key : 0);
+  const int clear_to = __reduce_min_sync(0xffffffffu, live ? pos : INT_MAX);
 #pragma unroll
   for (int it = 0; it < RW_STAGES - 1; it++) issue(it);
 
@@ -175,13 +179,11 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
     const int stage = it % RW_STAGES;
     const uint8_t* kst = sm + warp * RW_STAGES * S::STAGE + stage * S::STAGE + lane * 16;
     const uint8_t* vst = sm + warp * RW_STAGES * S::STAGE + stage * S::STAGE + RW_BLK * HD + lane * VB;
-    const float2 sc = scales[stage];
-    const int key0 = sp.first + (b_begin + warp + RW_WARPS * it) * RW_BLK + 2 * c;
+    const KeyInfo ki = info[it & 63];
+    const int blk0 = sp.first + (b_begin + warp + RW_WARPS * it) * RW_BLK, key0 = blk0 + 2 * c;
     // scores of 8 rows x 16 keys: this lane has keys key0, key0 + 1 (tile 0), key0 + 8, key0 + 9 (tile 1) of its row
     float y[4];
-    float e_v, mant, inv_pow;
-    split_scale(sc.y, &e_v, &mant, &inv_pow);
-    const float f = q_scale * sc.x;
+    const float f = q_scale * ki.k;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
       float d[4] = {0.f, 0.f, 0.f, 0.f};
@@ -196,17 +198,20 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
                    half2_of(__byte_perm(u, 0x64646464u, 0x4140)), half2_of(__byte_perm(u, 0x64646464u, 0x4342)));
         }
       }
+      y[2 * t] = fmaf(d[0] + d[2], f, ki.e);
+      y[2 * t + 1] = fmaf(d[1] + d[3], f, ki.e);
+    }
+    if (blk0 < clear_from || blk0 + RW_BLK - 1 > clear_to) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int key = key0 + 8 * t + i;
-        const float x = (d[i] + d[i + 2]) * f;
-        y[2 * t + i] = live && key <= pos && key >= first_key ? x + e_v : -INFINITY;
+      for (int i = 0; i < 4; i++) {
+        const int key = key0 + 8 * (i >> 1) + (i & 1);
+        if (!(live && key <= pos && key >= first_key)) y[i] = -INFINITY;
       }
     }
     float mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     if (__any_sync(0xffffffffu, mx > m_run + M_SLACK)) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float m_new = mx > m_run + M_SLACK ? mx : m_run;  // (a row's result does not depend on its neighbours)
       const float f_old = m_new == m_run ? 1.f : m_run == -INFINITY ? 0.f : exp2_fast(m_run - m_new);
       m_run = m_new;
@@ -221,8 +226,8 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const float w = exp2_fast(y[i] - m_use);
-      l_run += w * inv_pow;
-      p[i] = w * mant;
+      l_run = fmaf(w, ki.inv, l_run);
+      p[i] = w * ki.mant;
     }
     const uint32_t a0 = pack_half2(p[0], p[1]), a2 = pack_half2(p[2], p[3]);
     {

@@ -77,6 +77,11 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// What the softmax needs of 16 keys: the scale of K, the term of V's scale in the exponent, the factor that this leaves, and what
+// turns a weight back into the softmax's.
+struct __align__(16) KeyInfo {
+  float k, e, mant, inv;
+};
 // The scale of V is split as mantissa * 2^e: the exponent joins the score before the running maximum is taken, so that the
 // weights that enter the tensor cores never leave float16's range however the pages' scales differ; the mantissa
 // multiplies the weight. e is bounded so that 2^-e stays a normal number.

@@ -173,12 +173,6 @@ struct PromptCfg {
   static_assert(Q_AREA % 1024 == 0 && SMEM <= 226 * 1024, "shared memory budget");
 };
 
-// what the softmax needs of 16 keys: scale of K, the term of V's scale in the exponent, its factor (TERMS = 2), and what
-// turns a weight back into the softmax's
-struct __align__(16) KeyInfo {
-  float k, e, mant, inv;
-};
-
 // The weights of one tile of keys for one row: scores s (products of codes) to p = 2^(s f + e - m), packed as float16 (and the
 // remainders when two terms are kept); the sum of the softmax's weights is added to l. base = P_SHIFT - m.
 template <int TERMS, bool EDGE>
