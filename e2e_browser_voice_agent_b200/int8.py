@@ -82,12 +82,10 @@ def matmul(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Option
         if y_type is None:
             raise TypeError(f"out: float32, float16 or bfloat16 is wanted, not {out.dtype}")
         py, y_row = _matrix("out", out, index), out.stride(0)
-    work, need = None, 0
-    if x_scale is None and m:
-        # (h2c_i8_matmul_workspace: the codes, then their scales, each rounded up to 256 bytes)
-        need = (m * ((k + 15) // 16 * 16) + 255) // 256 * 256 + (4 * m + 255) // 256 * 256
-        work = torch.empty(need, dtype=torch.uint8, device=x.device)
-    _call(index, _lib.load().h2c_i8_matmul, x_type, px, x.stride(0), ps, pw, w.stride(0),
+    L = _lib.load()
+    need = L.h2c_i8_matmul_workspace(x_type, m, k)
+    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _call(index, L.h2c_i8_matmul, x_type, px, x.stride(0), ps, pw, w.stride(0),
           _want("w_scale", w_scale, torch.float32, index, (n,)), m, n, k, y_type, py, y_row,
           None if bias is None else _want("bias", bias, torch.float32, index, (n,)), None if work is None else work.data_ptr(), need)
     return out
