@@ -617,8 +617,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         const float4 x = *reinterpret_cast<const float4*>(&info[j / PR_INFO & 1][j % PR_INFO][g]);
         in[g] = {x.x * f_row, x.y, x.z, x.w};
       }
+      // (no way out of the loop when a wait expires: the other row tile's warp counts the turns; waits are short then)
       if (!ready && !wait_phase_warp(&s_full[q][j & 1], (j >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
-      if (!ok) break;
       tc_fence_after();
       float s[PR_KEYS];
       const uint32_t ts = tl + (j & 1) * PR_KEYS;
@@ -652,8 +652,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       }
       const float base = P_SHIFT - (m_run == -INFINITY ? 0.f : m_run);
       uint32_t p[PR_KEYS / 2], rest[C::TERMS == 2 ? PR_KEYS / 2 : 1];
+      // The two row tiles take turns at the exponentials (the two warps of a scheduler, which share its unit for them): each has
+      // the other's turn for everything else. Both at once, they also do everything else at once.
+      if (n_q_tiles == 2 && (q || j)) asm volatile("bar.sync %0, 64;" ::"r"(3 + 4 * q + w4) : "memory");
       if (edge) weights<C::TERMS, true>(s, in, base, key0, first_key, pos, p, rest, &l_run);
       else weights<C::TERMS, false>(s, in, base, key0, first_key, pos, p, rest, &l_run);
+      if (n_q_tiles == 2 && (!q || j + 1 < n_tiles)) asm volatile("bar.arrive %0, 64;" ::"r"(7 - 4 * q + w4) : "memory");
       tmem_st32(ts, p);
       if (C::TERMS == 2) tmem_st32(ts + 32, rest);
       // (the next scores are most often there: their test is under way while the stores are)
