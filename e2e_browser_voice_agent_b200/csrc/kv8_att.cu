@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
   constexpr int NT = HD / 8;    // output tiles of 8 dimensions
   extern __shared__ __align__(16) uint8_t sm[];
   const AttArgs& a = ra.a;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the joining kernel, which waits for this one's end)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x % ra.splits, th = blockIdx.x / ra.splits, head = th % a.kv_heads, tile = th / a.kv_heads;
   const int r = blockIdx.y;
@@ -426,6 +427,7 @@ __device__ __forceinline__ void join_row(const AttArgs& a, const float* part, si
 template <class T, int HD>
 __global__ void __launch_bounds__(256) k_att_join_rows(const RowArgs ra) {
   const AttArgs& a = ra.a;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int jr = blockIdx.x % RW_ROWS, th = blockIdx.x / RW_ROWS, head = th % a.kv_heads, tile = th / a.kv_heads;
   const int r = blockIdx.y;
   int n_all;
@@ -444,6 +446,7 @@ __global__ void __launch_bounds__(256) k_att_join_rows(const RowArgs ra) {
 template <class T, int HD>
 __global__ void __launch_bounds__(256) k_att_join_prompt(const PromptArgs pa) {
   const AttArgs& a = pa.a;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int jr = blockIdx.x % PR_ROWS, th = blockIdx.x / PR_ROWS, head = th % a.kv_heads, idx = th / a.kv_heads;
   const TileAt at = tile_at(pa, idx);
   if (at.r < 0) return;
@@ -510,6 +513,25 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g) {
   return p;
 }
 
+// A joining kernel (256 threads a CTA), launched while the kernel before it still runs (programmatic dependent launch): it waits
+// for that one's end itself.
+template <class A>
+int launch_after(const char* who, void (*kernel)(A), dim3 grid, const A& args, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t c = cudaLaunchKernelEx(&cfg, kernel, args);
+  if (c == cudaSuccess) return H2C_OK;
+  cudaGetLastError();
+  return op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
+}
+
 template <class T, int HD>
 int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaStream_t st) {
   float* part = static_cast<float*>(workspace);
@@ -528,8 +550,7 @@ int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaS
     k_att_prompt<T, HD><<<(unsigned)p.p_tiles * p.p_splits * a.kv_heads, PR_THREADS, smem, st>>>(pa);
     if (int rc = op_launched(who)) return rc;
     if (p.p_splits > 1) {
-      k_att_join_prompt<T, HD><<<(unsigned)p.p_tiles * a.kv_heads * PR_ROWS, 256, 0, st>>>(pa);
-      if (int rc = op_launched(who)) return rc;
+      if (int rc = launch_after(who, k_att_join_prompt<T, HD>, dim3((unsigned)p.p_tiles * a.kv_heads * PR_ROWS), pa, st)) return rc;
     }
   }
   if (p.rows) {
@@ -556,8 +577,7 @@ int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaS
       return op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
     }
     if (p.splits > 1 && !p.cluster) {
-      k_att_join_rows<T, HD><<<dim3((unsigned)RW_ROWS * a.kv_heads * p.tiles, a.n_req), 256, 0, st>>>(ra);
-      return op_launched(who);
+      return launch_after(who, k_att_join_rows<T, HD>, dim3((unsigned)RW_ROWS * a.kv_heads * p.tiles, a.n_req), ra, st);
     }
   }
   return H2C_OK;

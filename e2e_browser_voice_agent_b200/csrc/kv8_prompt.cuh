@@ -392,6 +392,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s;
   const AttArgs& a = pa.a;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the joining kernel, which waits for this one's end)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x % pa.splits, head = (blockIdx.x / pa.splits) % a.kv_heads;
   // the last tiles of a causal prompt have the most keys and go first
