@@ -379,56 +379,78 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
 }
 
 // Joins the spans of one row: the weights of span s relative to the common maximum are 2^(m_s - m). Span s of the row has
-// its sums at part + s * part_step and its (m, l) at ml + s * ml_step.
+// its sums at part + s * part_step and its (m, l) at ml + s * ml_step. By a warp for few spans (8 rows a CTA), by 8 warps for many,
+// each taking every 8th span: `n_warps`, `w` the warp's turn; the order of the additions goes by the spans' number alone.
+constexpr int JOIN_WARPS = 8, JOIN_WARP_SPANS = 12;
 template <class T, int HD>
 __device__ __forceinline__ void join_row(const AttArgs& a, const float* part, size_t part_step, const float2* ml, size_t ml_step,
-                                         int used, int tok, int hq) {
-  constexpr int TPR = HD / 4, LANES = 256 / TPR;  // threads for a row's dimensions, spans in flight
-  const int d = (threadIdx.x % TPR) * 4, s0 = threadIdx.x / TPR;
-  __shared__ float red[8];
-  __shared__ float acc[LANES][HD + 1];
+                                         int used, int tok, int hq, int w, int n_warps) {
+  constexpr int V = HD / 32;  // dimensions per lane
+  __shared__ float acc[JOIN_WARPS][HD], acc_l[JOIN_WARPS];
+  const int lane = threadIdx.x & 31;
   float m = -INFINITY;
-  for (int s = threadIdx.x; s < used; s += 256) m = fmaxf(m, ml[s * ml_step].x);
+  for (int s = lane; s < used; s += 32) m = fmaxf(m, ml[s * ml_step].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-  __syncthreads();
+  float v[V], l = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; w++) m = fmaxf(m, red[w]);
-  float v[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  for (int s = s0; s < used; s += LANES) {
+  for (int i = 0; i < V; i++) v[i] = 0.f;
+#pragma unroll 4
+  for (int s = w; s < used; s += n_warps) {
     const float2 x = ml[s * ml_step];
-    const float4 o = *reinterpret_cast<const float4*>(part + s * part_step + d);
+    float o[V];
+    if (V == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(part + s * part_step + V * lane);
+    else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(part + s * part_step + V * lane);
     const float f = x.x == -INFINITY ? 0.f : exp2_fast(x.x - m);
     l += f * x.y;
-    v[0] += f * o.x; v[1] += f * o.y; v[2] += f * o.z; v[3] += f * o.w;
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] += f * o[i];
   }
+  if (n_warps > 1) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) acc[s0][d + i] = v[i];
-  if (d == 0) acc[s0][HD] = l;
-  __syncthreads();
-  if (threadIdx.x >= TPR) return;
-  l = 0.f;
-  v[0] = v[1] = v[2] = v[3] = 0.f;
+    for (int i = 0; i < V; i++) acc[w][V * lane + i] = v[i];
+    if (lane == 0) acc_l[w] = l;
+    __syncthreads();
+    if (w) return;
+    for (int k = 1; k < n_warps; k++) {
+      l += acc_l[k];
 #pragma unroll
-  for (int s = 0; s < LANES; s++) {
-    l += acc[s][HD];
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] += acc[s][d + i];
+      for (int i = 0; i < V; i++) v[i] += acc[k][V * lane + i];
+    }
   }
   const float inv = l != 0.f ? 1.f / l : 1.f;
+  T* dst = static_cast<T*>(a.out) + (long long)tok * a.out_row + hq * a.out_head + V * lane;
 #pragma unroll
-  for (int i = 0; i < 4; i++) v[i] *= inv;
-  store4(static_cast<T*>(a.out) + (long long)tok * a.out_row + hq * a.out_head + d, v, a.out_vec);
-  if (d == 0 && a.lse)
+  for (int i = 0; i < V; i++) v[i] *= inv;
+  if (V == 4) {
+    store4(dst, v, a.out_vec);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) dst[i] = from_f<T>(v[i]);
+  }
+  if (lane == 0 && a.lse)
     a.lse[(size_t)tok * a.heads + hq] = l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
 }
 
+// Row `i` of the launch for this warp, its turn and the warps that share the row.
+struct JoinTurn {
+  int i, w, n;
+};
+__device__ __forceinline__ JoinTurn join_turn(int splits) {
+  const int warp = threadIdx.x >> 5;
+  if (splits <= JOIN_WARP_SPANS) return {(int)blockIdx.x * JOIN_WARPS + warp, 0, 1};
+  return {(int)blockIdx.x, warp, JOIN_WARPS};
+}
+inline unsigned join_ctas(long long rows, int splits) {
+  return (unsigned)(splits <= JOIN_WARP_SPANS ? (rows + JOIN_WARPS - 1) / JOIN_WARPS : rows);
+}
+
 template <class T, int HD>
-__global__ void __launch_bounds__(256) k_att_join_rows(const RowArgs ra) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_rows(const RowArgs ra) {
   const AttArgs& a = ra.a;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int jr = blockIdx.x % RW_ROWS, th = blockIdx.x / RW_ROWS, head = th % a.kv_heads, tile = th / a.kv_heads;
+  const JoinTurn t = join_turn(ra.splits);
+  const int jr = t.i % RW_ROWS, th = t.i / RW_ROWS, head = th % a.kv_heads, tile = th / a.kv_heads;
   const int r = blockIdx.y;
   int n_all;
   const Request R = request_of(a, r, &n_all);
@@ -439,15 +461,19 @@ __global__ void __launch_bounds__(256) k_att_join_rows(const RowArgs ra) {
   const Span sp = spans_of(lo, hi, ra.splits, ra.blocks, RW_BLK);
   if (sp.used == 1) return;  // (written by its only span)
   const size_t at = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits * RW_ROWS + jr;
-  join_row<T, HD>(a, ra.part + at * HD, (size_t)RW_ROWS * HD, ra.ml + at, RW_ROWS, sp.used, R.first + row / a.group,
-                  head * a.group + row % a.group);
+  int hq;
+  const int tok = token_of(a, row, &hq);
+  join_row<T, HD>(a, ra.part + at * HD, (size_t)RW_ROWS * HD, ra.ml + at, RW_ROWS, sp.used, R.first + tok, head * a.group + hq,
+                  t.w, t.n);
 }
 
 template <class T, int HD>
-__global__ void __launch_bounds__(256) k_att_join_prompt(const PromptArgs pa) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_prompt(const PromptArgs pa) {
   const AttArgs& a = pa.a;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int jr = blockIdx.x % PR_ROWS, th = blockIdx.x / PR_ROWS, head = th % a.kv_heads, idx = th / a.kv_heads;
+  const JoinTurn t = join_turn(pa.splits);
+  const int jr = t.i % PR_ROWS, th = t.i / PR_ROWS, head = th % a.kv_heads, idx = th / a.kv_heads;
+  if (idx >= pa.tiles) return;
   const TileAt at = tile_at(pa, idx);
   if (at.r < 0) return;
   const Request R = at.R;
@@ -458,8 +484,10 @@ __global__ void __launch_bounds__(256) k_att_join_prompt(const PromptArgs pa) {
   const Span sp = spans_of(lo, hi, pa.splits, pa.blocks, PR_KEYS);
   if (sp.used == 1) return;
   const size_t u = ((size_t)idx * a.kv_heads + head) * pa.splits * PR_ROWS + jr;
-  join_row<T, HD>(a, pa.part + u * HD, (size_t)PR_ROWS * HD, pa.ml + u, PR_ROWS, sp.used, R.first + row / a.group,
-                  head * a.group + row % a.group);
+  int hq;
+  const int tok = token_of(a, row, &hq);
+  join_row<T, HD>(a, pa.part + u * HD, (size_t)PR_ROWS * HD, pa.ml + u, PR_ROWS, sp.used, R.first + tok, head * a.group + hq, t.w,
+                  t.n);
 }
 
 // ---------------------------------------------------------------- host
@@ -513,13 +541,13 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g) {
   return p;
 }
 
-// A joining kernel (256 threads a CTA), launched while the kernel before it still runs (programmatic dependent launch): it waits
+// A joining kernel, launched while the kernel before it still runs (programmatic dependent launch): it waits
 // for that one's end itself.
 template <class A>
 int launch_after(const char* who, void (*kernel)(A), dim3 grid, const A& args, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(32 * JOIN_WARPS);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -550,7 +578,7 @@ int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaS
     k_att_prompt<T, HD><<<(unsigned)p.p_tiles * p.p_splits * a.kv_heads, PR_THREADS, smem, st>>>(pa);
     if (int rc = op_launched(who)) return rc;
     if (p.p_splits > 1) {
-      if (int rc = launch_after(who, k_att_join_prompt<T, HD>, dim3((unsigned)p.p_tiles * a.kv_heads * PR_ROWS), pa, st)) return rc;
+      if (int rc = launch_after(who, k_att_join_prompt<T, HD>, dim3(join_ctas((long long)p.p_tiles * a.kv_heads * PR_ROWS, p.p_splits)), pa, st)) return rc;
     }
   }
   if (p.rows) {
@@ -577,7 +605,8 @@ int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaS
       return op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
     }
     if (p.splits > 1 && !p.cluster) {
-      return launch_after(who, k_att_join_rows<T, HD>, dim3((unsigned)RW_ROWS * a.kv_heads * p.tiles, a.n_req), ra, st);
+      return launch_after(who, k_att_join_rows<T, HD>,
+                          dim3(join_ctas((long long)RW_ROWS * a.kv_heads * p.tiles, p.splits), a.n_req), ra, st);
     }
   }
   return H2C_OK;
