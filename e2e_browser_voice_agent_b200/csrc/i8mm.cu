@@ -57,12 +57,13 @@ __global__ void __launch_bounds__(1024) k_i8_quantize(const T* __restrict__ x, l
   const T* src = x + (long long)blockIdx.x * x_row;
   const int units = k >> 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned m = 0;
+#pragma unroll 4
   for (int u = threadIdx.x; u < units; u += blockDim.x) {
-    float v[4];
-    load4<VEC>(src + 4 * u, v);
-#pragma unroll
-    for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    Raw4<T, VEC> v;
+    v.load(src + 4 * u);
+    m = v.merge(m);
   }
+  m = Raw4<T, VEC>::bits(m);
   if ((int)threadIdx.x < (k & 3)) m = max(m, __float_as_uint(to_f(src[4 * units + threadIdx.x])) & 0x7fffffffu);
   m = __reduce_max_sync(0xffffffffu, m);
   if (lane == 0) red[warp] = m;
@@ -72,14 +73,18 @@ __global__ void __launch_bounds__(1024) k_i8_quantize(const T* __restrict__ x, l
   const float inv = rs.inv;
   if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
   uint32_t* dst = reinterpret_cast<uint32_t*>(q + (long long)blockIdx.x * q_row);
-  for (int u = threadIdx.x; u < k_pad >> 2; u += blockDim.x) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (u < units) {
-      load4<VEC>(src + 4 * u, v);
-    } else {
-      for (int i = 0; i < 4; i++)
-        if (4 * u + i < k) v[i] = to_f(src[4 * u + i]);
-    }
+#pragma unroll 4
+  for (int u = threadIdx.x; u < units; u += blockDim.x) {
+    Raw4<T, VEC> r;
+    float v[4];
+    r.load(src + 4 * u);
+    r.get(v);
+    dst[u] = round_bytes(__fmul_rn(v[0], inv), __fmul_rn(v[1], inv), __fmul_rn(v[2], inv), __fmul_rn(v[3], inv));
+  }
+  for (int u = units + threadIdx.x; u < k_pad >> 2; u += blockDim.x) {  // the row's end, and zeros to 16 bytes
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = 4 * u + i < k ? to_f(src[4 * u + i]) : 0.f;
     dst[u] = round_bytes(__fmul_rn(v[0], inv), __fmul_rn(v[1], inv), __fmul_rn(v[2], inv), __fmul_rn(v[3], inv));
   }
 }

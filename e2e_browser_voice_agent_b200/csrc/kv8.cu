@@ -198,46 +198,6 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   return round_bytes(v[0], v[1], v[2], v[3]);
 }
 
-// Four consecutive values as they lie in memory.
-template <class T, bool VEC>
-struct Raw4 {
-  uint32_t w[sizeof(T)];
-  __device__ __forceinline__ void load(const T* p) {
-    if (VEC) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T); i += 2) {
-        const uint2 x = reinterpret_cast<const uint2*>(p)[i / 2];
-        w[i] = x.x, w[i + 1] = x.y;
-      }
-    } else {
-      T v[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = p[i];
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T); i++) w[i] = reinterpret_cast<const uint32_t*>(v)[i];
-    }
-  }
-  __device__ __forceinline__ void get(float* v) const {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = to_f(reinterpret_cast<const T*>(w)[i]);
-  }
-  // Magnitudes order as their bits do, infinities and NaN above every number: 16-bit ones two at a time. merge() joins the largest
-  // so far with these; bits() makes the bits of a float32 of it.
-  __device__ __forceinline__ unsigned merge(unsigned m) const {
-    if (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T); i++) m = max(m, w[i] & 0x7fffffffu);
-      return m;
-    }
-    return __vmaxu2(m, __vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu));
-  }
-  static __device__ __forceinline__ unsigned bits(unsigned m) {
-    if (sizeof(T) == 4) return m;
-    const unsigned short u = (unsigned short)max(m & 0xffffu, m >> 16);
-    return __float_as_uint(to_f(*reinterpret_cast<const T*>(&u)));
-  }
-};
-
 // One run of one (K or V, head) by the threads i0 = 0 .. NT-1 of a warp (NT = 32) or of the CTA; reduce() combines the
 // largest magnitude bits over them. MAXU: units of 4 values that a thread keeps. A thread stays in one column of four.
 template <class T, bool VEC, int HD, int NT, int MAXU, class R>
