@@ -15,7 +15,8 @@ namespace {
 // thread writes is read by another (the tables' new entries are resolved through the ring, and the ring's new entries
 // lie behind its tail), so every CTA forms the sums for itself from the 8 bytes per request and no grid-wide step is
 // needed. Sums saturate at SUM_LIM, so that lengths without sense cannot wrap around to valid ones.
-// Bound: latency (launch, two dependent reads, the sums); the bytes are 8 per request, token and page.
+// Bound: latency (launch, two dependent reads, the sums); the bytes are 8 per request, token and page. 32 requests: 3.8 us;
+// 2,048 requests with prompts among them: 9.1 us, most of it the sums, which every CTA forms again.
 constexpr unsigned SUM_LIM = 0x3FFFFFFFu;
 constexpr int PLAN_THREADS = 512;
 
@@ -160,17 +161,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv8_plan(const PlanArgs a) {
 // ---------------------------------------------------------------- append
 //
 // The rows that one call brings to one page form a run; its (K or V, head) part is quantized together because it shares
-// a scale. grid.x covers windows of 16 rows, grid.y K and V and the heads: a CTA takes the runs that start in its window
+// a scale. grid.x covers windows of rows, grid.y K and V and the heads: a CTA takes the runs that start in its window
 // (a run longer than the window reaches beyond it). Runs of up to SHORT rows (decode steps: one row) take a warp each,
 // longer ones the whole CTA. A thread holds its values in registers between the maximum and the codes, so each input
-// is read once. Bound: bandwidth for prompts, latency for single rows.
-constexpr int APP_THREADS = 256, APP_WIN = 16, APP_SHORT = 2;
+// is read once. Bound: latency: one row, or a prompt's chain of slots, run, loads, maximum and codes, which 5 CTAs an SM (4: 21
+// us, 6: 24) hide in part. 32 rows of 4 heads of 128, bfloat16: 4.3 us; 16,392 rows: 19.6 us, 50 MB at 2.6 TB/s.
+constexpr int APP_THREADS = 256, APP_WIN = 16, APP_MAX_WIN = 128, APP_SHORT = 2;
 constexpr float SCALE_MIN = 0x1p-62f, SCALE_MAX = 0x1p63f;
 
 struct AppendArgs {
   int8_t* kv;
   float* scale;
-  int n_slots, page_log, kv_heads, rows, heads_per_cta;
+  int n_slots, page_log, kv_heads, rows, win;
   const void *k, *v;
   long long k_row, k_head, v_row, v_head;
   const int* slot;
@@ -258,28 +260,34 @@ __device__ __forceinline__ void append_run(const T* src, long long row_stride, i
 }
 
 template <class T, bool VEC, int HD>
-__global__ void __launch_bounds__(APP_THREADS, VEC && sizeof(T) == 2 ? 4 : 2) k_kv8_append(const AppendArgs a) {
-  __shared__ int run_row[APP_WIN], run_len[APP_WIN];
-  __shared__ int slots[APP_WIN + 128];  // of the window and of the rows that its last run may reach
+__global__ void __launch_bounds__(APP_THREADS, VEC && sizeof(T) == 2 ? 5 : 2) k_kv8_append(const AppendArgs a) {
+  static_assert(APP_MAX_WIN + 128 <= APP_THREADS, "a thread per slot");
+  __shared__ int run_row[APP_MAX_WIN], run_len[APP_MAX_WIN];
+  __shared__ int slots[APP_MAX_WIN + 128];  // of the window and of the rows that its last run may reach
   __shared__ int n_runs;
   __shared__ unsigned red[APP_THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int P = 1 << a.page_log;
-  const int w0 = blockIdx.x * APP_WIN;
-  if (tid < APP_WIN + 128) slots[tid] = w0 + tid < a.rows ? a.slot[w0 + tid] : -1;
+  const int w0 = blockIdx.x * a.win;
+  if (tid < a.win + 128) slots[tid] = w0 + tid < a.rows ? a.slot[w0 + tid] : -1;
   const int before = w0 > 0 && tid == 0 ? a.slot[w0 - 1] : -2;
   __syncthreads();
   if (warp == 0) {
     // a row starts a run unless the row before it is at the offset before its own in the same page
     const int last = __shfl_sync(0xffffffffu, before, 0);
-    bool lead = false;
-    if (lane < APP_WIN) {
-      const int s = slots[lane];
-      lead = s >= 0 && s < a.n_slots && ((s & (P - 1)) == 0 || (lane ? slots[lane - 1] : last) != s - 1);
+    int n = 0;
+    for (int t0 = 0; t0 < a.win; t0 += 32) {
+      const int t = t0 + lane;
+      bool lead = false;
+      if (t < a.win) {
+        const int s = slots[t];
+        lead = s >= 0 && s < a.n_slots && ((s & (P - 1)) == 0 || (t ? slots[t - 1] : last) != s - 1);
+      }
+      const unsigned b = __ballot_sync(0xffffffffu, lead);
+      if (lead) run_row[n + __popc(b & ((1u << lane) - 1))] = t;
+      n += __popc(b);
     }
-    const unsigned b = __ballot_sync(0xffffffffu, lead);
-    if (lead) run_row[__popc(b & ((1u << lane) - 1))] = lane;
-    if (lane == 0) n_runs = __popc(b);
+    if (lane == 0) n_runs = n;
   }
   __syncthreads();
   const int runs = n_runs;
@@ -297,44 +305,43 @@ __global__ void __launch_bounds__(APP_THREADS, VEC && sizeof(T) == 2 ? 4 : 2) k_
     if (lane == 0) run_len[i] = len;
   }
   __syncthreads();
-  for (int hh = blockIdx.y * a.heads_per_cta; hh < (int)(blockIdx.y + 1) * a.heads_per_cta; hh++) {
-    const int which = hh / a.kv_heads, head = hh - which * a.kv_heads;
-    const T* src = static_cast<const T*>(which ? a.v : a.k) + head * (which ? a.v_head : a.k_head);
-    const long long row_stride = which ? a.v_row : a.k_row;
-    auto page_of = [&](int s) {
-      return a.kv + (((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head) * ((size_t)P * HD);
-    };
-    auto scale_of = [&](int s) { return a.scale + ((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head; };
-    for (int i = warp; i < runs; i += APP_THREADS / 32) {
-      if (run_len[i] > APP_SHORT) continue;
-      const int t = w0 + run_row[i], s = slots[run_row[i]];
-      append_run<T, VEC, HD, 32, APP_SHORT * HD / 128>(src + t * row_stride, row_stride, run_len[i], page_of(s),
-                                                       s & (P - 1), scale_of(s), lane, [](unsigned m) {
-                                                         m = __reduce_max_sync(0xffffffffu, m);
-                                                         __syncwarp();  // (every lane has read the old scale)
-                                                         return m;
-                                                       });
-    }
-    for (int i = 0; i < runs; i++) {
-      if (run_len[i] <= APP_SHORT) continue;
-      const int t = w0 + run_row[i], s = slots[run_row[i]];
-      append_run<T, VEC, HD, APP_THREADS, 8>(src + t * row_stride, row_stride, run_len[i], page_of(s), s & (P - 1),
-                                             scale_of(s), tid, [&](unsigned m) {
-                                               m = __reduce_max_sync(0xffffffffu, m);
-                                               __syncthreads();  // (the run before is done with red[])
-                                               if (lane == 0) red[warp] = m;
-                                               __syncthreads();
-                                               unsigned x = red[lane % (APP_THREADS / 32)];
-                                               return __reduce_max_sync(0xffffffffu, x);
-                                             });
-    }
+  const int which = (int)blockIdx.y >= a.kv_heads, head = (int)blockIdx.y - which * a.kv_heads;
+  const T* src = static_cast<const T*>(which ? a.v : a.k) + head * (which ? a.v_head : a.k_head);
+  const long long row_stride = which ? a.v_row : a.k_row;
+  auto page_of = [&](int s) {
+    return a.kv + (((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head) * ((size_t)P * HD);
+  };
+  auto scale_of = [&](int s) { return a.scale + ((size_t)(s >> a.page_log) * 2 + which) * a.kv_heads + head; };
+  for (int i = warp; i < runs; i += APP_THREADS / 32) {
+    if (run_len[i] > APP_SHORT) continue;
+    const int t = w0 + run_row[i], s = slots[run_row[i]];
+    append_run<T, VEC, HD, 32, APP_SHORT * HD / 128>(src + t * row_stride, row_stride, run_len[i], page_of(s),
+                                                     s & (P - 1), scale_of(s), lane, [](unsigned m) {
+                                                       m = __reduce_max_sync(0xffffffffu, m);
+                                                       __syncwarp();  // (every lane has read the old scale)
+                                                       return m;
+                                                     });
+  }
+  for (int i = 0; i < runs; i++) {
+    if (run_len[i] <= APP_SHORT) continue;
+    const int t = w0 + run_row[i], s = slots[run_row[i]];
+    append_run<T, VEC, HD, APP_THREADS, 8>(src + t * row_stride, row_stride, run_len[i], page_of(s), s & (P - 1),
+                                           scale_of(s), tid, [&](unsigned m) {
+                                             m = __reduce_max_sync(0xffffffffu, m);
+                                             __syncthreads();  // (the run before is done with red[])
+                                             if (lane == 0) red[warp] = m;
+                                             __syncthreads();
+                                             unsigned x = red[lane % (APP_THREADS / 32)];
+                                             return __reduce_max_sync(0xffffffffu, x);
+                                           });
   }
 }
 
 // ---------------------------------------------------------------- read
 
 // A thread takes four consecutive codes of a row (blockDim.x threads across the row's K heads, then V heads) and goes from row to
-// row: its 16 or 8 bytes of output join its neighbours'. Four rows in flight. Bound: bandwidth.
+// row: its 16 or 8 bytes of output join its neighbours'. Four rows in flight (16,392 rows of 4 heads of 128 to float32, 84 MB: 19
+// us, 4.5 TB/s; one at a time 31). Bound: bandwidth; 32 rows: latency, 2.2 us.
 template <class T>
 __global__ void __launch_bounds__(256) k_kv8_read(const int8_t* __restrict__ kv, const float* __restrict__ scale, int n_slots,
                                                   int page_log, int kv_heads, int hd_log, const int* __restrict__ slot, int rows,
@@ -402,7 +409,7 @@ int cache_ok(const char* who, const void* kv, const float* scale, int n_pages, i
 
 template <class T, bool VEC>
 void launch_append(const AppendArgs& a, int head_dim, cudaStream_t st) {
-  const dim3 grid((a.rows + APP_WIN - 1) / APP_WIN, 2 * a.kv_heads / a.heads_per_cta);
+  const dim3 grid((a.rows + a.win - 1) / a.win, 2 * a.kv_heads);
   if (head_dim == 64) k_kv8_append<T, VEC, 64><<<grid, APP_THREADS, 0, st>>>(a);
   else k_kv8_append<T, VEC, 128><<<grid, APP_THREADS, 0, st>>>(a);
 }
@@ -460,10 +467,10 @@ int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size
   const size_t es = op_elem_size(type);
   if (((uintptr_t)k | (uintptr_t)v) & (es - 1))
     return op_error(H2C_ERR_INVALID, "%s: k and v must be aligned to their elements", who);
-  // few rows: a CTA for each (K or V, head), so that nothing waits in line; many: one for K and one for V, since most windows of
-  // a prompt begin no run and a CTA that finds none costs as much as its launch (16k rows: 41 us with one per head, 19 us so)
-  const int heads_per_cta = (long long)(rows + APP_WIN - 1) / APP_WIN * 2 * kv_heads > 1184 ? kv_heads : 1;
-  const AppendArgs a{static_cast<int8_t*>(kv), kv_scale, n_pages * page_size, log2_of(page_size), kv_heads, rows, heads_per_cta, k, v,
+  // few rows (decode steps): windows of 16, so that few single rows wait in line for a warp; many: windows of a page, so that
+  // every CTA of a prompt finds a run (16,392 rows into pages of 64: 19.6 us; with windows of 16, of which most begin no run, 29)
+  const int win = (long long)(rows + APP_WIN - 1) / APP_WIN * 2 * kv_heads > 1184 ? std::max(APP_WIN, page_size) : APP_WIN;
+  const AppendArgs a{static_cast<int8_t*>(kv), kv_scale, n_pages * page_size, log2_of(page_size), kv_heads, rows, win, k, v,
                      k_row, k_head, v_row, v_head, slot};
   // loads of four elements where every row and head starts at a multiple of four
   const bool vec = !(((uintptr_t)k | (uintptr_t)v) & (4 * es - 1)) && !((k_row | k_head | v_row | v_head) & 3);
