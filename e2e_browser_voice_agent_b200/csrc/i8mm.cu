@@ -13,7 +13,7 @@
 // Few tiles (few tokens on a small matrix): a cluster of up to 8 CTAs divides K and adds its partial tiles through
 // distributed shared memory, each CTA finishing a share of the tokens.
 // The tokens are quantized by a kernel of their own; the product is launched with it (programmatic dependent launch) and
-// has its weights under way before it waits for the codes. One to four tokens are quantized by every CTA for itself, its share
+// has its weights under way before it waits for the codes. One or two tokens are quantized by every CTA for itself, its share
 // of K into shared memory while the weights come: one launch.
 // Waits are bounded (1 s): on expiry the CTA records it (h2c_ops_check), drains its copies and returns.
 #include "ops.cuh"
@@ -28,7 +28,7 @@ namespace {
 
 constexpr int TN = 128;          // weight rows per product
 constexpr int KCH = 128;         // bytes of K per stage
-constexpr int FUSE_TOKENS = 4, FUSE_VALUES = 4096, FUSE_CHUNKS = 32;  // bounds of the form that quantizes its tokens itself
+constexpr int FUSE_TOKENS = 2, FUSE_VALUES = 4096, FUSE_CHUNKS = 32;  // bounds of the form that quantizes its tokens itself
 constexpr int X_CHUNK = 16 * KCH;  // its codes of one stage of K: 16 rows
 constexpr int MAX_STAGES = 12;
 constexpr int SMEM_RING = 220 * 1024;
@@ -404,7 +404,9 @@ void shape_of(int m, int n, int chunks, int* nt, int* mt, int* splits) {
   *splits = *mt > 1 ? 1 : std::max(1, std::min(std::min(8, chunks), 148 / tiles));
 }
 
-// Whether the product quantizes its tokens itself: few of them, and a CTA's share of K small enough for shared memory.
+// Whether the product quantizes its tokens itself: few of them, and a CTA's share of K small enough for shared memory. Through
+// 1152 x 896, bfloat16, in us on the device and per call: one token 5.8 and 15.7 (two launches: 6.2 and 19.5), two 6.4 and 14.6 (6.2
+// and 17.2), four 7.6 (6.2).
 bool fused(int x_type, int m, int k) { return x_type != H2C_TYPE_I8 && m <= FUSE_TOKENS && (long long)m * k <= FUSE_VALUES; }
 
 template <class T>
