@@ -1,8 +1,8 @@
 // Attention over the paged 8-bit cache (h2c_kv8_attention; the formula is stated in include/h2cuda.h).
 //
-// Many queries (k_att_prompt): kv8_prompt.cuh. Few queries (k_att_rows): a CTA takes 8 rows (query, head of the kv head's group) of one request and kv head and one
-// span of its keys; 4 warps take blocks of 16 keys in turn, each with its own running maximum, sum and output, joined at
-// the end; up to 8 spans are joined by their cluster, more by a second kernel.
+// Many queries (k_att_prompt): kv8_prompt.cuh. Few queries (k_att_rows): a CTA takes 8 rows (query, head of the kv head's
+// group) of one request and kv head and one span of its keys; 4 warps take blocks of 16 keys in turn, each with its own
+// running maximum, sum and output, joined at the end; up to 8 spans are joined by their cluster, more by a second kernel.
 // * Tensor cores (mma.sync m16n8k16, float16 in, float32 sums): codes are integers up to 127 and exact in float16. The
 //   16 rows of an operand tile hold 8 rows twice: a float16 term in rows 0-7 and the remainder in rows 8-15, for the
 //   queries (scaled by a power of two per row) and for the softmax weights, so the products carry 22 bits, whatever the
@@ -10,7 +10,10 @@
 // * The cache is the traffic: each lane copies its own 16-byte pieces of a block with cp.async into a ring that only it
 //   reads, so the ring needs no barrier; the order of dimensions inside a product is free as long as both operands use
 //   it, which lets a lane take 16 consecutive bytes of a key (QK) or of 4 keys (PV) without a transpose.
-// * Bound: the cache's bytes for long histories; latency for short ones.
+// * Bound: the cache's bytes for long histories, of which it reads 4.5 TB/s (28 heads over 4, 128 wide, bfloat16; 8 requests
+//   of 69,224-131,072 tokens, 876 MB: 195 us, of which the loads alone take 179: 3 CTAs of 168 registers an SM keep no more
+//   bytes on their way); latency for short ones (32 requests of 120-4,096 tokens, 51 MB: 20 us and 6 to join; one of 641
+//   tokens, 14 heads over 2, 64 wide, float32: 5.8 us, of which a launch is 2-3).
 #include "kv8_att.cuh"
 #include "kv8_prompt.cuh"
 
@@ -492,9 +495,14 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_prompt(const Promp
 
 // ---------------------------------------------------------------- host
 
-// Requests of up to RW_MAX rows take k_att_rows, others k_att_prompt, each CTA looking at its request's count on the device;
-// the host knows only max_q, and launches the one kernel or both. (A single request takes the one its max_q asks for.)
-constexpr int RW_MAX = 64;
+// k_att_rows reads a request's keys again for every 8 rows and starts in half the time; k_att_prompt takes 256 rows at once. A call
+// that visits few keys altogether (row tiles of 8 x keys, as many as max_q and max_kv allow; a tile's start counts as 256 keys)
+// is k_att_rows' whole: up to 2^17 visits 128 wide, 2^19 64 wide. In a call of more, each CTA looks at its request's rows on the
+// device: up to 16 (32) are k_att_rows', others k_att_prompt's, and the host launches the one kernel or both by max_q.
+// Measured, k_att_rows and k_att_prompt in us, bfloat16 128 wide, 28 heads over 4: 2 requests of 4,000 keys, 21 rows (96,000
+// visits) 17 and 21, 35 rows (160,000) 25 and 22, 252 rows (1,024,000) 71 and 29; 32 requests of 4,000 keys, 14 rows (1,024,000)
+// 73 and 82. float32 64 wide, 14 over 2: 8 requests of 4,000 keys, 35 rows (320,000) 20 and 23, 126 rows (1,024,000) 35 and 26; of
+// 16,000 keys, 21 rows (768,000) 32 and 47.
 struct WorkPlan {
   bool rows, prompt, cluster;
   int max_rows, splits, blocks, tiles;         // k_att_rows
@@ -505,12 +513,14 @@ struct WorkPlan {
 WorkPlan plan_work(const h2c_kv8_attention_args* g) {
   WorkPlan p = {};
   const long long group = g->heads / g->kv_heads, most_rows = g->max_q * group;
-  p.prompt = most_rows > RW_MAX;
-  p.rows = !p.prompt || g->n_req > 1;
   long long keys = g->max_kv;
   if (g->window > 0) keys = std::min(keys, (long long)g->window + g->max_q);
+  const long long visits = (most_rows + RW_ROWS - 1) / RW_ROWS * g->n_req * g->kv_heads * std::max(keys, 256LL);
+  const int few = g->head_dim == 64 ? 32 : 16;
+  p.prompt = most_rows > few && visits > (g->head_dim == 64 ? 1 << 19 : 1 << 17);
+  p.rows = !p.prompt || g->n_req > 1;
   if (p.rows) {
-    p.max_rows = p.prompt ? RW_MAX : INT_MAX;
+    p.max_rows = p.prompt ? few : INT_MAX;
     p.tiles = (int)((std::min<long long>(most_rows, p.max_rows) + RW_ROWS - 1) / RW_ROWS);
     // spans: enough CTAs for two waves of three per SM. Up to 8 are one cluster, whose join costs little: spans of 128 keys (2
     // blocks per warp) or more. More of them, for few rows over long histories, leave their parts in the workspace for a
@@ -526,7 +536,7 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g) {
     p.units = p.splits > 1 && !p.cluster ? (size_t)groups * p.splits : 0;
   }
   if (p.prompt) {
-    p.min_rows = p.rows ? RW_MAX + 1 : 0;
+    p.min_rows = p.rows ? few + 1 : 0;
     p.p_tiles = (int)std::min((long long)g->n_req * ((most_rows + PR_ROWS - 1) / PR_ROWS),
                               (long long)g->rows * group / PR_ROWS + g->n_req);
     // spans: as many as fill the SMs once (one CTA each), of at least 256 keys

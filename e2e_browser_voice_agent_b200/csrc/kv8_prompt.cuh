@@ -17,8 +17,14 @@
 //   O rescaled (by the softmax warps, in TMEM).
 // * float32 queries and weights are two float16 terms each (22 bits), one tcgen05.mma per term.
 // * V lies in shared memory as its rows come, [key][dimension]: the second product's B operand in MN-major form.
-// Bound: exponentials (256 x 64 per tile at 16 a cycle: 1,024 cycles) and tensor cores (about 1,280: the S products'
-// operands of 64 keys take 1.5 times their multiply time to read from shared memory) at about the same level.
+// * The softmaxes of the two row tiles take turns at the exponentials, so that one's wait for its scores falls into the
+//   other's turn (385 us in step with each other, 370 so).
+// Bound: a key tile of 256 rows needs 1,024 cycles of exponentials (16 a cycle) and about 1,280 of the tensor cores (the S
+// products' operands of 64 keys take 1.5 times their multiply time to read from shared memory). It takes about 2,350: the
+// softmax warps issue what lies between a score and its weight (maximum, scale, conversion, TMEM both ways) one after the
+// other, and each hand-over between warps costs 115-175 cycles. A CTA spends about 12,500 cycles more on its first scores and
+// its last outputs. Measured (4 prompts of 2,064-4,099 tokens, 28 heads over 4, 128 wide, bfloat16): 370 us, 684
+// TFLOP/s of the products that the mask leaves. Slower: tiles of 128 keys with one S slot (412), two threads a row (405).
 #pragma once
 #include "kv8_att.cuh"
 #include "tc5_ptx.cuh"
@@ -219,21 +225,23 @@ struct Raw8 {
   // the largest magnitude's bits as a float32 (infinities and NaN above every number)
   __device__ __forceinline__ unsigned largest() const {
     unsigned m = 0;
-    if (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < 8; i++) m = max(m, w[i] & 0x7fffffffu);
       return m;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-    m = max(m & 0xffffu, m >> 16);
-    const unsigned short u = (unsigned short)m;
-    return __float_as_uint(to_f(*reinterpret_cast<const T*>(&u)));
+      for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      m = max(m & 0xffffu, m >> 16);
+      const unsigned short u = (unsigned short)m;
+      return __float_as_uint(to_f(*reinterpret_cast<const T*>(&u)));
+    }
   }
 };
 
 // A warp's 32 rows of a row tile's queries (from row r0 of the tile, which begins at row tile0 of the request): HD / 8 lanes a
-// row; lane i has the place of row i in q (row_at). A row is scaled by a power of two so that its largest magnitude lies in
+// row; lane i has the place of row i in q (row_at). Rows past the last are zeros, and not read: all of them from one place took
+// a chunk of 10 float32 tokens on 16,000 positions from 19 to 35 us. A row is scaled by a power of two so that its largest magnitude lies in
 // [2^13, 2^14) and split into one or two float16 terms; what undoes the scaling, times the softmax scale, goes to row_scale.
 // The raw values are copied to where their terms will lie (8 of them take as many bytes as their terms do) and replaced
 // there by the same lane. Rolled loops: code that runs once waits for its own fetching.
@@ -250,9 +258,11 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
     for (int p = 0; p < PASSES; p++) {
       const T* src = q + __shfl_sync(0xffffffffu, row_at, p * RPP + sub);
       const uint32_t dst = su32(blk + sw128(r0 + p * RPP + sub, piece & 7));
+      const int bytes = tile0 + r0 + p * RPP + sub < n_rows ? 16 : 0;  // (what is not copied is filled with zeros)
 #pragma unroll
       for (int t = 0; t < C::TERMS; t++)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + t * C::Q_TILE), "l"(src + t * 4) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + t * C::Q_TILE), "l"(src + t * 4), "r"(bytes)
+                     : "memory");
     }
     asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
   } else {
@@ -260,9 +270,11 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
     for (int p = 0; p < PASSES; p++) {
       const T* src = q + __shfl_sync(0xffffffffu, row_at, p * RPP + sub);
       uint8_t* dst = blk + sw128(r0 + p * RPP + sub, piece & 7);
+      const bool live = tile0 + r0 + p * RPP + sub < n_rows;
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        *reinterpret_cast<T*>(dst + (i * (int)sizeof(T) >> 4) * C::Q_TILE + (i * (int)sizeof(T) & 15)) = src[i];
+        *reinterpret_cast<T*>(dst + (i * (int)sizeof(T) >> 4) * C::Q_TILE + (i * (int)sizeof(T) & 15)) =
+            live ? src[i] : from_f<T>(0.f);
     }
   }
 #pragma unroll 1
@@ -290,9 +302,7 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
       const int r = r0 + (p0 + b) * RPP + sub;
       const int e = (int)(m[b] >> 23);
       const int up = e == 255 || m[b] == 0 ? 127 : min(253, 267 - e);
-      // (the sign of the softmax scale goes into the query, so that larger products are larger scores; rows past the last
-      // are zeros)
-      const bool live = tile0 + r < n_rows;
+      // (the sign of the softmax scale goes into the query, so that larger products are larger scores)
       const float mul = copysignf(__int_as_float(up << 23), a.scale_log2);
       if (piece == 0) row_scale[r] = __int_as_float((254 - up) << 23) * fabsf(a.scale_log2);
       uint32_t h[4], rest[4];
@@ -300,8 +310,8 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
       for (int i = 0; i < 4; i++) {
         const float x0 = v[b].at(2 * i) * mul, x1 = v[b].at(2 * i + 1) * mul;
         const __half2 t = __floats2half2_rn(x0, x1);
-        h[i] = live ? *reinterpret_cast<const uint32_t*>(&t) : 0u;
-        if (C::TERMS == 2) rest[i] = live ? pack_half2(x0 - __low2float(t), x1 - __high2float(t)) : 0u;
+        h[i] = *reinterpret_cast<const uint32_t*>(&t);
+        if (C::TERMS == 2) rest[i] = pack_half2(x0 - __low2float(t), x1 - __high2float(t));
       }
       uint8_t* at = blk + sw128(r, piece & 7);
       *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
