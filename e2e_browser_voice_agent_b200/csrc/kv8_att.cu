@@ -12,7 +12,7 @@
 //   it, which lets a lane take 16 consecutive bytes of a key (QK) or of 4 keys (PV) without a transpose.
 // * Bound: the cache's bytes for long histories, of which it reads 4.5 TB/s (28 heads over 4, 128 wide, bfloat16; 8 requests
 //   of 69,224-131,072 tokens, 876 MB: 195 us, of which the loads alone take 179: 3 CTAs of 168 registers an SM keep no more
-//   bytes on their way); latency for short ones (32 requests of 120-4,096 tokens, 51 MB: 20 us and 6 to join; one of 641
+//   bytes on their way); latency for short ones (32 requests of 120-4,096 tokens, 51 MB: 20 us and 5 to join; one of 641
 //   tokens, 14 heads over 2, 64 wide, float32: 5.8 us, of which a launch is 2-3).
 #include "kv8_att.cuh"
 #include "kv8_prompt.cuh"
@@ -54,8 +54,16 @@ struct RowSmem {
   static constexpr int BYTES = (RING > JOIN ? RING : JOIN) + SCALES;
 };
 
+// In a call that launches k_att_prompt too, k_att_rows follows it by programmatic dependent launch: it uses nothing of it and
+// takes the SMs that its last CTAs leave (31 single tokens of 100-4,096 beside 2 prompts of 2,048: 134 -> 130 us). Its CTAs end after that one's, so that what follows on the stream finds both done. (They
+// start when all of the kernel before have started, so none waits for a CTA that needs its place.)
+struct EndAfterThePrompts {
+  __device__ __forceinline__ ~EndAfterThePrompts() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+};
+
 template <class T, int HD>
 __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
+  const EndAfterThePrompts end;
   using S = RowSmem<HD>;
   constexpr int KC = HD / 64;   // 16-byte pieces of a key per lane
   constexpr int VB = HD / 8;    // bytes of a value row per lane (16 or 8)
@@ -391,23 +399,44 @@ __device__ __forceinline__ void join_row(const AttArgs& a, const float* part, si
   constexpr int V = HD / 32;  // dimensions per lane
   __shared__ float acc[JOIN_WARPS][HD], acc_l[JOIN_WARPS];
   const int lane = threadIdx.x & 31;
-  float m = -INFINITY;
-  for (int s = lane; s < used; s += 32) m = fmaxf(m, ml[s * ml_step].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float v[V], l = 0.f;
-#pragma unroll
-  for (int i = 0; i < V; i++) v[i] = 0.f;
-#pragma unroll 4
-  for (int s = w; s < used; s += n_warps) {
-    const float2 x = ml[s * ml_step];
-    float o[V];
+  auto load = [&](int s, float* o) {
     if (V == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(part + s * part_step + V * lane);
     else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(part + s * part_step + V * lane);
+  };
+  float m = -INFINITY, v[V], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; i++) v[i] = 0.f;
+  auto add = [&](float2 x, const float* o) {
     const float f = x.x == -INFINITY ? 0.f : exp2_fast(x.x - m);
     l += f * x.y;
 #pragma unroll
     for (int i = 0; i < V; i++) v[i] += f * o[i];
+  };
+  if (n_warps == 1) {  // everything on its way at once (a chunk of 256 on 4,096 tokens, 10 spans: 30 -> 27 us)
+    float2 x[JOIN_WARP_SPANS];
+    float o[JOIN_WARP_SPANS][V];
+#pragma unroll
+    for (int s = 0; s < JOIN_WARP_SPANS; s++)
+      if (s < used) {
+        x[s] = ml[s * ml_step];
+        load(s, o[s]);
+      }
+#pragma unroll
+    for (int s = 0; s < JOIN_WARP_SPANS; s++)
+      if (s < used) m = fmaxf(m, x[s].x);
+#pragma unroll
+    for (int s = 0; s < JOIN_WARP_SPANS; s++)
+      if (s < used) add(x[s], o[s]);
+  } else {
+    for (int s = lane; s < used; s += 32) m = fmaxf(m, ml[s * ml_step].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll 4
+    for (int s = w; s < used; s += n_warps) {
+      float o[V];
+      load(s, o);
+      add(ml[s * ml_step], o);
+    }
   }
   if (n_warps > 1) {
 #pragma unroll
@@ -473,6 +502,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_rows(const RowArgs
 template <class T, int HD>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_prompt(const PromptArgs pa) {
   const AttArgs& a = pa.a;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (k_att_rows)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const JoinTurn t = join_turn(pa.splits);
   const int jr = t.i % PR_ROWS, th = t.i / PR_ROWS, head = th % a.kv_heads, idx = th / a.kv_heads;
@@ -604,11 +634,16 @@ int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaS
     cfg.blockDim = dim3(RW_WARPS * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {(unsigned)p.splits, 1, 1};
-    cfg.attrs = &attr;
-    cfg.numAttrs = p.cluster;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    if (p.cluster) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+      attr[cfg.numAttrs++].val.clusterDim = {(unsigned)p.splits, 1, 1};
+    }
+    if (p.prompt) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     const cudaError_t c = cudaLaunchKernelEx(&cfg, k_att_rows<T, HD>, ra);
     if (c != cudaSuccess) {
       cudaGetLastError();
