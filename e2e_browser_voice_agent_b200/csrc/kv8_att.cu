@@ -464,26 +464,25 @@ __device__ __forceinline__ void join_row(const AttArgs& a, const float* part, si
     a.lse[(size_t)tok * a.heads + hq] = l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
 }
 
-// Row `i` of the launch for this warp, its turn and the warps that share the row.
+// Row `i` of the CTAs that join, for this warp: its turn and the warps that share the row.
 struct JoinTurn {
   int i, w, n;
 };
-__device__ __forceinline__ JoinTurn join_turn(int splits) {
+__device__ __forceinline__ JoinTurn join_turn(int cta, int splits) {
   const int warp = threadIdx.x >> 5;
-  if (splits <= JOIN_WARP_SPANS) return {(int)blockIdx.x * JOIN_WARPS + warp, 0, 1};
-  return {(int)blockIdx.x, warp, JOIN_WARPS};
+  if (splits <= JOIN_WARP_SPANS) return {cta * JOIN_WARPS + warp, 0, 1};
+  return {cta, warp, JOIN_WARPS};
 }
 inline unsigned join_ctas(long long rows, int splits) {
   return (unsigned)(splits <= JOIN_WARP_SPANS ? (rows + JOIN_WARPS - 1) / JOIN_WARPS : rows);
 }
 
+// The first row_ctas CTAs join k_att_rows' spans, per_req of them a request's; the others k_att_prompt's.
 template <class T, int HD>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_rows(const RowArgs ra) {
+__device__ __forceinline__ void join_rows_at(const RowArgs& ra, int r, int cta) {
   const AttArgs& a = ra.a;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const JoinTurn t = join_turn(ra.splits);
+  const JoinTurn t = join_turn(cta, ra.splits);
   const int jr = t.i % RW_ROWS, th = t.i / RW_ROWS, head = th % a.kv_heads, tile = th / a.kv_heads;
-  const int r = blockIdx.y;
   int n_all;
   const Request R = request_of(a, r, &n_all);
   const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group, row = row0 + jr;
@@ -498,15 +497,14 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_rows(const RowArgs
   join_row<T, HD>(a, ra.part + at * HD, (size_t)RW_ROWS * HD, ra.ml + at, RW_ROWS, sp.used, R.first + tok, head * a.group + hq,
                   t.w, t.n);
 }
-
 template <class T, int HD>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_prompt(const PromptArgs pa) {
+__device__ __forceinline__ void join_prompts_at(const PromptArgs& pa, int cta) {
   const AttArgs& a = pa.a;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (k_att_rows)
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const JoinTurn t = join_turn(pa.splits);
+  const PromptShape shape = shape_of_call(pa);
+  if (shape.splits == 1) return;
+  const JoinTurn t = join_turn(cta, shape.splits);
   const int jr = t.i % PR_ROWS, th = t.i / PR_ROWS, head = th % a.kv_heads, idx = th / a.kv_heads;
-  if (idx >= pa.tiles) return;
+  if (idx >= shape.tiles) return;
   const TileAt at = tile_at(pa, idx);
   if (at.r < 0) return;
   const Request R = at.R;
@@ -514,13 +512,20 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_prompt(const Promp
   if (row >= n_rows) return;
   int lo, hi;
   key_range(a, R, n_all, at.row0 / a.group, min(at.row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-  const Span sp = spans_of(lo, hi, pa.splits, pa.blocks, PR_KEYS);
+  const Span sp = spans_of(lo, hi, shape.splits, shape.blocks, PR_KEYS);
   if (sp.used == 1) return;
-  const size_t u = ((size_t)idx * a.kv_heads + head) * pa.splits * PR_ROWS + jr;
+  const size_t u = ((size_t)idx * a.kv_heads + head) * shape.splits * PR_ROWS + jr;
   int hq;
   const int tok = token_of(a, row, &hq);
   join_row<T, HD>(a, pa.part + u * HD, (size_t)PR_ROWS * HD, pa.ml + u, PR_ROWS, sp.used, R.first + tok, head * a.group + hq, t.w,
                   t.n);
+}
+template <class T, int HD>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join(const RowArgs ra, const PromptArgs pa, int row_ctas, int per_req) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int b = blockIdx.x;
+  if (b < row_ctas) join_rows_at<T, HD>(ra, b / per_req, b % per_req);
+  else join_prompts_at<T, HD>(pa, b - row_ctas);
 }
 
 // ---------------------------------------------------------------- host
@@ -534,10 +539,12 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join_prompt(const Promp
 // 73 and 82. float32 64 wide, 14 over 2: 8 requests of 4,000 keys, 35 rows (320,000) 20 and 23, 126 rows (1,024,000) 35 and 26; of
 // 16,000 keys, 21 rows (768,000) 32 and 47.
 struct WorkPlan {
-  bool rows, prompt, cluster;
+  bool rows, prompt, cluster, counted;
   int max_rows, splits, blocks, tiles;         // k_att_rows
-  int min_rows, p_splits, p_blocks, p_tiles;   // k_att_prompt
-  size_t units, p_units;                       // row tiles x spans in the workspace
+  int min_rows, p_keys, p_units;               // k_att_prompt (see PromptArgs; p_units also without counting)
+  PromptShape shape;
+  unsigned p_join;                             // CTAs of its joining kernel, 0 without one
+  size_t units;                                // row tiles x spans in the workspace
   size_t bytes;
 };
 WorkPlan plan_work(const h2c_kv8_attention_args* g) {
@@ -567,44 +574,45 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g) {
   }
   if (p.prompt) {
     p.min_rows = p.rows ? few + 1 : 0;
-    p.p_tiles = (int)std::min((long long)g->n_req * ((most_rows + PR_ROWS - 1) / PR_ROWS),
-                              (long long)g->rows * group / PR_ROWS + g->n_req);
-    // spans: as many as fill the SMs once (one CTA each), of at least 256 keys
-    const long long groups = (long long)g->kv_heads * p.p_tiles;
-    const int n_blocks = (int)((keys + PR_KEYS - 1) / PR_KEYS) + (g->window > 0 ? 1 : 0);
-    p.p_splits = (int)std::max(1LL, std::min<long long>(148 / groups, n_blocks / 4));
-    p.p_blocks = std::max(1, (n_blocks + p.p_splits - 1) / p.p_splits);
-    p.p_splits = std::max(1, (n_blocks + p.p_blocks - 1) / p.p_blocks);
-    p.p_units = p.p_splits > 1 ? (size_t)groups * p.p_splits : 0;
+    const int tiles = (int)std::min<long long>({(long long)g->n_req * ((most_rows + PR_ROWS - 1) / PR_ROWS),
+                                                (long long)g->rows * group / PR_ROWS + g->n_req, (long long)INT_MAX / g->kv_heads});
+    p.p_keys = (int)((keys + PR_KEYS - 1) / PR_KEYS) + (g->window > 0 ? 1 : 0);
+    p.shape = prompt_shape(tiles, g->kv_heads, p.p_keys, g->n_req == 1 ? 148 : 0, 4);
+    if (g->n_req == 1) {
+      p.p_units = p.shape.splits > 1 ? tiles * g->kv_heads * p.shape.splits : 0;
+      p.p_join = p.p_units ? join_ctas((long long)tiles * g->kv_heads * PR_ROWS, p.shape.splits) : 0;
+    } else if (g->n_req <= 128 && (long long)g->rows * group / PR_ROWS * g->kv_heads <= 74 && g->kv_heads <= 74 && p.p_keys >= 16) {
+      // all rows together leave SMs idle: each CTA counts (which takes too long for more requests)
+      p.counted = true;
+      p.p_units = 148;
+      // rows that the joining kernel may find: of one in 2 .. JOIN_WARP_SPANS units (a warp each), or in more (a CTA each)
+      const long long groups = (long long)tiles * g->kv_heads;
+      p.p_join = std::max(join_ctas(std::min(groups, 148LL / 2) * PR_ROWS, 2),
+                          join_ctas(std::min(groups, 148LL / (JOIN_WARP_SPANS + 1)) * PR_ROWS, JOIN_WARP_SPANS + 1));
+    }
   }
-  p.bytes = (p.units * RW_ROWS + p.p_units * PR_ROWS) * ((size_t)g->head_dim * 4 + 8);
+  p.bytes = (p.units * RW_ROWS + (size_t)p.p_units * PR_ROWS) * ((size_t)g->head_dim * 4 + 8);
   return p;
-}
-
-// A joining kernel, launched while the kernel before it still runs (programmatic dependent launch): it waits
-// for that one's end itself.
-template <class A>
-int launch_after(const char* who, void (*kernel)(A), dim3 grid, const A& args, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(32 * JOIN_WARPS);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t c = cudaLaunchKernelEx(&cfg, kernel, args);
-  if (c == cudaSuccess) return H2C_OK;
-  cudaGetLastError();
-  return op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
 }
 
 template <class T, int HD>
 int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaStream_t st) {
   float* part = static_cast<float*>(workspace);
   float* p_part = part + p.units * RW_ROWS * HD;
-  float2* ml = reinterpret_cast<float2*>(p_part + p.p_units * PR_ROWS * HD);
+  float2* ml = reinterpret_cast<float2*>(p_part + (size_t)p.p_units * PR_ROWS * HD);
+  int* err = p.prompt ? op_err_words() : nullptr;
+  if (p.prompt && !err) return op_error(H2C_ERR_CUDA, "%s: no device", who);
+  const PromptArgs pa{a, p.min_rows, p.shape, p.p_keys, p.counted ? p.p_units : 0, p_part, ml + p.units * RW_ROWS, err};
+  const RowArgs ra{a, p.splits, p.blocks, p.tiles, p.max_rows, p.cluster, part, ml};
+  // a kernel that may start while the one before it still runs waits for that one's end itself
+  cudaLaunchAttribute dependent;
+  dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  dependent.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cudaError_t c = cudaSuccess;
   if (p.prompt) {
     static unsigned char done[OP_MAX_DEVICES];
     constexpr int smem = PromptCfg<T, HD>::SMEM;
@@ -612,14 +620,8 @@ int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaS
           return cudaFuncSetAttribute(k_att_prompt<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         }))
       return rc;
-    int* err = op_err_words();
-    if (!err) return op_error(H2C_ERR_CUDA, "%s: no device", who);
-    const PromptArgs pa{a, p.min_rows, p.p_tiles, p.p_splits, p.p_blocks, p_part, ml + p.units * RW_ROWS, err};
-    k_att_prompt<T, HD><<<(unsigned)p.p_tiles * p.p_splits * a.kv_heads, PR_THREADS, smem, st>>>(pa);
+    k_att_prompt<T, HD><<<std::max(p.shape.tiles * a.kv_heads, p.p_units), PR_THREADS, smem, st>>>(pa);
     if (int rc = op_launched(who)) return rc;
-    if (p.p_splits > 1) {
-      if (int rc = launch_after(who, k_att_join_prompt<T, HD>, dim3(join_ctas((long long)p.p_tiles * a.kv_heads * PR_ROWS, p.p_splits)), pa, st)) return rc;
-    }
   }
   if (p.rows) {
     static unsigned char done[OP_MAX_DEVICES];
@@ -628,33 +630,28 @@ int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaS
           return cudaFuncSetAttribute(k_att_rows<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         }))
       return rc;
-    const RowArgs ra{a, p.splits, p.blocks, p.tiles, p.max_rows, p.cluster, part, ml};
-    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.splits * a.kv_heads * p.tiles, a.n_req);
     cfg.blockDim = dim3(RW_WARPS * 32);
     cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    cfg.attrs = attr;
     if (p.cluster) {
       attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
       attr[cfg.numAttrs++].val.clusterDim = {(unsigned)p.splits, 1, 1};
     }
-    if (p.prompt) {
-      attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    const cudaError_t c = cudaLaunchKernelEx(&cfg, k_att_rows<T, HD>, ra);
-    if (c != cudaSuccess) {
-      cudaGetLastError();
-      return op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
-    }
-    if (p.splits > 1 && !p.cluster) {
-      return launch_after(who, k_att_join_rows<T, HD>,
-                          dim3(join_ctas((long long)RW_ROWS * a.kv_heads * p.tiles, p.splits), a.n_req), ra, st);
-    }
+    if (p.prompt) attr[cfg.numAttrs++] = dependent;
+    c = cudaLaunchKernelEx(&cfg, k_att_rows<T, HD>, ra);
   }
-  return H2C_OK;
+  const int per_req = p.rows && p.splits > 1 && !p.cluster ? (int)join_ctas((long long)RW_ROWS * a.kv_heads * p.tiles, p.splits) : 0;
+  if (c == cudaSuccess && (per_req || p.p_join)) {
+    cfg.gridDim = dim3((unsigned)per_req * a.n_req + p.p_join);
+    cfg.blockDim = dim3(32 * JOIN_WARPS);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    attr[0] = dependent;
+    c = cudaLaunchKernelEx(&cfg, k_att_join<T, HD>, ra, pa, per_req * a.n_req, std::max(1, per_req));
+  }
+  if (c == cudaSuccess) return H2C_OK;
+  cudaGetLastError();
+  return op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
 }
 
 template <class T>
@@ -710,7 +707,7 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
   if (p.bytes && (!g->workspace || g->workspace_bytes < p.bytes || ((uintptr_t)g->workspace & 15)))
     return op_error(H2C_ERR_INVALID, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
                     (unsigned long long)p.bytes, (unsigned long long)(g->workspace ? g->workspace_bytes : 0));
-  const long long most = std::max((long long)p.splits * p.tiles * RW_ROWS, (long long)p.p_splits * p.p_tiles * PR_ROWS);
+  const long long most = std::max((long long)p.splits * p.tiles * RW_ROWS, (long long)p.shape.tiles * PR_ROWS);
   if (most * g->kv_heads > INT_MAX) return op_error(H2C_ERR_INVALID, "%s: too many rows for one call", who);
   AttArgs a;
   a.q = g->q; a.q_row = g->q_row; a.q_head = g->q_head;

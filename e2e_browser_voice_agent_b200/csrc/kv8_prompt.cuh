@@ -35,14 +35,56 @@ namespace {
 constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 5 * 128, PR_INFO = 32;
 enum { PR_CONVERT = 21, PR_MMA = 22, PR_SOFTMAX = 23 };
 
+// The row tiles of all requests, the spans that each is cut into, and the 64-key tiles of a span.
+struct PromptShape {
+  int tiles, splits, blocks;
+};
+// Spans: as many as fill `units` CTAs once, of at least `least` key tiles.
+__host__ __device__ inline PromptShape prompt_shape(int tiles, int kv_heads, int key_tiles, int units, int least) {
+  PromptShape s{tiles, 1, key_tiles < 1 ? 1 : key_tiles};
+  const int ctas = tiles * kv_heads;
+  if (ctas > 0 && ctas <= units / 2 && key_tiles >= 2 * least) {
+    const int most = units / ctas, n = most < key_tiles / least ? most : key_tiles / least;
+    s.blocks = (key_tiles + n - 1) / n;
+    s.splits = (key_tiles + s.blocks - 1) / s.blocks;
+  }
+  return s;
+}
+
 struct PromptArgs {
   AttArgs a;
-  int min_rows;              // requests of fewer rows are k_att_rows'
-  int tiles, splits, blocks; // bound of the row tiles of all requests, spans per row tile, 64-key tiles per span
+  int min_rows;       // requests of fewer rows are k_att_rows'
+  PromptShape shape;  // as the host knows it: exact, or a bound of the row tiles, which are one span each
+  int key_tiles;      // bound of a history's 64-key tiles
+  int units;          // above 0: the shape is found here, for up to so many CTAs
   float* part;
   float2* ml;
   int* err;
 };
+
+// The host knows a single request's row tiles. Those of several depend on how their queries are spread (one chunk of a prompt
+// beside many single tokens has few), and are counted here by whole warps, as is the longest history among them. Spans of 512
+// keys or more: shorter ones take from k_att_rows' CTAs what they gain (31 single tokens of 100-4,096 and a chunk of 256 on 4,096, 28
+// heads over 4 of 128: 115 us in one span, 74 in 5; with a chunk of 512 on 512 instead: 50 us, 65 in two spans of 256 keys, and
+// 55 with the count that finds none).
+__device__ __forceinline__ PromptShape shape_of_call(const PromptArgs& pa) {
+  if (!pa.units) return pa.shape;
+  const AttArgs& a = pa.a;
+  int n = 0, keys = 0;
+#pragma unroll 4
+  for (int r = threadIdx.x & 31; r < a.n_req; r += 32) {
+    int n_all;
+    const Request R = request_of(a, r, &n_all);
+    const int rows = R.n_q * a.group;
+    if (rows >= pa.min_rows) {
+      n += (rows + PR_ROWS - 1) / PR_ROWS;
+      keys = max(keys, R.len);
+    }
+  }
+  n = min(pa.shape.tiles, __reduce_add_sync(0xffffffffu, n));
+  keys = min(pa.key_tiles, __reduce_max_sync(0xffffffffu, keys) / PR_KEYS + 1);
+  return prompt_shape(n, a.kv_heads, keys, pa.units, 8);
+}
 
 // The idx-th row tile over all requests: its request (r = -1 beyond the last), what it holds, and the tile's first row. Called
 // by whole warps.
@@ -402,20 +444,22 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s;
   const AttArgs& a = pa.a;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the joining kernel, which waits for this one's end)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (k_att_rows or the joining kernel; both wait for this one's end)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.x % pa.splits, head = (blockIdx.x / pa.splits) % a.kv_heads;
+  const PromptShape shape = shape_of_call(pa);
+  const int split = (int)blockIdx.x % shape.splits, head = ((int)blockIdx.x / shape.splits) % a.kv_heads;
   // the last tiles of a causal prompt have the most keys and go first
-  const int idx = pa.tiles - 1 - blockIdx.x / (pa.splits * a.kv_heads);
+  const int idx = shape.tiles - 1 - (int)blockIdx.x / (shape.splits * a.kv_heads);
+  if (idx < 0) return;
   const TileAt at = tile_at(pa, idx);
   if (at.r < 0) return;
   const Request R = at.R;
   const int n_all = at.n_all, n_rows = R.n_q * a.group;
   int lo, hi;
   key_range(a, R, n_all, at.row0 / a.group, min(at.row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-  const Span sp = spans_of(lo, hi, pa.splits, pa.blocks, PR_KEYS);
+  const Span sp = spans_of(lo, hi, shape.splits, shape.blocks, PR_KEYS);
   if (split >= sp.used) return;
-  const int t_begin = split * pa.blocks, t_end = split == sp.used - 1 ? sp.n_blocks : t_begin + pa.blocks;
+  const int t_begin = split * shape.blocks, t_end = split == sp.used - 1 ? sp.n_blocks : t_begin + shape.blocks;
   const int n_tiles = t_end - t_begin, key_begin = sp.first + t_begin * PR_KEYS;
   const int n_q_tiles = n_rows - at.row0 > 128 ? 2 : 1;
 
@@ -687,7 +731,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     if (ok) {
       const bool whole = sp.used == 1;
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
-      const size_t unit = ((size_t)idx * a.kv_heads + head) * pa.splits + split;
+      const size_t unit = ((size_t)idx * a.kv_heads + head) * shape.splits + split;
       uint8_t* stage = sm + q * C::Q_AREA + trow * C::OUT_LD;
       if (whole) {
         constexpr int NC = 256 / (int)sizeof(T) < HD ? 256 / (int)sizeof(T) : HD;

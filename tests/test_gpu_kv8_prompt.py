@@ -92,3 +92,13 @@ def test_long_prompts_through_the_kernel_for_few_rows(dtype):
     for hd in (64, 128):
         t.run_case(dtype, 16, 14, 2, hd, [1000], [300], max_kv=200)
         t.run_case(dtype, 64, 4, 2, hd, [800, 3, 129], [200, 3, 129], max_kv=100, window=70)
+
+
+@pytest.mark.parametrize("dtype", t.TYPES)
+@pytest.mark.parametrize("H,kvh,hd", [(14, 2, 64), (28, 4, 128), (7, 1, 128)])
+@pytest.mark.parametrize("singles", [1, 20, 130])
+def test_chunks_beside_single_tokens(dtype, H, kvh, hd, singles):
+    """A few row tiles over long histories among many requests: their spans are counted on the device (up to 128 requests)."""
+    lens, n_q = [1 + 37 * i % 500 for i in range(singles)], [1] * singles
+    t.run_case(dtype, 16, H, kvh, hd, lens[:1] + [2500] + lens[1:], n_q[:1] + [130] + n_q[1:])
+    t.run_case(dtype, 64, H, kvh, hd, lens + [0, 1800, 1500], n_q + [0, 60, 200], window=900 if hd == 64 else 0)
