@@ -140,6 +140,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
         "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* u) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -214,6 +222,11 @@ struct PromptCfg {
   static constexpr int OUT_LD = 256 + 16;                // bytes per row of a row tile's output staging: up to 256 of the row
   // a row tile's queries, later the staging of its output
   static constexpr int Q_AREA = TERMS * Q_TILE > 128 * OUT_LD ? TERMS * Q_TILE : 128 * OUT_LD;
+  // Tensor cores cut off what their float32 sums cannot hold, so a sum over many tiles of keys shrinks a little with each: with
+  // float32 queries of 64 dimensions, whose TMEM has the room, O holds FOLD tiles' sum and is then added to the sum so far by the
+  // softmax warps, which round. (4,000 keys: off by 7e-6 of the output's size without, 0.8e-6 so; a chunk of 256 on 4,096 tokens
+  // takes 30 us for 27.6.)
+  static constexpr int FOLD = TERMS == 2 && HD == 64 ? 4 : 0;
   static constexpr int OFF_K = 2 * Q_AREA;
   static constexpr int STAGES = TERMS * HD > 128 ? 2 : 3;   // K and V tiles each
   static constexpr int OFF_V = OFF_K + STAGES * KV_TILE;
@@ -364,15 +377,25 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
   __syncwarp();
 }
 
-// A thread's row of O, scaled, as NC values of type U at dst (a row of the warp's staging; columns col .. col + NC of the row).
+// A thread's row of O (and of the sum of what it held before, at sum_at if that is not 0), scaled, as NC values of type U at dst (a row of the warp's staging; columns col .. col + NC of the row).
 template <class U, int NC>
-__device__ __forceinline__ void stage_row(uint8_t* dst, uint32_t o_at, bool any, float inv) {
+__device__ __forceinline__ void stage_row(uint8_t* dst, uint32_t o_at, bool any, float inv, uint32_t sum_at) {
 #pragma unroll 1
   for (int c = 0; c < NC; c += 32) {
     float o[32];
     if (any) {
       tmem_ld32(o_at + c, o);
       tc_wait_ld();
+      if (sum_at) {
+#pragma unroll
+        for (int h = 0; h < 32; h += 16) {
+          uint32_t sum[16];
+          tmem_ld16(sum_at + c + h, sum);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[h + i] += __uint_as_float(sum[i]);
+        }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 32; i++) o[i] = 0.f;
@@ -614,11 +637,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
             tc_fence_after();
             const uint64_t kd = k_desc + s * (C::KV_TILE >> 4);
 #pragma unroll
-            for (int t = 0; t < C::TERMS; t++)
+            for (int t = C::TERMS - 1; t >= 0; t--)  // (the small term first: the sum is small while it is added)
 #pragma unroll
               for (int k = 0; k < HD / 16; k++)
                 mma_f16(base + (j & 1) * PR_KEYS, q_desc + ((t * C::Q_TILE + (k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
-                        kd + (((k >> 2) * (PR_KEYS * 128) + (k & 3) * 32) >> 4), id_s, t > 0 || k > 0);
+                        kd + (((k >> 2) * (PR_KEYS * 128) + (k & 3) * 32) >> 4), id_s, t < C::TERMS - 1 || k > 0);
             mma_commit(&s_full[q][j & 1]);
             mma_commit(k_empty + s);
           }
@@ -636,7 +659,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
 #pragma unroll
             for (int k = 0; k < PR_KEYS / 16; k++)
               mma_f16_ts(base + 128, base + (j & 1) * PR_KEYS + t * (PR_KEYS / 2) + 8 * k, vd + k * (2048 >> 4), id_o,
-                         j > 0 || t > 0 || k > 0);
+                         (C::FOLD ? j % (C::FOLD ? C::FOLD : 1) > 0 : j > 0) || t > 0 || k > 0);
           mma_commit(&pv_done[q][j & 1]);
           mma_commit(v_empty + s);
         }
@@ -665,6 +688,23 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     float m_run = -INFINITY, l_run = 0.f;
     bool ready = false;
     for (int j = 0; j < n_tiles; j++) {
+      if (C::FOLD && j > 0 && j % (C::FOLD ? C::FOLD : 1) == 0) {  // (the product with this tile's weights begins O anew)
+        if (!wait_phase_warp(&pv_done[q][(j - 1) & 1], ((j - 1) >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 16) {
+          uint32_t o[16], sum[16];
+          tmem_ld16(to + c, o);
+          tmem_ld16(to + HD + c, sum);  // (what lies there before the first time is not used)
+          tc_wait_ld();
+          if (j > C::FOLD) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(sum[i]));
+          }
+          tmem_st16(to + HD + c, o);
+        }
+        tc_wait_st();
+      }
       if (j % PR_INFO == 0 && !wait_phase_warp(i_full + (j / PR_INFO & 1), (j / PR_INFO >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
       KeyInfo in[PR_KEYS / 16];
 #pragma unroll
@@ -702,6 +742,17 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
             for (int i = 0; i < 32; i++) o[i] *= f_old;
             tmem_st32(to + c, reinterpret_cast<const uint32_t*>(o));
           }
+          if (C::FOLD && j >= C::FOLD) {
+#pragma unroll 1
+            for (int c = HD; c < 2 * HD; c += 32) {
+              float o[32];
+              tmem_ld32(to + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] *= f_old;
+              tmem_st32(to + c, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
           tc_wait_st();
         }
       }
@@ -733,19 +784,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
       const size_t unit = ((size_t)idx * a.kv_heads + head) * shape.splits + split;
       uint8_t* stage = sm + q * C::Q_AREA + trow * C::OUT_LD;
+      const uint32_t sum_at = C::FOLD && n_tiles > C::FOLD ? to + HD : 0;
       if (whole) {
         constexpr int NC = 256 / (int)sizeof(T) < HD ? 256 / (int)sizeof(T) : HD;
         T* dst = static_cast<T*>(a.out) + (long long)(R.first + tok) * a.out_row + hq * a.out_head;
 #pragma unroll 1
         for (int c = 0; c < HD; c += NC) {
-          stage_row<T, NC>(stage, to + c, n_tiles > 0, inv);
+          stage_row<T, NC>(stage, to + c, n_tiles > 0, inv, sum_at ? sum_at + c : 0);
           copy_row<T, NC>(dst + c, stage, live, a.out_vec16);
         }
       } else {
         float* dst = pa.part + (unit * PR_ROWS + q * 128 + trow) * HD;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 64) {
-          stage_row<float, 64>(stage, to + c, n_tiles > 0, 1.f);
+          stage_row<float, 64>(stage, to + c, n_tiles > 0, 1.f, sum_at ? sum_at + c : 0);
           copy_row<float, 64>(dst + c, stage, live, true);
         }
       }

@@ -102,3 +102,17 @@ def test_chunks_beside_single_tokens(dtype, H, kvh, hd, singles):
     lens, n_q = [1 + 37 * i % 500 for i in range(singles)], [1] * singles
     t.run_case(dtype, 16, H, kvh, hd, lens[:1] + [2500] + lens[1:], n_q[:1] + [130] + n_q[1:])
     t.run_case(dtype, 64, H, kvh, hd, lens + [0, 1800, 1500], n_q + [0, 60, 200], window=900 if hd == 64 else 0)
+
+
+def test_float32_sums_over_many_keys():
+    """64 wide, float32: no sum in the tensor cores takes more than 4 tiles of 64 keys, 32 additions that each cut off less than
+    2^-23 of it, so the output is off by less than 2^-18 of its size whatever the length."""
+    for kv_len, n_q in (([4000], [60]), ([3000, 4000], [300, 500])):
+        gen = torch.Generator(device=t.DEV)
+        gen.manual_seed(8)
+        kv, sc, table = t.make_cache(gen, kv_len, 16, 2, 64)
+        q = torch.randn(sum(n_q), 14, 64, generator=gen, device=t.DEV)
+        q_start = [0, n_q[0], sum(n_q)][: len(n_q) + 1]
+        o, _ = t.attend(q, kv, sc, table, q_start, kv_len)
+        want = t.ref_attention(q, kv, sc, table, q_start, kv_len, 0.125, 0)[0]
+        assert float((o.double() - want).norm() / want.norm()) < 2.0**-18
