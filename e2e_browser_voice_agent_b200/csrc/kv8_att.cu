@@ -7,6 +7,9 @@
 //   16 rows of an operand tile hold 8 rows twice: a float16 term in rows 0-7 and the remainder in rows 8-15, for the
 //   queries (scaled by a power of two per row) and for the softmax weights, so the products carry 22 bits, whatever the
 //   element type, at the price of one. The group of 7 or fewer heads of a single token fills no more than 8 rows anyway.
+// * The tensor cores cut off what a float32 sum cannot hold, so a sum kept there shrinks with every addition (16,000 keys in
+//   one span: 6e-6 of the output, 131,072: 9e-5). Each block's product with V starts from zero and is added to the output
+//   outside them, with rounding (1e-7 at any length).
 // * The cache is the traffic: each lane copies its own 16-byte pieces of a block with cp.async into a ring that only it
 //   reads, so the ring needs no barrier; the order of dimensions inside a product is free as long as both operands use
 //   it, which lets a lane take 16 consecutive bytes of a key (QK) or of 4 keys (PV) without a transpose.
@@ -39,6 +42,14 @@ __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the product alone
+__device__ __forceinline__ void mma16816_new(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
   if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -62,7 +73,7 @@ struct EndAfterThePrompts {
 };
 
 template <class T, int HD>
-__global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
+__global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(const RowArgs ra) {
   const EndAfterThePrompts end;
   using S = RowSmem<HD>;
   constexpr int KC = HD / 64;   // 16-byte pieces of a key per lane
@@ -135,9 +146,9 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
         }
   }
 
-  float o[NT][4];
+  unsigned long long o[NT];  // (two dimensions)
 #pragma unroll
-  for (int t = 0; t < NT; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+  for (int t = 0; t < NT; t++) o[t] = 0;
   float m_run = -INFINITY, l_run = 0.f;
 
   // ---- the warp's blocks: b_begin + warp + 4 it
@@ -229,9 +240,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
       m_run = m_new;
       l_run *= f_old;
 #pragma unroll
-      for (int t = 0; t < NT; t++) {
-        o[t][0] *= f_old; o[t][1] *= f_old; o[t][2] *= f_old; o[t][3] *= f_old;
-      }
+      for (int t = 0; t < NT; t++) o[t] = mul2(o[t], pair(f_old, f_old));
     }
     const float m_use = (m_run == -INFINITY ? 0.f : m_run) - P_SHIFT;
     float p[4], rest[4];
@@ -264,10 +273,14 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
       for (int hpair = 0; hpair < 2; hpair++) {
         const uint32_t k01 = __byte_perm(u[0], u[1], hpair ? 0x7362 : 0x5140);
         const uint32_t k23 = __byte_perm(u[2], u[3], hpair ? 0x7362 : 0x5140);
-        mma16816(o[4 * w + 2 * hpair], a0, a1, a2, a3, half2_of(__byte_perm(k01, 0x64646464u, 0x4140)),
-                 half2_of(__byte_perm(k23, 0x64646464u, 0x4140)));
-        mma16816(o[4 * w + 2 * hpair + 1], a0, a1, a2, a3, half2_of(__byte_perm(k01, 0x64646464u, 0x4342)),
-                 half2_of(__byte_perm(k23, 0x64646464u, 0x4342)));
+        float d0[4], d1[4];
+        mma16816_new(d0, a0, a1, a2, a3, half2_of(__byte_perm(k01, 0x64646464u, 0x4140)),
+                     half2_of(__byte_perm(k23, 0x64646464u, 0x4140)));
+        mma16816_new(d1, a0, a1, a2, a3, half2_of(__byte_perm(k01, 0x64646464u, 0x4342)),
+                     half2_of(__byte_perm(k23, 0x64646464u, 0x4342)));
+        unsigned long long* sum = &o[4 * w + 2 * hpair];
+        sum[0] = add2(sum[0], add2(pair(d0[0], d0[1]), pair(d0[2], d0[3])));
+        sum[1] = add2(sum[1], add2(pair(d1[0], d1[1]), pair(d1[2], d1[3])));
       }
     }
     issue(it + RW_STAGES - 1);
@@ -286,12 +299,15 @@ __global__ void __launch_bounds__(RW_WARPS * 32) k_att_rows(const RowArgs ra) {
     jl[warp * RW_ROWS + g] = l_run;
   }
 #pragma unroll
-  for (int i = 0; i < 2; i++)
+  for (int t = 0; t < NT; t += 4) {
+    float v[4][2];
 #pragma unroll
-    for (int t = 0; t < NT; t += 4)
+    for (int i = 0; i < 4; i++) unpair(o[t + i], &v[i][0], &v[i][1]);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
       *reinterpret_cast<float4*>(js + (warp * RW_ROWS + g) * HD + VB * (2 * c + i) + t) =
-          make_float4(o[t][i] + o[t][i + 2], o[t + 1][i] + o[t + 1][i + 2], o[t + 2][i] + o[t + 2][i + 2],
-                      o[t + 3][i] + o[t + 3][i + 2]);
+          make_float4(v[0][i], v[1][i], v[2][i], v[3][i]);
+  }
   __syncthreads();
   constexpr int TPR = RW_WARPS * 32 / RW_ROWS;  // threads per row
   const int jr = threadIdx.x / TPR, jt = threadIdx.x % TPR, orow = row0 + jr;

@@ -1,0 +1,89 @@
+"""How exact attention over the paged 8-bit cache is, relative to the output's size (2-norms), against the formula in 64 bits.
+
+Values of V have a mean, so that the output's size is that of the sum over the keys and what a sum loses shows. With n the keys
+of a row, in one span (a low max_kv makes k_att_rows take them so: 4 warps, and 4 lanes each that sum the weights):
+
+* A sum of N terms of like size, each addition rounded to nearest, is off by some 2^-24 sqrt(N) / 3 of itself (the i-th addition
+  rounds i / N of it). k_att_rows: 4 sums of n / 64 terms for the output, 16 of n / 16 for the weights, together 2^-24
+  sqrt(2 n) / 48. Three times that is allowed.
+* Weights of 22 bits, exponentials off by up to 2^-22 and float32 scores near 0: 2^-21 at most, less by averaging.
+* Larger scores: with standard deviation 2 and 128 dimensions the sum of the products' magnitudes is about 14; queries of 22 bits
+  and sums of up to 16 steps make a score off by less than 14 (2^-23 + 9 x 2^-24), which is 2^-17; twice that is allowed. (Queries of
+  11 bits would give 2^-12 of it, some 1e-4.)
+"""
+import math
+
+import pytest
+import torch
+
+import test_gpu_kv8 as t
+
+pytestmark = pytest.mark.gpu
+F32 = torch.float32
+
+
+def attend(dtype, heads, kvh, hd, n, n_q, spread, page=64, seed=0, **kw):
+    """(outputs, 64-bit outputs) of a few heads of one request of n positions whose last n_q are the queries; spread: the standard
+    deviation of the scores."""
+    gen = torch.Generator(device=t.DEV)
+    gen.manual_seed(seed + n + hd + n_q)
+    pages = -(-n // page)
+    kv = torch.randn(pages, 2, kvh, page, hd, generator=gen, device=t.DEV).mul_(34).round_().clamp_(-127, 127).to(torch.int8)
+    kv[:, 1] = kv[:, 1].div(2, rounding_mode="floor") + 40
+    sc = 0.03 * torch.exp(0.3 * torch.randn(pages, 2, kvh, generator=gen, device=t.DEV))
+    q = (torch.randn(n_q, heads, hd, generator=gen, device=t.DEV) * spread).to(dtype)
+    table = torch.randperm(pages, generator=gen, device=t.DEV).int()[None]
+    out, lse = t.attend(q, kv, sc, table, [0, n_q], [n], **kw)
+    some = sorted({0, heads // 2, heads - 1})
+    want = torch.empty(n_q, len(some), hd, dtype=torch.float64, device=t.DEV)
+    held = kv[table[0].long()].double() * sc[table[0].long()].double()[..., None, None]
+    key = torch.arange(n, device=t.DEV)
+    for i, h in enumerate(some):
+        k, v = (held[:, w, h // (heads // kvh)].reshape(-1, hd)[:n] for w in (0, 1))
+        for a in range(0, n_q, 100):
+            pos = n - n_q + torch.arange(a, min(n_q, a + 100), device=t.DEV)
+            x = (q[a:a + 100, h].double() @ k.t() * hd ** -0.5).masked_fill(key > pos[:, None], -math.inf)
+            want[a:a + 100, i] = torch.softmax(x, 1) @ v
+            assert float((lse[a:a + 100, h].double() - torch.logsumexp(x, 1)).abs().max()) < 2.0**-17 * max(1, spread)
+    return out[:, some], want
+
+
+def off(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+# ---------------------------------------------------------------------------------------------- the kernel for few rows
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [300, 1000, 4000, 16000, 64000, 131072])
+@pytest.mark.parametrize("n_q", [1, 10])
+def test_few_rows_in_one_span(hd, n, n_q):
+    got, want = attend(F32, 1, 1, hd, n, n_q, 0.1, max_kv=16)
+    assert off(got, want) < 2.0**-21 + 2.0**-24 * math.sqrt(2 * n) / 16
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [700, 1900, 30000])
+def test_few_rows_in_spans(hd, n):
+    """A cluster's spans, and spans that a second kernel joins: the sums are shorter."""
+    for heads, kvh, n_q in ((7, 1, 1), (1, 1, 10)):
+        got, want = attend(F32, heads, kvh, hd, n, n_q, 0.1)
+        assert off(got, want) < 2.0**-21 + 2.0**-24 * math.sqrt(2 * n) / 16
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kw", [{}, {"max_kv": 16}])
+def test_few_rows_with_larger_scores(hd, kw):
+    for n in (300, 5000):
+        got, want = attend(F32, 2, 1, hd, n, 4, 2.0, **kw)
+        assert off(got, want) < 2.0**-16
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_few_16_bit_rows_are_rounded_once(dtype, hd):
+    """The error is that of rounding the exact output (what is below 2^-18 before it adds to it in squares, and moves values
+    across a rounding boundary as often one way as the other)."""
+    for n in (300, 131072):
+        got, want = attend(dtype, 7, 1, hd, n, 4, 0.1 if n > 1000 else 2.0, max_kv=16)
+        assert off(got, want) < 1.02 * off(want.to(dtype), want)
