@@ -561,8 +561,16 @@ struct WorkPlan {
   PromptShape shape;
   unsigned p_join;                             // CTAs of its joining kernel, 0 without one
   size_t units;                                // row tiles x spans in the workspace
+  bool spill;                                  // its sums go through the workspace
   size_t bytes;
 };
+template <class C>
+int fold_of() { return C::SPILL ? C::FOLD : INT_MAX; }
+// Tiles of keys after which k_att_prompt's sums go to the workspace.
+int spill_after(int type, int head_dim) {
+  if (head_dim == 64) return INT_MAX;
+  return type == H2C_TYPE_F32 ? fold_of<PromptCfg<float, 128>>() : INT_MAX;
+}
 WorkPlan plan_work(const h2c_kv8_attention_args* g) {
   WorkPlan p = {};
   const long long group = g->heads / g->kv_heads, most_rows = g->max_q * group;
@@ -607,7 +615,12 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g) {
                           join_ctas(std::min(groups, 148LL / (JOIN_WARP_SPANS + 1)) * PR_ROWS, JOIN_WARP_SPANS + 1));
     }
   }
-  p.bytes = (p.units * RW_ROWS + (size_t)p.p_units * PR_ROWS) * ((size_t)g->head_dim * 4 + 8);
+  // whether a row tile can have more tiles of keys than a sum may take, whatever max_kv says
+  const long long room = (long long)g->table_cols * g->page_size;
+  const long long most_keys = g->window > 0 ? std::min(room, (long long)g->window + PR_ROWS + 16) : room;
+  p.spill = p.prompt && (most_keys + PR_KEYS - 1) / PR_KEYS + 1 > spill_after(g->type, g->head_dim);
+  p.bytes = (p.units * RW_ROWS + (size_t)p.p_units * PR_ROWS) * ((size_t)g->head_dim * 4 + 8) +
+            (p.spill ? (size_t)PR_SLOTS * PR_ROWS * g->head_dim * 4 : 0);
   return p;
 }
 
@@ -615,10 +628,11 @@ template <class T, int HD>
 int launch(const char* who, const WorkPlan& p, AttArgs a, void* workspace, cudaStream_t st) {
   float* part = static_cast<float*>(workspace);
   float* p_part = part + p.units * RW_ROWS * HD;
-  float2* ml = reinterpret_cast<float2*>(p_part + (size_t)p.p_units * PR_ROWS * HD);
+  float* sums = p_part + (size_t)p.p_units * PR_ROWS * HD;
+  float2* ml = reinterpret_cast<float2*>(sums + (p.spill ? (size_t)PR_SLOTS * PR_ROWS * HD : 0));
   int* err = p.prompt ? op_err_words() : nullptr;
   if (p.prompt && !err) return op_error(H2C_ERR_CUDA, "%s: no device", who);
-  const PromptArgs pa{a, p.min_rows, p.shape, p.p_keys, p.counted ? p.p_units : 0, p_part, ml + p.units * RW_ROWS, err};
+  const PromptArgs pa{a, p.min_rows, p.shape, p.p_keys, p.counted ? p.p_units : 0, p_part, ml + p.units * RW_ROWS, p.spill ? sums : nullptr, err};
   const RowArgs ra{a, p.splits, p.blocks, p.tiles, p.max_rows, p.cluster, part, ml};
   // a kernel that may start while the one before it still runs waits for that one's end itself
   cudaLaunchAttribute dependent;

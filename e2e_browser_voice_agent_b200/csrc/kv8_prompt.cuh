@@ -33,7 +33,8 @@ namespace h2 {
 namespace {
 
 constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 5 * 128, PR_INFO = 32;
-enum { PR_CONVERT = 21, PR_MMA = 22, PR_SOFTMAX = 23 };
+constexpr int PR_SLOTS = 192;  // places for spilled sums
+enum { PR_CONVERT = 21, PR_MMA = 22, PR_SOFTMAX = 23, PR_SLOT = 24 };
 
 // The row tiles of all requests, the spans that each is cut into, and the 64-key tiles of a span.
 struct PromptShape {
@@ -59,6 +60,7 @@ struct PromptArgs {
   int units;          // above 0: the shape is found here, for up to so many CTAs
   float* part;
   float2* ml;
+  float* sums;        // (PromptCfg::SPILL) PR_SLOTS places of 256 rows' sums; nullptr where no row tile has more than FOLD tiles of keys
   int* err;
 };
 
@@ -227,11 +229,18 @@ struct PromptCfg {
   static constexpr int OUT_LD = 256 + 16;                // bytes per row of a row tile's output staging: up to 256 of the row
   // a row tile's queries, later the staging of its output
   static constexpr int Q_AREA = TERMS * Q_TILE > 128 * OUT_LD ? TERMS * Q_TILE : 128 * OUT_LD;
-  // Tensor cores cut off what their float32 sums cannot hold, so a sum over many tiles of keys shrinks a little with each: with
-  // float32 queries of 64 dimensions, whose TMEM has the room, O holds FOLD tiles' sum and is then added to the sum so far by the
-  // softmax warps, which round. (4,000 keys: off by 7e-6 of the output's size without, 0.8e-6 so; a chunk of 256 on 4,096 tokens
-  // takes 30 us for 27.6.)
-  static constexpr int FOLD = TERMS == 2 && HD == 64 ? 4 : 0;
+  // Tensor cores cut off what their float32 sums cannot hold, so a sum over many tiles of keys shrinks with each. O therefore
+  // holds FOLD tiles' sum and is then added to the sum so far by the softmax warps, which round. 64 wide that lies beside O in
+  // TMEM; 128 wide there is no room, and it lies in a place of the workspace (SPILL, claim_slot). Float32 in one span of 4,000
+  // and 131,072 keys, relative to the output: off by 7e-6 and 4.5e-4 without; 4e-7 and 1.5e-6 so 64 wide (a chunk of 256 on 4,096
+  // tokens takes 30 us for 27.6), 8e-7 and 1.6e-6 128 wide (that chunk, 28 heads over 4, 59 us for 53, prompts of 2,064-4,099
+  // 760 for 650: the places' way to L2. 4 tiles: 63 and 830 us, 4e-7 and 1.4e-6; CTAs of one row tile, whose sum fits into the
+  // other's TMEM: 78 and 1,071).
+  static constexpr int FOLD = TERMS == 2 ? (HD == 64 ? 4 : 8) : 0;
+  static constexpr bool SPILL = FOLD && HD == 128;
+  static __device__ __forceinline__ bool folds(int j) {  // whether O begins anew with tile j of keys
+    return FOLD && j > 0 && j % (FOLD ? FOLD : 1) == 0;
+  }
   static constexpr int OFF_K = 2 * Q_AREA;
   static constexpr int STAGES = TERMS * HD > 128 ? 2 : 3;   // K and V tiles each
   static constexpr int OFF_V = OFF_K + STAGES * KV_TILE;
@@ -382,9 +391,58 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
   __syncwarp();
 }
 
-// A thread's row of O (and of the sum of what it held before, at sum_at if that is not 0), scaled, as NC values of type U at dst (a row of the warp's staging; columns col .. col + NC of the row).
+// A place for spilled sums that no other CTA at work holds, for a whole CTA until release_slot: by one thread. An SM has one CTA
+// of k_att_prompt at a time (its shared memory), so there are more places than CTAs at work in all streams together, and the first
+// that is tried, the SM's number, is nearly always free. -1 (and the abort flag) if none was within the time limit.
+__device__ int g_slot_held[PR_SLOTS];  // 0 between kernels
+__device__ __forceinline__ int claim_slot(const Abort& a) {
+  unsigned sm;
+  asm volatile("mov.u32 %0, %smid;" : "=r"(sm));
+  int at = (int)(sm % PR_SLOTS);
+  const unsigned long long t0 = now_ns();
+  for (unsigned it = 1;; it++) {
+    if (atomicCAS(g_slot_held + at, 0, 1) == 0) break;
+    at = at + 1 == PR_SLOTS ? 0 : at + 1;
+    if (it % PR_SLOTS == 0 && now_ns() - t0 > TIMEOUT_NS) {
+      raise_abort(a, PR_SLOT);
+      return -1;
+    }
+  }
+  __threadfence();
+  return at;
+}
+__device__ __forceinline__ void release_slot(int slot) {
+  __threadfence();
+  atomicExch(g_slot_held + slot, 0);
+}
+
+// The place of a thread's columns col .. col + 3 in a row tile's spilled sums: [columns / 4][128 rows], so that a warp's accesses are
+// whole lines. (Read and written in L2: the place was another SM's before.)
+__device__ __forceinline__ float4* spill_at(float* sums, int trow, int col) {
+  return reinterpret_cast<float4*>(sums) + (col >> 2) * 128 + trow;
+}
+// A row's O (128 columns) added to its spilled sum, which is multiplied by f first; the first time there is none.
+__device__ __forceinline__ void spill_row(float* sums, int trow, uint32_t o_at, float f, bool first) {
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 32) {
+    float4 sum[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum[i] = first ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(spill_at(sums, trow, c + 4 * i));
+    float o[32];
+    tmem_ld32(o_at + c, o);
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      __stcg(spill_at(sums, trow, c + 4 * i), make_float4(fmaf(sum[i].x, f, o[4 * i]), fmaf(sum[i].y, f, o[4 * i + 1]),
+                                                          fmaf(sum[i].z, f, o[4 * i + 2]), fmaf(sum[i].w, f, o[4 * i + 3])));
+  }
+}
+
+// A thread's row of O (and of the sum of what it held before: at sum_at in TMEM if that is not 0, or spilled, times f, if sums is
+// not null), scaled, as NC values of type U at dst (a row of the warp's staging; columns col .. col + NC of the row).
 template <class U, int NC>
-__device__ __forceinline__ void stage_row(uint8_t* dst, uint32_t o_at, bool any, float inv, uint32_t sum_at) {
+__device__ __forceinline__ void stage_row(uint8_t* dst, uint32_t o_at, bool any, float inv, uint32_t sum_at, float* sums, int trow,
+                                          int col, float f) {
 #pragma unroll 1
   for (int c = 0; c < NC; c += 32) {
     float o[32];
@@ -399,6 +457,16 @@ __device__ __forceinline__ void stage_row(uint8_t* dst, uint32_t o_at, bool any,
           tc_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; i++) o[h + i] += __uint_as_float(sum[i]);
+        }
+      }
+      if (sums) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float4 x = __ldcg(spill_at(sums, trow, col + c + 4 * i));
+          o[4 * i] = fmaf(x.x, f, o[4 * i]);
+          o[4 * i + 1] = fmaf(x.y, f, o[4 * i + 1]);
+          o[4 * i + 2] = fmaf(x.z, f, o[4 * i + 2]);
+          o[4 * i + 3] = fmaf(x.w, f, o[4 * i + 3]);
         }
       }
     } else {
@@ -470,7 +538,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   __shared__ int go[2][2];
   __shared__ float row_scale[PR_ROWS];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_s;
+  __shared__ int abort_s, slot_s;
   const AttArgs& a = pa.a;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (k_att_rows or the joining kernel; both wait for this one's end)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -513,6 +581,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     }
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (C::SPILL) slot_s = pa.sums && n_tiles > C::FOLD ? claim_slot(Abort{&abort_s, pa.err}) : -1;
   }
   if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_slot)) : "memory");
@@ -523,6 +592,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const Abort ab{&abort_s, pa.err};
+  const int slot = C::SPILL ? slot_s : -1;
 
   if (warp >= 8 && warp < 16) {  // ---------------- converters: warps 8-11 for K, warps 12-15 for V
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -664,7 +734,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
 #pragma unroll
             for (int k = 0; k < PR_KEYS / 16; k++)
               mma_f16_ts(base + 128, base + (j & 1) * PR_KEYS + t * (PR_KEYS / 2) + 8 * k, vd + k * (2048 >> 4), id_o,
-                         (C::FOLD ? j % (C::FOLD ? C::FOLD : 1) > 0 : j > 0) || t > 0 || k > 0);
+                         (j > 0 && !(C::folds(j) && (!C::SPILL || slot >= 0))) || t > 0 || k > 0);
           mma_commit(&pv_done[q][j & 1]);
           mma_commit(v_empty + s);
         }
@@ -691,13 +761,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     const float f_row = n_tiles > 0 ? row_scale[q * 128 + trow] : 0.f;
     const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + q * 256, to = tl + 128;
     float m_run = -INFINITY, l_run = 0.f;
+    // (spilled sums) the maximum that they are relative to
+    float m_sum = -INFINITY;
+    float* sums = C::SPILL && slot >= 0 ? pa.sums + ((size_t)slot * 2 + q) * (128 * HD) : nullptr;
     bool ready = false;
     for (int j = 0; j < n_tiles; j++) {
-      if (C::FOLD && j > 0 && j % (C::FOLD ? C::FOLD : 1) == 0) {  // (the product with this tile's weights begins O anew)
+      if (C::folds(j) && (!C::SPILL || slot >= 0)) {  // (the product with this tile's weights begins O anew)
         if (!wait_phase_warp(&pv_done[q][(j - 1) & 1], ((j - 1) >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
         tc_fence_after();
+        if (C::SPILL) {
+          spill_row(sums, trow, to, m_sum == m_run ? 1.f : exp2_fast(m_sum - m_run), j == C::FOLD);
+          m_sum = m_run;
+        }
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
+        for (int c = 0; c < (C::SPILL ? 0 : HD); c += 16) {
           uint32_t o[16], sum[16];
           tmem_ld16(to + c, o);
           tmem_ld16(to + HD + c, sum);  // (what lies there before the first time is not used)
@@ -747,7 +824,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
             for (int i = 0; i < 32; i++) o[i] *= f_old;
             tmem_st32(to + c, reinterpret_cast<const uint32_t*>(o));
           }
-          if (C::FOLD && j >= C::FOLD) {
+          if (C::FOLD && !C::SPILL && j >= C::FOLD) {
 #pragma unroll 1
             for (int c = HD; c < 2 * HD; c += 32) {
               float o[32];
@@ -789,20 +866,23 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
       const size_t unit = ((size_t)idx * a.kv_heads + head) * shape.splits + split;
       uint8_t* stage = sm + q * C::Q_AREA + trow * C::OUT_LD;
-      const uint32_t sum_at = C::FOLD && n_tiles > C::FOLD ? to + HD : 0;
+      const bool folded = C::FOLD && n_tiles > C::FOLD;
+      const uint32_t sum_at = folded && !C::SPILL ? to + HD : 0;
+      float* spilled = folded && C::SPILL ? sums : nullptr;  // (null without a place)
+      const float f_sum = m_sum == m_run ? 1.f : exp2_fast(m_sum - m_run);
       if (whole) {
         constexpr int NC = 256 / (int)sizeof(T) < HD ? 256 / (int)sizeof(T) : HD;
         T* dst = static_cast<T*>(a.out) + (long long)(R.first + tok) * a.out_row + hq * a.out_head;
 #pragma unroll 1
         for (int c = 0; c < HD; c += NC) {
-          stage_row<T, NC>(stage, to + c, n_tiles > 0, inv, sum_at ? sum_at + c : 0);
+          stage_row<T, NC>(stage, to + c, n_tiles > 0, inv, sum_at ? sum_at + c : 0, spilled, trow, c, f_sum);
           copy_row<T, NC>(dst + c, stage, live, a.out_vec16);
         }
       } else {
         float* dst = pa.part + (unit * PR_ROWS + q * 128 + trow) * HD;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 64) {
-          stage_row<float, 64>(stage, to + c, n_tiles > 0, 1.f, sum_at ? sum_at + c : 0);
+          stage_row<float, 64>(stage, to + c, n_tiles > 0, 1.f, sum_at ? sum_at + c : 0, spilled, trow, c, f_sum);
           copy_row<float, 64>(dst + c, stage, live, true);
         }
       }
@@ -816,6 +896,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   }
   tc_fence_before();
   __syncthreads();
+  if (C::SPILL && threadIdx.x == 0 && slot >= 0) release_slot(slot);
   if (warp == 16) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

@@ -87,3 +87,84 @@ def test_few_16_bit_rows_are_rounded_once(dtype, hd):
     for n in (300, 131072):
         got, want = attend(dtype, 7, 1, hd, n, 4, 0.1 if n > 1000 else 2.0, max_kv=16)
         assert off(got, want) < 1.02 * off(want.to(dtype), want)
+
+
+# ---------------------------------------------------------------------------------------------- the kernel for prompts
+#
+# Its sums lie in the tensor cores for 4 tiles of 64 keys (64 wide) or 8 (128 wide), 8 additions a tile for float32: each cuts off
+# less than 2^-23 of the sum, which grows evenly, so together less than F 2^-24 with F = 32 or 64. What is rounded: n / 16 additions
+# of a row's weights and n / 256 or more of its output: 2^-24 sqrt(n) / 12 together, three times that allowed.
+
+def prompt_bound(hd, n):
+    return (32 if hd == 64 else 64) * 2.0**-24 + 2.0**-21 + 2.0**-24 * math.sqrt(n) / 4
+
+
+def prompt_heads(hd):
+    """Heads, kv heads and queries whose row tiles fill the SMs, so that a history is one span."""
+    return (14, 2, 1400) if hd == 64 else (28, 4, 780)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1500, 4000, 16000, 64000, 131072])
+@pytest.mark.parametrize("kw", [{}, {"max_kv": 0}])
+def test_prompts_in_one_span(hd, n, kw):
+    heads, kvh, n_q = prompt_heads(hd)
+    got, want = attend(F32, heads, kvh, hd, n, n_q, 0.1, **kw)
+    assert off(got, want) < prompt_bound(hd, n)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [900, 20000, 131072])
+def test_prompts_in_spans(hd, n):
+    got, want = attend(F32, 14, 2, hd, n, 60, 0.1)
+    assert off(got, want) < prompt_bound(hd, n)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompts_with_larger_scores_and_a_window(hd):
+    heads, kvh, n_q = prompt_heads(hd)
+    got, want = attend(F32, heads, kvh, hd, 5000, n_q, 2.0)
+    assert off(got, want) < 2.0**-16
+    gen = torch.Generator(device=t.DEV)
+    gen.manual_seed(3)
+    t.run_case(F32, 16, heads, kvh, hd, [3000, 40], [n_q, 40], window=1100)
+
+
+def test_sums_that_change_their_scale():
+    """128 wide: keys whose scores rise along the history move the maximum between the sums that go to the workspace."""
+    gen = torch.Generator(device=t.DEV)
+    gen.manual_seed(4)
+    n, n_q = 6000, 900
+    kv, sc, table = t.make_cache(gen, [n], 64, 2, 128, spread=0.3)
+    rise = torch.linspace(0.0, 3.0, table.shape[1], device=t.DEV).exp()
+    sc[table[0].long(), 0] *= rise[:, None]
+    for dtype in t.TYPES:
+        q = torch.randn(n_q, 16, 128, generator=gen, device=t.DEV).mul(0.3).to(dtype)
+        out, lse = t.attend(q, kv, sc, table, [0, n_q], [n])
+        t.close(out, lse, t.ref_attention(q, kv, sc, table, [0, n_q], [n], 128 ** -0.5, 0), dtype, dtype != F32)
+
+
+def test_two_streams_at_once():
+    """Calls that run together keep their sums apart."""
+    gen = torch.Generator(device=t.DEV)
+    gen.manual_seed(5)
+    calls = []
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=t.DEV)
+    for n, n_q in ((9000, 300), (7000, 200)):
+        kv, sc, table = t.make_cache(gen, [n], 64, 4, 128)
+        q = torch.randn(n_q, 28, 128, generator=gen, device=t.DEV)
+        args = (q, kv, sc, table, i32(0, n_q), i32(n), n_q, n)
+        calls.append(lambda args=args: t.kv8().attention(*args))
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[], []]
+    for _ in range(10):
+        for s, c, g in zip(streams, calls, got):
+            with torch.cuda.stream(s):
+                g.append(c())
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in g)
+    from e2e_browser_voice_agent_b200 import _lib
+    _lib.check_ops()
