@@ -564,12 +564,12 @@ struct WorkPlan {
   bool spill;                                  // its sums go through the workspace
   size_t bytes;
 };
-template <class C>
-int fold_of() { return C::SPILL ? C::FOLD : INT_MAX; }
 // Tiles of keys after which k_att_prompt's sums go to the workspace.
 int spill_after(int type, int head_dim) {
   if (head_dim == 64) return INT_MAX;
-  return type == H2C_TYPE_F32 ? fold_of<PromptCfg<float, 128>>() : INT_MAX;
+  return type == H2C_TYPE_F32 ? PromptCfg<float, 128>::FOLD
+         : type == H2C_TYPE_F16 ? PromptCfg<__half, 128>::FOLD
+                                : PromptCfg<__nv_bfloat16, 128>::FOLD;
 }
 WorkPlan plan_work(const h2c_kv8_attention_args* g) {
   WorkPlan p = {};

@@ -29,6 +29,8 @@
 #include "kv8_att.cuh"
 #include "tc5_ptx.cuh"
 
+#include <type_traits>
+
 namespace h2 {
 namespace {
 
@@ -222,35 +224,35 @@ __device__ __forceinline__ uint32_t sw128(int r, int c) { return r * 128 + ((c ^
 
 template <class T, int HD>
 struct PromptCfg {
-  static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // float16 terms of queries and weights
+  static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int Q_TERMS = sizeof(T) == 4 ? 2 : 1;  // float16 terms of queries
+  static constexpr int P_TERMS = Q_TERMS;                 // and of weights
   static constexpr int BLKS = HD / 64;                   // 64-dimension blocks of a row
   static constexpr int Q_TILE = 128 * HD * 2;            // one row tile, one term
   static constexpr int KV_TILE = PR_KEYS * HD * 2;
   static constexpr int OUT_LD = 256 + 16;                // bytes per row of a row tile's output staging: up to 256 of the row
   // a row tile's queries, later the staging of its output
-  static constexpr int Q_AREA = TERMS * Q_TILE > 128 * OUT_LD ? TERMS * Q_TILE : 128 * OUT_LD;
+  static constexpr int Q_AREA = Q_TERMS * Q_TILE > 128 * OUT_LD ? Q_TERMS * Q_TILE : 128 * OUT_LD;
   // Tensor cores cut off what their float32 sums cannot hold, so a sum over many tiles of keys shrinks with each. O therefore
   // holds FOLD tiles' sum and is then added to the sum so far by the softmax warps, which round. 64 wide that lies beside O in
-  // TMEM; 128 wide there is no room, and it lies in a place of the workspace (SPILL, claim_slot). Float32 in one span of 4,000
-  // and 131,072 keys, relative to the output: off by 7e-6 and 4.5e-4 without; 4e-7 and 1.5e-6 so 64 wide (a chunk of 256 on 4,096
-  // tokens takes 30 us for 27.6), 8e-7 and 1.6e-6 128 wide (that chunk, 28 heads over 4, 59 us for 53, prompts of 2,064-4,099
-  // 760 for 650: the places' way to L2. 4 tiles: 63 and 830 us, 4e-7 and 1.4e-6; CTAs of one row tile, whose sum fits into the
-  // other's TMEM: 78 and 1,071).
-  static constexpr int FOLD = TERMS == 2 ? (HD == 64 ? 4 : 8) : 0;
-  static constexpr bool SPILL = FOLD && HD == 128;
-  static __device__ __forceinline__ bool folds(int j) {  // whether O begins anew with tile j of keys
-    return FOLD && j > 0 && j % (FOLD ? FOLD : 1) == 0;
-  }
+  // TMEM; 128 wide there is no room, and it lies in a place of the workspace (SPILL, claim_slot). One span of 4,000 and 131,072 keys,
+  // relative to the output: off by 7e-6 and 4.5e-4 without (16-bit types, before their rounding: 5e-6 and 4e-4). Float32 4e-7 and
+  // 1.5e-6 so 64 wide (a chunk of 256 on 4,096 tokens takes 30 us for 27.6), 8e-7 and 1.6e-6 128 wide (that chunk, 28 heads over 4, 60
+  // us for 53, prompts of 2,064-4,099 770 for 650: the places' way to L2. 4 tiles: 63 and 830 us, 4e-7 and 1.4e-6; CTAs of one row
+  // tile, whose sum fits into the other's TMEM: 78 and 1,071). 16-bit types 1.2e-5 and less, a twentieth of float16's rounding: chunks
+  // on 32,000 and more keys take 2-3% longer.
+  static constexpr int FOLD = sizeof(T) == 4 ? (HD == 64 ? 4 : 8) : HD == 64 ? 32 : BF16 ? 128 : 64;
+  static constexpr bool SPILL = HD == 128;
   static constexpr int OFF_K = 2 * Q_AREA;
-  static constexpr int STAGES = TERMS * HD > 128 ? 2 : 3;   // K and V tiles each
+  static constexpr int STAGES = Q_TERMS * HD > 128 ? 2 : 3;   // K and V tiles each
   static constexpr int OFF_V = OFF_K + STAGES * KV_TILE;
   static constexpr int SMEM = OFF_V + STAGES * KV_TILE + 1024;
   static_assert(Q_AREA % 1024 == 0 && SMEM <= 226 * 1024, "shared memory budget");
 };
 
-// The weights of one tile of keys for one row: scores s (products of codes) to p = 2^(s f + e - m), packed as float16 (and the
-// remainders when two terms are kept); the sum of the softmax's weights is added to l. base = P_SHIFT - m.
-template <int TERMS, bool EDGE>
+// The weights of one tile of keys for one row: scores s (products of codes) to p = 2^(s f + e - m), times V's mantissa where the
+// exponent does not hold it (MANT), packed as float16 (and the remainders when two terms are kept); the sum of the softmax's weights is added to l. base = P_SHIFT - m.
+template <int TERMS, bool MANT, bool EDGE>
 __device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float base, int key0, int first_key,
                                         int pos, uint32_t* p, uint32_t* rest, float* l) {
 #pragma unroll
@@ -270,9 +272,11 @@ __device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float
       w0 = exp2_fast(w0);
       w1 = exp2_fast(w1);
       sum = add2(sum, pair(w0, w1));
-      if (TERMS == 2) {
+      if (MANT) {
         w0 *= in[g].mant;
         w1 *= in[g].mant;
+      }
+      if (TERMS == 2) {
         const __half2 t = __floats2half2_rn(w0, w1);
         p[8 * g + i / 2] = *reinterpret_cast<const uint32_t*>(&t);
         rest[8 * g + i / 2] = pack_half2(w0 - __low2float(t), w1 - __high2float(t));
@@ -329,7 +333,7 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
       const uint32_t dst = su32(blk + sw128(r0 + p * RPP + sub, piece & 7));
       const int bytes = tile0 + r0 + p * RPP + sub < n_rows ? 16 : 0;  // (what is not copied is filled with zeros)
 #pragma unroll
-      for (int t = 0; t < C::TERMS; t++)
+      for (int t = 0; t < C::Q_TERMS; t++)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + t * C::Q_TILE), "l"(src + t * 4), "r"(bytes)
                      : "memory");
     }
@@ -355,7 +359,7 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
     for (int b = 0; b < NB; b++) {
       const uint8_t* at = blk + sw128(r0 + (p0 + b) * RPP + sub, piece & 7);
 #pragma unroll
-      for (int t = 0; t < C::TERMS; t++) {
+      for (int t = 0; t < C::Q_TERMS; t++) {
         const uint4 x = *reinterpret_cast<const uint4*>(at + t * C::Q_TILE);
         v[b].w[4 * t] = x.x, v[b].w[4 * t + 1] = x.y, v[b].w[4 * t + 2] = x.z, v[b].w[4 * t + 3] = x.w;
       }
@@ -380,11 +384,11 @@ __device__ __forceinline__ void put_queries(const AttArgs& a, long long row_at, 
         const float x0 = v[b].at(2 * i) * mul, x1 = v[b].at(2 * i + 1) * mul;
         const __half2 t = __floats2half2_rn(x0, x1);
         h[i] = *reinterpret_cast<const uint32_t*>(&t);
-        if (C::TERMS == 2) rest[i] = pack_half2(x0 - __low2float(t), x1 - __high2float(t));
+        if (C::Q_TERMS == 2) rest[i] = pack_half2(x0 - __low2float(t), x1 - __high2float(t));
       }
       uint8_t* at = blk + sw128(r, piece & 7);
       *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
-      if (C::TERMS == 2) *reinterpret_cast<uint4*>(at + C::Q_TILE) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+      if (C::Q_TERMS == 2) *reinterpret_cast<uint4*>(at + C::Q_TILE) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
     }
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -592,7 +596,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const Abort ab{&abort_s, pa.err};
-  const int slot = C::SPILL ? slot_s : -1;
+  const int fold = C::SPILL && slot_s < 0 ? n_tiles : C::FOLD;  // (at least n_tiles: never)
 
   if (warp >= 8 && warp < 16) {  // ---------------- converters: warps 8-11 for K, warps 12-15 for V
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -652,7 +656,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         KeyInfo ki;
         ki.k = sk[i];
         split_scale(sv[i], &ki.e, &ki.mant, &ki.inv);
-        if (C::TERMS == 1) {  // the whole scale goes into the exponent (its logarithm is off by 2^-22 of the result)
+        if (sizeof(T) == 2) {  // the whole scale goes into the exponent (its logarithm is off by 2^-22 of the result)
           const float mant = fmaxf(ki.mant, 1.f);  // (a scale below 2^-62, or 0, counts as 2^-62)
           ki.e += __log2f(mant);
           ki.inv = __fdividef(ki.inv, mant);
@@ -712,11 +716,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
             tc_fence_after();
             const uint64_t kd = k_desc + s * (C::KV_TILE >> 4);
 #pragma unroll
-            for (int t = C::TERMS - 1; t >= 0; t--)  // (the small term first: the sum is small while it is added)
+            for (int t = C::Q_TERMS - 1; t >= 0; t--)  // (the small term first: the sum is small while it is added)
 #pragma unroll
               for (int k = 0; k < HD / 16; k++)
                 mma_f16(base + (j & 1) * PR_KEYS, q_desc + ((t * C::Q_TILE + (k >> 2) * (128 * 128) + (k & 3) * 32) >> 4),
-                        kd + (((k >> 2) * (PR_KEYS * 128) + (k & 3) * 32) >> 4), id_s, t < C::TERMS - 1 || k > 0);
+                        kd + (((k >> 2) * (PR_KEYS * 128) + (k & 3) * 32) >> 4), id_s, t < C::Q_TERMS - 1 || k > 0);
             mma_commit(&s_full[q][j & 1]);
             mma_commit(k_empty + s);
           }
@@ -724,17 +728,20 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         const uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B in MN-major form
         // (V's blocks of 64 dimensions lie PR_KEYS rows apart)
         const uint64_t v_desc = desc_sw128(su32(sm + C::OFF_V), 1024) + ((uint64_t)(((PR_KEYS * 128) >> 4) - 1) << 16);
+        int anew = 0;  // the tile with which O begins anew
         for (int j = 0; j < n_tiles; j++) {
           const int s = j % STG;
+          const bool add = j != anew;
+          if (!add) anew += fold;
           if (!wait_two(v_full + s, (j / STG) & 1, &p_full[q][j & 1], (j >> 1) & 1, ab, PR_MMA)) break;
           tc_fence_after();
           const uint64_t vd = v_desc + s * (C::KV_TILE >> 4);
 #pragma unroll
-          for (int t = 0; t < C::TERMS; t++)
+          for (int t = 0; t < C::P_TERMS; t++)
 #pragma unroll
             for (int k = 0; k < PR_KEYS / 16; k++)
               mma_f16_ts(base + 128, base + (j & 1) * PR_KEYS + t * (PR_KEYS / 2) + 8 * k, vd + k * (2048 >> 4), id_o,
-                         (j > 0 && !(C::folds(j) && (!C::SPILL || slot >= 0))) || t > 0 || k > 0);
+                         add || t > 0 || k > 0);
           mma_commit(&pv_done[q][j & 1]);
           mma_commit(v_empty + s);
         }
@@ -761,33 +768,38 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     const float f_row = n_tiles > 0 ? row_scale[q * 128 + trow] : 0.f;
     const uint32_t tl = tmem + ((uint32_t)(32 * w4) << 16) + q * 256, to = tl + 128;
     float m_run = -INFINITY, l_run = 0.f;
-    // (spilled sums) the maximum that they are relative to
-    float m_sum = -INFINITY;
-    float* sums = C::SPILL && slot >= 0 ? pa.sums + ((size_t)slot * 2 + q) * (128 * HD) : nullptr;
+    float m_sum = -INFINITY;  // (spilled sums) the maximum that they are relative to
+    auto sums = [&] { return pa.sums + (slot_s * 2 + q) * (128 * HD); };
+    int anew = fold;
+    auto add_up = [&](int j) {  // O to the sum so far: the product with the weights of tile j begins it anew
+      anew += fold;
+      if (!wait_phase_warp(&pv_done[q][(j - 1) & 1], ((j - 1) >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
+      tc_fence_after();
+      if (C::SPILL) {
+        spill_row(sums(), trow, to, m_sum == m_run ? 1.f : exp2_fast(m_sum - m_run), j == C::FOLD);
+        m_sum = m_run;
+      }
+#pragma unroll 1
+      for (int c = 0; c < (C::SPILL ? 0 : HD); c += 16) {
+        uint32_t o[16], sum[16];
+        tmem_ld16(to + c, o);
+        tmem_ld16(to + HD + c, sum);  // (what lies there before the first time is not used)
+        tc_wait_ld();
+        if (j > C::FOLD) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(sum[i]));
+        }
+        tmem_st16(to + HD + c, o);
+      }
+      tc_wait_st();
+    };
     bool ready = false;
     for (int j = 0; j < n_tiles; j++) {
-      if (C::folds(j) && (!C::SPILL || slot >= 0)) {  // (the product with this tile's weights begins O anew)
-        if (!wait_phase_warp(&pv_done[q][(j - 1) & 1], ((j - 1) >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
-        tc_fence_after();
-        if (C::SPILL) {
-          spill_row(sums, trow, to, m_sum == m_run ? 1.f : exp2_fast(m_sum - m_run), j == C::FOLD);
-          m_sum = m_run;
-        }
-#pragma unroll 1
-        for (int c = 0; c < (C::SPILL ? 0 : HD); c += 16) {
-          uint32_t o[16], sum[16];
-          tmem_ld16(to + c, o);
-          tmem_ld16(to + HD + c, sum);  // (what lies there before the first time is not used)
-          tc_wait_ld();
-          if (j > C::FOLD) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) + __uint_as_float(sum[i]));
-          }
-          tmem_st16(to + HD + c, o);
-        }
-        tc_wait_st();
+      if (C::FOLD % PR_INFO && j == anew) add_up(j);
+      if (__builtin_expect(j % PR_INFO == 0, 0)) {
+        if (C::FOLD % PR_INFO == 0 && j == anew) add_up(j);
+        if (!wait_phase_warp(i_full + (j / PR_INFO & 1), (j / PR_INFO >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
       }
-      if (j % PR_INFO == 0 && !wait_phase_warp(i_full + (j / PR_INFO & 1), (j / PR_INFO >> 1) & 1, ab, PR_SOFTMAX)) ok = false;
       KeyInfo in[PR_KEYS / 16];
 #pragma unroll
       for (int g = 0; g < PR_KEYS / 16; g++) {
@@ -824,7 +836,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
             for (int i = 0; i < 32; i++) o[i] *= f_old;
             tmem_st32(to + c, reinterpret_cast<const uint32_t*>(o));
           }
-          if (C::FOLD && !C::SPILL && j >= C::FOLD) {
+          if (!C::SPILL && j >= C::FOLD) {
 #pragma unroll 1
             for (int c = HD; c < 2 * HD; c += 32) {
               float o[32];
@@ -839,15 +851,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
         }
       }
       const float base = P_SHIFT - (m_run == -INFINITY ? 0.f : m_run);
-      uint32_t p[PR_KEYS / 2], rest[C::TERMS == 2 ? PR_KEYS / 2 : 1];
+      uint32_t p[PR_KEYS / 2], rest[C::P_TERMS == 2 ? PR_KEYS / 2 : 1];
       // The two row tiles take turns at the exponentials (the two warps of a scheduler, which share its unit for them): each has
       // the other's turn for everything else. Both at once, they also do everything else at once.
       if (n_q_tiles == 2 && (q || j)) asm volatile("bar.sync %0, 64;" ::"r"(3 + 4 * q + w4) : "memory");
-      if (edge) weights<C::TERMS, true>(s, in, base, key0, first_key, pos, p, rest, &l_run);
-      else weights<C::TERMS, false>(s, in, base, key0, first_key, pos, p, rest, &l_run);
+      if (edge) weights<C::P_TERMS, sizeof(T) == 4, true>(s, in, base, key0, first_key, pos, p, rest, &l_run);
+      else weights<C::P_TERMS, sizeof(T) == 4, false>(s, in, base, key0, first_key, pos, p, rest, &l_run);
       if (n_q_tiles == 2 && (!q || j + 1 < n_tiles)) asm volatile("bar.arrive %0, 64;" ::"r"(7 - 4 * q + w4) : "memory");
       tmem_st32(ts, p);
-      if (C::TERMS == 2) tmem_st32(ts + 32, rest);
+      if (C::P_TERMS == 2) tmem_st32(ts + 32, rest);
       // (the next scores are most often there: their test is under way while the stores are)
       ready = __all_sync(0xffffffffu, bar_test(&s_full[q][(j + 1) & 1], ((j + 1) >> 1) & 1));
       tc_wait_st();
@@ -866,9 +878,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
       const size_t unit = ((size_t)idx * a.kv_heads + head) * shape.splits + split;
       uint8_t* stage = sm + q * C::Q_AREA + trow * C::OUT_LD;
-      const bool folded = C::FOLD && n_tiles > C::FOLD;
+      const bool folded = n_tiles > fold;
       const uint32_t sum_at = folded && !C::SPILL ? to + HD : 0;
-      float* spilled = folded && C::SPILL ? sums : nullptr;  // (null without a place)
+      float* spilled = folded && C::SPILL ? sums() : nullptr;
       const float f_sum = m_sum == m_run ? 1.f : exp2_fast(m_sum - m_run);
       if (whole) {
         constexpr int NC = 256 / (int)sizeof(T) < HD ? 256 / (int)sizeof(T) : HD;
@@ -896,7 +908,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   }
   tc_fence_before();
   __syncthreads();
-  if (C::SPILL && threadIdx.x == 0 && slot >= 0) release_slot(slot);
+  if (C::SPILL && threadIdx.x == 0 && slot_s >= 0) release_slot(slot_s);
   if (warp == 16) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

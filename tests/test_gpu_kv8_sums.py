@@ -130,6 +130,18 @@ def test_prompts_with_larger_scores_and_a_window(hd):
     t.run_case(F32, 16, heads, kvh, hd, [3000, 40], [n_q, 40], window=1100)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_16_bit_prompts_do_not_shrink(dtype, hd):
+    heads, kvh, n_q = prompt_heads(hd)
+    for n, spread in ((1500, 2.0), (20000, 0.1), (131072, 0.1)):
+        got, want = attend(dtype, heads, kvh, hd, n, n_q, spread)
+        exact = want.to(dtype)
+        # 2^-15 of the output more than the rounding does
+        lost = float(((got.double() - exact.double()) * want).sum() / (want * want).sum())
+        assert abs(lost) < 2.0**-15
+
+
 def test_sums_that_change_their_scale():
     """128 wide: keys whose scores rise along the history move the maximum between the sums that go to the workspace."""
     gen = torch.Generator(device=t.DEV)
