@@ -440,6 +440,13 @@ int h2c_kv8_plan(int32_t n_req, int32_t page_size, const int32_t* cached, const 
     return op_error(H2C_ERR_INVALID, "%s: table_cols %d out of range", who, table_cols);
   if (max_tokens < 0 || max_tokens >= (int)SUM_LIM)
     return op_error(H2C_ERR_INVALID, "%s: max_tokens %d out of range", who, max_tokens);
+  // (every CTA reads all of the inputs while others write)
+  const uint64_t n4 = 4ull * n_req, t4 = 4ull * max_tokens;
+  const OpRange in[] = {{"cached", cached, n4}, {"total", total, n4}, {"free_state", free_state, 16}};
+  const OpRange out[] = {{"block_table", block_table, n4 * table_cols}, {"free_ring", free_ring, 4ull * n_pages},
+                         {"free_state_out", free_state_out, 16}, {"kv_len", kv_len, n4}, {"q_start", q_start, n4 + 4},
+                         {"slot", slot, t4}, {"position", position, t4}, {"status", status, 8}};
+  if (int rc = op_disjoint(who, out, 8, in, 3)) return rc;
   static unsigned char done[OP_MAX_DEVICES];
   const int smem_max = 3 * (H2C_KV8_MAX_REQUESTS + 1) * (int)sizeof(unsigned);
   if (int rc = op_once(who, done, [&] {

@@ -24,6 +24,20 @@ int op_launched(const char* who) noexcept {
   return c == cudaSuccess ? H2C_OK : op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
 }
 
+int op_disjoint(const char* who, const OpRange* out, int n_out, const OpRange* in, int n_in) noexcept {
+  auto meet = [](const OpRange& a, const OpRange& b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return a.bytes && b.bytes && (x < y ? y - x < a.bytes : x - y < b.bytes);
+  };
+  for (int i = 0; i < n_out; i++) {
+    for (int j = 0; j < n_in; j++)
+      if (meet(out[i], in[j])) return op_error(H2C_ERR_INVALID, "%s: %s must not share memory with %s", who, out[i].name, in[j].name);
+    for (int j = 0; j < i; j++)
+      if (meet(out[i], out[j])) return op_error(H2C_ERR_INVALID, "%s: %s must not share memory with %s", who, out[i].name, out[j].name);
+  }
+  return H2C_OK;
+}
+
 namespace {
 __device__ int g_op_err[4];
 int* g_op_err_ptr[OP_MAX_DEVICES];

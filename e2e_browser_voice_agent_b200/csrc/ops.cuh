@@ -18,6 +18,16 @@ int op_launched(const char* who) noexcept;
 // (read by h2c_ops_check); nullptr when the device cannot be queried.
 int* op_err_words() noexcept;
 
+// An argument's memory: its name and the bytes from its lowest to its highest.
+struct OpRange {
+  const char* name;
+  const void* p;
+  uint64_t bytes;
+};
+// H2C_OK, or H2C_ERR_INVALID with "<who>: X must not share memory with Y" when one of the `n_out` ranges that a call writes shares
+// bytes with one of the `n_in` that it reads, or two that it writes do.
+int op_disjoint(const char* who, const OpRange* out, int n_out, const OpRange* in, int n_in) noexcept;
+
 constexpr int OP_MAX_DEVICES = 64;
 // Run fn() once per device (kernel attributes); its status, or H2C_OK when it has already run on this device.
 template <class F>

@@ -111,7 +111,8 @@ def plan(cached: torch.Tensor, total: torch.Tensor, block_table: torch.Tensor, f
          free_state: torch.Tensor, page_size: int, max_tokens: int, out: Optional[Plan] = None) -> Plan:
     """Take and give back pages so that request r goes from cached[r] to total[r] tokens, and map the new tokens to
     slots (h2c_kv8_plan). block_table (int32 [requests, columns]) and free_pages (int32 [pages], a ring) change in place.
-    out: a Plan of an earlier call of the same sizes, whose tensors are written again."""
+    out: a Plan of an earlier call of the same sizes, whose tensors are written again; none of them may be, or share memory
+    with, an argument of this call (cached = p.kv_len wants another Plan than p)."""
     if cached.dim() != 1:
         raise ValueError(f"cached: one length per request is wanted, not {tuple(cached.shape)}")
     index, n = cached.get_device(), cached.shape[0]

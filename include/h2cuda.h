@@ -283,7 +283,9 @@ int h2c_ops_check(void* stream);
  *                    or above table_cols * page_size, the new tokens are more than max_tokens, or the ring's state is
  *                    not that of n_pages pages. With a non-zero status nothing is taken or given back: kv_len is
  *                    cached (0 where that is invalid), q_start all 0, slot and position all -1, free_state_out =
- *                    free_state. */
+ *                    free_state.
+ * What is written shares no memory with what is read or with another output (refused): a loop that feeds kv_len back as the
+ * next step's cached keeps two sets of outputs in turn. */
 int h2c_kv8_plan(int32_t n_req, int32_t page_size, const int32_t* cached, const int32_t* total, int32_t* block_table,
                  int32_t table_cols, int32_t* free_ring, int32_t n_pages, const int64_t* free_state,
                  int64_t* free_state_out, int32_t* kv_len, int32_t* q_start, int32_t* slot, int32_t* position,
