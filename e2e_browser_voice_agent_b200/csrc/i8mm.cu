@@ -534,13 +534,27 @@ int h2c_i8_matmul(int32_t x_type, const void* x, int64_t x_row, const float* x_s
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return op_error(H2C_ERR_INVALID, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
                     (unsigned long long)need, (unsigned long long)(workspace ? workspace_bytes : 0));
+  const int64_t es = codes ? 1 : (int64_t)op_elem_size(x_type), ys = (int64_t)op_elem_size(y_type);
+  if (m > 1 && (y_row < 0 ? -y_row : y_row) < n)
+    return op_error(H2C_ERR_INVALID, "%s: rows of y overlap (%lld elements apart, %d long)", who, (long long)y_row, n);
+  const OpRows tokens{x, m, x_row * es, k * es}, out{y, m, y_row * ys, n * ys};
+  {
+    const OpRange in[] = {{"w", w, (uint64_t)(n - 1) * w_row + k}, {"w_scale", w_scale, 4ull * n}, {"bias", bias, bias ? 4ull * n : 0},
+                          {"x_scale", x_scale, codes ? 4ull * m : 0}};
+    const OpRange written[] = {op_range("y", out), {"workspace", workspace, need}};
+    if (int rc = op_disjoint(who, written, 2, in, 4)) return rc;
+    const OpRange x_range = op_range("x", tokens);
+    if (int rc = op_disjoint(who, written + 1, 1, &x_range, 1)) return rc;
+    if (codes && op_rows_meet(tokens, out)) return op_error(H2C_ERR_INVALID, "%s: y must not share memory with the codes x", who);
+  }
   cudaStream_t st = (cudaStream_t)stream;
   MmArgs a = {};
   a.err = op_err_words();
   if (!a.err) return op_error(H2C_ERR_CUDA, "%s: no device", who);
   a.n = n; a.m = m; a.k = k; a.chunks = (k + KCH - 1) / KCH;
   shape_of(m, n, a.chunks, &a.nt, &a.mt, &a.splits);
-  const bool fuse = fused(x_type, m, k);
+  // (a CTA of that form may write its outputs while another still reads the tokens, so y in their memory takes two kernels)
+  const bool fuse = fused(x_type, m, k) && !op_rows_meet(tokens, out);
   if (fuse) {  // (one tile of 16 tokens; K divided so that a share's codes fit)
     a.nt = 16;
     a.mt = 1;

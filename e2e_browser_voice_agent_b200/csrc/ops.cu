@@ -38,6 +38,23 @@ int op_disjoint(const char* who, const OpRange* out, int n_out, const OpRange* i
   return H2C_OK;
 }
 
+OpRange op_range(const char* name, const OpRows& r) noexcept {
+  const int64_t span = (r.rows - 1) * r.stride;
+  return {name, static_cast<const uint8_t*>(r.p) + (span < 0 ? span : 0), (uint64_t)((span < 0 ? -span : span) + r.bytes)};
+}
+
+bool op_rows_meet(const OpRows& a, const OpRows& b) noexcept {
+  const OpRange x = op_range("", a), y = op_range("", b);
+  const uintptr_t xp = (uintptr_t)x.p, yp = (uintptr_t)y.p;
+  if (xp + x.bytes <= yp || yp + y.bytes <= xp) return false;
+  int64_t s = a.rows == 1 ? b.stride : a.stride;
+  if ((a.rows > 1 && b.rows > 1 && a.stride != b.stride) || (a.rows == 1 && b.rows == 1)) return true;
+  if (s < 0) s = -s;
+  if (a.bytes > s || b.bytes > s) return true;
+  const uint64_t d = (yp > xp ? yp - xp : (uint64_t)s - (xp - yp) % s) % s;  // from a row of a to the next of b
+  return d < (uint64_t)a.bytes || (uint64_t)s - d < (uint64_t)b.bytes;
+}
+
 namespace {
 __device__ int g_op_err[4];
 int* g_op_err_ptr[OP_MAX_DEVICES];

@@ -28,6 +28,15 @@ struct OpRange {
 // bytes with one of the `n_in` that it reads, or two that it writes do.
 int op_disjoint(const char* who, const OpRange* out, int n_out, const OpRange* in, int n_in) noexcept;
 
+// Rows of `bytes` bytes, `stride` bytes apart (of either sign, or 0).
+struct OpRows {
+  const void* p;
+  int64_t rows, stride, bytes;
+};
+OpRange op_range(const char* name, const OpRows& r) noexcept;
+// Whether two sets of rows share bytes: exact for the same stride (columns of one buffer) and for one row, else by their ranges.
+bool op_rows_meet(const OpRows& a, const OpRows& b) noexcept;
+
 constexpr int OP_MAX_DEVICES = 64;
 // Run fn() once per device (kernel attributes); its status, or H2C_OK when it has already run on this device.
 template <class F>

@@ -47,7 +47,8 @@ def matmul(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Option
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = x w^T in 8-bit integers, scaled, plus bias (h2c_i8_matmul). x is [m, k] values, or with x_scale the codes of
     quantize, whose k must then be given; w int8 [n, at least k] with rows a multiple of 16 apart; w_scale and bias
-    float32 [n]. The result has x's type (float32 for codes) unless out_dtype or out says otherwise."""
+    float32 [n]. The result has x's type (float32 for codes) unless out_dtype or out says otherwise. out may be x's values, in
+    place; it shares no memory with another argument."""
     index = x.get_device()
     px, pw = _matrix("x", x, index), _matrix("w", w, index)
     if w.dtype is not torch.int8:

@@ -361,7 +361,8 @@ int h2c_i8_quantize(int32_t type, const void* x, int64_t x_row, int32_t rows, in
  * in the workspace (x_scale is not looked at), x_type H2C_TYPE_I8 takes x as codes (x_row bytes apart) with x_scale.
  * w: int8 [n] rows w_row bytes apart. Codes and w are 16-byte aligned with rows a multiple of 16 bytes apart, at least k;
  * what lies beyond k is not looked at. y: row i at y + i * y_row elements. bias: float32 [n] or NULL. workspace:
- * h2c_i8_matmul_workspace bytes, 16-byte aligned (NULL when that is 0). m = 0 or n = 0 does nothing. */
+ * h2c_i8_matmul_workspace bytes, 16-byte aligned (NULL when that is 0). m = 0 or n = 0 does nothing. y may lie in the memory of
+ * x's values, which are read before it is written; it shares none with another argument, nor do its rows (refused). */
 uint64_t h2c_i8_matmul_workspace(int32_t x_type, int32_t m, int32_t k);
 int h2c_i8_matmul(int32_t x_type, const void* x, int64_t x_row, const float* x_scale, const void* w, int64_t w_row,
                   const float* w_scale, int32_t m, int32_t n, int32_t k, int32_t y_type, void* y, int64_t y_row,

@@ -42,3 +42,30 @@ def test_plan_refuses_outputs_over_other_arguments(lib, written, other):
             refused(lib, rc, "h2c_kv8_plan", "free_state_out")
         else:
             refused(lib, rc, "h2c_kv8_plan", "share memory", NAMES.get(written, written), NAMES.get(other, other))
+
+
+MATMUL = dict(x_type=0, x=A[0], x_row=64, x_scale=None, w=A[1], w_row=64, w_scale=A[2], m=5, n=30, k=50, y_type=0, y=A[3], y_row=30,
+              bias=A[4], workspace=A[5], workspace_bytes=1 << 16, stream=None)
+CODES = {**MATMUL, "x_type": 3, "x_scale": A[6], "workspace": None, "workspace_bytes": 0}
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(y=A[1] + 29 * 64 + 48), ("y", "w")), (dict(y=A[2] + 116), ("y", "w_scale")), (dict(y=A[4] - 5 * 120 + 4), ("y", "bias")),
+    (dict(y=A[5]), ("workspace", "y")), (dict(workspace=A[0]), ("workspace", "x")), (dict(workspace=A[1] + 16), ("workspace", "w")),
+    (dict(workspace=A[2]), ("workspace", "w_scale")),
+])
+def test_matmul_refuses_outputs_over_other_arguments(lib, change, words):
+    refused(lib, lib.h2c_i8_matmul(*{**MATMUL, **change}.values()), "h2c_i8_matmul", "share memory", *words)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(y=A[0]), ("y", "codes")), (dict(y=A[0] + 4 * 64 + 48), ("y", "codes")), (dict(y=A[6] + 16), ("y", "x_scale")),
+    (dict(y=A[0] - 4 * 120 - 4), ("y", "codes")),
+])
+def test_matmul_of_codes_refuses_outputs_over_them(lib, change, words):
+    refused(lib, lib.h2c_i8_matmul(*{**CODES, **change}.values()), "h2c_i8_matmul", "share memory", *words)
+
+
+@pytest.mark.parametrize("y_row", [0, 29, -29, 1])
+def test_matmul_refuses_rows_of_y_that_overlap(lib, y_row):
+    refused(lib, lib.h2c_i8_matmul(*{**MATMUL, "y_row": y_row}.values()), "h2c_i8_matmul", "rows of y overlap")
