@@ -503,6 +503,12 @@ int h2c_i8_quantize(int32_t type, const void* x, int64_t x_row, int32_t rows, in
   if ((uintptr_t)x & (op_elem_size(type) - 1)) return op_error(H2C_ERR_INVALID, "%s: x must be aligned to its elements", who);
   if (((uintptr_t)q & 15) || (q_row & 15) || q_row < k)
     return op_error(H2C_ERR_INVALID, "%s: q must be 16-byte aligned with rows of a multiple of 16 bytes, at least k", who);
+  const int64_t es = (int64_t)op_elem_size(type), k_pad = (k + 15) / 16 * 16;
+  const OpRows values{x, rows, x_row * es, k * es}, codes{q, rows, q_row, k_pad};
+  const OpRange in = op_range("x", values), out[] = {op_range("q", codes), {"scale", scale, 4ull * rows}};
+  if (op_rows_meet(values, codes)) return op_error(H2C_ERR_INVALID, "%s: q must not share memory with x", who);
+  if (int rc = op_disjoint(who, out, 2, &in, 0)) return rc;
+  if (int rc = op_disjoint(who, out + 1, 1, &in, 1)) return rc;
   return quantize(who, type, x, x_row, rows, k, q, q_row, scale, (cudaStream_t)stream);
 }
 

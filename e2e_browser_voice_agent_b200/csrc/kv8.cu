@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 
 namespace h2 {
 namespace {
@@ -474,6 +475,17 @@ int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size
   const size_t es = op_elem_size(type);
   if (((uintptr_t)k | (uintptr_t)v) & (es - 1))
     return op_error(H2C_ERR_INVALID, "%s: k and v must be aligned to their elements", who);
+  {
+    auto range = [&](const char* name, const void* at, long long row, long long head) {  // of all rows and heads
+      const long long r = (rows - 1LL) * row, h = (kv_heads - 1LL) * head;
+      return OpRange{name, static_cast<const uint8_t*>(at) + (std::min(0LL, r) + std::min(0LL, h)) * (long long)es,
+                     (uint64_t)(std::abs(r) + std::abs(h) + head_dim) * es};
+    };
+    const OpRange in[] = {range("k", k, k_row, k_head), range("v", v, v_row, v_head), {"slot", slot, 4ull * rows}};
+    const OpRange out[] = {{"kv", kv, 2ull * n_pages * kv_heads * page_size * head_dim},
+                           {"kv_scale", kv_scale, 8ull * n_pages * kv_heads}};
+    if (int rc = op_disjoint(who, out, 2, in, 3)) return rc;
+  }
   // few rows (decode steps): windows of 16, so that few single rows wait in line for a warp; many: windows of a page, so that
   // every CTA of a prompt finds a run (16,392 rows into pages of 64: 19.6 us; with windows of 16, of which most begin no run, 29)
   const int win = (long long)(rows + APP_WIN - 1) / APP_WIN * 2 * kv_heads > 1184 ? std::max(APP_WIN, page_size) : APP_WIN;
@@ -499,6 +511,11 @@ int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t
   if (!slot || !k_out || !v_out) return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15)
     return op_error(H2C_ERR_INVALID, "%s: k_out and v_out must be 16-byte aligned", who);
+  const uint64_t bytes = (uint64_t)rows * kv_heads * head_dim * op_elem_size(type);
+  const OpRange in[] = {{"kv", kv, 2ull * n_pages * kv_heads * page_size * head_dim},
+                        {"kv_scale", kv_scale, 8ull * n_pages * kv_heads}, {"slot", slot, 4ull * rows}};
+  const OpRange out[] = {{"k_out", k_out, bytes}, {"v_out", v_out, bytes}};
+  if (int rc = op_disjoint(who, out, 2, in, 3)) return rc;
   const int across = std::min(256, (2 * kv_heads * (head_dim / 4) + 31) / 32 * 32);
   const dim3 block(across, 256 / across);
   const int ctas = std::min((rows + (int)block.y - 1) / (int)block.y, 148 * 8);

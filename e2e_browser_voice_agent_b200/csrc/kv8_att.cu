@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 
 namespace h2 {
 namespace {
@@ -737,6 +738,32 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
   if (p.bytes && (!g->workspace || g->workspace_bytes < p.bytes || ((uintptr_t)g->workspace & 15)))
     return op_error(H2C_ERR_INVALID, "%s: needs %llu bytes of 16-byte aligned workspace, got %llu", who,
                     (unsigned long long)p.bytes, (unsigned long long)(g->workspace ? g->workspace_bytes : 0));
+  const long long hd = g->head_dim;
+  if (op_vectors_overlap(g->rows, g->out_row, g->heads, g->out_head, hd))
+    return op_error(H2C_ERR_INVALID, "%s: vectors of out overlap (rows %lld elements apart, heads %lld)", who,
+                    (long long)g->out_row, (long long)g->out_head);
+  {
+    // a token's vectors as one row, between the lowest and the highest
+    auto rows_of = [&](const void* at, long long row, long long head) {
+      const long long span = (g->heads - 1) * head;
+      return OpRows{static_cast<const uint8_t*>(at) + std::min(0LL, span) * (long long)es, g->rows, row * (long long)es,
+                    (std::abs(span) + hd) * (long long)es};
+    };
+    const OpRows q = rows_of(g->q, g->q_row, g->q_head), out = rows_of(g->out, g->out_row, g->out_head);
+    // (in place is safe: the CTAs that read a vector are done with it before one of them writes it)
+    const bool in_place = g->out == g->q && (g->out_row == g->q_row || g->rows == 1) && (g->out_head == g->q_head || g->heads == 1);
+    if (!in_place && op_rows_meet(q, out))
+      return op_error(H2C_ERR_INVALID, "%s: out must be q itself or share no memory with it", who);
+    const uint64_t kv_bytes = 2ull * g->n_pages * g->kv_heads * g->page_size * g->head_dim;
+    const OpRange in[] = {{"kv", g->kv, kv_bytes}, {"kv_scale", g->kv_scale, 8ull * g->n_pages * g->kv_heads},
+                          {"block_table", g->block_table, 4ull * g->n_req * g->table_cols},
+                          {"q_start", g->q_start, 4ull * g->n_req + 4}, {"kv_len", g->kv_len, 4ull * g->n_req}};
+    const OpRange written[] = {op_range("out", out), {"lse", g->lse, g->lse ? 4ull * g->rows * g->heads : 0},
+                               {"workspace", g->workspace, p.bytes}};
+    if (int rc = op_disjoint(who, written, 3, in, 5)) return rc;
+    const OpRange q_range = op_range("q", q);
+    if (int rc = op_disjoint(who, written + 1, 2, &q_range, 1)) return rc;
+  }
   const long long most = std::max((long long)p.splits * p.tiles * RW_ROWS, (long long)p.shape.tiles * PR_ROWS);
   if (most * g->kv_heads > INT_MAX) return op_error(H2C_ERR_INVALID, "%s: too many rows for one call", who);
   AttArgs a;

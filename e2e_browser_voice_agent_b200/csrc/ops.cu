@@ -55,6 +55,18 @@ bool op_rows_meet(const OpRows& a, const OpRows& b) noexcept {
   return d < (uint64_t)a.bytes || (uint64_t)s - d < (uint64_t)b.bytes;
 }
 
+bool op_vectors_overlap(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t len) noexcept {
+  if (row < 0) row = -row;
+  if (head < 0) head = -head;
+  if ((rows > 1 && row < len) || (heads > 1 && head < len)) return true;
+  if (rows <= 1 || heads <= 1 || row >= (heads - 1) * head + len || head >= (rows - 1) * row + len) return false;
+  for (int64_t h = 1; h < heads; h++) {  // vectors h heads apart, and the rows' distance that comes nearest
+    const int64_t r = h * head / row, over = h * head - r * row;
+    if ((r < rows && over < len) || (r + 1 < rows && row - over < len)) return true;
+  }
+  return false;
+}
+
 namespace {
 __device__ int g_op_err[4];
 int* g_op_err_ptr[OP_MAX_DEVICES];

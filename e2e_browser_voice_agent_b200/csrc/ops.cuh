@@ -36,6 +36,8 @@ struct OpRows {
 OpRange op_range(const char* name, const OpRows& r) noexcept;
 // Whether two sets of rows share bytes: exact for the same stride (columns of one buffer) and for one row, else by their ranges.
 bool op_rows_meet(const OpRows& a, const OpRows& b) noexcept;
+// Whether of rows x heads vectors of `len` elements, `row` and `head` elements apart, two share elements (exact).
+bool op_vectors_overlap(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t len) noexcept;
 
 constexpr int OP_MAX_DEVICES = 64;
 // Run fn() once per device (kernel attributes); its status, or H2C_OK when it has already run on this device.

@@ -178,7 +178,8 @@ def attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, block_t
     """Causal grouped-query attention of a ragged batch over the cache (h2c_kv8_attention). q is [rows, heads, head dim]
     with any row and head stride; scale defaults to head_dim ** -0.5; window > 0 limits each query to that many positions.
     max_q and max_kv bound the requests' query counts and lengths. Returns out ([rows, heads, head dim], q's type), or
-    (out, lse) with lse float32 [rows, heads]; rows that belong to no request keep what out held."""
+    (out, lse) with lse float32 [rows, heads]; rows that belong to no request keep what out held. out may be q itself, or
+    share no memory with the arguments."""
     index, pkv, ps, n_pages, page, kvh, hd = _cache(kv, kv_scale)
     if q.dim() != 3:
         raise ValueError(f"q: [rows, heads, {hd}] is wanted, not {tuple(q.shape)}")

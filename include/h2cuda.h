@@ -299,13 +299,14 @@ int h2c_kv8_plan(int32_t n_req, int32_t page_size, const int32_t* cached, const 
  * codes at earlier offsets become round(code * (s0 / s)); else s = s0. The new codes are round(x * (1 / s)), within
  * [-127, 127] (float32 operations, halves to even). A code is re-rounded only when the scale grows, which it does by at
  * least 1.25 each time, so a cached value is off by at most 2.5 final steps. A row with an infinity or NaN makes its
- * page's scale NaN until the page is new again: every read of that page and head gives NaN. */
+ * page's scale NaN until the page is new again: every read of that page and head gives NaN. The cache shares no memory with k, v or
+ * slot (refused). */
 int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
                    int32_t type, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                    int64_t v_head, int32_t rows, const int32_t* slot, void* stream);
 
 /* The cached values at slot[t], t < rows: k_out and v_out [rows][kv_heads][head_dim] of element type `type` (16-byte
- * aligned); zeros where the slot is not in the cache. To move a session elsewhere, or to look at what the cache holds. */
+ * aligned, sharing no memory with the cache, slot or each other); zeros where the slot is not in the cache. To move a session elsewhere, or to look at what the cache holds. */
 int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t page_size, int32_t kv_heads,
                  int32_t head_dim, const int32_t* slot, int32_t rows, int32_t type, void* k_out, void* v_out,
                  void* stream);
@@ -315,7 +316,8 @@ int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t
  * positions 0 .. p, or p - window + 1 .. p with window > 0. Head h reads kv head h / (heads / kv_heads).
  *   x = scale * (q . k),  out = sum softmax(x) v  (rounded once to `type`),  lse = log sum exp x  (natural logarithm)
  * A query with no position to attend to (p < 0) gives zeros and lse = -infinity. Rows of q that belong to no request are
- * not touched. Scores, softmax statistics and sums are float32; codes and float16 / bfloat16 queries enter the tensor
+ * not touched. out may be q itself (the same address and strides); otherwise what is written (out, lse, the workspace) shares no
+ * memory with another argument, nor do two vectors of out (refused). Scores, softmax statistics and sums are float32; codes and float16 / bfloat16 queries enter the tensor
  * cores exactly, float32 queries as two float16 terms (22 bits). */
 typedef struct h2c_kv8_attention_args {
   const void* q;          /* row t of head h at t * q_row + h * q_head elements, head_dim values */
@@ -351,7 +353,7 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* args, void* stream);
  * row's largest magnitude, scale = a / 127 and q = round(x * min(127 / a, FLT_MAX)) (float32 operations, halves to even;
  * a row of zeros gives zeros). Rows of q start q_row bytes apart (a multiple of 16, at least k, q 16-byte aligned); the
  * bytes from k to the next multiple of 16 become 0. A row with an infinity or NaN has the scale NaN (and codes without
- * meaning): every product with it is NaN. For weights (rows = output channels), once, and for activations that
+ * meaning): every product with it is NaN. q and scale share no memory with x or each other (refused). For weights (rows = output channels), once, and for activations that
  * several products share. */
 int h2c_i8_quantize(int32_t type, const void* x, int64_t x_row, int32_t rows, int32_t k, void* q, int64_t q_row,
                     float* scale, void* stream);

@@ -35,3 +35,51 @@ def test_columns_of_one_buffer_stay_one_launch():
     w, ws = int8.quantize(torch.randn(128, 400, device=DEV))
     want = int8.matmul(x[:, :400].contiguous(), w, ws)
     assert torch.equal(int8.matmul(x[:, :400], w, ws, out=x[:, 450:578]), want)
+
+
+def attention_case(dtype, hd, kv_len, n_q, heads=14, kvh=2, seed=0):
+    import test_gpu_kv8 as t
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(seed + hd + sum(kv_len))
+    kv, sc, table = t.make_cache(gen, kv_len, 16, kvh, hd)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    start = [0]
+    for n in n_q:
+        start.append(start[-1] + n)
+    q = torch.randn(start[-1], heads, hd, generator=gen, device=DEV).to(dtype)
+    call = lambda q, **kw: t.kv8().attention(q, kv, sc, table, i32(start), i32(kv_len), max(n_q), max(kv_len), return_lse=True, **kw)
+    return q, call
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kv_len,n_q", [([700], [1]), ([5000, 90], [1, 1]), ([3000], [200]), ([900, 2000, 30], [1, 150, 30]),
+                                        ([300], [9])])
+def test_attention_over_its_queries(dtype, hd, kv_len, n_q):
+    """One span, a cluster's, spans joined by a second kernel, both kernels in one call."""
+    q, call = attention_case(dtype, hd, kv_len, n_q)
+    want, want_lse = call(q)
+    for _ in range(5):
+        z = q.clone()
+        got, lse = call(z, out=z)
+        assert got is z and torch.equal(z, want) and torch.equal(lse, want_lse)
+
+
+def test_attention_into_columns_and_interleaved_heads():
+    """Layouts that share no memory although the ranges of their tokens or heads do."""
+    q, call = attention_case(torch.float32, 64, [500, 40], [3, 2])
+    want, _ = call(q)
+    wide = torch.zeros(5, 31, 64, device=DEV)
+    wide[:, 1:15] = q
+    got, _ = call(wide[:, 1:15], out=wide[:, 15:29])     # beside the queries
+    assert torch.equal(got, want) and torch.equal(wide[:, 1:15], q) and (wide[:, 29:] == 0).all()
+    flat = torch.zeros(5 * 14 * 64 * 3, device=DEV)
+    for row, head in ((64, 5 * 64), (3 * 64, 15 * 64), (15 * 64, 64), (29 * 64, 128)):
+        out = flat.as_strided((5, 14, 64), (row, head, 1))
+        got, _ = call(q, out=out)
+        assert torch.equal(got, want)
+    q, call = attention_case(torch.float32, 64, [50, 40], [1, 1])
+    want, _ = call(q)
+    out = flat.as_strided((2, 14, 64), (13 * 64, 128, 1))   # one token's heads between the other's
+    got, _ = call(q, out=out)
+    assert torch.equal(got, want)

@@ -69,3 +69,57 @@ def test_matmul_of_codes_refuses_outputs_over_them(lib, change, words):
 @pytest.mark.parametrize("y_row", [0, 29, -29, 1])
 def test_matmul_refuses_rows_of_y_that_overlap(lib, y_row):
     refused(lib, lib.h2c_i8_matmul(*{**MATMUL, "y_row": y_row}.values()), "h2c_i8_matmul", "rows of y overlap")
+
+
+def attention(lib, **change):
+    a = dict(q=A[0], q_row=256, q_head=64, out=A[1], out_row=256, out_head=64, lse=A[2], kv=A[3], kv_scale=A[4], n_pages=8,
+             page_size=16, kv_heads=2, head_dim=64, heads=4, type=0, block_table=A[5], table_cols=4, n_req=2, q_start=A[6],
+             kv_len=A[7], rows=3, max_q=2, max_kv=60, window=0, scale=0.125, workspace=None, workspace_bytes=0)
+    assert set(change) <= set(a)
+    return lib.h2c_kv8_attention(C.byref(_lib.Kv8AttentionArgs(**{**a, **change})), None)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(out=A[0] + 4), ("out", "q itself")), (dict(out=A[0] - 3 * 1024 + 16), ("out", "q itself")),
+    (dict(out=A[0], out_row=320), ("out", "q itself")), (dict(out=A[0], out_row=64, out_head=192), ("out", "q itself")),
+    (dict(out=A[3]), ("out", "kv")), (dict(out=A[4]), ("out", "kv_scale")), (dict(out=A[5]), ("out", "block_table")),
+    (dict(out=A[6]), ("out", "q_start")), (dict(out=A[7]), ("out", "kv_len")), (dict(lse=A[1] + 64), ("lse", "out")),
+    (dict(lse=A[0]), ("lse", "q")), (dict(lse=A[7] - 44), ("lse", "kv_len")),
+    (dict(max_kv=4000, workspace=A[1], workspace_bytes=1 << 30), ("workspace", "out")),
+    (dict(max_kv=4000, workspace=A[0], workspace_bytes=1 << 30), ("workspace", "q")),
+])
+def test_attention_refuses_outputs_over_other_arguments(lib, change, words):
+    # (the workspace lies below the other addresses: its size does not reach them)
+    refused(lib, attention(lib, **change), "h2c_kv8_attention", *words)
+
+
+@pytest.mark.parametrize("row,head", [(0, 64), (256, 0), (63, 1024), (256, 63), (100, 240), (192, 64), (-128, 64), (130, 64)])
+def test_attention_refuses_vectors_of_out_that_overlap(lib, row, head):
+    refused(lib, attention(lib, out=A[1] + 4096, out_row=row, out_head=head), "h2c_kv8_attention", "vectors of out overlap")
+
+
+APPEND = dict(kv=A[0], scale=A[1], n_pages=8, page=16, kv_heads=2, head_dim=64, type=0, k=A[2], k_row=128, k_head=64, v=A[3],
+              v_row=128, v_head=64, rows=3, slot=A[4], stream=None)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(k=A[0] + 32764), ("kv", "k")), (dict(v=A[0] - 1532), ("kv", "v")), (dict(slot=A[0] + 16), ("kv", "slot")),
+    (dict(scale=A[2] + 16), ("kv_scale", "k")), (dict(scale=A[4] - 124), ("kv_scale", "slot")), (dict(scale=A[0] + 64), ("kv_scale", "kv")),
+    (dict(k=A[0] + 40000, k_row=-4096), ("kv", "k")),
+])
+def test_append_refuses_a_cache_over_its_rows(lib, change, words):
+    refused(lib, lib.h2c_kv8_append(*{**APPEND, **change}.values()), "h2c_kv8_append", "share memory", *words)
+
+
+@pytest.mark.parametrize("k_out,v_out,words", [(A[0] + 16, A[6], ("k_out", "kv")), (A[6], A[1], ("v_out", "kv_scale")),
+                                               (A[6], A[6] + 1520, ("v_out", "k_out")), (A[4] - 1520, A[6], ("k_out", "slot"))])
+def test_read_refuses_outputs_over_other_arguments(lib, k_out, v_out, words):
+    rc = lib.h2c_kv8_read(A[0], A[1], 8, 16, 2, 64, A[4], 3, 0, k_out, v_out, None)
+    refused(lib, rc, "h2c_kv8_read", "share memory", *words)
+
+
+@pytest.mark.parametrize("change,words", [(dict(q=A[0]), ("q", "x")), (dict(q=A[0] + 2 * 200 - 16), ("q", "x")),
+                                          (dict(scale=A[0] + 4), ("scale", "x")), (dict(scale=A[1] + 64), ("scale", "q"))])
+def test_quantize_refuses_outputs_over_its_values(lib, change, words):
+    a = dict(type=0, x=A[0], x_row=50, rows=3, k=50, q=A[1], q_row=64, scale=A[2], stream=None)
+    refused(lib, lib.h2c_i8_quantize(*{**a, **change}.values()), "h2c_i8_quantize", "share memory", *words)
