@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
   const int tok = token_of(a, live ? row : row0, &hq);
   hq += head * a.group;
   const int pos = R.len - n_all + tok;               // its position, and the keys it may see: [first_key, pos]
-  const int first_key = a.window > 0 ? pos + 1 - a.window : 0;
+  const int first_key = first_key_of(a, pos);
   uint32_t qa[KC * 4][4];
   float q_scale;  // what a product of codes is multiplied by: power of two of the row, softmax scale
   {

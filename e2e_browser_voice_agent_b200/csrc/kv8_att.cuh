@@ -55,11 +55,15 @@ __device__ __forceinline__ Request request_of(const AttArgs& a, int r, int* n_al
   return R;
 }
 
+// The first key that the query at position pos sees. (Before position 0 it sees none; with the largest windows the difference would
+// not fit there.)
+__device__ __forceinline__ int first_key_of(const AttArgs& a, int pos) { return a.window > 0 ? max(pos, 0) + 1 - a.window : 0; }
+
 // The keys that queries t0 .. t1 of a request may attend to: [lo, hi), hi <= lo when there are none.
 __device__ __forceinline__ void key_range(const AttArgs& a, const Request& R, int n_all, int t0, int t1, int* lo, int* hi) {
   const int p0 = R.len - n_all + t0, p1 = R.len - n_all + t1;
   *hi = min(p1 + 1, R.len);
-  *lo = a.window > 0 ? max(0, p0 + 1 - a.window) : 0;
+  *lo = max(0, first_key_of(a, p0));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2 ulp, 0 for -infinity

@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     int hq;
     const int tok = token_of(a, rr, &hq);
     hq += head * a.group;
-    const int pos = R.len - n_all + tok, first_key = a.window > 0 ? pos + 1 - a.window : 0;
+    const int pos = R.len - n_all + tok, first_key = first_key_of(a, pos);
     bool ok = true;
     if (n_tiles > 0) {
       put_queries<T, HD>(a, (long long)(R.first + tok) * a.q_row + hq * a.q_head, n_rows, at.row0 + q * 128, 32 * w4,
