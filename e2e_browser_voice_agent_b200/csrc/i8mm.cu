@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                   put<T>(a, tok0 + c + i, row, (int)u[i], FUSE ? fused_scale[i & (FUSE_TOKENS - 1)] : a.xs[tok0 + c + i], ws, b);
             }
           }
+          __syncwarp();
         }
       }
       tc_fence_before();
@@ -369,6 +370,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
       }
       if (row < a.n) put<T>(a, tok0 + c, row, acc, FUSE ? fused_scale[c & (FUSE_TOKENS - 1)] : a.xs[tok0 + c], ws, b);
     }
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   tc_fence_before();

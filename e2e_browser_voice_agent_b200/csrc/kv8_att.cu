@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
           ll == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(ll) + mm - P_SHIFT);
   }
   if (!ra.cluster) return;
+  __syncwarp();
 
   // ---- the cluster's spans, each CTA a share of the rows' pieces of four dimensions, through distributed shared memory
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -202,7 +202,7 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
 // in turn, so that every thread of the group takes the same way; false when the wait expired.
 __device__ __forceinline__ bool wait_group(uint64_t* b, unsigned parity, const Abort& a, int role, int id, volatile int* go, int j) {
   if ((threadIdx.x & 127) == 0) go[j & 1] = wait_phase(b, parity, a, role);
-  asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+  asm volatile("barrier.sync %0, 128;" ::"r"(id) : "memory");  // (a warp need not have come together)
   return go[j & 1] != 0;
 }
 // whether the phase has completed, without waiting
@@ -494,15 +494,17 @@ template <class U, int NC>
 __device__ __forceinline__ void copy_row(U* dst, const uint8_t* src, bool store, bool bulk) {
   if (bulk) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    if (store)
-      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(__cvta_generic_to_global(dst)),
-                   "r"(su32(src)), "r"(NC * (int)sizeof(U))
-                   : "memory");
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %3, 0;\n @p cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n}\n" ::"l"(
+            __cvta_generic_to_global(dst)),
+        "r"(su32(src)), "r"(NC * (int)sizeof(U)), "r"((int)store)
+        : "memory");
     asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group.read 0;" ::: "memory");
   } else if (store) {
 #pragma unroll 1
     for (int i = 0; i < NC; i++) dst[i] = reinterpret_cast<const U*>(src)[i];
   }
+  if (!bulk) __syncwarp();
 }
 
 // The largest score of one tile of keys among those the row sees, with the exponent of V's scale.
@@ -589,6 +591,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (C::SPILL) slot_s = pa.sums && n_tiles > C::FOLD ? claim_slot(Abort{&abort_s, pa.err}) : -1;
   }
+  __syncwarp();
   if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(su32(&tmem_slot)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -863,11 +866,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       tmem_st32(ts, p);
       if (C::P_TERMS == 2) tmem_st32(ts + 32, rest);
       // (the next scores are most often there: their test is under way while the stores are)
-      ready = __all_sync(0xffffffffu, bar_test(&s_full[q][(j + 1) & 1], ((j + 1) >> 1) & 1));
+      const bool next = bar_test(&s_full[q][(j + 1) & 1], ((j + 1) >> 1) & 1);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) bar_arrive(&p_full[q][j & 1]);
+      ready = __all_sync(0xffffffffu, next);  // (which also brings the warp together for the next aligned instruction)
     }
     // ---- the rows' output: each thread stages its row in the place of the row tile's queries (their last product was issued
     // before the last update of O, whose completion is waited for; without keys they were not written) and copies it out
@@ -908,6 +912,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       }
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (C::SPILL && threadIdx.x == 0 && slot_s >= 0) release_slot(slot_s);
