@@ -55,6 +55,12 @@ def _call(index: int, fn, *args) -> None:
         _lib.check(rc)
 
 
+def _int32(names: str, *numbers: int) -> None:
+    """Refuse numbers that a 32-bit argument of the library would cut off."""
+    if max(numbers) >= 2**31 or min(numbers) < -2**31:
+        raise ValueError(f"{names}: {numbers}: not all fit in 32 bits")
+
+
 def _want(name: str, t: torch.Tensor, dtype: torch.dtype, index: int, shape: Optional[Tuple] = None) -> int:
     """The address of a contiguous tensor of this type and shape on device `index`."""
     if t.dtype is dtype and t.get_device() == index and t.is_contiguous() and (shape is None or t.shape == shape):
@@ -74,6 +80,8 @@ def _cache(kv: torch.Tensor, kv_scale: torch.Tensor):
     if len(shape) != 5 or shape[1] != 2:
         raise ValueError(f"kv: [pages, 2, kv heads, page size, head dim] is wanted, not {tuple(shape)}")
     n_pages, _, kv_heads, page, head_dim = shape
+    if n_pages >= 2**31 or kv_heads >= 2**31 or page >= 2**31 or head_dim >= 2**31:
+        raise ValueError(f"kv: {tuple(shape)} does not fit in 32 bits")
     index = kv.get_device()
     return (index, _want("kv", kv, torch.int8, index),
             _want("kv_scale", kv_scale, torch.float32, index, (n_pages, 2, kv_heads)), n_pages, page, kv_heads, head_dim)
@@ -82,7 +90,7 @@ def _cache(kv: torch.Tensor, kv_scale: torch.Tensor):
 def _rows(name: str, t: torch.Tensor, index: int, heads: int, head_dim: int) -> Tuple[int, int, int, int]:
     """(address, element type, row stride, head stride) of [rows, heads, head_dim] values, the last axis dense."""
     shape = t.shape
-    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+    if len(shape) != 3 or shape[0] >= 2**31 or shape[1] != heads or shape[2] != head_dim:
         raise ValueError(f"{name}: [rows, {heads}, {head_dim}] is wanted, not {tuple(shape)}")
     kind = _TYPES.get(t.dtype)
     if kind is None:
@@ -122,6 +130,7 @@ def plan(cached: torch.Tensor, total: torch.Tensor, block_table: torch.Tensor, f
         raise ValueError(f"free_pages: one number per page is wanted, not {tuple(free_pages.shape)}")
     if max_tokens < 0:
         raise ValueError(f"max_tokens: {max_tokens}")
+    _int32("page_size, max_tokens, columns, pages, requests", page_size, max_tokens, block_table.shape[1], free_pages.shape[0], n)
     i32, i64 = torch.int32, torch.int64
     args = (n, page_size, _want("cached", cached, i32, index), _want("total", total, i32, index, (n,)),
             _want("block_table", block_table, i32, index), block_table.shape[1],
@@ -166,6 +175,7 @@ def read(kv: torch.Tensor, kv_scale: torch.Tensor, slot: torch.Tensor,
     if slot.dim() != 1:
         raise ValueError(f"slot: one entry per row is wanted, not {tuple(slot.shape)}")
     rows = slot.shape[0]
+    _int32("rows", rows, 0)
     k, v = (torch.empty(rows, cache[4], cache[5], dtype=dtype, device=kv.device) for _ in range(2))
     _call(index, _lib.load().h2c_kv8_read, *cache, _want("slot", slot, torch.int32, index), rows, _TYPES[dtype], k.data_ptr(),
           v.data_ptr())
@@ -188,6 +198,7 @@ def attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, block_t
     n = kv_len.shape[0]
     if block_table.dim() != 2 or block_table.shape[0] != n:
         raise ValueError(f"block_table: [{n}, columns] is wanted, not {tuple(block_table.shape)}")
+    _int32("heads, max_q, max_kv, window, columns", heads, max_q, max_kv, window, block_table.shape[1])
     i32, dev = torch.int32, kv.device
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
