@@ -499,7 +499,7 @@ int h2c_i8_quantize(int32_t type, const void* x, int64_t x_row, int32_t rows, in
                     float* scale, void* stream) {
   const char* who = "h2c_i8_quantize";
   if (!op_type_ok(type)) return op_error(H2C_ERR_BAD_TYPE, "%s: element type %d", who, type);
-  if (rows < 0 || k < 1 || k > H2C_I8_MAX_K) return op_error(H2C_ERR_INVALID, "%s: %d rows of %d", who, rows, k);
+  if (rows < 0 || rows > OP_MAX_ROWS || k < 1 || k > H2C_I8_MAX_K) return op_error(H2C_ERR_INVALID, "%s: %d rows of %d", who, rows, k);
   if (rows == 0) return H2C_OK;
   if (!x || !q || !scale) return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
   if ((uintptr_t)x & (op_elem_size(type) - 1)) return op_error(H2C_ERR_INVALID, "%s: x must be aligned to its elements", who);
@@ -526,7 +526,7 @@ int h2c_i8_matmul(int32_t x_type, const void* x, int64_t x_row, const float* x_s
   const bool codes = x_type == H2C_TYPE_I8;
   if (!codes && !op_type_ok(x_type)) return op_error(H2C_ERR_BAD_TYPE, "%s: element type %d of x", who, x_type);
   if (!op_type_ok(y_type)) return op_error(H2C_ERR_BAD_TYPE, "%s: element type %d of y", who, y_type);
-  if (m < 0 || n < 0 || k < 1 || k > H2C_I8_MAX_K)
+  if (m < 0 || n < 0 || m > OP_MAX_ROWS || n > OP_MAX_ROWS || k < 1 || k > H2C_I8_MAX_K)
     return op_error(H2C_ERR_INVALID, "%s: sizes m %d, n %d, k %d (k is 1 to %d)", who, m, n, k, H2C_I8_MAX_K);
   if (m == 0 || n == 0) return H2C_OK;
   if (!x || !w || !w_scale || !y || (codes && !x_scale)) return op_error(H2C_ERR_INVALID, "%s: null pointer", who);

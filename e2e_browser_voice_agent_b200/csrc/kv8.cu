@@ -469,7 +469,7 @@ int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size
   const char* who = "h2c_kv8_append";
   if (int rc = cache_ok(who, kv, kv_scale, n_pages, page_size, kv_heads, head_dim)) return rc;
   if (!op_type_ok(type)) return op_error(H2C_ERR_BAD_TYPE, "%s: element type %d", who, type);
-  if (rows < 0) return op_error(H2C_ERR_INVALID, "%s: rows %d", who, rows);
+  if (rows < 0 || rows > OP_MAX_ROWS) return op_error(H2C_ERR_INVALID, "%s: rows %d", who, rows);
   if (rows == 0) return H2C_OK;
   if (!k || !v || !slot) return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
   const size_t es = op_elem_size(type);
@@ -506,7 +506,7 @@ int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t
   const char* who = "h2c_kv8_read";
   if (int rc = cache_ok(who, kv, kv_scale, n_pages, page_size, kv_heads, head_dim)) return rc;
   if (!op_type_ok(type)) return op_error(H2C_ERR_BAD_TYPE, "%s: element type %d", who, type);
-  if (rows < 0) return op_error(H2C_ERR_INVALID, "%s: rows %d", who, rows);
+  if (rows < 0 || rows > OP_MAX_ROWS) return op_error(H2C_ERR_INVALID, "%s: rows %d", who, rows);
   if (rows == 0) return H2C_OK;
   if (!slot || !k_out || !v_out) return op_error(H2C_ERR_INVALID, "%s: null pointer", who);
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15)

@@ -706,6 +706,7 @@ int check_args(const char* who, const h2c_kv8_attention_args* g) {
     return op_error(H2C_ERR_INVALID, "%s: n_req must be 0 to %d, not %d", who, H2C_KV8_MAX_REQUESTS, g->n_req);
   if (g->rows < 0 || g->max_q < 0 || g->max_kv < 0 || g->window < 0 || g->table_cols < 0)
     return op_error(H2C_ERR_INVALID, "%s: a size is negative", who);
+  if (g->rows > OP_MAX_ROWS) return op_error(H2C_ERR_INVALID, "%s: rows %d out of range", who, g->rows);
   if ((long long)g->max_q * (g->heads / g->kv_heads) > INT_MAX / 2)
     return op_error(H2C_ERR_INVALID, "%s: max_q %d out of range", who, g->max_q);
   return H2C_OK;

@@ -39,6 +39,8 @@ bool op_rows_meet(const OpRows& a, const OpRows& b) noexcept;
 // Whether of rows x heads vectors of `len` elements, `row` and `head` elements apart, two share elements (exact).
 bool op_vectors_overlap(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t len) noexcept;
 
+// Most rows of a call: kernels count past the last by up to a grid's stride.
+constexpr int OP_MAX_ROWS = 0x7fffffff - (1 << 16);
 constexpr int OP_MAX_DEVICES = 64;
 // Run fn() once per device (kernel attributes); its status, or H2C_OK when it has already run on this device.
 template <class F>

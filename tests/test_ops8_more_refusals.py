@@ -1,5 +1,5 @@
 """The C entries of the 8-bit serving operators refuse outputs that share memory with what other threads still read, or with one
-another, before anything touches a device (so these run without one)."""
+another, and sizes that counters do not hold, before anything touches a device (so these run without one)."""
 import ctypes as C
 
 import pytest
@@ -123,3 +123,14 @@ def test_read_refuses_outputs_over_other_arguments(lib, k_out, v_out, words):
 def test_quantize_refuses_outputs_over_its_values(lib, change, words):
     a = dict(type=0, x=A[0], x_row=50, rows=3, k=50, q=A[1], q_row=64, scale=A[2], stream=None)
     refused(lib, lib.h2c_i8_quantize(*{**a, **change}.values()), "h2c_i8_quantize", "share memory", *words)
+
+
+def test_rows_up_to_the_integers_last_are_refused(lib):
+    """Counters that step past the last row would wrap around."""
+    for rows in (2**31 - 1, 2**31 - 60000):
+        refused(lib, lib.h2c_i8_matmul(*{**MATMUL, "m": rows}.values()), "h2c_i8_matmul", "sizes")
+        refused(lib, lib.h2c_i8_matmul(*{**MATMUL, "n": rows}.values()), "h2c_i8_matmul", "sizes")
+        refused(lib, lib.h2c_i8_quantize(0, A[0], 50, rows, 50, A[1], 64, A[2], None), "h2c_i8_quantize", "rows")
+        refused(lib, lib.h2c_kv8_append(*{**APPEND, "rows": rows}.values()), "h2c_kv8_append", "rows")
+        refused(lib, lib.h2c_kv8_read(A[0], A[1], 8, 16, 2, 64, A[4], rows, 0, A[5], A[6], None), "h2c_kv8_read", "rows")
+        refused(lib, attention(lib, rows=rows), "h2c_kv8_attention", "rows")
