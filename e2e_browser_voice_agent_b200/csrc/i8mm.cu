@@ -31,10 +31,11 @@ namespace {
 
 constexpr int TN = 128;          // weight rows per product
 constexpr int KCH = 128;         // bytes of K per stage
-constexpr int FUSE_TOKENS = 2, FUSE_VALUES = 4096, FUSE_CHUNKS = 32;  // bounds of the form that quantizes its tokens itself
+constexpr int FUSE_TOKENS = 2, FUSE_VALUES = 4096;  // bounds of the form that quantizes its tokens itself
 constexpr int X_CHUNK = 16 * KCH;  // its codes of one stage of K: 16 rows
 constexpr int MAX_STAGES = 12;
 constexpr int SMEM_RING = 220 * 1024;
+static_assert(FUSE_VALUES / KCH * X_CHUNK + 2 * TN * KCH <= SMEM_RING, "all of such a call's codes, and two stages of weights");
 constexpr int MM_THREADS = 256;
 enum { I8_PRODUCER = 11, I8_MMA = 12, I8_EPILOGUE = 13 };
 
@@ -563,10 +564,9 @@ int h2c_i8_matmul(int32_t x_type, const void* x, int64_t x_row, const float* x_s
   shape_of(m, n, a.chunks, &a.nt, &a.mt, &a.splits);
   // (a CTA of that form may write its outputs while another still reads the tokens, so y in their memory takes two kernels)
   const bool fuse = fused(x_type, m, k) && !op_rows_meet(tokens, out);
-  if (fuse) {  // (one tile of 16 tokens; K divided so that a share's codes fit)
+  if (fuse) {  // (one tile of 16 tokens)
     a.nt = 16;
     a.mt = 1;
-    a.splits = std::max(a.splits, (a.chunks + FUSE_CHUNKS - 1) / FUSE_CHUNKS);
   }
   const int x_smem = fuse ? (a.chunks + a.splits - 1) / a.splits * X_CHUNK : 0;
   const int stage_bytes = a.mt * TN * KCH + (fuse ? 0 : a.nt * KCH);
