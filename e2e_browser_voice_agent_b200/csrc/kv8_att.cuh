@@ -49,7 +49,7 @@ __device__ __forceinline__ Request request_of(const AttArgs& a, int r, int* n_al
   const int s0 = a.q_start[r], s1 = a.q_start[r + 1];
   *n_all = s1 - s0;
   R.first = max(s0, 0);
-  R.n_q = min(min(s1, a.rows) - R.first, a.max_q);
+  R.n_q = max(0, min(max(0, min(s1, a.rows)) - R.first, a.max_q));  // (not negative: products with the group must not wrap around)
   const long long room = (long long)a.table_cols << a.page_log;
   R.len = max(0, (int)min((long long)a.kv_len[r], room));
   return R;
