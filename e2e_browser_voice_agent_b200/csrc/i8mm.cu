@@ -508,10 +508,10 @@ int h2c_i8_quantize(int32_t type, const void* x, int64_t x_row, int32_t rows, in
     return op_error(H2C_ERR_INVALID, "%s: q must be 16-byte aligned with rows of a multiple of 16 bytes, at least k", who);
   const int64_t es = (int64_t)op_elem_size(type), k_pad = (k + 15) / 16 * 16;
   const OpRows values{x, rows, x_row * es, k * es}, codes{q, rows, q_row, k_pad};
-  const OpRange in = op_range("x", values), out[] = {op_range("q", codes), {"scale", scale, 4ull * rows}};
+  const OpRange in = op_range("x", values), out[] = {op_range("q", codes), {"scale", scale, 4ull * rows, 4}};
   if (op_rows_meet(values, codes)) return op_error(H2C_ERR_INVALID, "%s: q must not share memory with x", who);
-  if (int rc = op_disjoint(who, out, 2, &in, 0)) return rc;
-  if (int rc = op_disjoint(who, out + 1, 1, &in, 1)) return rc;
+  if (int rc = op_check_ranges(who, out, 2, &in, 0)) return rc;
+  if (int rc = op_check_ranges(who, out + 1, 1, &in, 1)) return rc;
   return quantize(who, type, x, x_row, rows, k, q, q_row, scale, (cudaStream_t)stream);
 }
 
@@ -548,12 +548,12 @@ int h2c_i8_matmul(int32_t x_type, const void* x, int64_t x_row, const float* x_s
     return op_error(H2C_ERR_INVALID, "%s: rows of y overlap (%lld elements apart, %d long)", who, (long long)y_row, n);
   const OpRows tokens{x, m, x_row * es, k * es}, out{y, m, y_row * ys, n * ys};
   {
-    const OpRange in[] = {{"w", w, (uint64_t)(n - 1) * w_row + k}, {"w_scale", w_scale, 4ull * n}, {"bias", bias, bias ? 4ull * n : 0},
-                          {"x_scale", x_scale, codes ? 4ull * m : 0}};
+    const OpRange in[] = {{"w", w, (uint64_t)(n - 1) * w_row + k}, {"w_scale", w_scale, 4ull * n, 4}, {"bias", bias, bias ? 4ull * n : 0, 4},
+                          {"x_scale", x_scale, codes ? 4ull * m : 0, 4}};
     const OpRange written[] = {op_range("y", out), {"workspace", workspace, need}};
-    if (int rc = op_disjoint(who, written, 2, in, 4)) return rc;
+    if (int rc = op_check_ranges(who, written, 2, in, 4)) return rc;
     const OpRange x_range = op_range("x", tokens);
-    if (int rc = op_disjoint(who, written + 1, 1, &x_range, 1)) return rc;
+    if (int rc = op_check_ranges(who, written + 1, 1, &x_range, 1)) return rc;
     if (codes && op_rows_meet(tokens, out)) return op_error(H2C_ERR_INVALID, "%s: y must not share memory with the codes x", who);
   }
   cudaStream_t st = (cudaStream_t)stream;

@@ -443,11 +443,11 @@ int h2c_kv8_plan(int32_t n_req, int32_t page_size, const int32_t* cached, const 
     return op_error(H2C_ERR_INVALID, "%s: max_tokens %d out of range", who, max_tokens);
   // (every CTA reads all of the inputs while others write)
   const uint64_t n4 = 4ull * n_req, t4 = 4ull * max_tokens;
-  const OpRange in[] = {{"cached", cached, n4}, {"total", total, n4}, {"free_state", free_state, 16}};
-  const OpRange out[] = {{"block_table", block_table, n4 * table_cols}, {"free_ring", free_ring, 4ull * n_pages},
-                         {"free_state_out", free_state_out, 16}, {"kv_len", kv_len, n4}, {"q_start", q_start, n4 + 4},
-                         {"slot", slot, t4}, {"position", position, t4}, {"status", status, 8}};
-  if (int rc = op_disjoint(who, out, 8, in, 3)) return rc;
+  const OpRange in[] = {{"cached", cached, n4, 4}, {"total", total, n4, 4}, {"free_state", free_state, 16, 8}};
+  const OpRange out[] = {{"block_table", block_table, n4 * table_cols, 4}, {"free_ring", free_ring, 4ull * n_pages, 4},
+                         {"free_state_out", free_state_out, 16, 8}, {"kv_len", kv_len, n4, 4}, {"q_start", q_start, n4 + 4, 4},
+                         {"slot", slot, t4, 4}, {"position", position, t4, 4}, {"status", status, 8, 4}};
+  if (int rc = op_check_ranges(who, out, 8, in, 3)) return rc;
   static unsigned char done[OP_MAX_DEVICES];
   const int smem_max = 3 * (H2C_KV8_MAX_REQUESTS + 1) * (int)sizeof(unsigned);
   if (int rc = op_once(who, done, [&] {
@@ -481,10 +481,10 @@ int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size
       return OpRange{name, static_cast<const uint8_t*>(at) + (std::min(0LL, r) + std::min(0LL, h)) * (long long)es,
                      (uint64_t)(std::abs(r) + std::abs(h) + head_dim) * es};
     };
-    const OpRange in[] = {range("k", k, k_row, k_head), range("v", v, v_row, v_head), {"slot", slot, 4ull * rows}};
+    const OpRange in[] = {range("k", k, k_row, k_head), range("v", v, v_row, v_head), {"slot", slot, 4ull * rows, 4}};
     const OpRange out[] = {{"kv", kv, 2ull * n_pages * kv_heads * page_size * head_dim},
-                           {"kv_scale", kv_scale, 8ull * n_pages * kv_heads}};
-    if (int rc = op_disjoint(who, out, 2, in, 3)) return rc;
+                           {"kv_scale", kv_scale, 8ull * n_pages * kv_heads, 4}};
+    if (int rc = op_check_ranges(who, out, 2, in, 3)) return rc;
   }
   // few rows (decode steps): windows of 16, so that few single rows wait in line for a warp; many: windows of a page, so that
   // every CTA of a prompt finds a run (16,392 rows into pages of 64: 19.6 us; with windows of 16, of which most begin no run, 29)
@@ -513,9 +513,9 @@ int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t
     return op_error(H2C_ERR_INVALID, "%s: k_out and v_out must be 16-byte aligned", who);
   const uint64_t bytes = (uint64_t)rows * kv_heads * head_dim * op_elem_size(type);
   const OpRange in[] = {{"kv", kv, 2ull * n_pages * kv_heads * page_size * head_dim},
-                        {"kv_scale", kv_scale, 8ull * n_pages * kv_heads}, {"slot", slot, 4ull * rows}};
+                        {"kv_scale", kv_scale, 8ull * n_pages * kv_heads, 4}, {"slot", slot, 4ull * rows, 4}};
   const OpRange out[] = {{"k_out", k_out, bytes}, {"v_out", v_out, bytes}};
-  if (int rc = op_disjoint(who, out, 2, in, 3)) return rc;
+  if (int rc = op_check_ranges(who, out, 2, in, 3)) return rc;
   const int across = std::min(256, (2 * kv_heads * (head_dim / 4) + 31) / 32 * 32);
   const dim3 block(across, 256 / across);
   const int ctas = std::min((rows + (int)block.y - 1) / (int)block.y, 148 * 8);

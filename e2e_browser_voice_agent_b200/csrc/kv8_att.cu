@@ -757,14 +757,14 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* g, void* stream) {
     if (!in_place && op_rows_meet(q, out))
       return op_error(H2C_ERR_INVALID, "%s: out must be q itself or share no memory with it", who);
     const uint64_t kv_bytes = 2ull * g->n_pages * g->kv_heads * g->page_size * g->head_dim;
-    const OpRange in[] = {{"kv", g->kv, kv_bytes}, {"kv_scale", g->kv_scale, 8ull * g->n_pages * g->kv_heads},
-                          {"block_table", g->block_table, 4ull * g->n_req * g->table_cols},
-                          {"q_start", g->q_start, 4ull * g->n_req + 4}, {"kv_len", g->kv_len, 4ull * g->n_req}};
-    const OpRange written[] = {op_range("out", out), {"lse", g->lse, g->lse ? 4ull * g->rows * g->heads : 0},
+    const OpRange in[] = {{"kv", g->kv, kv_bytes}, {"kv_scale", g->kv_scale, 8ull * g->n_pages * g->kv_heads, 4},
+                          {"block_table", g->block_table, 4ull * g->n_req * g->table_cols, 4},
+                          {"q_start", g->q_start, 4ull * g->n_req + 4, 4}, {"kv_len", g->kv_len, 4ull * g->n_req, 4}};
+    const OpRange written[] = {op_range("out", out), {"lse", g->lse, g->lse ? 4ull * g->rows * g->heads : 0, 4},
                                {"workspace", g->workspace, p.bytes}};
-    if (int rc = op_disjoint(who, written, 3, in, 5)) return rc;
+    if (int rc = op_check_ranges(who, written, 3, in, 5)) return rc;
     const OpRange q_range = op_range("q", q);
-    if (int rc = op_disjoint(who, written + 1, 2, &q_range, 1)) return rc;
+    if (int rc = op_check_ranges(who, written + 1, 2, &q_range, 1)) return rc;
   }
   const long long most = std::max((long long)p.splits * p.tiles * RW_ROWS, (long long)p.shape.tiles * PR_ROWS);
   if (most * g->kv_heads > INT_MAX) return op_error(H2C_ERR_INVALID, "%s: too many rows for one call", who);

@@ -24,7 +24,7 @@ int op_launched(const char* who) noexcept {
   return c == cudaSuccess ? H2C_OK : op_error(H2C_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(c));
 }
 
-int op_disjoint(const char* who, const OpRange* out, int n_out, const OpRange* in, int n_in) noexcept {
+int op_check_ranges(const char* who, const OpRange* out, int n_out, const OpRange* in, int n_in) noexcept {
   auto meet = [](const OpRange& a, const OpRange& b) {
     const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
     return a.bytes && b.bytes && (x < y ? y - x < a.bytes : x - y < b.bytes);
@@ -34,6 +34,10 @@ int op_disjoint(const char* who, const OpRange* out, int n_out, const OpRange* i
       if (meet(out[i], in[j])) return op_error(H2C_ERR_INVALID, "%s: %s must not share memory with %s", who, out[i].name, in[j].name);
     for (int j = 0; j < i; j++)
       if (meet(out[i], out[j])) return op_error(H2C_ERR_INVALID, "%s: %s must not share memory with %s", who, out[i].name, out[j].name);
+  }
+  for (int i = 0; i < n_out + n_in; i++) {
+    const OpRange& r = i < n_out ? out[i] : in[i - n_out];
+    if (r.bytes && (uintptr_t)r.p % r.align) return op_error(H2C_ERR_INVALID, "%s: %s must be aligned to %u bytes", who, r.name, r.align);
   }
   return H2C_OK;
 }

@@ -18,15 +18,16 @@ int op_launched(const char* who) noexcept;
 // (read by h2c_ops_check); nullptr when the device cannot be queried.
 int* op_err_words() noexcept;
 
-// An argument's memory: its name and the bytes from its lowest to its highest.
+// An argument's memory: its name, the bytes from its lowest to its highest, and the alignment that it needs.
 struct OpRange {
   const char* name;
   const void* p;
   uint64_t bytes;
+  unsigned align = 1;
 };
-// H2C_OK, or H2C_ERR_INVALID with "<who>: X must not share memory with Y" when one of the `n_out` ranges that a call writes shares
-// bytes with one of the `n_in` that it reads, or two that it writes do.
-int op_disjoint(const char* who, const OpRange* out, int n_out, const OpRange* in, int n_in) noexcept;
+// H2C_OK, or H2C_ERR_INVALID with "<who>: X must be aligned to N bytes" when one is not, or "<who>: X must not share memory with Y"
+// when one of the `n_out` ranges that a call writes shares bytes with one of the `n_in` that it reads, or two that it writes do.
+int op_check_ranges(const char* who, const OpRange* out, int n_out, const OpRange* in, int n_in) noexcept;
 
 // Rows of `bytes` bytes, `stride` bytes apart (of either sign, or 0).
 struct OpRows {

@@ -246,8 +246,9 @@ int h2c_q4_matvec_noalloc(const void* w, int32_t n_rows, int32_t k, const float*
 /* ---- 8-bit serving operators: a paged 8-bit KV cache and matrix products in 8-bit integers. Stand-alone device
  * operations (no engine): every pointer is a DEVICE pointer unless said otherwise, `stream` is a cudaStream_t of the
  * current device (0 = default) and a call only enqueues work on it, nothing is allocated, and a call whose arguments
- * do not fit returns a status with a message in h2c_last_error(NULL) before anything is enqueued. Sizes of zero
- * (requests, rows) are valid and do nothing; more than 2^31 - 65537 rows are refused. Results do not depend on the stream, the launch or other calls.
+ * do not fit (sizes, alignment to their elements, outputs over other arguments) returns a status with a message in
+ * h2c_last_error(NULL) before anything is enqueued. Sizes of zero (requests, rows) are valid and do nothing; more than
+ * 2^31 - 65537 rows are refused. A call's results do not depend on the stream, on what else runs, or on earlier calls.
  *
  * The cache: `kv` holds int8 codes [n_pages][2][kv_heads][page_size][head_dim] (index 0 of the second axis: K, 1: V;
  * 16-byte aligned), `kv_scale` float32 [n_pages][2][kv_heads], not negative; a cached value is code * scale. page_size is 16, 32, 64 or

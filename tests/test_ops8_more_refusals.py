@@ -134,3 +134,20 @@ def test_rows_up_to_the_integers_last_are_refused(lib):
         refused(lib, lib.h2c_kv8_append(*{**APPEND, "rows": rows}.values()), "h2c_kv8_append", "rows")
         refused(lib, lib.h2c_kv8_read(A[0], A[1], 8, 16, 2, 64, A[4], rows, 0, A[5], A[6], None), "h2c_kv8_read", "rows")
         refused(lib, attention(lib, rows=rows), "h2c_kv8_attention", "rows")
+
+
+def test_arrays_that_are_not_aligned_to_their_elements_are_refused(lib):
+    for name in SIZES:
+        rc = lib.h2c_kv8_plan(*{**PLAN, name: PLAN[name] + 2}.values())
+        refused(lib, rc, "h2c_kv8_plan", NAMES.get(name, name), "aligned")
+    refused(lib, lib.h2c_kv8_plan(*{**PLAN, "state": PLAN["state"] + 4}.values()), "h2c_kv8_plan", "free_state", "8 bytes")
+    for name in ("lse", "kv_scale", "block_table", "q_start", "kv_len"):
+        refused(lib, attention(lib, **{name: A[9] + 1}), "h2c_kv8_attention", name, "aligned")
+    for name, word in (("scale", "kv_scale"), ("slot", "slot")):
+        refused(lib, lib.h2c_kv8_append(*{**APPEND, name: A[9] + 2}.values()), "h2c_kv8_append", word, "aligned")
+    refused(lib, lib.h2c_kv8_read(A[0], A[1] + 2, 8, 16, 2, 64, A[4], 3, 0, A[5], A[6], None), "h2c_kv8_read", "kv_scale", "aligned")
+    refused(lib, lib.h2c_kv8_read(A[0], A[1], 8, 16, 2, 64, A[4] + 2, 3, 0, A[5], A[6], None), "h2c_kv8_read", "slot", "aligned")
+    for name in ("w_scale", "bias"):
+        refused(lib, lib.h2c_i8_matmul(*{**MATMUL, name: A[9] + 2}.values()), "h2c_i8_matmul", name, "aligned")
+    refused(lib, lib.h2c_i8_matmul(*{**CODES, "x_scale": A[9] + 2}.values()), "h2c_i8_matmul", "x_scale", "aligned")
+    refused(lib, lib.h2c_i8_quantize(0, A[0], 50, 3, 50, A[1], 64, A[2] + 2, None), "h2c_i8_quantize", "scale", "aligned")
