@@ -607,8 +607,10 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g) {
     if (g->n_req == 1) {
       p.p_units = p.shape.splits > 1 ? tiles * g->kv_heads * p.shape.splits : 0;
       p.p_join = p.p_units ? join_ctas((long long)tiles * g->kv_heads * PR_ROWS, p.shape.splits) : 0;
-    } else if (g->n_req <= 128 && (long long)g->rows * group / PR_ROWS * g->kv_heads <= 74 && g->kv_heads <= 74 && p.p_keys >= 16) {
-      // all rows together leave SMs idle: each CTA counts (which takes too long for more requests)
+    } else if (g->n_req <= 256 && (long long)g->rows * group / PR_ROWS * g->kv_heads <= 74 && g->kv_heads <= 74 && p.p_keys >= 16) {
+      // all rows together leave half of the SMs or more idle: each CTA counts. A chunk of 256 on 4,096 beside 31, 127, 255 and 511 single
+      // tokens (28 heads over 4 of 128, bfloat16): 72, 97, 138 and 270 us, without the count 121, 137, 176 and 270, so up to 256 requests.
+      // On histories of 16 tiles of keys or more: 128 beside 7 on 768, 1,024 and 1,536 tokens: 36, 40 and 41, without 31, 37 and 47
       p.counted = true;
       p.p_units = 148;
       // rows that the joining kernel may find: of one in 2 .. JOIN_WARP_SPANS units (a warp each), or in more (a CTA each)
