@@ -16,9 +16,11 @@
 // has its weights under way before it waits for the codes. One or two tokens are quantized by every CTA for itself, its share
 // of K into shared memory while the weights come: one launch.
 // Bound and measured: 1 x 896 by 1152 rows, float32: latency, 5.9 us. 32 x 3584 by 37888, bfloat16: the weights' bytes, 33 us with
-// the codes of the tokens (136 MB, 4.6 TB/s over the product's 30). 4099 x 18944 by 3584: 270 us with the codes, the product alone
-// 235 (2,370 Top/s): the operands' way from L2.
-// Waits are bounded (1 s): on expiry the CTA records it (h2c_ops_check), drains its copies and returns.
+// the codes of the tokens (136 MB, 4.6 TB/s over the product's 30). 4099 x 18944 by 3584: 267 us with the codes, the product alone
+// 235 (2,370 Top/s): the operands' way from L2. (In bursts of ten; in a run of seconds the power limit brings the SMs to 1,695 MHz,
+// and it takes 301 us.)
+// Waits for data are bounded (1 s): on expiry the CTA records it (h2c_ops_check), drains its copies and returns. The allocation of
+// TMEM waits for the SM's other CTAs to free theirs, which they do at their end, whether their own waits expire or not.
 #include "ops.cuh"
 #include "tc5_ptx.cuh"
 

@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv8_plan(const PlanArgs a) {
 // (a run longer than the window reaches beyond it). Runs of up to SHORT rows (decode steps: one row) take a warp each,
 // longer ones the whole CTA. A thread holds its values in registers between the maximum and the codes, so each input
 // is read once. Bound: latency: one row, or a prompt's chain of slots, run, loads, maximum and codes, which 5 CTAs an SM (4: 21
-// us, 6: 24) hide in part. 32 rows of 4 heads of 128, bfloat16: 4.3 us; 16,392 rows: 19.6 us, 50 MB at 2.6 TB/s.
+// us, 6: 24) hide in part. 32 rows of 4 heads of 128, bfloat16: 4.5 us; 16,392 rows: 19.5 us, 50 MB at 2.6 TB/s. Float32 rows, which
+// take twice the registers, 2 CTAs an SM: 4.2 and 31 us (4, which spill: 4.6 and 27; 200 prompts of 20 rows 11.8 and 12.7).
 constexpr int APP_THREADS = 256, APP_WIN = 16, APP_MAX_WIN = 128, APP_SHORT = 2;
 constexpr float SCALE_MIN = 0x1p-62f, SCALE_MAX = 0x1p63f;
 

@@ -13,10 +13,12 @@
 // * The cache is the traffic: each lane copies its own 16-byte pieces of a block with cp.async into a ring that only it
 //   reads, so the ring needs no barrier; the order of dimensions inside a product is free as long as both operands use
 //   it, which lets a lane take 16 consecutive bytes of a key (QK) or of 4 keys (PV) without a transpose.
-// * Bound: the cache's bytes for long histories, of which it reads 4.5 TB/s (28 heads over 4, 128 wide, bfloat16; 8 requests
-//   of 69,224-131,072 tokens, 876 MB: 195 us, of which the loads alone take 179: 3 CTAs of 168 registers an SM keep no more
-//   bytes on their way); latency for short ones (32 requests of 120-4,096 tokens, 51 MB: 20 us and 5 to join; one of 641
-//   tokens, 14 heads over 2, 64 wide, float32: 5.8 us, of which a launch is 2-3).
+// * Bound: long histories (28 heads over 4, 128 wide, bfloat16; 8 requests of 69,224-131,072 tokens, 876 MB: 193 us, 4.5 TB/s)
+//   not by the bytes that can be on their way (12 warps an SM, 3 blocks of 4 KB each), nor by DRAM (48% of its cycles), but by
+//   what the warps wait for between them: shared memory (1.6 stalls an issue), fixed latencies (1.2), the matrix pipe (0.6);
+//   the loads alone take 179 us in this ring. The time goes with the SMs' clock: 210 us in a run of seconds, in which the power
+//   limit brings it to 1,750 MHz. Short ones by latency (32 requests of 120-4,096 tokens, 51 MB: 19 us and 5 to join; one of
+//   641 tokens, 14 heads over 2, 64 wide, float32: 5.9 us, of which a launch is 2-3).
 #include "kv8_att.cuh"
 #include "kv8_prompt.cuh"
 
@@ -409,7 +411,9 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
 
 // Joins the spans of one row: the weights of span s relative to the common maximum are 2^(m_s - m). Span s of the row has
 // its sums at part + s * part_step and its (m, l) at ml + s * ml_step. By a warp for few spans (8 rows a CTA), by 8 warps for many,
-// each taking every 8th span: `n_warps`, `w` the warp's turn; the order of the additions goes by the spans' number alone.
+// each taking every 8th span: `n_warps`, `w` the warp's turn; the order of the additions goes by the spans' number alone. A warp up
+// to 12 spans (a chunk of 256 on 4,096, 10 spans: 30 us, 41 by 8 warps, 33 with room for 24 in a warp's registers; 32 single tokens,
+// 7 spans: 19, 21, 19; a chunk of 100 on 16,000, 18 spans: 43 by 8 warps, 39 by one with room for 24).
 constexpr int JOIN_WARPS = 8, JOIN_WARP_SPANS = 12;
 template <class T, int HD>
 __device__ __forceinline__ void join_row(const AttArgs& a, const float* part, size_t part_step, const float2* ml, size_t ml_step,
@@ -552,10 +556,12 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) k_att_join(const RowArgs ra, 
 // that visits few keys altogether (row tiles of 8 x keys, as many as max_q and max_kv allow; a tile's start counts as 256 keys)
 // is k_att_rows' whole: up to 2^17 visits 128 wide, 2^19 64 wide. In a call of more, each CTA looks at its request's rows on the
 // device: up to 16 (32) are k_att_rows', others k_att_prompt's, and the host launches the one kernel or both by max_q.
-// Measured, k_att_rows and k_att_prompt in us, bfloat16 128 wide, 28 heads over 4: 2 requests of 4,000 keys, 21 rows (96,000
-// visits) 17 and 21, 35 rows (160,000) 25 and 22, 252 rows (1,024,000) 71 and 29; 32 requests of 4,000 keys, 14 rows (1,024,000)
-// 73 and 82. float32 64 wide, 14 over 2: 8 requests of 4,000 keys, 35 rows (320,000) 20 and 23, 126 rows (1,024,000) 35 and 26; of
-// 16,000 keys, 21 rows (768,000) 32 and 47.
+// Measured, k_att_rows and k_att_prompt in us. bfloat16 128 wide, 28 heads over 4, one request of 4,000 keys: 35 rows (80,000
+// visits) 14 and 21, 70 rows (144,000) 21 and 22, 126 rows (256,000) 31 and 23; of 16,000, 35 rows (320,000) 32 and 26. Several
+// requests, whose spans are longer, cross later: 2 of 4,000 keys, 35 rows (160,000) 24 and 32, 70 rows (288,000) 36 and 33, 252 rows
+// (1,024,000) 67 and 38. float32: 70 rows of one 21 and 26, 126 rows 31 and 28. 64 wide, 14 over 2, bfloat16 and float32: one of
+// 4,000 keys, 504 rows (504,000) 23, 22 and 27, 1,008 rows (1,008,000) 36, 27 and 32; of 16,000, 126 rows (512,000) 24, 18 and 22;
+// 8 of 4,000 keys, 63 rows (512,000) 23, 28 and 34, 126 rows (1,024,000) 35, 29 and 35.
 struct WorkPlan {
   bool rows, prompt, cluster, counted;
   int max_rows, splits, blocks, tiles;         // k_att_rows
@@ -585,7 +591,9 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g) {
   if (p.rows) {
     p.max_rows = p.prompt ? few : INT_MAX;
     p.tiles = (int)((std::min<long long>(most_rows, p.max_rows) + RW_ROWS - 1) / RW_ROWS);
-    // spans: enough CTAs for two waves of three per SM. Up to 8 are one cluster, whose join costs little: spans of 128 keys (2
+    // spans: enough CTAs for two waves of three per SM (28 heads over 4, 128 wide, bfloat16; 888, half and one and a half times as
+    // many in us: 32 requests of 100-4,096 keys 19, 23 and 19; 64 of them 33, 44 and 35; 2 of 30,000-60,000 42, 38 and 47; 8 of
+    // 60,000-131,072 175, 176 and 164; 32 of 4,000-16,000 89, 81 and 75). Up to 8 are one cluster, whose join costs little: spans of 128 keys (2
     // blocks per warp) or more. More of them, for few rows over long histories, leave their parts in the workspace for a
     // second kernel: spans of 256 keys or more, below which a span's start-up costs more than it shares out
     const long long groups = (long long)g->n_req * g->kv_heads * p.tiles, want = (888 + groups - 1) / groups;

@@ -15,16 +15,19 @@
 // * A page's scale of K multiplies its scores; its scale of V joins the exponent (see split_scale), so a row's weights
 //   are powers of two relative to one running maximum, which moves only when a score passes it by M_SLACK: only then is
 //   O rescaled (by the softmax warps, in TMEM).
-// * float32 queries and weights are two float16 terms each (22 bits), one tcgen05.mma per term.
+// * float32 queries and float32 and float16 rows' weights are two float16 terms each (22 bits), one tcgen05.mma per term.
+// * The tensor cores' sums are added up outside them every few tiles of keys (see FOLD).
 // * V lies in shared memory as its rows come, [key][dimension]: the second product's B operand in MN-major form.
 // * The softmaxes of the two row tiles take turns at the exponentials, so that one's wait for its scores falls into the
 //   other's turn (385 us in step with each other, 370 so).
 // Bound: a key tile of 256 rows needs 1,024 cycles of exponentials (16 a cycle) and about 1,280 of the tensor cores (the S
 // products' operands of 64 keys take 1.5 times their multiply time to read from shared memory). It takes about 2,350: the
 // softmax warps issue what lies between a score and its weight (maximum, scale, conversion, TMEM both ways) one after the
-// other, and each hand-over between warps costs 115-175 cycles. A CTA spends about 12,500 cycles more on its first scores and
-// its last outputs. Measured (4 prompts of 2,064-4,099 tokens, 28 heads over 4, 128 wide, bfloat16): 370 us, 684
-// TFLOP/s of the products that the mask leaves. Slower: tiles of 128 keys with one S slot (412), two threads a row (405).
+// other, and each hand-over between warps costs 115-175 cycles (2.0 stalls an issue at barriers, 1.8 for fixed latencies; tensor
+// pipe 27%, issue 45% busy). That is where this form stands, not a bound of the hardware. A CTA spends about 12,500 cycles more
+// on its first scores and its last outputs. Measured (4 prompts of 2,064-4,099 tokens, 28 heads over 4, 128 wide, bfloat16): 382
+// us, 662 TFLOP/s of the products that the mask leaves. Slower: tiles of 128 keys with one S slot (412), two threads a row (405).
+// Waits for data are bounded; the allocation of TMEM waits for an SM's other CTAs, which free theirs at their end in any case.
 #pragma once
 #include "kv8_att.cuh"
 #include "tc5_ptx.cuh"
