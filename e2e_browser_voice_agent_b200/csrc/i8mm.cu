@@ -16,8 +16,8 @@
 // has its weights under way before it waits for the codes. One or two tokens are quantized by every CTA for itself, its share
 // of K into shared memory while the weights come: one launch.
 // Bound and measured: 1 x 896 by 1152 rows, float32: latency, 5.9 us. 32 x 3584 by 37888, bfloat16: the weights' bytes, 33 us with
-// the codes of the tokens (136 MB, 4.6 TB/s over the product's 30). 4099 x 18944 by 3584: 267 us with the codes, the product alone
-// 235 (2,370 Top/s): the operands' way from L2. (In bursts of ten; in a run of seconds the power limit brings the SMs to 1,695 MHz,
+// the codes of the tokens (136 MB, 4.4 TB/s over the product's 31). 4099 x 18944 by 3584: 270 us with the codes, the product alone
+// 227 (2,455 Top/s): the operands' way from L2. (In bursts of ten; in a run of seconds the power limit brings the SMs to 1,695 MHz,
 // and it takes 301 us.)
 // Waits for data are bounded (1 s): on expiry the CTA records it (h2c_ops_check), drains its copies and returns. The allocation of
 // TMEM waits for the SM's other CTAs to free theirs, which they do at their end, whether their own waits expire or not.
@@ -44,7 +44,7 @@ enum { I8_PRODUCER = 11, I8_MMA = 12, I8_EPILOGUE = 13 };
 // ---------------------------------------------------------------- quantize rows
 //
 // A CTA a row, read twice (the second time from L2), four loads ahead. Bound: bandwidth for many rows (4,099 x 18,944 bfloat16, 233
-// MB: 56 us, 4.2 TB/s), latency for few (32 x 3,584: 4.5 us). Rows of more than 4,096 get 1,024 threads while there are too few to
+// MB: 54 us, 4.3 TB/s), latency for few (32 x 3,584: 2.4 us). Rows of more than 4,096 get 1,024 threads while there are too few to
 // fill the SMs (32 x 18,944 with its product through 3,584 rows: 36.9 us, with 256 threads 39.1; 4,099 rows: 270 with 256, 289).
 
 // A row's scale and what its values are multiplied by, from its largest magnitude's bits (magnitudes order as their bits do,

@@ -75,6 +75,7 @@ struct EndAfterThePrompts {
   __device__ __forceinline__ ~EndAfterThePrompts() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 };
 
+// (the CTAs an SM that shared memory has room for 128 wide, and registers 64 wide: without the bound the compiler spills for one more)
 template <class T, int HD>
 __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(const RowArgs ra) {
   const EndAfterThePrompts end;

@@ -256,7 +256,8 @@ struct PromptCfg {
 };
 
 // The weights of one tile of keys for one row: scores s (products of codes) to p = 2^(s f + e - m), times V's mantissa where the
-// exponent does not hold it (MANT), packed as float16 (and the remainders when two terms are kept); the sum of the softmax's weights is added to l. base = P_SHIFT - m.
+// exponent does not hold it (MANT), packed as float16 (and the remainders when two terms are kept); the sum of the softmax's weights
+// is added to l. base = P_SHIFT - m.
 template <int TERMS, bool MANT, bool EDGE>
 __device__ __forceinline__ void weights(const float* s, const KeyInfo* in, float base, int key0, int first_key,
                                         int pos, uint32_t* p, uint32_t* rest, float* l) {

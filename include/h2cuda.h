@@ -251,7 +251,8 @@ int h2c_q4_matvec_noalloc(const void* w, int32_t n_rows, int32_t k, const float*
  * 2^31 - 65537 rows are refused. A call's results do not depend on the stream, on what else runs, or on earlier calls.
  *
  * The cache: `kv` holds int8 codes [n_pages][2][kv_heads][page_size][head_dim] (index 0 of the second axis: K, 1: V;
- * 16-byte aligned), `kv_scale` float32 [n_pages][2][kv_heads], not negative; a cached value is code * scale. page_size is 16, 32, 64 or
+ * 16-byte aligned), `kv_scale` float32 [n_pages][2][kv_heads], not negative; a cached value is code * scale. page_size is
+ * 16, 32, 64 or
  * 128, head_dim 64 or 128, n_pages * page_size < 2^31. A slot is page * page_size + offset. A request's position p lies
  * in page block_table[request][p / page_size] at offset p % page_size; no page belongs to two requests. ---- */
 
@@ -299,15 +300,18 @@ int h2c_kv8_plan(int32_t n_req, int32_t page_size, const int32_t* cached, const 
  * page new whatever it held): if a > 127.5 s0 the scale becomes s = max(a / 127, 1.25 s0), within [2^-62, 2^63], and the
  * codes at earlier offsets become round(code * (s0 / s)); else s = s0. The new codes are round(x * (1 / s)), within
  * [-127, 127] (float32 operations, halves to even). A code is re-rounded only when the scale grows, which it does by at
- * least 1.25 each time, so a cached value is off by at most 2.5 final steps. A row with an infinity or NaN makes its
- * page's scale NaN until the page is new again: every read of that page and head gives NaN. The cache shares no memory with k, v or
+ * least 1.25 each time, so a cached value is off by at most 2.5 final steps (magnitudes above 127 * 2^63 become that). A
+ * row with an infinity or NaN makes its
+ * page's scale NaN until the page is new again: every read of that page and head gives NaN. The cache shares no memory
+ * with k, v or
  * slot (refused). */
 int h2c_kv8_append(void* kv, float* kv_scale, int32_t n_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
                    int32_t type, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                    int64_t v_head, int32_t rows, const int32_t* slot, void* stream);
 
 /* The cached values at slot[t], t < rows: k_out and v_out [rows][kv_heads][head_dim] of element type `type` (16-byte
- * aligned, sharing no memory with the cache, slot or each other); zeros where the slot is not in the cache. To move a session elsewhere, or to look at what the cache holds. */
+ * aligned, sharing no memory with the cache, slot or each other); zeros where the slot is not in the cache. To move a
+ * session elsewhere, or to look at what the cache holds. */
 int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t page_size, int32_t kv_heads,
                  int32_t head_dim, const int32_t* slot, int32_t rows, int32_t type, void* k_out, void* v_out,
                  void* stream);
@@ -317,9 +321,17 @@ int h2c_kv8_read(const void* kv, const float* kv_scale, int32_t n_pages, int32_t
  * positions 0 .. p, or p - window + 1 .. p with window > 0. Head h reads kv head h / (heads / kv_heads).
  *   x = scale * (q . k),  out = sum softmax(x) v  (rounded once to `type`),  lse = log sum exp x  (natural logarithm)
  * A query with no position to attend to (p < 0) gives zeros and lse = -infinity. Rows of q that belong to no request are
- * not touched. out may be q itself (the same address and strides); otherwise what is written (out, lse, the workspace) shares no
- * memory with another argument, nor do two vectors of out (refused). Scores, softmax statistics and sums are float32; codes and float16 / bfloat16 queries enter the tensor
- * cores exactly, float32 queries as two float16 terms (22 bits). */
+ * not touched. out may be q itself (the same address and strides); otherwise what is written (out, lse, the workspace)
+ * shares no
+ * memory with another argument, nor do two vectors of out (refused).
+ * Scores, softmax statistics and sums are float32. Codes and 16-bit queries enter the tensor cores exactly, float32 queries
+ * as two float16 terms (22 bits), the softmax's weights as two, too, save in bfloat16 prompts, which round each weight to 11
+ * bits (2^-12 of it; the output's own rounding is 2^-9 of itself). 16-bit prompts take V's scales through their logarithm
+ * (2^-22), and one below 2^-62 as 2^-62. Prompts' sums are the tensor cores' for 4 to 128 tiles of 64 keys, which cut off
+ * what float32 does not hold, and are rounded between: that puts float32 outputs off by some 1e-6 of their size at any
+ * length of the history, 16-bit outputs by 2e-5 beside their rounding. How a call is divided (n_req, max_q, max_kv,
+ * window, and so the
+ * requests beside a request) moves results within these errors; the same call gives the same bits every time. */
 typedef struct h2c_kv8_attention_args {
   const void* q;          /* row t of head h at t * q_row + h * q_head elements, head_dim values */
   int64_t q_row, q_head;
@@ -354,7 +366,8 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* args, void* stream);
  * row's largest magnitude, scale = a / 127 and q = round(x * min(127 / a, FLT_MAX)) (float32 operations, halves to even;
  * a row of zeros gives zeros). Rows of q start q_row bytes apart (a multiple of 16, at least k, q 16-byte aligned); the
  * bytes from k to the next multiple of 16 become 0. A row with an infinity or NaN has the scale NaN (and codes without
- * meaning): every product with it is NaN. q and scale share no memory with x or each other (refused). For weights (rows = output channels), once, and for activations that
+ * meaning): every product with it is NaN. q and scale share no memory with x or each other (refused). For weights (rows =
+ * output channels), once, and for activations that
  * several products share. */
 int h2c_i8_quantize(int32_t type, const void* x, int64_t x_row, int32_t rows, int32_t k, void* q, int64_t q_row,
                     float* scale, void* stream);
