@@ -51,8 +51,11 @@ class Server:
         """Pages and slots for the step that takes the sessions to these lengths."""
         p = kv8.plan(self.kv_len, torch.tensor(total, dtype=torch.int32, device="cuda"), self.table, self.free,
                      self.free_state, self.page, tokens)
-        if p.status[0] != 0:  # (the one place where the host waits for the step's plan)
-            raise RuntimeError(f"out of pages: {int(p.status[1])} missing")
+        code, missing = p.status.tolist()  # (the one place where the host waits for the step's plan)
+        if code == 1:
+            raise RuntimeError(f"out of pages: {missing} missing")
+        if code:
+            raise RuntimeError(f"lengths {total} do not fit tables of {self.table.shape[1] * self.page} positions")
         self.kv_len, self.free_state, self.length = p.kv_len, p.free_state, total
         return p
 
