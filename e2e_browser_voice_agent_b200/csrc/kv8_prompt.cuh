@@ -119,7 +119,7 @@ __device__ __forceinline__ TileAt tile_at(const PromptArgs& pa, int idx) {
       const int u = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += u;
     }
-    const int at = idx - before;  // among this round's tiles
+    const int at = idx - before;  // among these requests' tiles
     const unsigned in = __ballot_sync(0xffffffffu, at >= sum - n && at < sum);
     if (in) {
       const int l = __ffs(in) - 1;

@@ -22,7 +22,7 @@ def _matrix(name: str, t: torch.Tensor, index: int) -> int:
         raise ValueError(f"{name}: a matrix is wanted, not {tuple(t.shape)}")
     if t.get_device() != index:
         raise ValueError(f"{name}: on {t.device}, not cuda:{index}")
-    if t.shape[0] >= 2**31 or t.shape[1] >= 2**31:
+    if t.numel() >= 2**31 and max(t.shape) >= 2**31:
         raise ValueError(f"{name}: {tuple(t.shape)} does not fit in 32 bits")
     if t.stride(1) != 1 and t.shape[1] > 1:
         raise ValueError(f"{name}: rows must be dense")
