@@ -230,7 +230,7 @@ struct PromptCfg {
   static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   static constexpr int Q_TERMS = sizeof(T) == 4 ? 2 : 1;  // float16 terms of queries
   // ... and of weights. One where the output is bfloat16: 2^-12 of each weight, an eighth of that rounding. With float16 outputs one
-  // term's error would be as large as theirs (some 1.2 times the error in all; 445 us for the prompts below, 541 with two).
+  // term's error would be as large as theirs (some 1.2 times the error in all; 445 us for the prompts below, 543 with two).
   static constexpr int P_TERMS = BF16 ? 1 : 2;
   static constexpr int BLKS = HD / 64;                   // 64-dimension blocks of a row
   static constexpr int Q_TILE = 128 * HD * 2;            // one row tile, one term
@@ -242,8 +242,8 @@ struct PromptCfg {
   // holds FOLD tiles' sum and is then added to the sum so far by the softmax warps, which round. 64 wide that lies beside O in
   // TMEM; 128 wide there is no room, and it lies in a place of the workspace (SPILL, claim_slot). One span of 4,000 and 131,072 keys,
   // relative to the output: off by 7e-6 and 4.5e-4 without (16-bit types, before their rounding: 5e-6 and 4e-4). Float32 4e-7 and
-  // 1.5e-6 so 64 wide (a chunk of 256 on 4,096 tokens takes 30 us for 27.6), 8e-7 and 1.6e-6 128 wide (that chunk, 28 heads over 4, 60
-  // us for 53, prompts of 2,064-4,099 770 for 650: the places' way to L2. 4 tiles: 63 and 830 us, 4e-7 and 1.4e-6; CTAs of one row
+  // 1.5e-6 so 64 wide (a chunk of 256 on 4,096 tokens takes 30 us for 27.6), 8e-7 and 1.6e-6 128 wide (that chunk, 28 heads over 4, 62
+  // us for 53, prompts of 2,064-4,099 797 for 650: the places' way to L2. 4 tiles: 63 and 830 us, 4e-7 and 1.4e-6; CTAs of one row
   // tile, whose sum fits into the other's TMEM: 78 and 1,071). 16-bit types 1.2e-5 and less, a twentieth of float16's rounding: chunks
   // on 32,000 and more keys take 2-3% longer.
   static constexpr int FOLD = sizeof(T) == 4 ? (HD == 64 ? 4 : 8) : HD == 64 ? 32 : BF16 ? 128 : 64;
