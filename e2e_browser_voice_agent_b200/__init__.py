@@ -6,7 +6,9 @@ Public surface (mirrors the reference engine, h2-own-inference-engine/engine/):
   llm       LLM.load / feed / generate_ids / reset (llm.js)
   synth     seeded benchmark models
   kv8       a paged 8-bit KV cache over torch tensors: plan, append, attention
-  int8      matrix products in 8-bit integers over torch tensors
+  int8      matrix products in 8-bit integers over torch tensors, and the norm that makes their codes
+  rope      rotary positions of queries and keys
+  logits    penalties, biases and masks on a step's logits
 The CUDA library itself is csrc/ -> libh2cuda.so, declared in include/h2cuda.h.
 """
 __all__ = ["gguf", "synth"]

@@ -23,6 +23,7 @@ DECODE_AUTO, DECODE_GRAPH, DECODE_PERSISTENT = 0, 1, 2
 MATMUL_AUTO, MATMUL_MMA_SYNC, MATMUL_TCGEN05 = 0, 1, 2
 TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8 = 0, 1, 2, 3
 I8_MAX_K = 131072
+LOGITS_MAX_BIASES = 1024
 KV8_MAX_REQUESTS = 8192
 PROFILE_NAMES = ["embed", "norm+quantize", "matvec qkv", "rope+kv", "attention", "quantize", "matvec o",
                  "matvec gate+up", "swiglu+quantize", "matvec down", "matvec output"]  # cpu-worker.js:32
@@ -35,7 +36,8 @@ EXPORTS = ["h2c_create", "h2c_set_tensor", "h2c_forward", "h2c_forward_batch", "
            "h2c_q4_matvec", "h2c_q4_matvec_noalloc", "h2c_set_matmul_kernel", "h2c_matmul_kernel",
            "h2c_tp_unique_id", "h2c_create_tp", "h2c_tp_rank", "h2c_tp_world",
            "h2c_ops_check", "h2c_kv8_plan", "h2c_kv8_append", "h2c_kv8_read", "h2c_kv8_attention_workspace",
-           "h2c_kv8_attention", "h2c_i8_quantize", "h2c_i8_matmul_workspace", "h2c_i8_matmul"]
+           "h2c_kv8_attention", "h2c_i8_quantize", "h2c_i8_matmul_workspace", "h2c_i8_matmul",
+           "h2c_i8_norm", "h2c_i8_values", "h2c_rope", "h2c_logits_adjust"]
 
 
 class Config(C.Structure):
@@ -122,12 +124,18 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     L.h2c_i8_matmul_workspace.argtypes = [i32, i32, i32]
     L.h2c_i8_matmul_workspace.restype = u64
     L.h2c_i8_matmul.argtypes = [i32, p, i64, p, p, i64, p, i32, i32, i32, i32, p, i64, p, p, u64, p]
+    f32, f64 = C.c_float, C.c_double
+    L.h2c_i8_norm.argtypes = [i32, p, i64, i32, p, i64, p, i64, p, f64, i32, i32, p, i64, p, p]
+    L.h2c_i8_values.argtypes = [p, i64, p, i32, i32, i32, p, p]
+    L.h2c_rope.argtypes = [i32, p, i64, i64, p, i64, i64, i32, p, i64, i64, p, i64, i64, i32, i32, i32, p, p, i32, i32, f32, p]
+    L.h2c_logits_adjust.argtypes = [i32, p, i64, p, i64, i32, i32, p, i64, i32, p, p, p, p, p, p, i32, p, i64, p]
     for name in ("h2c_create", "h2c_set_tensor", "h2c_forward", "h2c_forward_batch", "h2c_generate_batch", "h2c_batch_kernels", "h2c_generate", "h2c_decode_kernels", "h2c_set_decode_mode",
                  "h2c_decode_path", "h2c_trace_decode", "h2c_decode_ctas", "h2c_set_decode_fault", "h2c_read_logits",
                  "h2c_profile", "h2c_selftest_math",
                  "h2c_destroy", "h2c_q4_pack", "h2c_q4_matvec", "h2c_q4_matvec_noalloc", "h2c_set_matmul_kernel",
                  "h2c_matmul_kernel", "h2c_tp_unique_id", "h2c_create_tp", "h2c_ops_check", "h2c_kv8_plan",
-                 "h2c_kv8_append", "h2c_kv8_read", "h2c_kv8_attention", "h2c_i8_quantize", "h2c_i8_matmul"):
+                 "h2c_kv8_append", "h2c_kv8_read", "h2c_kv8_attention", "h2c_i8_quantize", "h2c_i8_matmul",
+                 "h2c_i8_norm", "h2c_i8_values", "h2c_rope", "h2c_logits_adjust"):
         getattr(L, name).restype = C.c_int
     _lib = L
     return L

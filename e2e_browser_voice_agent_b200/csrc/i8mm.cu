@@ -47,18 +47,6 @@ enum { I8_PRODUCER = 11, I8_MMA = 12, I8_EPILOGUE = 13 };
 // MB: 54 us, 4.3 TB/s), latency for few (32 x 3,584: 2.4 us). Rows of more than 4,096 get 1,024 threads while there are too few to
 // fill the SMs (32 x 18,944 with its product through 3,584 rows: 36.9 us, with 256 threads 39.1; 4,099 rows: 270 with 256, 289).
 
-// A row's scale and what its values are multiplied by, from its largest magnitude's bits (magnitudes order as their bits do,
-// infinities and NaN above every number: they make the scale NaN). 127 / a overflows for denormal rows, whose largest code is then
-// below 127.
-struct RowScale {
-  float scale, inv;
-};
-__device__ __forceinline__ RowScale row_scale_of(unsigned m) {
-  const float a = __uint_as_float(m);
-  return {m >= 0x7f800000u ? __int_as_float(0x7fc00000) : __fdiv_rn(a, 127.f),
-          a > 0.f ? fminf(__fdiv_rn(127.f, a), 3.4028234663852886e38f) : 0.f};
-}
-
 template <class T, bool VEC>
 __global__ void __launch_bounds__(1024) k_i8_quantize(const T* __restrict__ x, long long x_row, int k, int8_t* __restrict__ q,
                                                       long long q_row, int k_pad, float* __restrict__ scale) {

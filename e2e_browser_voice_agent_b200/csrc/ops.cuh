@@ -82,6 +82,18 @@ __device__ __forceinline__ uint32_t round_bytes(float a, float b, float c, float
   return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
 }
 
+// A row's scale and what its values are multiplied by, from its largest magnitude's bits (magnitudes order as their bits do,
+// infinities and NaN above every number: they make the scale NaN). 127 / a overflows for denormal rows, whose largest code is then
+// below 127.
+struct RowScale {
+  float scale, inv;
+};
+__device__ __forceinline__ RowScale row_scale_of(unsigned m) {
+  const float a = __uint_as_float(m);
+  return {m >= 0x7f800000u ? __int_as_float(0x7fc00000) : __fdiv_rn(a, 127.f),
+          a > 0.f ? fminf(__fdiv_rn(127.f, a), 3.4028234663852886e38f) : 0.f};
+}
+
 // four consecutive values; VEC: the address is aligned to four of them
 template <bool VEC>
 __device__ __forceinline__ void load4(const float* p, float* v) {

@@ -4,17 +4,29 @@ h2c_i8_* operators of libh2cuda (include/h2cuda.h states their formulas).
   w8, w_scale = quantize(weight)                 # once: [n, k] values -> int8 [n, k padded to 16], float32 [n]
   y = matmul(x, w8, w_scale, bias=bias)          # x [m, k] -> y [m, n], the tokens quantized on the way
 
-or, where several products share their input, matmul(xq, w8, w_scale, x_scale=xs, k=k) with xq, xs = quantize(x). Every call
-enqueues kernels on the current stream of the tensors' device and returns; nothing is kept between calls.
+or, where several products share their input, matmul(xq, w8, w_scale, x_scale=xs, k=k) with xq, xs = quantize(x). norm makes such
+codes of a normed residual stream:
+
+  n = norm(x, weight, eps, residual=r)           # n.sum = x + r, n.codes and n.scale of its root-mean-square norm
+  y = matmul(n.codes, w8, w_scale, x_scale=n.scale, k=k)
+
+Every call enqueues kernels on the current stream of the tensors' device and returns; nothing is kept between calls.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
 from .kv8 import _TYPES, _call, _want
+
+
+class Norm(NamedTuple):
+    """What norm returns."""
+    codes: torch.Tensor          # int8 [rows, k padded to a multiple of 16]
+    scale: torch.Tensor          # float32 [rows]
+    sum: Optional[torch.Tensor]  # x + residual, None without a residual
 
 
 def _matrix(name: str, t: torch.Tensor, index: int) -> int:
@@ -92,3 +104,57 @@ def matmul(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Option
           _want("w_scale", w_scale, torch.float32, index, (n,)), m, n, k, y_type, py, y_row,
           None if bias is None else _want("bias", bias, torch.float32, index, (n,)), None if work is None else work.data_ptr(), need)
     return out
+
+
+def norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+         out: Optional[torch.Tensor] = None) -> Norm:
+    """The codes of rows of x ([rows, k], float32, float16 or bfloat16, any row stride), or of x + residual, normed by their root mean
+    square and multiplied by weight (float32 [k]) (h2c_i8_norm). residual has x's type or float32 and gives the sum its type; out takes
+    the sum: residual itself, x itself, a tensor that shares no memory with the arguments, or None for a new one."""
+    index = x.get_device()
+    px = _matrix("x", x, index)
+    if x.dtype not in _TYPES:
+        raise TypeError(f"x: float32, float16 or bfloat16 is wanted, not {x.dtype}")
+    rows, k = x.shape
+    pr = po = None
+    r_type = r_row = o_row = 0
+    if residual is not None:
+        pr, r_row = _matrix("residual", residual, index), residual.stride(0)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual: {tuple(x.shape)} is wanted, not {tuple(residual.shape)}")
+        if residual.dtype is not x.dtype and residual.dtype is not torch.float32:
+            raise TypeError(f"residual: {x.dtype} or float32 is wanted, not {residual.dtype}")
+        r_type = _TYPES[residual.dtype]
+        if out is None:
+            out = torch.empty(rows, k, dtype=residual.dtype, device=x.device)
+        elif out.shape != x.shape:
+            raise ValueError(f"out: {tuple(x.shape)} is wanted, not {tuple(out.shape)}")
+        elif out.dtype is not residual.dtype:
+            raise TypeError(f"out: {residual.dtype} is wanted, not {out.dtype}")
+        po, o_row = _matrix("out", out, index), out.stride(0)
+    elif out is not None:
+        raise ValueError("out: there is no residual, so no sum")
+    q = torch.empty(rows, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _call(index, _lib.load().h2c_i8_norm, _TYPES[x.dtype], px, x.stride(0), r_type, pr, r_row, po, o_row,
+          _want("weight", weight, torch.float32, index, (k,)), eps, rows, k, q.data_ptr(), q.shape[1], scale.data_ptr())
+    return Norm(q, scale, out)
+
+
+def values(codes: torch.Tensor, scale: torch.Tensor, k: Optional[int] = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """What codes of quantize or norm stand for: [rows, k] values of dtype (h2c_i8_values). k: how many of a row's codes count, all
+    unless given."""
+    index = codes.get_device()
+    pq = _matrix("codes", codes, index)
+    if codes.dtype is not torch.int8:
+        raise TypeError(f"codes: int8 is wanted, not {codes.dtype}")
+    if dtype not in _TYPES:
+        raise TypeError(f"dtype: float32, float16 or bfloat16 is wanted, not {dtype}")
+    rows = codes.shape[0]
+    k = codes.shape[1] if k is None else k
+    if not 0 < k <= codes.shape[1]:
+        raise ValueError(f"k: 1 to {codes.shape[1]} is wanted, not {k}")
+    y = torch.empty(rows, k, dtype=dtype, device=codes.device)
+    _call(index, _lib.load().h2c_i8_values, pq, codes.stride(0), _want("scale", scale, torch.float32, index, (rows,)), rows, k,
+          _TYPES[dtype], y.data_ptr())
+    return y

@@ -1,0 +1,114 @@
+"""Rotary positions over torch CUDA tensors: the h2c_rope operator of libh2cuda (include/h2cuda.h states its formula).
+
+  f = frequencies(128, base=1e6)                                   # once: float64 [64], radians per position
+  q, k = rotate(q, p.position, f, k=k)                             # q and k [tokens, heads, head dim], any strides
+
+rotate enqueues one kernel on the current stream of the tensors' device and returns; nothing is kept between calls.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .kv8 import _TYPES, _call, _want
+
+SCALINGS = ("none", "linear", "ntk", "yarn")
+
+
+def frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 0,
+                fast: float = 32.0, slow: float = 1.0, device="cuda") -> torch.Tensor:
+    """The frequencies base ** (-2 j / rotary_dim) of a head's rotary_dim / 2 pairs, in radians per position (float64), as they are or
+    for contexts `factor` times as long as the model's:
+      linear  all divided by factor
+      ntk     the base raised by factor ** (rotary_dim / (rotary_dim - 2)): the slowest is divided by factor, the fastest stays
+      yarn    pairs that turn more than `fast` times within `original` positions stay, those that turn less than `slow` times are
+              divided by factor, and between them the share of both goes linearly with the turns (YaRN, Peng et al. 2023; the
+              attention temperature that belongs to it is yarn_magnitude(factor), an argument of rotate).
+    A model whose frequencies are made otherwise brings its own tensor."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim: an even number is wanted, not {rotary_dim}")
+    if not base > 1 or not factor >= 1:
+        raise ValueError(f"base {base}, factor {factor}: a base above 1 and a factor of at least 1 are wanted")
+    if scaling not in SCALINGS:
+        raise ValueError(f"scaling: one of {SCALINGS} is wanted, not {scaling!r}")
+    half = rotary_dim // 2
+    if scaling == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("scaling ntk: the one pair of rotary_dim 2 has nothing to be stretched against")
+        base *= factor ** (rotary_dim / (rotary_dim - 2))
+    f = [base ** (-2 * j / rotary_dim) for j in range(half)]
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    if scaling == "yarn":
+        if original < 1 or not fast > slow > 0:
+            raise ValueError(f"scaling yarn: original ({original}) positions and fast ({fast}) above slow ({slow}) are wanted")
+        for j in range(half):
+            kept = min(1.0, max(0.0, (f[j] * original / (2 * math.pi) - slow) / (fast - slow)))
+            f[j] *= kept + (1 - kept) / factor
+    return torch.tensor(f, dtype=torch.float64, device=device)
+
+
+def yarn_magnitude(factor: float) -> float:
+    """The magnitude of queries and keys that goes with scaling yarn."""
+    return 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+
+def _vectors(name: str, t: torch.Tensor, like: torch.Tensor, index: int):
+    """(address, row stride, head stride) of [tokens, heads, head dim] values, the last axis dense, of like's type and device."""
+    if t.dim() != 3:
+        raise ValueError(f"{name}: [tokens, heads, head dim] is wanted, not {tuple(t.shape)}")
+    if t.dtype is not like.dtype:
+        raise TypeError(f"{name}: {like.dtype} is wanted, not {t.dtype}")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on {t.device}, not cuda:{index}")
+    row, head, dense = t.stride()
+    if dense != 1:
+        raise ValueError(f"{name}: the head dimension must be dense")
+    return t.data_ptr(), row, head
+
+
+def rotate(q: torch.Tensor, position: torch.Tensor, frequency: torch.Tensor, k: Optional[torch.Tensor] = None,
+           interleaved: bool = False, magnitude: float = 1.0, out: Optional[torch.Tensor] = None,
+           k_out: Optional[torch.Tensor] = None):
+    """q ([tokens, heads, head dim], float32, float16 or bfloat16, any row and head stride) and, with it, k with their first 2 *
+    len(frequency) values turned to their tokens' positions (h2c_rope). position: int32, one per token or more; tokens whose
+    position is negative stay as they are. Pairs are (j, j + len(frequency)), or neighbours with `interleaved`. out and k_out:
+    q and k themselves (in place), tensors that share no memory with the arguments, or None for new ones. Returns q's, or (q's,
+    k's) with k."""
+    index = q.get_device()
+    kind = _TYPES.get(q.dtype)
+    if kind is None:
+        raise TypeError(f"q: float32, float16 or bfloat16 is wanted, not {q.dtype}")
+    pq, q_row, q_head = _vectors("q", q, q, index)
+    tokens, heads, head_dim = q.shape
+    k_heads, pk, k_row, k_head, pko, ko_row, ko_head = 0, None, 0, 0, None, 0, 0
+    if k is not None:
+        pk, k_row, k_head = _vectors("k", k, q, index)
+        k_heads = k.shape[1]
+        if k.shape[0] != tokens or k.shape[2] != head_dim:
+            raise ValueError(f"k: [{tokens}, heads, {head_dim}] is wanted, not {tuple(k.shape)}")
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        elif k_out.shape != k.shape:
+            raise ValueError(f"k_out: {tuple(k.shape)} is wanted, not {tuple(k_out.shape)}")
+        pko, ko_row, ko_head = _vectors("k_out", k_out, q, index)
+    elif k_out is not None:
+        raise ValueError("k_out: there is no k")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out: {tuple(q.shape)} is wanted, not {tuple(out.shape)}")
+    po, o_row, o_head = _vectors("out", out, q, index)
+    if position.dim() != 1 or position.shape[0] < tokens:
+        raise ValueError(f"position: at least {tokens} entries are wanted, not {tuple(position.shape)}")
+    if frequency.dim() != 1 or not 1 <= frequency.shape[0] <= head_dim // 2:
+        raise ValueError(f"frequency: 1 to {head_dim // 2} entries are wanted, not {tuple(frequency.shape)}")
+    if tokens >= 2**31 or heads >= 2**31 or k_heads >= 2**31 or head_dim >= 2**31:
+        raise ValueError(f"q: {tuple(q.shape)} does not fit in 32 bits")
+    _call(index, _lib.load().h2c_rope, kind, pq, q_row, q_head, po, o_row, o_head, heads, pk, k_row, k_head, pko, ko_row, ko_head,
+          k_heads, tokens, head_dim, _want("position", position, torch.int32, index),
+          _want("frequency", frequency, torch.float64, index), 2 * frequency.shape[0], int(bool(interleaved)), magnitude)
+    return out if k is None else (out, k_out)

@@ -384,6 +384,57 @@ int h2c_i8_matmul(int32_t x_type, const void* x, int64_t x_row, const float* x_s
                   const float* w_scale, int32_t m, int32_t n, int32_t k, int32_t y_type, void* y, int64_t y_row,
                   const float* bias, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---- The operators of a serving step beside its cache and its products, to the same rules as those above: device pointers, the
+ * caller's stream, nothing allocated, arguments that do not fit refused before anything is enqueued. ---- */
+
+/* Norm and codes of rows r < rows of k <= H2C_I8_MAX_K values, in one pass. With a residual:
+ *   s = x + residual, rounded to the residual's type and written to sum (row r at sum + r * sum_row elements)
+ * else s = x (residual and sum NULL, res_type and the strides not looked at). Then, with the mean over the row in 64 bits,
+ *   f = 1 / sqrt(mean(s^2) + eps) rounded to float32,  y = (s * f) * weight
+ * and q, scale are the codes and scales that h2c_i8_quantize has for y: a = max |y|, scale = a / 127, q = round(y * min(127 / a,
+ * FLT_MAX)), single float32 operations, halves to even; q as there (rows a multiple of 16 bytes apart, zeros from k to the next
+ * multiple of 16), ready for h2c_i8_matmul with x_type H2C_TYPE_I8. A row whose y holds an infinity or NaN has the scale NaN.
+ * x_type F32, F16 or BF16; res_type x_type or F32; weight float32 [k]; eps not negative. sum may be residual itself or x itself (same
+ * address, strides and type); beside that what is written shares no memory with another argument, nor do rows of sum (refused). */
+int h2c_i8_norm(int32_t x_type, const void* x, int64_t x_row, int32_t res_type, const void* residual, int64_t res_row, void* sum,
+                int64_t sum_row, const float* weight, double eps, int32_t rows, int32_t k, void* q, int64_t q_row, float* scale,
+                void* stream);
+
+/* What codes stand for: y[r][i] = q[r][i] * scale[r], rounded to `type`, rows of y k elements apart. q as above, of which the bytes
+ * from k on are not looked at; y shares no memory with q or scale (refused). */
+int h2c_i8_values(const void* q, int64_t q_row, const float* scale, int32_t rows, int32_t k, int32_t type, void* y, void* stream);
+
+/* Rotary positions. Token t's vectors of q_heads queries (row t of head h at q + t * q_row + h * q_head elements, head_dim values, 2
+ * to 1024) and of k_heads keys (likewise; either may be 0) go to q_out and k_out with the first rotary_dim (even) values turned and
+ * the others as they are. Pair j < rotary_dim / 2 is (x[j], x[j + rotary_dim / 2]), or with `interleaved` (x[2j], x[2j + 1]):
+ *   (a, b) -> (a c - b s, b c + a s),  c = magnitude * cos(u), s = magnitude * sin(u),  u = position[t] * frequency[j]
+ * frequency: float64 [rotary_dim / 2], radians per position. The angle's whole turns are dropped in 64 bits, so it is as exact far
+ * out as near 0; the rest is float32, rounded once. A token whose position is negative (h2c_kv8_plan's beyond the last) is not turned,
+ * magnitude included. q_out may be q itself (same address and strides), k_out k; beside that what is written shares no memory with
+ * another argument, nor do two vectors of it (refused). */
+int h2c_rope(int32_t type, const void* q, int64_t q_row, int64_t q_head, void* q_out, int64_t q_out_row, int64_t q_out_head,
+             int32_t q_heads, const void* k, int64_t k_row, int64_t k_head, void* k_out, int64_t k_out_row, int64_t k_out_head,
+             int32_t k_heads, int32_t tokens, int32_t head_dim, const int32_t* position, const double* frequency,
+             int32_t rotary_dim, int32_t interleaved, float magnitude, void* stream);
+
+#define H2C_LOGITS_MAX_BIASES 1024
+
+/* Penalties, biases and masks on the logits of `rows` rows, `vocab` each (row r at logits + r * in_row elements of `type`, out
+ * likewise). With c the number of times that token i stands among the row's tokens so far (tokens[r * tokens_row + 0 ..
+ * length[r] - 1], at most `columns`; numbers outside the vocabulary count for none), in single float32 operations:
+ *   c > 0:  x = x > 0 ? x / repetition[r] : x * repetition[r],  then  x = x - (frequency[r] * c + presence[r])
+ *   i among bias_id[r][0 .. n_bias):  x = x + the sum of its biases, in the list's order (an id outside the vocabulary, as -1, is
+ *                                     skipped)
+ *   bit i % 32 of allowed[r * allowed_row + i / 32] is 0:  x = -infinity, whatever it was (a row may be left with nothing)
+ * and rounded to `type`. tokens and length NULL: no penalties (repetition, presence and frequency then NULL, too, each of which
+ * may be NULL otherwise: 1, 0 and 0); bias_id and bias int32 and float32 [rows][n_bias], n_bias <= H2C_LOGITS_MAX_BIASES, 0: none;
+ * allowed NULL: all. out may be logits itself (same address and stride); beside that it shares no memory with another argument, nor do
+ * its rows (refused). */
+int h2c_logits_adjust(int32_t type, const void* logits, int64_t in_row, void* out, int64_t out_row, int32_t rows, int32_t vocab,
+                      const int32_t* tokens, int64_t tokens_row, int32_t columns, const int32_t* length, const float* repetition,
+                      const float* presence, const float* frequency, const int32_t* bias_id, const float* bias, int32_t n_bias,
+                      const int32_t* allowed, int64_t allowed_row, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
