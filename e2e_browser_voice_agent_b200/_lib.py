@@ -37,7 +37,8 @@ EXPORTS = ["h2c_create", "h2c_set_tensor", "h2c_forward", "h2c_forward_batch", "
            "h2c_tp_unique_id", "h2c_create_tp", "h2c_tp_rank", "h2c_tp_world",
            "h2c_ops_check", "h2c_kv8_plan", "h2c_kv8_append", "h2c_kv8_read", "h2c_kv8_attention_workspace",
            "h2c_kv8_attention", "h2c_i8_quantize", "h2c_i8_matmul_workspace", "h2c_i8_matmul",
-           "h2c_i8_norm", "h2c_i8_values", "h2c_rope", "h2c_logits_adjust"]
+           "h2c_i8_norm", "h2c_i8_values", "h2c_rope", "h2c_logits_adjust",
+           "h2c_kv8_prefix_attention_workspace", "h2c_kv8_prefix_attention"]
 
 
 class Config(C.Structure):
@@ -57,6 +58,12 @@ class Kv8AttentionArgs(C.Structure):
                 ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("rows", C.c_int32), ("max_q", C.c_int32),
                 ("max_kv", C.c_int32), ("window", C.c_int32), ("scale", C.c_float),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class Kv8PrefixArgs(C.Structure):
+    """h2c_kv8_prefix_args of include/h2cuda.h."""
+    _fields_ = [("own", Kv8AttentionArgs), ("prefix_table", C.c_void_p), ("prefix_len", C.c_void_p), ("group_start", C.c_void_p),
+                ("prefix_cols", C.c_int32), ("n_groups", C.c_int32), ("max_prefix", C.c_int32)]
 
 
 class H2CError(RuntimeError):
@@ -124,6 +131,9 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     L.h2c_i8_matmul_workspace.argtypes = [i32, i32, i32]
     L.h2c_i8_matmul_workspace.restype = u64
     L.h2c_i8_matmul.argtypes = [i32, p, i64, p, p, i64, p, i32, i32, i32, i32, p, i64, p, p, u64, p]
+    L.h2c_kv8_prefix_attention_workspace.argtypes = [C.POINTER(Kv8PrefixArgs)]
+    L.h2c_kv8_prefix_attention_workspace.restype = u64
+    L.h2c_kv8_prefix_attention.argtypes = [C.POINTER(Kv8PrefixArgs), p]
     f32, f64 = C.c_float, C.c_double
     L.h2c_i8_norm.argtypes = [i32, p, i64, i32, p, i64, p, i64, p, f64, i32, i32, p, i64, p, p]
     L.h2c_i8_values.argtypes = [p, i64, p, i32, i32, i32, p, p]
@@ -135,7 +145,7 @@ def load(path: str = LIB_PATH) -> C.CDLL:
                  "h2c_destroy", "h2c_q4_pack", "h2c_q4_matvec", "h2c_q4_matvec_noalloc", "h2c_set_matmul_kernel",
                  "h2c_matmul_kernel", "h2c_tp_unique_id", "h2c_create_tp", "h2c_ops_check", "h2c_kv8_plan",
                  "h2c_kv8_append", "h2c_kv8_read", "h2c_kv8_attention", "h2c_i8_quantize", "h2c_i8_matmul",
-                 "h2c_i8_norm", "h2c_i8_values", "h2c_rope", "h2c_logits_adjust"):
+                 "h2c_i8_norm", "h2c_i8_values", "h2c_rope", "h2c_logits_adjust", "h2c_kv8_prefix_attention"):
         getattr(L, name).restype = C.c_int
     _lib = L
     return L

@@ -22,6 +22,13 @@ struct AttArgs {
   float scale_log2;       // scale * log2(e): scores are kept in powers of two
 };
 
+// The same for a pass of h2c_kv8_prefix_attention, whose kernels leave all they compute to a joining kernel: over the requests' own
+// positions, or (group_start) over the prefixes, where a "request" is a group of n_own requests and every row sees all positions.
+struct SharedArgs : AttArgs {
+  const int* group_start;
+  int n_own;
+};
+
 #ifdef __CUDACC__
 
 namespace {
@@ -44,9 +51,8 @@ __device__ __forceinline__ Span spans_of(int lo, int hi, int splits, int blocks,
 struct Request {
   int first, n_q, len;  // first row of q, queries, cached positions
 };
-__device__ __forceinline__ Request request_of(const AttArgs& a, int r, int* n_all) {  // n_all: the queries, max_q or not
+__device__ __forceinline__ Request request_of_rows(const AttArgs& a, int r, int s0, int s1, int* n_all) {
   Request R;
-  const int s0 = a.q_start[r], s1 = a.q_start[r + 1];
   *n_all = s1 - s0;
   R.first = max(s0, 0);
   R.n_q = max(0, min(max(0, min(s1, a.rows)) - R.first, a.max_q));  // (not negative: products with the group must not wrap around)
@@ -54,14 +60,29 @@ __device__ __forceinline__ Request request_of(const AttArgs& a, int r, int* n_al
   R.len = max(0, (int)min((long long)a.kv_len[r], room));
   return R;
 }
+__device__ __forceinline__ Request request_of(const AttArgs& a, int r, int* n_all) {  // n_all: the queries, max_q or not
+  return request_of_rows(a, r, a.q_start[r], a.q_start[r + 1], n_all);
+}
+__device__ __forceinline__ Request request_of(const SharedArgs& a, int r, int* n_all) {
+  if (!a.group_start) return request_of_rows(a, r, a.q_start[r], a.q_start[r + 1], n_all);
+  const int g0 = max(0, min(a.group_start[r], a.n_own)), g1 = max(g0, min(a.group_start[r + 1], a.n_own));
+  return request_of_rows(a, r, a.q_start[g0], a.q_start[g1], n_all);
+}
+
+// The position of a request's query, among the cached ones.
+__device__ __forceinline__ int position_of(const AttArgs&, const Request& R, int n_all, int query) { return R.len - n_all + query; }
+__device__ __forceinline__ int position_of(const SharedArgs& a, const Request& R, int n_all, int query) {
+  return a.group_start ? R.len - 1 : R.len - n_all + query;
+}
 
 // The first key that the query at position pos sees. (Before position 0 it sees none; with the largest windows the difference would
 // not fit there.)
 __device__ __forceinline__ int first_key_of(const AttArgs& a, int pos) { return a.window > 0 ? max(pos, 0) + 1 - a.window : 0; }
 
 // The keys that queries t0 .. t1 of a request may attend to: [lo, hi), hi <= lo when there are none.
-__device__ __forceinline__ void key_range(const AttArgs& a, const Request& R, int n_all, int t0, int t1, int* lo, int* hi) {
-  const int p0 = R.len - n_all + t0, p1 = R.len - n_all + t1;
+template <class A>
+__device__ __forceinline__ void key_range(const A& a, const Request& R, int n_all, int t0, int t1, int* lo, int* hi) {
+  const int p0 = position_of(a, R, n_all, t0), p1 = position_of(a, R, n_all, t1);
   *hi = min(p1 + 1, R.len);
   *lo = max(0, first_key_of(a, p0));
 }

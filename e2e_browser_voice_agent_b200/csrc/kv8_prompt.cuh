@@ -37,6 +37,20 @@
 namespace h2 {
 namespace {
 
+// Whether a kernel leaves its sums to a joining kernel in any case.
+template <class A>
+constexpr bool PARTS_ONLY = std::is_same<A, SharedArgs>::value;
+
+// A kernel that was launched to start while the one before it on the stream still runs (programmatic dependent launch), and uses nothing
+// of it, ends after it, so that what follows on the stream finds both done. (Such kernels start when all CTAs of the kernel before
+// have started, so none waits for a CTA that needs its place.)
+template <bool DO>
+struct EndAfterTheOthers {
+  __device__ __forceinline__ ~EndAfterTheOthers() {
+    if (DO) asm volatile("griddepcontrol.wait;" ::: "memory");
+  }
+};
+
 constexpr int PR_ROWS = 256, PR_KEYS = 64, PR_THREADS = 5 * 128, PR_INFO = 32;
 constexpr int PR_SLOTS = 192;  // places for spilled sums
 enum { PR_CONVERT = 21, PR_MMA = 22, PR_SOFTMAX = 23, PR_SLOT = 24 };
@@ -57,8 +71,9 @@ __host__ __device__ inline PromptShape prompt_shape(int tiles, int kv_heads, int
   return s;
 }
 
-struct PromptArgs {
-  AttArgs a;
+template <class A>
+struct PromptArgsOf {
+  A a;
   int min_rows;       // requests of fewer rows are k_att_rows'
   PromptShape shape;  // as the host knows it: exact, or a bound of the row tiles, which are one span each
   int key_tiles;      // bound of a history's 64-key tiles
@@ -68,15 +83,17 @@ struct PromptArgs {
   float* sums;        // (PromptCfg::SPILL) PR_SLOTS places of 256 rows' sums; nullptr where no row tile has more than FOLD tiles of keys
   int* err;
 };
+using PromptArgs = PromptArgsOf<AttArgs>;
 
 // The host knows a single request's row tiles. Those of several depend on how their queries are spread (one chunk of a prompt
 // beside many single tokens has few), and are counted here by whole warps, as is the longest history among them. Spans of 512
 // keys or more: shorter ones take from k_att_rows' CTAs what they gain (31 single tokens of 100-4,096 and a chunk of 256 on 4,096, 28
 // heads over 4 of 128: 115 us in one span, 74 in 5; with a chunk of 512 on 512 instead: 50 us, 65 in two spans of 256 keys, and
 // 55 with the count that finds none).
-__device__ __forceinline__ PromptShape shape_of_call(const PromptArgs& pa) {
+template <class A>
+__device__ __forceinline__ PromptShape shape_of_call(const PromptArgsOf<A>& pa) {
   if (!pa.units) return pa.shape;
-  const AttArgs& a = pa.a;
+  const A& a = pa.a;
   int n = 0, keys = 0;
 #pragma unroll 4
   for (int r = threadIdx.x & 31; r < a.n_req; r += 32) {
@@ -99,8 +116,9 @@ struct TileAt {
   int r, row0, n_all;  // n_all: the request's queries, max_q or not
   Request R;
 };
-__device__ __forceinline__ TileAt tile_at(const PromptArgs& pa, int idx) {
-  const AttArgs& a = pa.a;
+template <class A>
+__device__ __forceinline__ TileAt tile_at(const PromptArgsOf<A>& pa, int idx) {
+  const A& a = pa.a;
   const int lane = threadIdx.x & 31;
   TileAt t{-1, 0, 0, {0, 0, 0}};
   int before = 0;
@@ -538,8 +556,9 @@ __device__ __forceinline__ float tile_max(const float* s, const KeyInfo* in, int
   return mx;
 }
 
-template <class T, int HD>
-__global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs pa) {
+template <class T, int HD, class A>
+__global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgsOf<A> pa) {
+  const EndAfterTheOthers<PARTS_ONLY<A>> end;
   using C = PromptCfg<T, HD>;
   constexpr int STG = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -551,7 +570,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
   __shared__ float row_scale[PR_ROWS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_s, slot_s;
-  const AttArgs& a = pa.a;
+  const A& a = pa.a;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (k_att_rows or the joining kernel; both wait for this one's end)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PromptShape shape = shape_of_call(pa);
@@ -767,7 +786,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
     int hq;
     const int tok = token_of(a, rr, &hq);
     hq += head * a.group;
-    const int pos = R.len - n_all + tok, first_key = first_key_of(a, pos);
+    const int pos = position_of(a, R, n_all, tok), first_key = first_key_of(a, pos);
     bool ok = true;
     if (n_tiles > 0) {
       put_queries<T, HD>(a, (long long)(R.first + tok) * a.q_row + hq * a.q_head, n_rows, at.row0 + q * 128, 32 * w4,
@@ -884,7 +903,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgs p
       tc_fence_after();
     }
     if (ok) {
-      const bool whole = sp.used == 1;
+      const bool whole = !PARTS_ONLY<A> && sp.used == 1;
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
       const size_t unit = ((size_t)idx * a.kv_heads + head) * shape.splits + split;
       uint8_t* stage = sm + q * C::Q_AREA + trow * C::OUT_LD;

@@ -182,14 +182,8 @@ def read(kv: torch.Tensor, kv_scale: torch.Tensor, slot: torch.Tensor,
     return k, v
 
 
-def attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, block_table: torch.Tensor,
-              q_start: torch.Tensor, kv_len: torch.Tensor, max_q: int, max_kv: int, scale: Optional[float] = None,
-              window: int = 0, out: Optional[torch.Tensor] = None, return_lse: bool = False):
-    """Causal grouped-query attention of a ragged batch over the cache (h2c_kv8_attention). q is [rows, heads, head dim]
-    with any row and head stride; scale defaults to head_dim ** -0.5; window > 0 limits each query to that many positions.
-    max_q and max_kv bound the requests' query counts and lengths. Returns out ([rows, heads, head dim], q's type), or
-    (out, lse) with lse float32 [rows, heads]; rows that belong to no request keep what out held. out may be q itself, or
-    share no memory with the arguments."""
+def _attention_args(q, kv, kv_scale, block_table, q_start, kv_len, max_q, max_kv, scale, window, out, return_lse):
+    """(device, arguments without a workspace, out, lse)"""
     index, pkv, ps, n_pages, page, kvh, hd = _cache(kv, kv_scale)
     if q.dim() != 3:
         raise ValueError(f"q: [rows, heads, {hd}] is wanted, not {tuple(q.shape)}")
@@ -212,10 +206,46 @@ def attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, block_t
                               page, kvh, hd, heads, tq, _want("block_table", block_table, i32, index), block_table.shape[1], n,
                               _want("q_start", q_start, i32, index, (n + 1,)), _want("kv_len", kv_len, i32, index, (n,)), rows,
                               max_q, max_kv, window, hd ** -0.5 if scale is None else scale, None, 0)
+    return index, a, out, lse
+
+
+def attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, block_table: torch.Tensor,
+              q_start: torch.Tensor, kv_len: torch.Tensor, max_q: int, max_kv: int, scale: Optional[float] = None,
+              window: int = 0, out: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Causal grouped-query attention of a ragged batch over the cache (h2c_kv8_attention). q is [rows, heads, head dim]
+    with any row and head stride; scale defaults to head_dim ** -0.5; window > 0 limits each query to that many positions.
+    max_q and max_kv bound the requests' query counts and lengths. Returns out ([rows, heads, head dim], q's type), or
+    (out, lse) with lse float32 [rows, heads]; rows that belong to no request keep what out held. out may be q itself, or
+    share no memory with the arguments."""
+    index, a, out, lse = _attention_args(q, kv, kv_scale, block_table, q_start, kv_len, max_q, max_kv, scale, window, out, return_lse)
     L = _lib.load()
     need = L.h2c_kv8_attention_workspace(a)
     if need:
-        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        work = torch.empty(need, dtype=torch.uint8, device=kv.device)
         a.workspace, a.workspace_bytes = work.data_ptr(), need
     _call(index, L.h2c_kv8_attention, a)
+    return (out, lse) if return_lse else out
+
+
+def prefix_attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, prefix_table: torch.Tensor, prefix_len: torch.Tensor,
+                     group_start: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, max_q: int,
+                     max_kv: int, max_prefix: int, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                     return_lse: bool = False):
+    """attention of requests that share prefixes, whose keys are read once for all of them (h2c_kv8_prefix_attention). Requests
+    group_start[g] .. group_start[g + 1] - 1 (int32 [groups + 1]) also see the first prefix_len[g] (int32 [groups]) positions of the
+    pages prefix_table[g] (int32 [groups, columns]), which come before their own; block_table, kv_len and max_kv are of their own
+    positions alone. max_prefix bounds the prefixes' lengths. The rest is as in attention."""
+    index, own, out, lse = _attention_args(q, kv, kv_scale, block_table, q_start, kv_len, max_q, max_kv, scale, 0, out, return_lse)
+    i32, n = torch.int32, prefix_len.shape[0]
+    if prefix_table.dim() != 2 or prefix_table.shape[0] != n:
+        raise ValueError(f"prefix_table: [{n}, columns] is wanted, not {tuple(prefix_table.shape)}")
+    _int32("groups, columns, max_prefix", n, prefix_table.shape[1], max_prefix)
+    a = _lib.Kv8PrefixArgs(own, _want("prefix_table", prefix_table, i32, index), _want("prefix_len", prefix_len, i32, index, (n,)),
+                           _want("group_start", group_start, i32, index, (n + 1,)), prefix_table.shape[1], n, max_prefix)
+    L = _lib.load()
+    need = L.h2c_kv8_prefix_attention_workspace(a)
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=kv.device)
+        a.own.workspace, a.own.workspace_bytes = work.data_ptr(), need
+    _call(index, L.h2c_kv8_prefix_attention, a)
     return (out, lse) if return_lse else out

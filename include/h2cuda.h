@@ -358,6 +358,26 @@ typedef struct h2c_kv8_attention_args {
 uint64_t h2c_kv8_attention_workspace(const h2c_kv8_attention_args* args);
 int h2c_kv8_attention(const h2c_kv8_attention_args* args, void* stream);
 
+/* Attention of requests that share prefixes (a system prompt of many sessions): as h2c_kv8_attention, with the positions of a prefix
+ * before a request's own. Requests group_start[g] .. group_start[g + 1]-1 share prefix g, the first prefix_len[g] positions of the
+ * pages prefix_table[g] (which no request's own table needs to name: a prefix is held like a session of its own, and may end
+ * anywhere in a page); requests of no group have none. Request r's queries see all positions of its prefix and, causally, its own: query
+ * i of n its own positions 0 .. kv_len[r] - n + i. The softmax is over both, and a prefix's keys are read once for all of a group's
+ * rows of a kv head, or for every 256 of them. A query that sees nothing gives zeros and lse = -infinity.
+ * own.window must be 0. What is rounded where is as in h2c_kv8_attention, where a group's rows count as one prompt for the prefix; the
+ * parts are joined in float32. group_start is clamped to 0 .. own.n_req and should not decrease (a row in two groups has the first's
+ * prefix). The workspace is h2c_kv8_prefix_attention_workspace bytes. */
+typedef struct h2c_kv8_prefix_args {
+  h2c_kv8_attention_args own;
+  const int32_t* prefix_table; /* [n_groups][prefix_cols] */
+  const int32_t* prefix_len;   /* [n_groups] */
+  const int32_t* group_start;  /* [n_groups + 1] */
+  int32_t prefix_cols, n_groups;
+  int32_t max_prefix;          /* bounds the prefixes' lengths, for the division of the work */
+} h2c_kv8_prefix_args;
+uint64_t h2c_kv8_prefix_attention_workspace(const h2c_kv8_prefix_args* args);
+int h2c_kv8_prefix_attention(const h2c_kv8_prefix_args* args, void* stream);
+
 /* Matrix products in 8-bit integers, with a scale for each token and each output channel. */
 #define H2C_TYPE_I8 3         /* codes, where an entry says so */
 #define H2C_I8_MAX_K 131072   /* (sums of k products of two codes stay within 32 bits) */

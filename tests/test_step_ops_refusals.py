@@ -1,9 +1,11 @@
-"""The C entries of the norm, rotary positions and logits refuse arguments that do not fit with a status and a message, before anything
+"""The C entries of the norm, rotary positions, logits and attention behind shared prefixes refuse arguments that do not fit with a status and a message, before anything
 touches a device (so these run without one), and so do the Python calls."""
+import ctypes as C
+
 import pytest
 import torch
 
-from e2e_browser_voice_agent_b200 import _lib, build, int8, logits, rope
+from e2e_browser_voice_agent_b200 import _lib, build, int8, kv8, logits, rope
 
 
 @pytest.fixture(scope="module")
@@ -197,3 +199,60 @@ L, T, N, S = torch.zeros(3, 100), torch.zeros(3, 9, dtype=torch.int32), torch.ze
 def test_logits_calls_refuse(call, error, word):
     with pytest.raises(error, match=word):
         call()
+
+
+def prefix_args(**change):
+    a = dict(q=A[0], q_row=256, q_head=64, out=A[1], out_row=256, out_head=64, lse=A[2], kv=A[3], kv_scale=A[4], n_pages=8, page_size=16,
+             kv_heads=2, head_dim=64, heads=4, type=0, block_table=A[5], table_cols=4, n_req=2, q_start=A[6], kv_len=A[7], rows=3,
+             max_q=2, max_kv=60, window=0, scale=0.125, workspace=A[12], workspace_bytes=1 << 20)
+    p = dict(prefix_table=A[8], prefix_len=A[9], group_start=A[10], prefix_cols=4, n_groups=2, max_prefix=60)
+    assert set(change) <= {*a, *p}
+    own = _lib.Kv8AttentionArgs(**{k: change.get(k, v) for k, v in a.items()})
+    return _lib.Kv8PrefixArgs(own, **{k: change.get(k, v) for k, v in p.items()})
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(page_size=48), ("page_size",)), (dict(head_dim=32), ("head_dim",)), (dict(heads=5), ("multiple",)), (dict(n_req=9000), ("n_req",)),
+    (dict(max_kv=-1), ("negative",)), (dict(window=5), ("window",)), (dict(n_groups=-1), ("n_groups",)), (dict(n_groups=9000), ("n_groups",)),
+    (dict(prefix_cols=-1), ("negative",)), (dict(max_prefix=-1), ("negative",)), (dict(rows=2**31 - 70000), ("rows",)),
+    (dict(q=None), ("null",)), (dict(block_table=None), ("null",)), (dict(prefix_table=None), ("null",)), (dict(prefix_len=None), ("null",)),
+    (dict(group_start=None), ("null",)), (dict(kv=A[3] + 4), ("aligned",)), (dict(q=A[0] + 2), ("aligned",)),
+    (dict(prefix_table=A[8] + 2), ("prefix_table", "aligned")), (dict(prefix_len=A[9] + 1), ("prefix_len", "aligned")),
+    (dict(group_start=A[10] + 2), ("group_start", "aligned")), (dict(workspace=None), ("workspace",)), (dict(workspace=A[12] + 8), ("workspace",)),
+    (dict(workspace_bytes=100), ("workspace",)), (dict(out=A[0] + 4), ("out", "q itself")), (dict(out=A[0], out_row=320), ("out", "q itself")),
+    (dict(out_row=0), ("vectors of out overlap",)),
+    *[(dict(out=A[i]), ("out", n)) for i, n in ((3, "kv"), (4, "kv_scale"), (5, "block_table"), (6, "q_start"), (7, "kv_len"), (8, "prefix_table"),
+                                                (9, "prefix_len"), (10, "group_start"))],
+    *[(dict(lse=A[i]), ("lse", n)) for i, n in ((0, "q"), (1, "out"), (8, "prefix_table"), (9, "prefix_len"), (10, "group_start"))],
+    *[(dict(workspace=A[i]), ("workspace", n)) for i, n in ((0, "q"), (1, "out"), (5, "block_table"), (8, "prefix_table"), (10, "group_start"))],
+])
+def test_prefix_attention_refuses(lib, change, words):
+    refused(lib, lib.h2c_kv8_prefix_attention(C.byref(prefix_args(**change)), None), "h2c_kv8_prefix_attention", *words)
+
+
+def test_prefix_attention_of_nothing_and_its_workspace(lib):
+    assert lib.h2c_kv8_prefix_attention(None, None) == _lib.ERR_INVALID
+    refused(lib, lib.h2c_kv8_prefix_attention(C.byref(prefix_args(type=3)), None), "h2c_kv8_prefix_attention", code=_lib.ERR_BAD_TYPE)
+    for change in (dict(n_req=0), dict(rows=0), dict(max_q=0)):
+        assert lib.h2c_kv8_prefix_attention(C.byref(prefix_args(q=None, **change)), None) == _lib.OK
+        assert lib.h2c_kv8_prefix_attention_workspace(C.byref(prefix_args(**change))) == 0
+    need = lib.h2c_kv8_prefix_attention_workspace(C.byref(prefix_args()))
+    assert 0 < need < 1 << 20
+    assert lib.h2c_kv8_prefix_attention_workspace(C.byref(prefix_args(n_groups=0))) < need
+    refused(lib, lib.h2c_kv8_prefix_attention(C.byref(prefix_args(workspace_bytes=need - 1)), None), "h2c_kv8_prefix_attention", str(need))
+
+
+KV, KS, I = torch.zeros(8, 2, 2, 16, 64, dtype=torch.int8), torch.zeros(8, 2, 2), torch.zeros(9, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("change,error,word", [
+    ({}, ValueError, "CUDA"), (dict(ptable=I[:2]), ValueError, "prefix_table"), (dict(ptable=I.view(3, 3)), ValueError, "prefix_table"),
+    (dict(ptable=I[:8].view(2, 4).long()), TypeError, "prefix_table"), (dict(plen=I[:2].long()), TypeError, "prefix_len"),
+    (dict(gs=I[:2]), ValueError, "group_start"), (dict(q=Q.long()), TypeError, "q:"), (dict(max_prefix=2**31), ValueError, "32 bits"),
+    (dict(table=I[:2]), ValueError, "block_table"), (dict(out=Q[:2]), ValueError, "out"),
+])
+def test_prefix_attention_calls_refuse(change, error, word):
+    a = {**dict(q=Q, kv=KV, sc=KS, ptable=I[:8].view(2, 4), plen=I[:2], gs=I[:3], table=I[:8].view(2, 4), q_start=I[:3], kv_len=I[:2], max_q=2,
+                max_kv=60, max_prefix=60), **change}
+    with pytest.raises(error, match=word):
+        kv8.prefix_attention(*[v for k, v in a.items() if k != "out"], out=a.get("out"))
