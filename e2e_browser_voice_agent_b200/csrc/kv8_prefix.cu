@@ -26,15 +26,18 @@ struct Parts {
   int used;  // 0: the row is in no request (group)
 };
 
-// The parts of row t (of q) and head hq. By whole warps: 32 requests at a time, until the one that has the row; the row tiles of
-// k_att_prompt before it are counted on the way.
-template <int HD>
-__device__ __forceinline__ Parts parts_of(const Pass& p, int t, int hq) {
+// The request (group) that has row t of q, and the row tiles of k_att_prompt before its own. By all threads of the CTA, which test as
+// many requests at a time.
+struct Owner {
+  int r, n_all, before;  // r = -1: no request has it
+  Request R;
+};
+__device__ __forceinline__ void find_owner(const Pass& p, int t, Owner* owner, int* sums) {
   const SharedArgs& a = p.ra.a;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int before = 0;
-  for (int base = 0; base < a.n_req; base += 32) {
-    const int r = base + lane;
+  for (int base = 0;; base += 32 * JOIN_WARPS) {
+    const int r = base + threadIdx.x;
     int n = 0, n_all = 0;
     Request R{0, 0, 0};
     if (r < a.n_req) {
@@ -42,105 +45,148 @@ __device__ __forceinline__ Parts parts_of(const Pass& p, int t, int hq) {
       const int rows = R.n_q * a.group;
       if (p.prompt && rows >= p.pa.min_rows) n = (rows + PR_ROWS - 1) / PR_ROWS;
     }
-    const unsigned in = __ballot_sync(0xffffffffu, t >= R.first && t - R.first < R.n_q);
-    if (!in) {
-      before += __reduce_add_sync(0xffffffffu, n);
-      continue;
+    const bool in = t >= R.first && t - R.first < R.n_q;
+    int first = __reduce_min_sync(0xffffffffu, in ? r : INT_MAX);  // (of several, the first)
+    const int sum = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) sums[warp] = sum, sums[JOIN_WARPS + warp] = first;
+    __syncthreads();
+    int all = 0, mine = before;
+    first = INT_MAX;
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; w++) {
+      first = min(first, sums[JOIN_WARPS + w]);
+      if (w < warp) mine += sums[w];
+      all += sums[w];
     }
-    const int l = __ffs(in) - 1;
-    before += __reduce_add_sync(0xffffffffu, lane < l ? n : 0);
-    n_all = __shfl_sync(0xffffffffu, n_all, l);
-    R.first = __shfl_sync(0xffffffffu, R.first, l);
-    R.n_q = __shfl_sync(0xffffffffu, R.n_q, l);
-    R.len = __shfl_sync(0xffffffffu, R.len, l);
-    const int head = hq / a.group, row = (t - R.first) * a.group + (hq - head * a.group), n_rows = R.n_q * a.group;
-    int lo, hi;
-    if (p.prompt && n_rows >= p.pa.min_rows) {
-      const PromptShape shape = shape_of_call(p.pa);
-      const int idx = before + row / PR_ROWS, row0 = row / PR_ROWS * PR_ROWS;
-      if (idx >= shape.tiles) break;  // (starts of requests without sense: not computed)
-      key_range(a, R, n_all, row0 / a.group, min(row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-      const size_t u = ((size_t)idx * a.kv_heads + head) * shape.splits * PR_ROWS + (row - row0);
-      return {p.pa.part + u * HD, p.pa.ml + u, (size_t)PR_ROWS * HD, PR_ROWS, spans_of(lo, hi, shape.splits, shape.blocks, PR_KEYS).used};
+    if (first != INT_MAX) {
+      if (first >> 5 == r >> 5) {  // (its warp)
+        mine += __reduce_add_sync(0xffffffffu, r < first ? n : 0);
+        if (r == first) *owner = {r, n_all, mine, R};
+      }
+    } else if (base + 32 * JOIN_WARPS >= a.n_req) {
+      if (threadIdx.x == 0) owner->r = -1;
     }
-    const int tile = row / RW_ROWS, row0 = tile * RW_ROWS;
-    if (tile >= p.ra.tiles) break;
-    key_range(a, R, n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-    const size_t u = (((size_t)(base + l) * a.kv_heads + head) * p.ra.tiles + tile) * p.ra.splits * RW_ROWS + (row - row0);
-    return {p.ra.part + u * HD, p.ra.ml + u, (size_t)RW_ROWS * HD, RW_ROWS, spans_of(lo, hi, p.ra.splits, p.ra.blocks, RW_BLK).used};
+    __syncthreads();
+    if (first != INT_MAX || base + 32 * JOIN_WARPS >= a.n_req) return;
+    before += all;
   }
-  return {nullptr, nullptr, 0, 0, 0};
 }
 
-// NW warps (1 or JOIN_WARPS) a row and head: see JOIN_WARPS.
+// The parts of row t of q, which `o` has, and head hq. (idx, tile: beyond what was computed only with starts of requests without sense.)
+template <int HD>
+__device__ __forceinline__ Parts parts_of(const Pass& p, const PromptShape& shape, const Owner& o, int t, int hq) {
+  if (o.r < 0) return {nullptr, nullptr, 0, 0, 0};
+  const SharedArgs& a = p.ra.a;
+  const Request& R = o.R;
+  const int head = hq / a.group, row = (t - R.first) * a.group + (hq - head * a.group), n_rows = R.n_q * a.group;
+  int lo, hi;
+  if (p.prompt && n_rows >= p.pa.min_rows) {
+    const int idx = o.before + row / PR_ROWS, row0 = row / PR_ROWS * PR_ROWS;
+    if (idx >= shape.tiles) return {nullptr, nullptr, 0, 0, 0};
+    key_range(a, R, o.n_all, row0 / a.group, min(row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
+    const size_t u = ((size_t)idx * a.kv_heads + head) * shape.splits * PR_ROWS + (row - row0);
+    return {p.pa.part + u * HD, p.pa.ml + u, (size_t)PR_ROWS * HD, PR_ROWS, spans_of(lo, hi, shape.splits, shape.blocks, PR_KEYS).used};
+  }
+  const int tile = row / RW_ROWS, row0 = tile * RW_ROWS;
+  if (tile >= p.ra.tiles) return {nullptr, nullptr, 0, 0, 0};
+  key_range(a, R, o.n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
+  const size_t u = (((size_t)o.r * a.kv_heads + head) * p.ra.tiles + tile) * p.ra.splits * RW_ROWS + (row - row0);
+  return {p.ra.part + u * HD, p.ra.ml + u, (size_t)RW_ROWS * HD, RW_ROWS, spans_of(lo, hi, p.ra.splits, p.ra.blocks, RW_BLK).used};
+}
+
+// A CTA takes `heads` heads of one token, NW warps (1 or JOIN_WARPS, see there) a head. What it looks up needs nothing of the passes and
+// goes on while they end.
 template <class T, int HD, int NW>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) k_prefix_join(const Pass prefix, const Pass own) {
-  constexpr int V = HD / 32, UN = 4;
-  __shared__ float acc[NW][HD], acc_l[NW];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+__global__ void __launch_bounds__(32 * JOIN_WARPS) k_prefix_join(const Pass prefix, const Pass own, int heads) {
+  constexpr int V = HD / 32, UN = 6;
+  __shared__ float acc[NW][HD];
+  __shared__ float2 acc_ml[NW];
+  __shared__ Owner owner[2];
+  __shared__ int sums[2 * JOIN_WARPS];
   const AttArgs& a = own.ra.a;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = NW > 1 ? warp : 0;
-  const long long i = NW > 1 ? blockIdx.x : (long long)blockIdx.x * JOIN_WARPS + warp;
-  const int t = (int)(i / a.heads), hq = (int)(i - (long long)t * a.heads);
-  if (t >= a.rows) return;
-  const Parts o = parts_of<HD>(own, t, hq);
-  if (o.used == 0) return;  // (a row of no request is not touched)
-  const Parts p = parts_of<HD>(prefix, t, hq);
-  const int all = p.used + o.used;
-  auto ml_of = [&](int s) { return s < p.used ? p.ml[s * p.ml_step] : o.ml[(s - p.used) * o.ml_step]; };
-  float m = -INFINITY;
-  for (int s = lane; s < all; s += 32) m = fmaxf(m, ml_of(s).x);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = NW > 1 ? warp : 0, t = blockIdx.x;
+  const int h0 = blockIdx.y * heads, h1 = min(h0 + heads, a.heads);
+  find_owner(own, t, &owner[1], sums);
+  find_owner(prefix, t, &owner[0], sums);
+  const PromptShape own_shape = shape_of_call(own.pa), prefix_shape = shape_of_call(prefix.pa);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int hq = h0 + (NW > 1 ? 0 : warp); hq < h1; hq += NW > 1 ? 1 : JOIN_WARPS) {
+    const Parts o = parts_of<HD>(own, own_shape, owner[1], t, hq);
+    if (o.used == 0) return;  // (a row of no request is not touched)
+    const Parts p = parts_of<HD>(prefix, prefix_shape, owner[0], t, hq);
+    const int all = p.used + o.used;
+    // UN spans at a time, everything of them on its way at once; the sums are relative to the largest maximum so far
+    float m = -INFINITY, v[V], l = 0.f;
 #pragma unroll
-  for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-  float v[V], l = 0.f;
+    for (int k = 0; k < V; k++) v[k] = 0.f;
+    for (int s0 = w; s0 < all; s0 += UN * NW) {
+      float x[UN][V];
+      float2 ml[UN];
 #pragma unroll
-  for (int k = 0; k < V; k++) v[k] = 0.f;
-  for (int s0 = w; s0 < all; s0 += UN * NW) {
-    float x[UN][V];
-    float2 ml[UN];
+      for (int k = 0; k < UN; k++) {
+        const int s = s0 + k * NW;
+        ml[k] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-    for (int k = 0; k < UN; k++) {
-      const int s = s0 + k * NW;
-      if (s < all) {
-        const float* src = (s < p.used ? p.part + s * p.part_step : o.part + (s - p.used) * o.part_step) + V * lane;
-        ml[k] = ml_of(s);
-        if (V == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(src);
-        else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(src);
+        for (int j = 0; j < V; j++) x[k][j] = 0.f;
+        if (s < all) {
+          const bool shared = s < p.used;
+          const int i = shared ? s : s - p.used;
+          const float* src = (shared ? p.part + i * p.part_step : o.part + i * o.part_step) + V * lane;
+          ml[k] = shared ? p.ml[i * p.ml_step] : o.ml[i * o.ml_step];
+          if (V == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(src);
+          else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(src);
+        }
       }
-    }
+      float top = m;
 #pragma unroll
-    for (int k = 0; k < UN; k++)
-      if (s0 + k * NW < all) {
+      for (int k = 0; k < UN; k++) top = fmaxf(top, ml[k].x);
+      const float f_old = m == -INFINITY ? 0.f : exp2_fast(m - top);
+      m = top;
+      l *= f_old;
+#pragma unroll
+      for (int j = 0; j < V; j++) v[j] *= f_old;
+#pragma unroll
+      for (int k = 0; k < UN; k++) {
         const float f = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - m);
         l = fmaf(f, ml[k].y, l);
 #pragma unroll
         for (int j = 0; j < V; j++) v[j] = fmaf(f, x[k][j], v[j]);
       }
-  }
-  if (NW > 1) {
+    }
+    if (NW > 1) {
 #pragma unroll
-    for (int k = 0; k < V; k++) acc[w][V * lane + k] = v[k];
-    if (lane == 0) acc_l[w] = l;
-    __syncthreads();
-    if (w) return;
-    for (int n = 1; n < NW; n++) {
-      l += acc_l[n];
+      for (int k = 0; k < V; k++) acc[w][V * lane + k] = v[k];
+      if (lane == 0) acc_ml[w] = make_float2(m, l);
+      __syncthreads();
+      if (w == 0) {
+        for (int n = 1; n < NW; n++) m = fmaxf(m, acc_ml[n].x);
+        l = 0.f;
 #pragma unroll
-      for (int k = 0; k < V; k++) v[k] += acc[n][V * lane + k];
+        for (int k = 0; k < V; k++) v[k] = 0.f;
+        for (int n = 0; n < NW; n++) {
+          const float f = acc_ml[n].x == -INFINITY ? 0.f : exp2_fast(acc_ml[n].x - m);
+          l = fmaf(f, acc_ml[n].y, l);
+#pragma unroll
+          for (int k = 0; k < V; k++) v[k] = fmaf(f, acc[n][V * lane + k], v[k]);
+        }
+      }
+      __syncthreads();
+    }
+    if (w == 0) {
+      const float inv = l != 0.f ? 1.f / l : 1.f;
+      T* dst = static_cast<T*>(a.out) + (long long)t * a.out_row + hq * a.out_head + V * lane;
+#pragma unroll
+      for (int k = 0; k < V; k++) v[k] *= inv;
+      if (V == 4) {
+        store4(dst, v, a.out_vec);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; k++) dst[k] = from_f<T>(v[k]);
+      }
+      if (lane == 0 && a.lse)
+        a.lse[(size_t)t * a.heads + hq] = l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
     }
   }
-  const float inv = l != 0.f ? 1.f / l : 1.f;
-  T* dst = static_cast<T*>(a.out) + (long long)t * a.out_row + hq * a.out_head + V * lane;
-#pragma unroll
-  for (int k = 0; k < V; k++) v[k] *= inv;
-  if (V == 4) {
-    store4(dst, v, a.out_vec);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; k++) dst[k] = from_f<T>(v[k]);
-  }
-  if (lane == 0 && a.lse)
-    a.lse[(size_t)t * a.heads + hq] = l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
 }
 
 // ---------------------------------------------------------------- host
@@ -255,13 +301,15 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
     auto most = [&](const WorkPlan& p) {  // spans of a row
       return std::max(p.rows ? p.splits : 0, p.prompt ? p.counted ? 148 / g->own.kv_heads : p.shape.splits : 0);
     };
-    const long long rows = (long long)g->own.rows * g->own.heads;
-    const int spans = most(plan.own) + most(plan.prefix);
-    cfg.gridDim = dim3(join_ctas(rows, spans));
+    // eight warps a head where spans are many and rows few; else a warp a head, eight heads a CTA or, of many tokens, all
+    const long long all = (long long)g->own.rows * g->own.heads;
+    const bool many = most(plan.own) + most(plan.prefix) > JOIN_WARP_SPANS && all <= 148 * 8;
+    const int heads = many ? 1 : all <= 148 * 64 ? JOIN_WARPS : g->own.heads;
+    cfg.gridDim = dim3(g->own.rows, (g->own.heads + heads - 1) / heads);
     cfg.blockDim = dim3(32 * JOIN_WARPS);
     cfg.dynamicSmemBytes = 0;
-    c = spans <= JOIN_WARP_SPANS ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, 1>, pass[0], pass[1])
-                                 : cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, JOIN_WARPS>, pass[0], pass[1]);
+    c = many ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, JOIN_WARPS>, pass[0], pass[1], heads)
+             : cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, 1>, pass[0], pass[1], heads);
   }
   if (c == cudaSuccess) return H2C_OK;
   cudaGetLastError();
