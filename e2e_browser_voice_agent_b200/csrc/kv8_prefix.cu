@@ -22,98 +22,111 @@ struct Pass {
 struct Parts {
   const float* part;
   const float2* ml;
-  size_t part_step, ml_step;
+  unsigned part_step, ml_step;
   int used;  // 0: the row is in no request (group)
 };
 
-// The request (group) that has row t of q, and the row tiles of k_att_prompt before its own. By all threads of the CTA, which test as
-// many requests at a time.
-struct Owner {
-  int r, n_all, before;  // r = -1: no request has it
-  Request R;
+// Quotients of numbers below 2^31 by multiplication: the joining kernel would spend most of its instructions on divisions else.
+struct Divisor {
+  unsigned d, magic;
+  __device__ __forceinline__ explicit Divisor(int n) : d(n), magic(0xffffffffu / (unsigned)n) {}
+  __device__ __forceinline__ Divisor(int n, unsigned m) : d(n), magic(m) {}
+  __device__ __forceinline__ int quotient(int n) const {
+    const unsigned q = __umulhi((unsigned)n, magic);  // (one too few at most)
+    return (int)(q + ((unsigned)n - q * d >= d));
+  }
+  __device__ __forceinline__ int rounded_up(int n) const { return quotient(n + (int)d - 1); }
 };
-__device__ __forceinline__ void find_owner(const Pass& p, int t, Owner* owner, int* sums) {
+
+// The request (group) that has row t of q, and k_att_prompt's spans before its own, `blocks` tiles of keys each. By whole warps.
+struct Owner {
+  int r, n_all;      // r = -1: no request has it
+  long long before;
+  Request R;
+  int tiles, spans;  // its row tiles in k_att_prompt, if it takes them, the spans of each and the tiles of keys of a span
+  Divisor blocks;
+};
+__device__ __forceinline__ Owner owner_of(const Pass& p, int blocks, int t) {
   const SharedArgs& a = p.ra.a;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int before = 0;
-  for (int base = 0;; base += 32 * JOIN_WARPS) {
-    const int r = base + threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  Owner o{-1, 0, 0, {0, 0, 0}, 0, 1, Divisor(1)};
+  for (int base = 0; base < a.n_req; base += 32) {
+    const int r = base + lane;
     int n = 0, n_all = 0;
     Request R{0, 0, 0};
     if (r < a.n_req) {
       R = request_of(a, r, &n_all);
-      const int rows = R.n_q * a.group;
-      if (p.prompt && rows >= p.pa.min_rows) n = (rows + PR_ROWS - 1) / PR_ROWS;
+      if (p.prompt) n = units_of(p.pa, row_tiles_of(p.pa, R), spans_of_len(p.pa, R.len, blocks));
     }
-    const bool in = t >= R.first && t - R.first < R.n_q;
-    int first = __reduce_min_sync(0xffffffffu, in ? r : INT_MAX);  // (of several, the first)
-    const int sum = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) sums[warp] = sum, sums[JOIN_WARPS + warp] = first;
-    __syncthreads();
-    int all = 0, mine = before;
-    first = INT_MAX;
-#pragma unroll
-    for (int w = 0; w < JOIN_WARPS; w++) {
-      first = min(first, sums[JOIN_WARPS + w]);
-      if (w < warp) mine += sums[w];
-      all += sums[w];
-    }
-    if (first != INT_MAX) {
-      if (first >> 5 == r >> 5) {  // (its warp)
-        mine += __reduce_add_sync(0xffffffffu, r < first ? n : 0);
-        if (r == first) *owner = {r, n_all, mine, R};
+    const unsigned in = __ballot_sync(0xffffffffu, t >= R.first && t - R.first < R.n_q);
+    const int l = in ? __ffs(in) - 1 : 32;  // (of several, the first)
+    o.before += __reduce_add_sync(0xffffffffu, lane < l ? n : 0);
+    if (in) {
+      o.r = base + l;
+      o.n_all = __shfl_sync(0xffffffffu, n_all, l);
+      o.R.first = __shfl_sync(0xffffffffu, R.first, l);
+      o.R.n_q = __shfl_sync(0xffffffffu, R.n_q, l);
+      o.R.len = __shfl_sync(0xffffffffu, R.len, l);
+      if (p.prompt) {
+        o.tiles = row_tiles_of(p.pa, o.R);
+        o.spans = spans_of_len(p.pa, o.R.len, blocks);
+        o.blocks = Divisor(even_blocks(p.pa, o.R.len, o.spans));
       }
-    } else if (base + 32 * JOIN_WARPS >= a.n_req) {
-      if (threadIdx.x == 0) owner->r = -1;
+      break;
     }
-    __syncthreads();
-    if (first != INT_MAX || base + 32 * JOIN_WARPS >= a.n_req) return;
-    before += all;
   }
+  return o;
 }
 
-// The parts of row t of q, which `o` has, and head hq. (idx, tile: beyond what was computed only with starts of requests without sense.)
+// The parts of row t of q, which `o` has, and head h of kv head `head`'s group. row_blocks: blocks of k_att_rows' spans. (Beyond what was computed only with starts of requests without sense.)
 template <int HD>
-__device__ __forceinline__ Parts parts_of(const Pass& p, const PromptShape& shape, const Owner& o, int t, int hq) {
+__device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_blocks, const Owner& o, int t, int head, int h) {
   if (o.r < 0) return {nullptr, nullptr, 0, 0, 0};
   const SharedArgs& a = p.ra.a;
-  const Request& R = o.R;
-  const int head = hq / a.group, row = (t - R.first) * a.group + (hq - head * a.group), n_rows = R.n_q * a.group;
-  int lo, hi;
-  if (p.prompt && n_rows >= p.pa.min_rows) {
-    const int idx = o.before + row / PR_ROWS, row0 = row / PR_ROWS * PR_ROWS;
-    if (idx >= shape.tiles) return {nullptr, nullptr, 0, 0, 0};
-    key_range(a, R, o.n_all, row0 / a.group, min(row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-    const size_t u = ((size_t)idx * a.kv_heads + head) * shape.splits * PR_ROWS + (row - row0);
-    return {p.pa.part + u * HD, p.pa.ml + u, (size_t)PR_ROWS * HD, PR_ROWS, spans_of(lo, hi, shape.splits, shape.blocks, PR_KEYS).used};
+  const Divisor group(a.group, a.group_magic);
+  const int row = (t - o.R.first) * a.group + h;
+  // the keys before the end of what the tile's last row sees
+  auto end_of = [&](int last_row) { return min(position_of(a, o.R, o.n_all, group.quotient(min(last_row, o.R.n_q * a.group - 1))) + 1, o.R.len); };
+  if (o.tiles) {
+    const int tile = row / PR_ROWS, n_blocks = (max(0, end_of(tile * PR_ROWS + PR_ROWS - 1)) + PR_KEYS - 1) / PR_KEYS;
+    const long long unit = o.before + ((o.tiles - 1LL - tile) * a.kv_heads + head) * o.spans;
+    if (unit + o.spans > p.pa.cap) return {nullptr, nullptr, 0, 0, 0};
+    const size_t u = (size_t)unit * PR_ROWS + (row - tile * PR_ROWS);
+    return {p.pa.part + u * HD, p.pa.ml + u, PR_ROWS * HD, PR_ROWS, max(1, min(o.spans, o.blocks.rounded_up(n_blocks)))};
   }
-  const int tile = row / RW_ROWS, row0 = tile * RW_ROWS;
+  const int tile = row / RW_ROWS, n_blocks = (max(0, end_of(tile * RW_ROWS + RW_ROWS - 1)) + RW_BLK - 1) / RW_BLK;
   if (tile >= p.ra.tiles) return {nullptr, nullptr, 0, 0, 0};
-  key_range(a, R, o.n_all, row0 / a.group, min(row0 + RW_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-  const size_t u = (((size_t)o.r * a.kv_heads + head) * p.ra.tiles + tile) * p.ra.splits * RW_ROWS + (row - row0);
-  return {p.ra.part + u * HD, p.ra.ml + u, (size_t)RW_ROWS * HD, RW_ROWS, spans_of(lo, hi, p.ra.splits, p.ra.blocks, RW_BLK).used};
+  const size_t u = (((size_t)o.r * a.kv_heads + head) * p.ra.tiles + tile) * p.ra.splits * RW_ROWS + (row - tile * RW_ROWS);
+  return {p.ra.part + u * HD, p.ra.ml + u, RW_ROWS * HD, RW_ROWS, max(1, min(p.ra.splits, row_blocks.rounded_up(n_blocks)))};
 }
 
-// A CTA takes `heads` heads of one token, NW warps (1 or JOIN_WARPS, see there) a head. What it looks up needs nothing of the passes and
-// goes on while they end.
+// A CTA takes `heads` heads of `tokens` (at most JOIN_TOKENS) rows of q, NW warps (1, or JOIN_WARPS for one row) a head. What it looks up
+// needs nothing of the passes and goes on while they end; the host makes no more CTAs than the SMs hold where it can.
+constexpr int JOIN_TOKENS = JOIN_WARPS / 2, JOIN_CTAS = 148 * 3;
 template <class T, int HD, int NW>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) k_prefix_join(const Pass prefix, const Pass own, int heads) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS, 3) k_prefix_join(const Pass prefix, const Pass own, int tokens, int heads) {
   constexpr int V = HD / 32, UN = 6;
   __shared__ float acc[NW][HD];
   __shared__ float2 acc_ml[NW];
-  __shared__ Owner owner[2];
-  __shared__ int sums[2 * JOIN_WARPS];
+  __shared__ __align__(16) uint8_t owner_s[JOIN_TOKENS * 2 * sizeof(Owner)];
+  Owner(*owner)[2] = reinterpret_cast<Owner(*)[2]>(owner_s);
   const AttArgs& a = own.ra.a;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = NW > 1 ? warp : 0, t = blockIdx.x;
-  const int h0 = blockIdx.y * heads, h1 = min(h0 + heads, a.heads);
-  find_owner(own, t, &owner[1], sums);
-  find_owner(prefix, t, &owner[0], sums);
-  const PromptShape own_shape = shape_of_call(own.pa), prefix_shape = shape_of_call(prefix.pa);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = NW > 1 ? warp : 0, t0 = blockIdx.x * tokens;
+  const int h0 = blockIdx.y * heads, nh = min(heads, a.heads - h0), n = min(tokens, a.rows - t0) * nh;
+  if (warp < 2 * tokens) {  // two warps a token: its prefix's group, its request
+    const Pass& p = warp & 1 ? own : prefix;
+    const int blocks = p.prompt ? blocks_of_call(p.pa) : 1;
+    const Owner o = owner_of(p, blocks, t0 + (warp >> 1));
+    if (lane == 0) owner[warp >> 1][warp & 1] = o;
+  }
+  __syncthreads();
+  const Divisor by_heads(nh), by_group(a.group, a.group_magic), prefix_row_blocks(max(1, prefix.ra.blocks)), own_row_blocks(max(1, own.ra.blocks));
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int hq = h0 + (NW > 1 ? 0 : warp); hq < h1; hq += NW > 1 ? 1 : JOIN_WARPS) {
-    const Parts o = parts_of<HD>(own, own_shape, owner[1], t, hq);
-    if (o.used == 0) return;  // (a row of no request is not touched)
-    const Parts p = parts_of<HD>(prefix, prefix_shape, owner[0], t, hq);
+  for (int i = NW > 1 ? 0 : warp; i < n; i += NW > 1 ? 1 : JOIN_WARPS) {
+    const int k_t = by_heads.quotient(i), t = t0 + k_t, hq = h0 + i - k_t * nh, head = by_group.quotient(hq), h = hq - head * a.group;
+    const Parts o = parts_of<HD>(own, own_row_blocks, owner[k_t][1], t, head, h);
+    if (o.used == 0) continue;  // (a row of no request is not touched)
+    const Parts p = parts_of<HD>(prefix, prefix_row_blocks, owner[k_t][0], t, head, h);
     const int all = p.used + o.used;
     // UN spans at a time, everything of them on its way at once; the sums are relative to the largest maximum so far
     float m = -INFINITY, v[V], l = 0.f;
@@ -130,9 +143,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) k_prefix_join(const Pass pref
         for (int j = 0; j < V; j++) x[k][j] = 0.f;
         if (s < all) {
           const bool shared = s < p.used;
-          const int i = shared ? s : s - p.used;
-          const float* src = (shared ? p.part + i * p.part_step : o.part + i * o.part_step) + V * lane;
-          ml[k] = shared ? p.ml[i * p.ml_step] : o.ml[i * o.ml_step];
+          const unsigned n = shared ? s : s - p.used;
+          const float* src = (shared ? p.part : o.part) + (size_t)n * (shared ? p.part_step : o.part_step) + V * lane;
+          ml[k] = (shared ? p.ml : o.ml)[(size_t)n * (shared ? p.ml_step : o.ml_step)];
           if (V == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(src);
           else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(src);
         }
@@ -221,7 +234,11 @@ PrefixPlan plan_prefix(const h2c_kv8_prefix_args* g) {
   p.bytes = p.own.bytes + p.prefix.bytes - (p.own.spill && p.prefix.spill ? sums : 0);
   return p;
 }
-long long tiles_of(const WorkPlan& p) { return std::max((long long)p.splits * p.tiles * RW_ROWS, (long long)p.shape.tiles * PR_ROWS * std::max(1, p.shape.splits)); }
+// Whether a pass's counts fit their types: rows of the workspace, axes of the grids.
+bool fits(const WorkPlan& p, long long kv_heads) {
+  return (long long)p.splits * p.tiles * RW_ROWS * kv_heads <= INT_MAX && p.splits <= 65535 &&
+         spans_at_most((long long)p.shape.tiles * kv_heads, p.p_keys) * PR_ROWS <= INT_MAX;
+}
 
 template <class T, int HD>
 int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g, cudaStream_t st) {
@@ -254,7 +271,7 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
     pass[i].rows = p.rows;
     pass[i].prompt = p.prompt;
     pass[i].ra = {a, p.splits, p.blocks, p.tiles, p.max_rows, 0, part, nullptr};
-    pass[i].pa = {a, p.min_rows, p.shape, p.p_keys, p.counted ? 148 : 0, p_part, nullptr, p.spill ? sums : nullptr, err};
+    pass[i].pa = {a, p.min_rows, p.shape, p.p_keys, p.counted, p_part, nullptr, p.spill ? sums : nullptr, err, p.p_units};
   }
   for (int i = 0; i < 2; i++) {
     const WorkPlan& p = i ? plan.own : plan.prefix;
@@ -282,7 +299,7 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
   for (int i = 0; i < 2 && c == cudaSuccess; i++) {
     const WorkPlan& p = i ? plan.own : plan.prefix;
     if (!p.prompt) continue;
-    cfg.gridDim = dim3((unsigned)std::max(p.shape.tiles * g->own.kv_heads * p.shape.splits, p.counted ? 148 : 0));
+    cfg.gridDim = dim3(p.p_units);
     cfg.blockDim = dim3(PR_THREADS);
     cfg.dynamicSmemBytes = p_smem;
     c = cudaLaunchKernelEx(&cfg, k_att_prompt<T, HD, SharedArgs>, pass[i].pa);
@@ -291,7 +308,7 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
   for (int i = 0; i < 2 && c == cudaSuccess; i++) {
     const WorkPlan& p = i ? plan.own : plan.prefix;
     if (!p.rows) continue;
-    cfg.gridDim = dim3((unsigned)p.splits * g->own.kv_heads * p.tiles, pass[i].ra.a.n_req);
+    cfg.gridDim = dim3((g->own.kv_heads * p.tiles + RW_WARPS - 1) / RW_WARPS, pass[i].ra.a.n_req, p.splits);
     cfg.blockDim = dim3(RW_WARPS * 32);
     cfg.dynamicSmemBytes = r_smem;
     c = cudaLaunchKernelEx(&cfg, k_att_rows<T, HD, SharedArgs>, pass[i].ra);
@@ -299,17 +316,19 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
   }
   if (c == cudaSuccess) {
     auto most = [&](const WorkPlan& p) {  // spans of a row
-      return std::max(p.rows ? p.splits : 0, p.prompt ? p.counted ? 148 / g->own.kv_heads : p.shape.splits : 0);
+      return std::max(p.rows ? p.splits : 0, p.prompt ? p.p_units / (p.shape.tiles * g->own.kv_heads) : 0);
     };
-    // eight warps a head where spans are many and rows few; else a warp a head, eight heads a CTA or, of many tokens, all
+    // eight warps a head where spans are many and rows few; else a warp a head, and no more CTAs than the SMs hold at a time
     const long long all = (long long)g->own.rows * g->own.heads;
     const bool many = most(plan.own) + most(plan.prefix) > JOIN_WARP_SPANS && all <= 148 * 8;
-    const int heads = many ? 1 : all <= 148 * 64 ? JOIN_WARPS : g->own.heads;
-    cfg.gridDim = dim3(g->own.rows, (g->own.heads + heads - 1) / heads);
+    const int heads = many ? 1 : all <= JOIN_CTAS * JOIN_WARPS * JOIN_TOKENS ? std::min(JOIN_WARPS, g->own.heads) : g->own.heads;
+    const long long ctas = (long long)g->own.rows * ((g->own.heads + heads - 1) / heads);
+    const int tokens = many ? 1 : (int)std::min<long long>(JOIN_TOKENS, (ctas + JOIN_CTAS - 1) / JOIN_CTAS);
+    cfg.gridDim = dim3((g->own.rows + tokens - 1) / tokens, (g->own.heads + heads - 1) / heads);
     cfg.blockDim = dim3(32 * JOIN_WARPS);
     cfg.dynamicSmemBytes = 0;
-    c = many ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, JOIN_WARPS>, pass[0], pass[1], heads)
-             : cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, 1>, pass[0], pass[1], heads);
+    c = many ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, JOIN_WARPS>, pass[0], pass[1], tokens, heads)
+             : cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, 1>, pass[0], pass[1], tokens, heads);
   }
   if (c == cudaSuccess) return H2C_OK;
   cudaGetLastError();
@@ -366,7 +385,7 @@ int h2c_kv8_prefix_attention(const h2c_kv8_prefix_args* g, void* stream) {
                         {"kv_len", o->kv_len, n4, 4},                          {"prefix_table", g->prefix_table, g4 * g->prefix_cols, 4},
                         {"prefix_len", g->prefix_len, g4, 4},                  {"group_start", g->group_start, g4 ? g4 + 4 : 0, 4}};
   if (int rc = check_memory(who, o, in, 6, p.bytes)) return rc;
-  if (std::max(tiles_of(p.own), p.shared ? tiles_of(p.prefix) : 0LL) * o->kv_heads > INT_MAX || (long long)o->rows * o->heads > INT_MAX)
+  if (!fits(p.own, o->kv_heads) || !fits(p.prefix, o->kv_heads) || (long long)o->rows * o->heads > INT_MAX)
     return op_error(H2C_ERR_INVALID, "%s: too many rows for one call", who);
   cudaStream_t st = (cudaStream_t)stream;
   if (o->type == H2C_TYPE_F32) return launch_typed<float>(who, p, g, st);

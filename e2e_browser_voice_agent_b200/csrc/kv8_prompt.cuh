@@ -82,6 +82,7 @@ struct PromptArgsOf {
   float2* ml;
   float* sums;        // (PromptCfg::SPILL) PR_SLOTS places of 256 rows' sums; nullptr where no row tile has more than FOLD tiles of keys
   int* err;
+  int cap;            // (SharedArgs) CTAs, and spans that the workspace has room for
 };
 using PromptArgs = PromptArgsOf<AttArgs>;
 
@@ -152,6 +153,121 @@ __device__ __forceinline__ TileAt tile_at(const PromptArgsOf<A>& pa, int idx) {
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
   return t;
+}
+
+// What a CTA does: span `split` of the at most `splits` spans of `blocks` tiles of keys that the row tile `at` of a kv head is cut into
+// (r = -1: nothing), and the number of that span in the workspace.
+struct Work {
+  TileAt at;
+  int head, split, splits, blocks;
+  size_t unit;
+};
+__device__ __forceinline__ Work work_of(const PromptArgsOf<AttArgs>& pa) {
+  const AttArgs& a = pa.a;
+  Work w{};
+  w.at.r = -1;
+  const PromptShape shape = shape_of_call(pa);
+  w.split = (int)blockIdx.x % shape.splits, w.head = ((int)blockIdx.x / shape.splits) % a.kv_heads;
+  w.splits = shape.splits, w.blocks = shape.blocks;
+  // the last tiles of a causal prompt have the most keys and go first
+  const int idx = shape.tiles - 1 - (int)blockIdx.x / (shape.splits * a.kv_heads);
+  if (idx < 0) return w;
+  w.at = tile_at(pa, idx);
+  w.unit = ((size_t)idx * a.kv_heads + w.head) * shape.splits + w.split;
+  return w;
+}
+
+// Requests of different lengths whose spans a joining kernel adds up in any case (SharedArgs): every row tile is cut into spans of
+// `blocks` tiles of keys, as many as its request's length needs. With u tiles of keys an SM in all, spans of B cost about
+// u + u / B c + B / 2, where c = SPAN_COST tiles is what a span's start and end take and B / 2 what the last ones leave idle: least at
+// B = sqrt(2 u c). (One request: what fills the SMs once, known to the host.) Row tiles for SPAN_TILES CTAs and more are not cut.
+constexpr int SPAN_COST = 5, SPAN_LEAST = 8, SPAN_TILES = 148 * 4;
+__host__ __device__ inline long long spans_at_most(long long ctas, long long key_tiles) {  // of `ctas` uncut row tiles
+  const double cut = (double)(ctas < SPAN_TILES ? ctas : SPAN_TILES) * (double)key_tiles;
+  return ctas + (long long)sqrt(cut * 148 / (2 * SPAN_COST)) + 2;
+}
+// A request's row tiles, and the spans that each is cut into.
+__device__ __forceinline__ int row_tiles_of(const PromptArgsOf<SharedArgs>& pa, const Request& R) {
+  const int rows = R.n_q * pa.a.group;
+  return rows >= pa.min_rows ? (rows + PR_ROWS - 1) / PR_ROWS : 0;
+}
+__device__ __forceinline__ int spans_of_len(const PromptArgsOf<SharedArgs>& pa, int len, int blocks) {
+  return max(1, (min((len + PR_KEYS - 1) / PR_KEYS, pa.key_tiles) + blocks - 1) / blocks);
+}
+// ... and their tiles of keys, as even as they can be.
+__device__ __forceinline__ int even_blocks(const PromptArgsOf<SharedArgs>& pa, int len, int spans) {
+  return max(1, (min((len + PR_KEYS - 1) / PR_KEYS, pa.key_tiles) + spans - 1) / spans);
+}
+// All its spans, of all kv heads; starts of requests without sense can make more than there is room for, which counts as one too many.
+__device__ __forceinline__ int units_of(const PromptArgsOf<SharedArgs>& pa, int tiles, int spans) {
+  return (int)min((long long)tiles * pa.a.kv_heads * spans, pa.cap + 1LL);
+}
+// Tiles of keys a span. By whole warps.
+__device__ __forceinline__ int blocks_of_call(const PromptArgsOf<SharedArgs>& pa) {
+  if (!pa.units) return pa.shape.blocks;
+  const SharedArgs& a = pa.a;
+  int n = 0;
+  float all = 0.f;
+#pragma unroll 4
+  for (int r = threadIdx.x & 31; r < a.n_req; r += 32) {
+    int n_all;
+    const Request R = request_of(a, r, &n_all);
+    const int tiles = row_tiles_of(pa, R);
+    n += tiles;
+    all += (float)tiles * (float)min((R.len + PR_KEYS - 1) / PR_KEYS, pa.key_tiles);
+  }
+  n = __reduce_add_sync(0xffffffffu, n);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  if ((long long)n * a.kv_heads >= SPAN_TILES) return max(1, pa.key_tiles);
+  // (rounded up, so that there are no more spans than spans_at_most has)
+  return max(SPAN_LEAST, (int)ceilf(1.001f * sqrtf(all * a.kv_heads * (2.f * SPAN_COST / 148.f))));
+}
+__device__ __forceinline__ Work work_of(const PromptArgsOf<SharedArgs>& pa) {
+  const SharedArgs& a = pa.a;
+  const int lane = threadIdx.x & 31, unit = blockIdx.x;
+  Work w{};
+  w.at.r = -1;
+  const int blocks = blocks_of_call(pa);
+  w.unit = unit;
+  int before = 0;
+  for (int base = 0; base < a.n_req; base += 32) {
+    const int r = base + lane;
+    int n = 0, n_all = 0, spans = 1, tiles = 0;
+    Request R{0, 0, 0};
+    if (r < a.n_req) {
+      R = request_of(a, r, &n_all);
+      tiles = row_tiles_of(pa, R);
+      spans = spans_of_len(pa, R.len, blocks);
+      n = units_of(pa, tiles, spans);
+    }
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += u;
+    }
+    const int at = unit - before;  // among these requests' spans
+    const unsigned in = __ballot_sync(0xffffffffu, at >= sum - n && at < sum);
+    if (in) {
+      const int l = __ffs(in) - 1, i = at - __shfl_sync(0xffffffffu, sum - n, l);
+      w.splits = __shfl_sync(0xffffffffu, spans, l);
+      tiles = __shfl_sync(0xffffffffu, tiles, l);
+      w.at.r = base + l;
+      w.at.n_all = __shfl_sync(0xffffffffu, n_all, l);
+      w.at.R.first = __shfl_sync(0xffffffffu, R.first, l);
+      w.at.R.n_q = __shfl_sync(0xffffffffu, R.n_q, l);
+      w.at.R.len = __shfl_sync(0xffffffffu, R.len, l);
+      w.blocks = even_blocks(pa, w.at.R.len, w.splits);
+      const int th = i / w.splits;
+      w.split = i - th * w.splits;
+      w.head = th % a.kv_heads;
+      w.at.row0 = (tiles - 1 - th / a.kv_heads) * PR_ROWS;  // (the last tiles of a causal prompt first)
+      return w;
+    }
+    before = min(before + __shfl_sync(0xffffffffu, sum, 31), pa.cap + 1);  // (32 of them fit)
+  }
+  return w;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -573,20 +689,28 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgsOf
   const A& a = pa.a;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (k_att_rows or the joining kernel; both wait for this one's end)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const PromptShape shape = shape_of_call(pa);
-  const int split = (int)blockIdx.x % shape.splits, head = ((int)blockIdx.x / shape.splits) % a.kv_heads;
-  // the last tiles of a causal prompt have the most keys and go first
-  const int idx = shape.tiles - 1 - (int)blockIdx.x / (shape.splits * a.kv_heads);
-  if (idx < 0) return;
-  const TileAt at = tile_at(pa, idx);
+  Work wk;
+  if constexpr (PARTS_ONLY<A>) {  // by one warp for all: its search is longer
+    __shared__ Work found;
+    if (warp == 0) {
+      wk = work_of(pa);
+      if (lane == 0) found = wk;
+    }
+    __syncthreads();
+    wk = found;
+  } else {
+    wk = work_of(pa);
+  }
+  const TileAt& at = wk.at;
   if (at.r < 0) return;
+  const int head = wk.head;
   const Request R = at.R;
   const int n_all = at.n_all, n_rows = R.n_q * a.group;
   int lo, hi;
   key_range(a, R, n_all, at.row0 / a.group, min(at.row0 + PR_ROWS - 1, n_rows - 1) / a.group, &lo, &hi);
-  const Span sp = spans_of(lo, hi, shape.splits, shape.blocks, PR_KEYS);
-  if (split >= sp.used) return;
-  const int t_begin = split * shape.blocks, t_end = split == sp.used - 1 ? sp.n_blocks : t_begin + shape.blocks;
+  const Span sp = spans_of(lo, hi, wk.splits, wk.blocks, PR_KEYS);
+  if (wk.split >= sp.used) return;
+  const int t_begin = wk.split * wk.blocks, t_end = wk.split == sp.used - 1 ? sp.n_blocks : t_begin + wk.blocks;
   const int n_tiles = t_end - t_begin, key_begin = sp.first + t_begin * PR_KEYS;
   const int n_q_tiles = n_rows - at.row0 > 128 ? 2 : 1;
 
@@ -905,7 +1029,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgsOf
     if (ok) {
       const bool whole = !PARTS_ONLY<A> && sp.used == 1;
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
-      const size_t unit = ((size_t)idx * a.kv_heads + head) * shape.splits + split;
+      const size_t unit = wk.unit;
       uint8_t* stage = sm + q * C::Q_AREA + trow * C::OUT_LD;
       const bool folded = n_tiles > fold;
       const uint32_t sum_at = folded && !C::SPILL ? to + HD : 0;

@@ -87,7 +87,12 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
   const A& a = ra.a;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the joining kernel, which waits for this one's end)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int split = blockIdx.x % ra.splits, th = blockIdx.x / ra.splits, head = th % a.kv_heads, tile = th / a.kv_heads;
+  // Where parts are left to a joining kernel in any case, a warp takes a span for itself: no warp waits for another, and four times as
+  // many spans are on their way (256 single tokens of 16-2,000 keys, 28 heads over 4 of 128). Spans are the grid's slowest axis and the
+  // last go first: only long requests have them, and the CTAs without one are over before the work begins.
+  constexpr bool ALONE = PARTS_ONLY<A>;
+  const int split = ALONE ? ra.splits - 1 - blockIdx.z : blockIdx.x % ra.splits, th = ALONE ? blockIdx.x * RW_WARPS + warp : blockIdx.x / ra.splits;
+  const int head = th % a.kv_heads, tile = th / a.kv_heads;
   const int r = blockIdx.y;
   int n_all;
   const Request R = request_of(a, r, &n_all);
@@ -155,8 +160,10 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
   for (int t = 0; t < NT; t++) o[t] = 0;
   float m_run = -INFINITY, l_run = 0.f;
 
-  // ---- the warp's blocks: b_begin + warp + 4 it
-  const int n_it = max(0, (b_end - b_begin - warp + RW_WARPS - 1) / RW_WARPS);
+  // ---- the warp's blocks: b_first + B_STEP it
+  const int b_first = b_begin + (ALONE ? 0 : warp);
+  constexpr int B_STEP = ALONE ? 1 : RW_WARPS;
+  const int n_it = max(0, (b_end - b_first + B_STEP - 1) / B_STEP);
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * RW_STAGES * S::STAGE;
   KeyInfo* info = reinterpret_cast<KeyInfo*>(sm + S::BYTES - S::SCALES) + warp * 64;
   const int P = 1 << a.page_log;
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
   auto issue = [&](int it) {
     if (it < n_it) {
       if ((it & 31) == 0) {  // places and scales of the next 32 blocks, one per lane
-        const int b = b_begin + warp + RW_WARPS * (it + lane);
+        const int b = b_first + B_STEP * (it + lane);
         if (b < b_end) {
           const int key = sp.first + b * RW_BLK;
           int pg = a.table[(size_t)r * a.table_cols + (key >> a.page_log)];
@@ -207,7 +214,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
     const uint8_t* kst = sm + warp * RW_STAGES * S::STAGE + stage * S::STAGE + lane * 16;
     const uint8_t* vst = sm + warp * RW_STAGES * S::STAGE + stage * S::STAGE + RW_BLK * HD + lane * VB;
     const KeyInfo ki = info[it & 63];
-    const int blk0 = sp.first + (b_begin + warp + RW_WARPS * it) * RW_BLK, key0 = blk0 + 2 * c;
+    const int blk0 = sp.first + (b_first + B_STEP * it) * RW_BLK, key0 = blk0 + 2 * c;
     // scores of 8 rows x 16 keys: this lane has keys key0, key0 + 1 (tile 0), key0 + 8, key0 + 9 (tile 1) of its row
     float y[4];
     const float f = q_scale * ki.k;
@@ -292,6 +299,23 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
   l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
   l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
 
+  const size_t unit = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits + split;
+  if constexpr (ALONE) {
+    if (!live) return;
+    if (c == 0) ra.ml[unit * RW_ROWS + g] = make_float2(m_run, l_run);
+    float* dst = ra.part + (unit * RW_ROWS + g) * HD;
+#pragma unroll
+    for (int t = 0; t < NT; t += 4) {
+      float v[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; i++) unpair(o[t + i], &v[i][0], &v[i][1]);
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        *reinterpret_cast<float4*>(dst + VB * (2 * c + i) + t) = make_float4(v[0][i], v[1][i], v[2][i], v[3][i]);
+    }
+    return;
+  }
+
   // ---- join the warps: [warp][8][HD] sums, [warp][8] maxima, [warp][8] sums of weights
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
@@ -324,8 +348,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
     fw[w] = mw == -INFINITY ? 0.f : exp2_fast(mw - mm);
     ll += fw[w] * jl[w * RW_ROWS + jr];
   }
-  const size_t unit = (((size_t)r * a.kv_heads + head) * ra.tiles + tile) * ra.splits + split;
-  const bool whole = !PARTS_ONLY<A> && sp.used == 1 && !ra.cluster;
+  const bool whole = sp.used == 1 && !ra.cluster;
   const float inv = whole && ll != 0.f ? 1.f / ll : 1.f;
   int oh;
   const int otok = token_of(a, orow, &oh);
@@ -359,7 +382,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
       a.lse[(size_t)(R.first + otok) * a.heads + oh] =
           ll == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(ll) + mm - P_SHIFT);
   }
-  if (PARTS_ONLY<A> || !ra.cluster) return;
+  if (!ra.cluster) return;
   __syncwarp();
 
   // ---- the cluster's spans, each CTA a share of the rows' pieces of four dimensions, through distributed shared memory
@@ -465,12 +488,15 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
     // 60,000-131,072 175, 176 and 164; 32 of 4,000-16,000 89, 81 and 75). Up to 8 are one cluster, whose join costs little: spans of 128 keys (2
     // blocks per warp) or more. More of them, for few rows over long histories, leave their parts in the workspace for a
     // second kernel: spans of 256 keys or more, below which a span's start-up costs more than it shares out
-    const long long groups = (long long)g->n_req * g->kv_heads * p.tiles, want = (888 + groups - 1) / groups;
+    // (a warp's spans, where they are joined in any case: four waves of 12 warps an SM, of 128 keys or more, or of 64 where those are few)
+    const long long groups = (long long)g->n_req * g->kv_heads * p.tiles, want = ((parts ? 7104 : 888) + groups - 1) / groups;
     const int n_blocks = (int)((keys + RW_BLK - 1) / RW_BLK) + (g->window > 0 ? 1 : 0);
     p.cluster = !parts && groups * RW_CLUSTER <= 444 && n_blocks / 16 <= RW_CLUSTER;
+    const int least = !parts ? 16 : groups * (n_blocks / 4) <= 888 && n_blocks <= 256 ? 4 : 8;
     p.splits = (int)std::max(1LL, p.cluster ? std::min<long long>({(long long)RW_CLUSTER, want, (n_blocks + 7LL) / 8})
-                                            : std::min<long long>(want, n_blocks / 16));
-    p.blocks = std::max(RW_WARPS, ((n_blocks + p.splits - 1) / p.splits + RW_WARPS - 1) / RW_WARPS * RW_WARPS);
+                                            : std::min<long long>(want, n_blocks / least));
+    const int step = parts ? 1 : RW_WARPS;  // blocks of a span: a multiple of the warps that share it
+    p.blocks = std::max(step, ((n_blocks + p.splits - 1) / p.splits + step - 1) / step * step);
     p.splits = std::max(1, (n_blocks + p.blocks - 1) / p.blocks);
     p.cluster = p.cluster && p.splits > 1;
     p.units = parts || (p.splits > 1 && !p.cluster) ? (size_t)groups * p.splits : 0;
@@ -497,8 +523,9 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
     }
   }
   if (parts && p.prompt) {
-    const long long units = (long long)p.shape.tiles * g->kv_heads * p.shape.splits;
-    p.p_units = (int)std::min<long long>(INT_MAX, p.counted ? std::max(148LL, units) : units);
+    const long long ctas = (long long)p.shape.tiles * g->kv_heads;
+    p.counted = g->n_req > 1;
+    p.p_units = (int)std::min<long long>(INT_MAX / PR_ROWS, p.counted ? spans_at_most(ctas, p.p_keys) : ctas * p.shape.splits);
     p.p_join = 0;
   }
   // whether a row tile can have more tiles of keys than a sum may take, whatever max_kv says
