@@ -1,10 +1,12 @@
 // Penalties for repeated tokens, biases and masks of allowed tokens on a step's logits (h2c_logits_adjust; the formula is
 // stated in include/h2cuda.h).
 //
-// A CTA takes one row's tokens c0 .. c1 of the vocabulary: it counts the row's earlier tokens that fall there in shared memory
-// (whole numbers, so the order of the counting does not matter), and then passes over its logits once. The few biased tokens of
-// the chunk are computed beside the pass, each by one thread that adds the token's biases up in the list's order, and written
-// after it. Bound: bandwidth for many rows; each chunk reads the row's history again (from L2), so chunks are long where histories are.
+// A CTA takes a chunk of one row's vocabulary, whose logits are on their way to registers (all of them but of the longest chunks) while it
+// counts the row's earlier tokens that fall there in shared memory (whole numbers, so the order does not matter) and its first
+// warp looks for the biased tokens among them and adds the biases of each up in the list's order. Then it changes, masks and writes
+// the logits, and at last the few biased ones.
+// Bound: bandwidth for many rows, and the instructions of the pass: a token that was said is found in nearly every warp's 256 logits, so
+// its division is one of five multiplications where it can be. Each chunk goes through the row's history (from L2), so chunks are long.
 #include "ops.cuh"
 
 #include <algorithm>
@@ -14,9 +16,10 @@
 namespace h2 {
 namespace {
 
-constexpr int LG_THREADS = 512, LG_BIASES = H2C_LOGITS_MAX_BIASES, LG_OWN = (LG_BIASES + LG_THREADS - 1) / LG_THREADS;
-constexpr int LG_CHUNK = 32768;  // the longest chunk (of 16-bit counts)
-constexpr int LG_SMEM = 2 * LG_CHUNK + 4 * LG_BIASES;
+constexpr int LG_THREADS = 512, LG_PER_SM = 3, LG_BIASES = H2C_LOGITS_MAX_BIASES;
+constexpr int LG_AHEAD = 4;                     // units of 16 bytes that a thread has on their way
+constexpr int LG_UNITS = LG_AHEAD * LG_THREADS;  // of the longest chunk
+constexpr int LG_SAID = 2;                      // units of 4 earlier tokens that a thread has on their way
 
 struct LogitArgs {
   const void* in;
@@ -32,100 +35,220 @@ struct LogitArgs {
 
 struct Strength {
   float rep, pres, freq;
+  float inv;  // 1 / rep, rounded; 0: quotients are formed by division
 };
+__device__ __forceinline__ Strength strength_of(const LogitArgs& a, int row) {
+  Strength s{a.repetition ? a.repetition[row] : 1.f, a.presence ? a.presence[row] : 0.f, a.frequency ? a.frequency[row] : 0.f, 0.f};
+  if (s.rep >= 0x1p-20f && s.rep <= 0x1p20f) s.inv = __fdiv_rn(1.f, s.rep);
+  return s;
+}
+// x / rep as division rounds it. An approximation q is corrected by its remainder, which fma gives exactly: once makes q the quotient
+// or one of its neighbours, and from there a correction with the rounded reciprocal rounds right (Markstein 1990), as long as no
+// term leaves the normal numbers.
+__device__ __forceinline__ float quotient(float x, const Strength& s) {
+  if (!(s.inv > 0.f && x > 0x1p-60f && x < 0x1p60f)) return __fdiv_rn(x, s.rep);
+  float q = __fmul_rn(x, s.inv);
+  q = __fmaf_rn(__fmaf_rn(-q, s.rep, x), s.inv, q);
+  return __fmaf_rn(__fmaf_rn(-q, s.rep, x), s.inv, q);
+}
 // the logit of a token that was said `count` times (single float32 operations)
 __device__ __forceinline__ float penalized(float x, unsigned count, const Strength& s) {
-  if (count) {
-    x = x > 0.f ? __fdiv_rn(x, s.rep) : __fmul_rn(x, s.rep);
-    x = __fsub_rn(x, __fadd_rn(__fmul_rn(s.freq, (float)count), s.pres));
-  }
-  return x;
+  x = x > 0.f ? quotient(x, s) : __fmul_rn(x, s.rep);
+  return __fsub_rn(x, __fadd_rn(__fmul_rn(s.freq, (float)count), s.pres));
 }
+
+// -infinity's bits, in each logit of a word
+template <class T>
+constexpr uint32_t MINUS_INF = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+
+// Logit i of a word as a number, and put into it.
+template <class T>
+__device__ __forceinline__ float value_of(uint32_t w, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(w);
+  } else {
+    const unsigned short u = (unsigned short)(i ? w >> 16 : w);
+    return to_f(*reinterpret_cast<const T*>(&u));
+  }
+}
+template <class T>
+__device__ __forceinline__ void put_value(uint32_t* w, int i, T x) {
+  if constexpr (sizeof(T) == 4) *w = __float_as_uint(x);
+  else *w = __byte_perm(*w, *reinterpret_cast<const unsigned short*>(&x), i ? 0x5410 : 0x3254);
+}
+
+// The biased tokens of a chunk, in the list's order, in shared memory: their places in the chunk and their entries, and for a token's
+// first entry the sum of its biases and its logit.
+struct Biased {
+  int *n, *at, *entry;
+  float *sum, *x;
+  int* first;
+  __device__ __forceinline__ Biased(uint8_t* p, int most) {
+    n = reinterpret_cast<int*>(p);
+    at = n + 4, entry = at + most;
+    sum = reinterpret_cast<float*>(entry + most), x = sum + most;
+    first = reinterpret_cast<int*>(x + most);
+  }
+  static size_t bytes(int most) { return most ? 16 + 20 * (size_t)most : 0; }
+};
 
 // C: type of the counts
 template <class T, class C, bool VEC>
-__global__ void __launch_bounds__(LG_THREADS) k_logits(const LogitArgs a) {
+__global__ void __launch_bounds__(LG_THREADS, LG_PER_SM) k_logits(const LogitArgs a) {
   extern __shared__ __align__(16) uint8_t sm[];
-  constexpr int V = 16 / (int)sizeof(T);
-  const int tid = threadIdx.x, row = blockIdx.x / a.chunks, c0 = (blockIdx.x - row * a.chunks) * a.chunk, n = min(a.chunk, a.vocab - c0);
-  C* count = reinterpret_cast<C*>(sm);
-  int* id = reinterpret_cast<int*>(sm + (a.tokens ? a.chunk * sizeof(C) : 0));
+  constexpr int V = 16 / (int)sizeof(T), UN = LG_AHEAD, CPW = 4 / (int)sizeof(C);  // logits of 16 bytes, counts of a word
+  const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.x / a.chunks, c0 = (blockIdx.x - row * a.chunks) * a.chunk;
+  const int n = min(a.chunk, a.vocab - c0);
+  unsigned* counts = reinterpret_cast<unsigned*>(sm);
+  const Biased biased(sm + (a.tokens ? a.chunk * sizeof(C) : 0), a.n_bias);
   const T* in = static_cast<const T*>(a.in) + row * a.in_row + c0;
   T* out = static_cast<T*>(a.out) + row * a.out_row + c0;
   const unsigned* allowed = a.allowed ? a.allowed + row * a.allowed_row + (c0 >> 5) : nullptr;
-  const Strength s{a.repetition ? a.repetition[row] : 1.f, a.presence ? a.presence[row] : 0.f, a.frequency ? a.frequency[row] : 0.f};
+  auto is_allowed = [&](int i) { return !allowed || (allowed[i >> 5] >> (i & 31) & 1u); };
+  // the first units of V logits are on their way while the history is counted
+  const int units = VEC ? n / V : 0;
+  uint4 raw[UN];
+  auto fetch = [&](int u0) {
+#pragma unroll
+    for (int k = 0; k < UN; k++) {
+      const int u = u0 + k * LG_THREADS;
+      if (u < units) raw[k] = reinterpret_cast<const uint4*>(in)[u];
+    }
+  };
+  fetch(tid);
+  const Strength s = strength_of(a, row);
+  auto count_of = [&](unsigned i) { return CPW == 1 ? counts[i] : counts[i >> 1] >> (16 * (i & 1)) & 0xffffu; };
   if (a.tokens) {
+    const int* history = a.tokens + row * a.tokens_row;
+    const int len = max(0, min(a.length[row], a.columns)), skip = min(len, (int)(((16 - ((uintptr_t)history & 15)) & 15) >> 2));
+    const int quads = (len - skip) >> 2, ends = skip + ((len - skip) & 3);  // (at most 6 before the first 16 bytes and after the last)
+    const int4* history4 = reinterpret_cast<const int4*>(history + skip);
+    // (by all warps but the first where that has biases to look for)
+    const int busy = a.n_bias ? 32 : 0, threads = LG_THREADS - busy, me = tid - busy;
+    int4 t[LG_SAID];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int k = 0; k < LG_SAID; k++)
+        if (me >= 0 && i0 + k * threads < quads) t[k] = history4[i0 + k * threads];
+    };
+    load(me);
+    const int rest = me >= 0 && me < ends ? history[me < skip ? me : len - ends + me] : -1;
     for (int i = tid; i < a.chunk * (int)sizeof(C) / 16; i += LG_THREADS) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    const int* said = a.tokens + row * a.tokens_row;
-    const int len = max(0, min(a.length[row], a.columns));
-#pragma unroll 4
-    for (int i = tid; i < len; i += LG_THREADS) {
-      const unsigned t = (unsigned)said[i] - (unsigned)c0;
-      if (t < (unsigned)n) {
-        if (sizeof(C) == 4) atomicAdd(reinterpret_cast<unsigned*>(count) + t, 1u);
-        else atomicAdd(reinterpret_cast<unsigned*>(count) + (t >> 1), 1u << (16 * (t & 1)));  // (up to 65,535: no carry)
+    auto add = [&](int token) {
+      const unsigned i = (unsigned)token - (unsigned)c0;
+      if (i < (unsigned)n) atomicAdd(counts + i / CPW, CPW == 1 ? 1u : 1u << (16 * (i & 1)));  // (up to 65,535: no carry)
+    };
+    if (me >= 0) {
+      if (me < ends) add(rest);
+      for (int i = me; i < quads; i += LG_SAID * threads) {
+        if (i != me) load(i);
+#pragma unroll
+        for (int k = 0; k < LG_SAID; k++)
+          if (i + k * threads < quads) add(t[k].x), add(t[k].y), add(t[k].z), add(t[k].w);
       }
     }
   }
-  for (int i = tid; i < a.n_bias; i += LG_THREADS) id[i] = a.bias_id[row * a.bias_row + i];
-  __syncthreads();
-  auto count_of = [&](int i) { return a.tokens ? (unsigned)count[i] : 0u; };
-  auto is_allowed = [&](int i) { return !allowed || (allowed[i >> 5] >> (i & 31) & 1u); };
-  // a biased token is the thread's that has its first entry
-  float own[LG_OWN];
-  unsigned mine = 0;
-  if (a.n_bias) {
+  if (a.n_bias && tid < 32) {
+    int m = 0;
+    for (int e0 = 0; e0 < a.n_bias; e0 += 32) {
+      const int e = e0 + lane, token = e < a.n_bias ? a.bias_id[row * a.bias_row + e] : -1, at = token - c0;
+      const bool here = token >= c0 && at < n;
+      const unsigned b = __ballot_sync(0xffffffffu, here);
+      if (here) {
+        const int k = m + __popc(b & ((1u << lane) - 1));
+        biased.at[k] = at;
+        biased.entry[k] = e;
+      }
+      m += __popc(b);
+    }
+    if (lane == 0) *biased.n = m;
+    __syncwarp();
     const float* b = a.bias + row * a.bias_row;
-#pragma unroll
-    for (int k = 0; k < LG_OWN; k++) {
-      const int e = tid + k * LG_THREADS, t = e < a.n_bias ? id[e] : -1;
-      bool first = t >= c0 && t - c0 < n;
-      for (int j = 0; first && j < e; j++) first = id[j] != t;
-      if (!first) continue;
-      float sum = b[e];
-      for (int j = e + 1; j < a.n_bias; j++)
-        if (id[j] == t) sum = __fadd_rn(sum, b[j]);
-      own[k] = is_allowed(t - c0) ? __fadd_rn(penalized(to_f(in[t - c0]), count_of(t - c0), s), sum) : -INFINITY;
-      mine |= 1u << k;
+    for (int k = lane; k < m; k += 32) {
+      const int at = biased.at[k];
+      const float x = to_f(in[at]);  // (before it is written, where out is in)
+      float sum = b[biased.entry[k]];
+      bool first = true;
+      for (int j = 0; first && j < k; j++) first = biased.at[j] != at;
+      for (int j = k + 1; first && j < m; j++)
+        if (biased.at[j] == at) sum = __fadd_rn(sum, b[biased.entry[j]]);
+      biased.sum[k] = sum;
+      biased.x[k] = x;
+      biased.first[k] = first;
     }
-    __syncthreads();  // (out may be in: they are read before any is written)
   }
-  if (VEC) {
-    for (int i = tid * V; i + V <= n; i += LG_THREADS * V) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(in + i);
-      const T* h = reinterpret_cast<const T*>(&raw);
-      alignas(16) T o[V];
-      const unsigned bits = allowed ? allowed[i >> 5] >> (i & 31) : ~0u;
+  __syncthreads();
+  // (most units hold no token that was said: their counts are looked at together)
+  constexpr int CW = V * (int)sizeof(C) / 4, PER = 4 / (int)sizeof(T);  // words of a unit's counts; logits of a word
+  for (int u0 = tid; u0 < units; u0 += UN * LG_THREADS) {
+    if (u0 != tid) fetch(u0);
 #pragma unroll
-      for (int k = 0; k < V; k++) {
-        const float x = penalized(to_f(h[k]), count_of(i + k), s);
-        o[k] = from_f<T>(bits >> k & 1u ? x : -INFINITY);
+    for (int k = 0; k < UN; k++) {
+      const int u = u0 + k * LG_THREADS;
+      if (u >= units) break;
+      uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+      if (a.tokens) {
+        uint32_t c[CW], any = 0;
+#pragma unroll
+        for (int i = 0; i < CW; i += 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(counts + u * CW + i);
+          c[i] = x.x, c[i + 1] = x.y;
+          any |= x.x | x.y;
+        }
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < V; i++) {
+            const unsigned said = CPW == 1 ? c[i / CPW] : i % CPW ? c[i / CPW] >> 16 : c[i / CPW] & 0xffffu;
+            if (said) {
+              const T x = from_f<T>(penalized(value_of<T>(w[i / PER], i % PER), said, s));
+              put_value<T>(&w[i / PER], i % PER, x);
+            }
+          }
+        }
       }
-      *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(o);
+      if (allowed) {
+        const unsigned bits = ~(allowed[u * V >> 5] >> (u * V & 31));  // of those that may not come
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t m;
+          if (sizeof(T) == 4) m = bits >> i & 1u ? ~0u : 0u;
+          else m = (bits >> (2 * i) & 1u ? 0xffffu : 0u) | (bits >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+          w[i] = (w[i] & ~m) | (MINUS_INF<T> & m);
+        }
+      }
+      reinterpret_cast<uint4*>(out)[u] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  for (int i = (VEC ? n / V * V : 0) + tid; i < n; i += LG_THREADS)
-    out[i] = from_f<T>(is_allowed(i) ? penalized(to_f(in[i]), count_of(i), s) : -INFINITY);
+  for (int i = units * V + tid; i < n; i += LG_THREADS) {
+    const unsigned said = a.tokens ? count_of(i) : 0u;
+    if (!is_allowed(i)) out[i] = from_f<T>(-INFINITY);
+    else if (said) out[i] = from_f<T>(penalized(to_f(in[i]), said, s));
+    else out[i] = in[i];
+  }
   if (a.n_bias) {
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < LG_OWN; k++)
-      if (mine >> k & 1u) out[id[tid + k * LG_THREADS] - c0] = from_f<T>(own[k]);
+    for (int k = tid; k < *biased.n; k += LG_THREADS) {
+      const int at = biased.at[k];
+      if (!biased.first[k] || !is_allowed(at)) continue;
+      const unsigned said = a.tokens ? count_of(at) : 0u;
+      out[at] = from_f<T>(__fadd_rn(said ? penalized(biased.x[k], said, s) : biased.x[k], biased.sum[k]));
+    }
   }
 }
 
 template <class T, class C>
-int launch_logits(const char* who, const LogitArgs& a, int rows, int chunks, bool vec, cudaStream_t st) {
+int launch_logits(const char* who, const LogitArgs& a, int rows, bool vec, cudaStream_t st) {
   static unsigned char done[OP_MAX_DEVICES];
+  constexpr int most = LG_UNITS * (16 / (int)sizeof(T)) * (int)sizeof(C) + 16 + 20 * LG_BIASES;
   if (int rc = op_once(who, done, [] {
-        const cudaError_t c = cudaFuncSetAttribute(k_logits<T, C, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SMEM);
-        return c != cudaSuccess ? c : cudaFuncSetAttribute(k_logits<T, C, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SMEM);
+        const cudaError_t c = cudaFuncSetAttribute(k_logits<T, C, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        return c != cudaSuccess ? c : cudaFuncSetAttribute(k_logits<T, C, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       }))
     return rc;
-  const size_t smem = (a.tokens ? (size_t)a.chunk * sizeof(C) : 0) + 4 * a.n_bias;
-  if (vec) k_logits<T, C, true><<<rows * chunks, LG_THREADS, smem, st>>>(a);
-  else k_logits<T, C, false><<<rows * chunks, LG_THREADS, smem, st>>>(a);
+  const size_t smem = (a.tokens ? (size_t)a.chunk * sizeof(C) : 0) + Biased::bytes(a.n_bias);
+  if (vec) k_logits<T, C, true><<<rows * a.chunks, LG_THREADS, smem, st>>>(a);
+  else k_logits<T, C, false><<<rows * a.chunks, LG_THREADS, smem, st>>>(a);
   return op_launched(who);
 }
 
@@ -179,14 +302,14 @@ extern "C" int h2c_logits_adjust(int32_t type, const void* logits, int64_t in_ro
   a.allowed = reinterpret_cast<const unsigned*>(allowed);
   const bool wide = columns > 65535;  // counts of 32 bits
   // the longest chunks that leave every SM a few CTAs
-  a.chunk = wide ? LG_CHUNK / 2 : LG_CHUNK;
-  while (a.chunk > 1024 && rows * ((vocab + a.chunk - 1LL) / a.chunk) < 148 * 4) a.chunk /= 2;
+  a.chunk = LG_UNITS * (int)(16 / es);
+  while (a.chunk > 1024 && rows * ((vocab + a.chunk - 1LL) / a.chunk) < 148 * 2) a.chunk /= 2;
   const long long chunks = (vocab + a.chunk - 1LL) / a.chunk;
   if (chunks * rows > INT_MAX) return op_error(H2C_ERR_INVALID, "%s: too many logits for one call", who);
   a.chunks = (int)chunks;
   const bool vec = !(((uintptr_t)logits | (uintptr_t)out | (rows > 1 ? in_row * es | out_row * es : 0)) & 15);
   cudaStream_t st = (cudaStream_t)stream;
-#define H2_LOGITS(T) (wide ? launch_logits<T, uint32_t>(who, a, rows, a.chunks, vec, st) : launch_logits<T, uint16_t>(who, a, rows, a.chunks, vec, st))
+#define H2_LOGITS(T) (wide ? launch_logits<T, uint32_t>(who, a, rows, vec, st) : launch_logits<T, uint16_t>(who, a, rows, vec, st))
   if (type == H2C_TYPE_F32) return H2_LOGITS(float);
   if (type == H2C_TYPE_F16) return H2_LOGITS(__half);
   return H2_LOGITS(__nv_bfloat16);
