@@ -1,18 +1,20 @@
 // Rotary positions of queries and keys (h2c_rope; the formula is stated in include/h2cuda.h).
 //
-// A CTA takes a few tokens: the angles of each token's pairs are the same for every head, so a thread makes one cosine and sine for
-// all of them into shared memory, and then the CTA's vectors are turned with 16-byte loads and stores where the layout has them.
+// A warp takes a token, or some of its heads where tokens are few: its lanes make the cosines and sines of the token's pairs, once for all
+// heads, and hand them around through shared memory. A lane then has the same few pairs of every head that it turns, so it keeps their
+// cosines and sines, and goes from head to head with loads and stores of 16 bytes where the layout has them.
 // The angle is formed in turns: position * (frequency / 2 pi) in 64 bits, whose whole turns are dropped before it becomes a
 // float32, so far positions are as exact as near ones.
 #include "ops.cuh"
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace h2 {
 namespace {
 
-constexpr int ROPE_THREADS = 256, ROPE_PAIRS = 1024;  // pairs that a CTA holds angles of
+constexpr int ROPE_WARPS = 8, ROPE_AHEAD = 4;  // of a CTA; heads that a lane has under way
 
 struct RopeSide {  // queries or keys
   const void* in;
@@ -25,7 +27,7 @@ struct RopeArgs {
   const int* position;
   const double* frequency;
   float magnitude;
-  int tokens, head_dim, half, per_cta;  // half = pairs of a head; tokens of a CTA
+  int tokens, head_dim, half, parts;  // half = pairs of a head; parts: warps that share a token's heads
 };
 
 // A pair turned: one product rounded, the other exact within its addition, whatever the layout.
@@ -36,7 +38,7 @@ __device__ __forceinline__ float turned_b(float a, float b, float2 cs) { return 
 template <class T, int W>
 struct Piece {
   static constexpr int B = W * (int)sizeof(T);
-  T v[W];
+  alignas(W * sizeof(T) >= 16 ? 16 : W * sizeof(T)) T v[W];
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (B % 16 == 0) {
 #pragma unroll
@@ -64,82 +66,149 @@ struct Piece {
   }
 };
 
-// One unit of work: W neighbouring values and, in the half layout, the W that are their partners. PAIR: values of a unit that
-// hold whole pairs (interleaved).
-template <class T, int W, bool INTER>
-__global__ void __launch_bounds__(ROPE_THREADS) k_rope(const RopeArgs a) {
-  extern __shared__ float2 turn[];  // [token][pair]: cosine and sine, times the magnitude
-  constexpr int PP = INTER ? (W == 1 ? 1 : W / 2) : W;  // pairs of a unit
-  const int t0 = blockIdx.x * a.per_cta, n = min(a.per_cta, a.tokens - t0);
-  for (int i = threadIdx.x; i < n * a.half; i += ROPE_THREADS) {
-    const int t = i / a.half, j = i - t * a.half, pos = a.position[t0 + t];
-    const double turns = (double)max(pos, 0) * (a.frequency[j] * 0.15915494309189533577);
-    float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    // (a token without a position is copied; an infinite frequency gives NaN, and so does every use of it)
-    turn[i] = make_float2(c * a.magnitude, s * a.magnitude);
+// Quotients of small numbers by multiplication (what lies where would be most of the instructions else).
+struct Quotient {
+  unsigned d, magic;
+  __device__ __forceinline__ explicit Quotient(unsigned n) : d(n), magic(0xffffffffu / n) {}
+  __device__ __forceinline__ unsigned of(unsigned n, unsigned* rest) const {
+    unsigned q = __umulhi(n, magic), r = n - q * d;  // (one too few at most)
+    if (r >= d) q++, r -= d;
+    *rest = r;
+    return q;
   }
-  __syncthreads();
-  const int rot = a.half / PP, rest = (a.head_dim - 2 * a.half) / W, units = rot + rest;  // of a head
-  const int heads = a.side[0].heads + a.side[1].heads, all = n * heads * units;
-  for (int i = threadIdx.x; i < all; i += ROPE_THREADS) {
-    const int th = i / units, u = i - th * units, t = th / heads;
-    int h = th - t * heads;
-    const bool keys = h >= a.side[0].heads;
-    const RopeSide& s = a.side[keys];
-    if (keys) h -= a.side[0].heads;
-    const T* in = static_cast<const T*>(s.in) + (t0 + t) * s.in_row + h * s.in_head;
-    T* out = static_cast<T*>(s.out) + (t0 + t) * s.out_row + h * s.out_head;
-    if (u >= rot) {
-      if (!s.copy) continue;
-      Piece<T, W> p;
-      const int d = 2 * a.half + (u - rot) * W;
-      p.load(in + d);
-      p.store(out + d);
-      continue;
+};
+
+// Two 16-bit values of a word as float32, and float32 rounded to them.
+template <class T>
+__device__ __forceinline__ float2 two_of(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <class T>
+__device__ __forceinline__ uint32_t word_of(float a, float b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+// A unit's pairs turned: (p[i], q[i]), or the neighbours of p.
+template <bool INTER, class T, int N, int W>
+__device__ __forceinline__ void turn_unit(Piece<T, N>& p, Piece<T, W>& q, const float2* cs) {
+  if constexpr (sizeof(T) == 2 && W > 1) {
+    uint32_t* pw = reinterpret_cast<uint32_t*>(p.v);
+    uint32_t* qw = reinterpret_cast<uint32_t*>(q.v);
+#pragma unroll
+    for (int i = 0; i < W / 2; i++) {
+      const float2 x = two_of<T>(pw[i]);
+      if constexpr (INTER) {
+        const float2 c = cs[i];
+        pw[i] = word_of<T>(turned_a(x.x, x.y, c), turned_b(x.x, x.y, c));
+      } else {
+        const float2 y = two_of<T>(qw[i]);
+        const float4 c = reinterpret_cast<const float4*>(cs)[i];
+        const float2 c0 = make_float2(c.x, c.y), c1 = make_float2(c.z, c.w);
+        pw[i] = word_of<T>(turned_a(x.x, y.x, c0), turned_a(x.y, y.y, c1));
+        qw[i] = word_of<T>(turned_b(x.x, y.x, c0), turned_b(x.y, y.y, c1));
+      }
     }
-    const float2* cs = turn + t * a.half + u * PP;
-    const bool turned = a.position[t0 + t] >= 0;
-    if (!turned && !s.copy) continue;
-    if constexpr (INTER) {
-      Piece<T, 2 * PP> p;
-      p.load(in + u * 2 * PP);
-      if (turned) {
+  } else {
 #pragma unroll
-        for (int k = 0; k < PP; k++) {
-          const float x = to_f(p.v[2 * k]), y = to_f(p.v[2 * k + 1]);
-          p.v[2 * k] = from_f<T>(turned_a(x, y, cs[k]));
-          p.v[2 * k + 1] = from_f<T>(turned_b(x, y, cs[k]));
-        }
-      }
-      p.store(out + u * 2 * PP);
-    } else {
-      Piece<T, W> p, q;
-      p.load(in + u * W);
-      q.load(in + a.half + u * W);
-      if (turned) {
-#pragma unroll
-        for (int k = 0; k < W; k++) {
-          const float x = to_f(p.v[k]), y = to_f(q.v[k]);
-          p.v[k] = from_f<T>(turned_a(x, y, cs[k]));
-          q.v[k] = from_f<T>(turned_b(x, y, cs[k]));
-        }
-      }
-      p.store(out + u * W);
-      q.store(out + a.half + u * W);
+    for (int i = 0; i < (INTER ? N / 2 : W); i++) {
+      T& a = INTER ? p.v[2 * i] : p.v[i];
+      T& b = INTER ? p.v[2 * i + 1] : q.v[i];
+      const float x = to_f(a), y = to_f(b);
+      a = from_f<T>(turned_a(x, y, cs[i]));
+      b = from_f<T>(turned_b(x, y, cs[i]));
     }
   }
 }
 
+// One unit of work is W neighbouring values and, in the half layout, the W that are their partners; of the part that is not turned, W
+// values. FEW: a head has at most 32 units, so a lane has one of them, of several heads at a time, and keeps its cosines and sines; else
+// the lanes go through a head's units together.
+template <class T, int W, bool INTER, bool FEW>
+__global__ void __launch_bounds__(32 * ROPE_WARPS, 3) k_rope(const RopeArgs a) {
+  extern __shared__ __align__(16) float2 turn[];  // [warp][pair]: cosine and sine, times the magnitude
+  constexpr int PP = INTER ? (W == 1 ? 1 : W / 2) : W;  // pairs of a unit
+  constexpr int IW = INTER ? 2 * PP : W;                // values of its first piece
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long job = (long long)blockIdx.x * ROPE_WARPS + warp;
+  const int t = (int)(job / a.parts), part = (int)(job - (long long)t * a.parts);
+  if (t >= a.tokens) return;
+  float2* cs = turn + warp * ((a.half + 1) & ~1);
+  const int pos = a.position[t];
+  for (int j = lane; j < a.half; j += 32) {
+    const double turns = (double)max(pos, 0) * (a.frequency[j] * 0.15915494309189533577);
+    float s, c;
+    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    // (a token without a position is copied; an infinite frequency gives NaN, and so does every use of it)
+    cs[j] = make_float2(c * a.magnitude, s * a.magnitude);
+  }
+  __syncwarp();
+  const int rot = a.half / PP, units = rot + (a.head_dim - 2 * a.half) / W, heads = a.side[0].heads + a.side[1].heads;
+  // heads at a time, and what of them this lane has; it goes from its first head by as many as all warps of the token take at a time
+  const int at_once = FEW ? 32 / units : 1, mine = FEW ? lane / units : 0, step = at_once * a.parts;
+  if (mine >= at_once) return;
+  auto go = [&](int u, const float2* c) {
+    const bool pair = u < rot, turned = pair && pos >= 0;
+    const int d = pair ? u * IW : 2 * a.half + (u - rot) * W;
+    for (int h0 = part * at_once + mine; h0 < heads; h0 += ROPE_AHEAD * step) {
+      Piece<T, IW> p[ROPE_AHEAD];
+      Piece<T, W> q[ROPE_AHEAD];
+      auto side_of = [&](int h) -> const RopeSide& { return a.side[h >= a.side[0].heads]; };
+      auto in_side = [&](int h) { return h >= a.side[0].heads ? h - a.side[0].heads : h; };
+#pragma unroll
+      for (int k = 0; k < ROPE_AHEAD; k++) {
+        const int h = h0 + k * step;
+        if (h >= heads) break;
+        const RopeSide& s = side_of(h);
+        const T* in = static_cast<const T*>(s.in) + t * s.in_row + in_side(h) * s.in_head + d;
+        if (!turned && !s.copy) continue;
+        if (IW == W || pair) p[k].load(in);
+        else p[k].v[0] = in[0];
+        if (!INTER && pair) q[k].load(in + a.half);
+      }
+#pragma unroll
+      for (int k = 0; k < ROPE_AHEAD; k++) {
+        const int h = h0 + k * step;
+        if (h >= heads) break;
+        const RopeSide& s = side_of(h);
+        T* out = static_cast<T*>(s.out) + t * s.out_row + in_side(h) * s.out_head + d;
+        if (!turned && !s.copy) continue;
+        if (turned) turn_unit<INTER>(p[k], q[k], c);
+        if (IW == W || pair) p[k].store(out);
+        else out[0] = p[k].v[0];
+        if (!INTER && pair) q[k].store(out + a.half);
+      }
+    }
+  };
+  if (FEW) {
+    const int u = lane - mine * units;
+    alignas(16) float2 kept[PP];
+#pragma unroll
+    for (int i = 0; i < PP; i++) kept[i] = u < rot ? cs[u * PP + i] : make_float2(1.f, 0.f);
+    go(u, kept);
+  } else {
+    for (int u = lane; u < units; u += 32) go(u, cs + (u < rot ? u * PP : 0));
+  }
+}
+
+template <class T, int W, bool INTER>
+void launch_rope_w(const RopeArgs& a, cudaStream_t st) {
+  const int units = a.half / (INTER ? (W == 1 ? 1 : W / 2) : W) + (a.head_dim - 2 * a.half) / W;
+  const unsigned ctas = (unsigned)(((long long)a.tokens * a.parts + ROPE_WARPS - 1) / ROPE_WARPS);
+  const size_t smem = ROPE_WARPS * ((a.half + 1) & ~1) * sizeof(float2);
+  if (units <= 32) k_rope<T, W, INTER, true><<<ctas, 32 * ROPE_WARPS, smem, st>>>(a);
+  else k_rope<T, W, INTER, false><<<ctas, 32 * ROPE_WARPS, smem, st>>>(a);
+}
 template <class T>
 void launch_rope(const RopeArgs& a, bool interleaved, bool vec, cudaStream_t st) {
   constexpr int W = 16 / (int)sizeof(T);
-  const int ctas = (a.tokens + a.per_cta - 1) / a.per_cta;
-  const size_t smem = (size_t)a.per_cta * a.half * sizeof(float2);
-  if (interleaved)
-    vec ? k_rope<T, W, true><<<ctas, ROPE_THREADS, smem, st>>>(a) : k_rope<T, 1, true><<<ctas, ROPE_THREADS, smem, st>>>(a);
-  else
-    vec ? k_rope<T, W, false><<<ctas, ROPE_THREADS, smem, st>>>(a) : k_rope<T, 1, false><<<ctas, ROPE_THREADS, smem, st>>>(a);
+  if (interleaved) vec ? launch_rope_w<T, W, true>(a, st) : launch_rope_w<T, 1, true>(a, st);
+  else vec ? launch_rope_w<T, W, false>(a, st) : launch_rope_w<T, 1, false>(a, st);
 }
 
 }  // namespace
@@ -204,10 +273,8 @@ extern "C" int h2c_rope(int32_t type, const void* q, int64_t q_row, int64_t q_he
         return op_error(H2C_ERR_INVALID, "%s: %s must not share memory with %s", who, out_name[i], in_name[1 - i]);
     if (op_rows_meet(out[0], out[1])) return op_error(H2C_ERR_INVALID, "%s: q_out must not share memory with k_out", who);
   }
-  const long long per_token = ((long long)q_heads + k_heads) * head_dim;
-  // tokens of a CTA: some 8 vectors a thread, while that leaves every SM a CTA
-  long long per = std::min<long long>({std::max(1LL, 16384 / per_token), ROPE_PAIRS / a.half, (tokens + 295LL) / 296});
-  a.per_cta = (int)std::max(1LL, per);
+  // warps of a token: as few as fill the SMs (some 32 warps each), at most one for every four heads
+  a.parts = (int)std::max<long long>(1, std::min<long long>((q_heads + k_heads + 3) / 4, 148 * 32 / tokens));
   cudaStream_t st = (cudaStream_t)stream;
   if (type == H2C_TYPE_F32) launch_rope<float>(a, interleaved, vec, st);
   else if (type == H2C_TYPE_F16) launch_rope<__half>(a, interleaved, vec, st);
