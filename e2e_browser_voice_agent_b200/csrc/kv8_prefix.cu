@@ -18,6 +18,20 @@ struct Pass {
   int rows, prompt;  // whether k_att_rows, k_att_prompt take part
 };
 
+// k_att_rows of both passes in one launch: the groups, then the requests.
+struct BothRows {
+  RowArgsOf<SharedArgs> ra[2];
+  unsigned across[2], first_own;  // CTAs that a request's rows take; the requests' first CTA
+};
+template <class T, int HD>
+__global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_prefix_rows(const __grid_constant__ BothRows both) {
+  const EndAfterTheOthers<true> end;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int own = blockIdx.x >= both.first_own;
+  const unsigned at = own ? blockIdx.x - both.first_own : blockIdx.x, across = both.across[own], rz = at / across, n = both.ra[own].a.n_req;
+  att_rows<T, HD>(both.ra[own], at - rz * across, rz % n, rz / n);
+}
+
 // Where the spans of a row lie: span s has its sums at part + s * part_step and its (m, l) at ml + s * ml_step.
 struct Parts {
   const float* part;
@@ -234,9 +248,9 @@ PrefixPlan plan_prefix(const h2c_kv8_prefix_args* g) {
   p.bytes = p.own.bytes + p.prefix.bytes - (p.own.spill && p.prefix.spill ? sums : 0);
   return p;
 }
-// Whether a pass's counts fit their types: rows of the workspace, axes of the grids.
-bool fits(const WorkPlan& p, long long kv_heads) {
-  return (long long)p.splits * p.tiles * RW_ROWS * kv_heads <= INT_MAX && p.splits <= 65535 &&
+// Whether a pass's counts fit their types: CTAs and rows of the workspace.
+bool fits(const WorkPlan& p, long long kv_heads, long long requests) {
+  return (long long)p.splits * p.tiles * RW_ROWS * kv_heads <= INT_MAX && (p.tiles * kv_heads / RW_WARPS + 1) * requests * p.splits <= INT_MAX / 2 &&
          spans_at_most((long long)p.shape.tiles * kv_heads, p.p_keys) * PR_ROWS <= INT_MAX;
 }
 
@@ -285,7 +299,7 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
   constexpr int p_smem = PromptCfg<T, HD>::SMEM, r_smem = RowSmem<HD>::BYTES;
   if (int rc = op_once(who, done, [] {
         const cudaError_t c = cudaFuncSetAttribute(k_att_prompt<T, HD, SharedArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, p_smem);
-        return c != cudaSuccess ? c : cudaFuncSetAttribute(k_att_rows<T, HD, SharedArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, r_smem);
+        return c != cudaSuccess ? c : cudaFuncSetAttribute(k_prefix_rows<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, r_smem);
       }))
     return rc;
   // each kernel but the first may start while the one before it still runs, and ends after it
@@ -305,13 +319,20 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
     c = cudaLaunchKernelEx(&cfg, k_att_prompt<T, HD, SharedArgs>, pass[i].pa);
     cfg.numAttrs = 1;
   }
-  for (int i = 0; i < 2 && c == cudaSuccess; i++) {
-    const WorkPlan& p = i ? plan.own : plan.prefix;
-    if (!p.rows) continue;
-    cfg.gridDim = dim3((g->own.kv_heads * p.tiles + RW_WARPS - 1) / RW_WARPS, pass[i].ra.a.n_req, p.splits);
+  if (c == cudaSuccess && (plan.own.rows || plan.prefix.rows)) {
+    BothRows both{{pass[0].ra, pass[1].ra}, {1, 1}, 0};
+    unsigned ctas = 0;
+    for (int i = 0; i < 2; i++) {
+      const WorkPlan& p = i ? plan.own : plan.prefix;
+      both.first_own = i ? ctas : 0;
+      if (!p.rows) continue;
+      both.across[i] = (unsigned)(g->own.kv_heads * p.tiles + RW_WARPS - 1) / RW_WARPS;
+      ctas += both.across[i] * pass[i].ra.a.n_req * p.splits;
+    }
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(RW_WARPS * 32);
     cfg.dynamicSmemBytes = r_smem;
-    c = cudaLaunchKernelEx(&cfg, k_att_rows<T, HD, SharedArgs>, pass[i].ra);
+    c = cudaLaunchKernelEx(&cfg, k_prefix_rows<T, HD>, both);
     cfg.numAttrs = 1;
   }
   if (c == cudaSuccess) {
@@ -385,7 +406,7 @@ int h2c_kv8_prefix_attention(const h2c_kv8_prefix_args* g, void* stream) {
                         {"kv_len", o->kv_len, n4, 4},                          {"prefix_table", g->prefix_table, g4 * g->prefix_cols, 4},
                         {"prefix_len", g->prefix_len, g4, 4},                  {"group_start", g->group_start, g4 ? g4 + 4 : 0, 4}};
   if (int rc = check_memory(who, o, in, 6, p.bytes)) return rc;
-  if (!fits(p.own, o->kv_heads) || !fits(p.prefix, o->kv_heads) || (long long)o->rows * o->heads > INT_MAX)
+  if (!fits(p.own, o->kv_heads, o->n_req) || !fits(p.prefix, o->kv_heads, g->n_groups) || (long long)o->rows * o->heads > INT_MAX)
     return op_error(H2C_ERR_INVALID, "%s: too many rows for one call", who);
   cudaStream_t st = (cudaStream_t)stream;
   if (o->type == H2C_TYPE_F32) return launch_typed<float>(who, p, g, st);

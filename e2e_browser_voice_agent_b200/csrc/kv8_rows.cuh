@@ -75,25 +75,23 @@ struct RowSmem {
 // In a call that launches k_att_prompt too, k_att_rows follows it by programmatic dependent launch: it uses nothing of it and
 // takes the SMs that its last CTAs leave (31 single tokens of 100-4,096 beside 2 prompts of 2,048: 134 -> 130 us), and ends after it.
 
-// (the CTAs an SM that shared memory has room for 128 wide, and registers 64 wide: without the bound the compiler spills for one more)
+// The CTA's work among those of `ra`: request r, and x and z as in the grid.
 template <class T, int HD, class A>
-__global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(const RowArgsOf<A> ra) {
-  const EndAfterTheOthers<true> end;
+__device__ __forceinline__ void att_rows(const RowArgsOf<A>& ra, const int x, const int r, const int z) {
   using S = RowSmem<HD>;
   constexpr int KC = HD / 64;   // 16-byte pieces of a key per lane
   constexpr int VB = HD / 8;    // bytes of a value row per lane (16 or 8)
   constexpr int NT = HD / 8;    // output tiles of 8 dimensions
   extern __shared__ __align__(16) uint8_t sm[];
   const A& a = ra.a;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the joining kernel, which waits for this one's end)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   // Where parts are left to a joining kernel in any case, a warp takes a span for itself: no warp waits for another, and four times as
   // many spans are on their way (256 single tokens of 16-2,000 keys, 28 heads over 4 of 128). Spans are the grid's slowest axis and the
   // last go first: only long requests have them, and the CTAs without one are over before the work begins.
   constexpr bool ALONE = PARTS_ONLY<A>;
-  const int split = ALONE ? ra.splits - 1 - blockIdx.z : blockIdx.x % ra.splits, th = ALONE ? blockIdx.x * RW_WARPS + warp : blockIdx.x / ra.splits;
+  const int split = ALONE ? ra.splits - 1 - z : x % ra.splits, th = ALONE ? x * RW_WARPS + warp : x / ra.splits;
   const int head = th % a.kv_heads, tile = th / a.kv_heads;
-  const int r = blockIdx.y;
+  if (ALONE && split < 0) return;
   int n_all;
   const Request R = request_of(a, r, &n_all);
   const int row0 = tile * RW_ROWS, n_rows = R.n_q * a.group;
@@ -431,6 +429,14 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(c
   __syncwarp();
   // (the others may still read this CTA's part)
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// (the CTAs an SM that shared memory has room for 128 wide, and registers 64 wide: without the bound the compiler spills for one more)
+template <class T, int HD, class A>
+__global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_att_rows(const RowArgsOf<A> ra) {
+  const EndAfterTheOthers<true> end;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the joining kernel, which waits for this one's end)
+  att_rows<T, HD>(ra, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 // A row's spans are joined by a warp where they are few (8 rows a CTA), by 8 warps where they are many, each taking every 8th span; the
