@@ -30,6 +30,8 @@ class Norm(NamedTuple):
 
 
 def _matrix(name: str, t: torch.Tensor, index: int) -> int:
+    if t.dim() == 2 and t.get_device() == index and t.stride(1) == 1 and t.numel() < 2**31:  # (the usual case)
+        return t.data_ptr()
     if t.dim() != 2:
         raise ValueError(f"{name}: a matrix is wanted, not {tuple(t.shape)}")
     if t.get_device() != index:
@@ -126,18 +128,21 @@ def norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Opt
             raise TypeError(f"residual: {x.dtype} or float32 is wanted, not {residual.dtype}")
         r_type = _TYPES[residual.dtype]
         if out is None:
-            out = torch.empty(rows, k, dtype=residual.dtype, device=x.device)
-        elif out.shape != x.shape:
-            raise ValueError(f"out: {tuple(x.shape)} is wanted, not {tuple(out.shape)}")
-        elif out.dtype is not residual.dtype:
-            raise TypeError(f"out: {residual.dtype} is wanted, not {out.dtype}")
-        po, o_row = _matrix("out", out, index), out.stride(0)
+            out = residual.new_empty((rows, k))
+            po, o_row = out.data_ptr(), k
+        else:
+            if out.shape != x.shape:
+                raise ValueError(f"out: {tuple(x.shape)} is wanted, not {tuple(out.shape)}")
+            if out.dtype is not residual.dtype:
+                raise TypeError(f"out: {residual.dtype} is wanted, not {out.dtype}")
+            po, o_row = _matrix("out", out, index), out.stride(0)
     elif out is not None:
         raise ValueError("out: there is no residual, so no sum")
-    q = torch.empty(rows, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    k_pad = (k + 15) // 16 * 16
+    q = x.new_empty((rows, k_pad), dtype=torch.int8)
+    scale = weight.new_empty((rows,), dtype=torch.float32)
     _call(index, _lib.load().h2c_i8_norm, _TYPES[x.dtype], px, x.stride(0), r_type, pr, r_row, po, o_row,
-          _want("weight", weight, torch.float32, index, (k,)), eps, rows, k, q.data_ptr(), q.shape[1], scale.data_ptr())
+          _want("weight", weight, torch.float32, index, (k,)), eps, rows, k, q.data_ptr(), k_pad, scale.data_ptr())
     return Norm(q, scale, out)
 
 
@@ -154,7 +159,7 @@ def values(codes: torch.Tensor, scale: torch.Tensor, k: Optional[int] = None, dt
     k = codes.shape[1] if k is None else k
     if not 0 < k <= codes.shape[1]:
         raise ValueError(f"k: 1 to {codes.shape[1]} is wanted, not {k}")
-    y = torch.empty(rows, k, dtype=dtype, device=codes.device)
+    y = codes.new_empty((rows, k), dtype=dtype)
     _call(index, _lib.load().h2c_i8_values, pq, codes.stride(0), _want("scale", scale, torch.float32, index, (rows,)), rows, k,
           _TYPES[dtype], y.data_ptr())
     return y

@@ -50,7 +50,7 @@ def adjust(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, length: 
     rows, vocab = logits.shape
     p_in, in_row = _lines("logits", logits, logits.dtype, index, rows)
     if out is None:
-        out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty((rows, vocab))
         p_out, out_row = out.data_ptr(), vocab
     else:
         p_out, out_row = _lines("out", out, logits.dtype, index, rows, vocab)
@@ -59,7 +59,6 @@ def adjust(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, length: 
         raise ValueError("tokens and length belong together")
     if (bias_id is None) != (bias is None):
         raise ValueError("bias_id and bias belong together")
-    given = [(n, t) for n, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)) if t is not None]
     if tokens is not None:
         said, said_row = _lines("tokens", tokens, torch.int32, index, rows)
         columns = tokens.shape[1]
@@ -69,12 +68,15 @@ def adjust(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, length: 
             said = p_len = None
         else:
             p_len = _want("length", length, torch.int32, index, (rows,))
-        strengths = [None if t is None else _want(n, t, torch.float32, index, (rows,))
-                     for n, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency))]
+        f32, one = torch.float32, (rows,)
+        strengths = [None if repetition is None else _want("repetition", repetition, f32, index, one),
+                     None if presence is None else _want("presence", presence, f32, index, one),
+                     None if frequency is None else _want("frequency", frequency, f32, index, one)]
         if not columns:
             strengths = [None, None, None]
-    elif given:
-        raise ValueError(f"{given[0][0]}: the tokens that it is for are wanted with it")
+    elif not (repetition is presence is frequency is None):
+        name = "repetition" if repetition is not None else "presence" if presence is not None else "frequency"
+        raise ValueError(f"{name}: the tokens that it is for are wanted with it")
     p_id = p_bias = None
     n_bias = 0
     if bias_id is not None:

@@ -83,32 +83,37 @@ def rotate(q: torch.Tensor, position: torch.Tensor, frequency: torch.Tensor, k: 
     if kind is None:
         raise TypeError(f"q: float32, float16 or bfloat16 is wanted, not {q.dtype}")
     pq, q_row, q_head = _vectors("q", q, q, index)
-    tokens, heads, head_dim = q.shape
+    tokens, heads, head_dim = shape = q.shape
     k_heads, pk, k_row, k_head, pko, ko_row, ko_head = 0, None, 0, 0, None, 0, 0
     if k is not None:
         pk, k_row, k_head = _vectors("k", k, q, index)
-        k_heads = k.shape[1]
-        if k.shape[0] != tokens or k.shape[2] != head_dim:
+        k_tokens, k_heads, k_dim = k.shape
+        if k_tokens != tokens or k_dim != head_dim:
             raise ValueError(f"k: [{tokens}, heads, {head_dim}] is wanted, not {tuple(k.shape)}")
         if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        elif k_out.shape != k.shape:
-            raise ValueError(f"k_out: {tuple(k.shape)} is wanted, not {tuple(k_out.shape)}")
-        pko, ko_row, ko_head = _vectors("k_out", k_out, q, index)
+            k_out = k.new_empty((tokens, k_heads, head_dim))
+            pko, ko_row, ko_head = k_out.data_ptr(), k_heads * head_dim, head_dim
+        else:
+            if k_out.shape != k.shape:
+                raise ValueError(f"k_out: {tuple(k.shape)} is wanted, not {tuple(k_out.shape)}")
+            pko, ko_row, ko_head = _vectors("k_out", k_out, q, index)
     elif k_out is not None:
         raise ValueError("k_out: there is no k")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape:
-        raise ValueError(f"out: {tuple(q.shape)} is wanted, not {tuple(out.shape)}")
-    po, o_row, o_head = _vectors("out", out, q, index)
+        out = q.new_empty((tokens, heads, head_dim))
+        po, o_row, o_head = out.data_ptr(), heads * head_dim, head_dim
+    else:
+        if out.shape != shape:
+            raise ValueError(f"out: {tuple(shape)} is wanted, not {tuple(out.shape)}")
+        po, o_row, o_head = _vectors("out", out, q, index)
     if position.dim() != 1 or position.shape[0] < tokens:
         raise ValueError(f"position: at least {tokens} entries are wanted, not {tuple(position.shape)}")
-    if frequency.dim() != 1 or not 1 <= frequency.shape[0] <= head_dim // 2:
+    pairs = frequency.shape[0] if frequency.dim() == 1 else 0
+    if not 1 <= pairs <= head_dim // 2:
         raise ValueError(f"frequency: 1 to {head_dim // 2} entries are wanted, not {tuple(frequency.shape)}")
     if tokens >= 2**31 or heads >= 2**31 or k_heads >= 2**31 or head_dim >= 2**31:
         raise ValueError(f"q: {tuple(q.shape)} does not fit in 32 bits")
     _call(index, _lib.load().h2c_rope, kind, pq, q_row, q_head, po, o_row, o_head, heads, pk, k_row, k_head, pko, ko_row, ko_head,
           k_heads, tokens, head_dim, _want("position", position, torch.int32, index),
-          _want("frequency", frequency, torch.float64, index), 2 * frequency.shape[0], int(bool(interleaved)), magnitude)
+          _want("frequency", frequency, torch.float64, index), 2 * pairs, 1 if interleaved else 0, magnitude)
     return out if k is None else (out, k_out)
