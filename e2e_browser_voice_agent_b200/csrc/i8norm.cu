@@ -16,8 +16,12 @@ namespace {
 // whatever the division of a row among threads.
 // Rows of aligned units of four values, up to 8,192 units (k_i8_norm): one warp a row to 32, a few short rows a CTA, each thread holding
 // up to eight units in registers between the three steps (sum of squares, largest magnitude, codes), so every input is read once and
-// all of a row is on its way together; the sizes are the compiler's, for the instructions, not the bytes, were what bound it. Few
-// rows: two units a thread. Other rows (k_i8_norm_any): a CTA each, whose values that do not fit its registers are read again.
+// all of a row is on its way together. The sizes are the compiler's: with loops over sizes known at run time the instructions were what
+// bound it (16,392 x 3,584 bfloat16 with a float32 residual: 146 us; now 97, 6.7 TB/s). Few rows: two units a thread, four times
+// the warps, as latency is what counts (k_i8_norm's launch below). Other rows (k_i8_norm_any): a CTA each, whose values that do not fit
+// its registers are read again.
+// Bound: bandwidth for many rows (16,392 x 3,584 with a bfloat16 residual 63 us, 6.5 TB/s; float32 x 896 31 us, 6.1 TB/s); rows without a
+// residual have the fewest bytes for the same sums in 64 bits and are bound by those (47 us, 3.7 TB/s). One row: 2.3 us, a launch.
 constexpr int NORM_V = 4;        // values of a unit: 16 bytes of float32, so that a warp's accesses are whole lines
 constexpr int NORM_WARPS = 8;    // of a CTA whose rows take fewer
 constexpr int NORM_MOST = 32768; // values of a row that registers hold
@@ -330,7 +334,10 @@ void launch_norm_w(const NormArgs& a, cudaStream_t st) {
 }
 template <class TX, class TR>
 void launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
-  const bool few = a.rows <= 148;
+  // Few rows, some 3 of them an SM: more warps each. us with more and with fewer warps, bfloat16 with a residual: 896 wide 32 rows 2.2
+  // and 3.0, 600 rows 2.8 and 3.3, 1,200 rows 4.0 and 3.8; 3,584 wide 32 rows 2.7 and 3.4, 400 rows 3.7 and 4.1, 600 rows 5.1 and 4.7;
+  // 8,192 wide 32 rows 3.6 and 3.6, 200 rows 4.7 and 4.1, so there all rows take 8 warps.
+  const bool few = a.rows <= 148 * 3;
   if (!vec || a.k > NORM_MOST) {
     if (vec) k_i8_norm_any<TX, TR, true><<<a.rows, 1024, 0, st>>>(a);
     else k_i8_norm_any<TX, TR, false><<<a.rows, 1024, 0, st>>>(a);
@@ -341,8 +348,7 @@ void launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
     if (few) launch_norm_w<TX, TR, 16, 2>(a, st);
     else launch_norm_w<TX, TR, 4, 8>(a, st);
   } else if (a.k <= 8192) {
-    if (few) launch_norm_w<TX, TR, 32, 2>(a, st);
-    else launch_norm_w<TX, TR, 8, 8>(a, st);
+    launch_norm_w<TX, TR, 8, 8>(a, st);
   } else {
     launch_norm_w<TX, TR, 32, 8>(a, st);
   }

@@ -115,6 +115,20 @@ def test_groups_counted_on_the_device(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_more_groups_and_requests_than_a_warp(dtype):
+    sizes = [1 + (5 * i) % 4 for i in range(41)]
+    gs = [0] + np.cumsum(sizes).tolist()
+    n = gs[-1] + 3
+    kv_len = [(11 * i) % 70 for i in range(n)]
+    n_q = [min(1, x) for x in kv_len]
+    run_case(dtype, 16, 14, 2, 64, [(97 * i) % 400 for i in range(41)], gs, kv_len, n_q)
+    n_q[70], kv_len[70] = 300, 333                      # a prompt behind many single tokens
+    run_case(dtype, 32, 8, 4, 128, [(97 * i) % 400 for i in range(41)], gs, kv_len, n_q)
+    n = 130                                             # a group whose own requests are counted warp by warp
+    n_q = [1] * 100 + [40] + [1] * 29
+    run_case(dtype, 16, 7, 1, 64, [2100], [0, n], [x + i for i, x in enumerate(n_q)], n_q)
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_prompts_behind_a_prefix(dtype):
     run_case(dtype, 64, 8, 2, 128, [1500], [0, 3], [400, 90, 1000], [400, 90, 300])
     run_case(dtype, 16, 14, 2, 64, [513], [0, 1], [700], [700])

@@ -98,6 +98,36 @@ def test_one_penalty_alone(only):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_strong_and_weak_penalties(dtype):
+    """Logits of all magnitudes over and times strengths of all: single float32 operations, as the host's."""
+    some = [0.0, 1e-45, 1e-30, 2.0**-21, 2.0**-20, 0.3, 1 / 3, 0.9999999, 1.0, 1.0000001, 1.3, 3.0, 7.0, 2.0**20, 2.0**21, 1e30, math.inf, -1.3, -math.inf]
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(5)
+    x = torch.exp2(torch.randint(-149, 128, (len(some), 40000), generator=gen, device=DEV).double())
+    x = (x * (1 + torch.rand(x.shape, generator=gen, device=DEV))).float()
+    x[:, 20000:] = torch.exp2(8 * torch.rand(len(some), 20000, generator=gen, device=DEV) - 4)
+    x[:, ::7] *= -1
+    x = x.to(dtype)
+    rep = torch.tensor(some, device=DEV)
+    tokens = torch.arange(40000, device=DEV).int().expand(len(some), -1)
+    got = adjust(x, tokens=tokens, length=torch.full((len(some),), 40000, device=DEV).int(), repetition=rep)
+    y, r = x.cpu().float(), rep.cpu()[:, None]
+    same(got, torch.where(y > 0, y / r, y * r).sub(torch.zeros(1)).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,columns,n_bias", [(3, 40000, 9000, 5), (300, 2100, 9000, 3), (2, 3000, 70001, 1024), (450, 4000, 10, 1024)])
+def test_long_histories_and_long_lists_in_place(dtype, rows, vocab, columns, n_bias):
+    a = inputs(rows, vocab, columns, dtype, n_bias, 0, seed=3)
+    a["bias_id"][:, : n_bias // 2] %= 50
+    a["tokens"][:, : columns // 2] %= 3
+    a["length"][:] = columns
+    want = formula(a["logits"], **{k: v for k, v in a.items() if k != "logits"})
+    same(adjust(**a), want)
+    adjust(**a, out=a["logits"])
+    same(a["logits"], want)
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_strides_and_starts(dtype):
     a = inputs(5, 3001, 40, dtype, 6, 0)
     want = adjust(**a)

@@ -58,6 +58,19 @@ def test_codes_are_the_formulas(dtype, rows, k, residual):
     check(int8().norm(x, w, 1e-6, residual=res), formula(x, w, 1e-6, res), k)
 
 
+@pytest.mark.parametrize("dtype,residual", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                            (torch.bfloat16, None)])
+@pytest.mark.parametrize("k", [4, 1020, 1024, 1028, 3584, 4096, 4100, 5003, 8192, 8196, 18944, 32768, 32772])
+def test_every_division_of_a_row(dtype, residual, k):
+    for rows in (444, 445):
+        x, w = stream(rows, k, dtype)
+        r = None if residual is None else stream(rows, k, residual, 1)[0]
+        want = formula(x, w, 1e-6, r)
+        n = int8().norm(x, w, 1e-6, residual=r)
+        check(n, want, k)
+        if r is not None:
+            check(int8().norm(x, w, 1e-6, residual=r, out=r), want, k)
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_strides_places_and_in_place(dtype):
     rows, k = 6, 200

@@ -67,6 +67,23 @@ def test_layouts(dtype, interleaved, tokens, heads, kv_heads, hd, rotary):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,heads,kv_heads,hd,rotary", [
+    (1, 200, 9, 64, 64), (3, 65, 0, 128, 96), (40, 71, 3, 16, 16), (2, 130, 130, 8, 4), (300, 5, 2, 1024, 512), (3000, 14, 2, 64, 64),
+    (2400, 3, 1, 66, 66), (1, 65536, 1, 16, 16)])
+def test_heads_shared_out_among_warps(dtype, interleaved, tokens, heads, kv_heads, hd, rotary):
+    q, k, position = case(tokens, heads, kv_heads, hd, dtype, seed=7)
+    f = rope().frequencies(rotary, 1e4)
+    position[tokens // 2] = -1
+    gq, gk = rope().rotate(q, position, f, k=k, interleaved=interleaved)
+    for got, x in ((gq, q), (gk, k)):
+        if x.numel():
+            near(got, want_of(x, position, f, interleaved), x, position, f)
+        assert torch.equal(got[..., rotary:], x[..., rotary:]) and torch.equal(got[tokens // 2], x[tokens // 2])
+    rope().rotate(q, position, f, k=k, interleaved=interleaved, out=q, k_out=k)
+    assert torch.equal(q, gq) and torch.equal(k, gk)
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
 def test_slices_of_a_product(dtype, interleaved):
     """q, k and v as columns of one buffer, at any start, turned in place: nothing else is touched."""
     heads, kvh, hd, tokens = 6, 2, 64, 19
