@@ -1,6 +1,7 @@
 // Attention over the paged 8-bit cache (h2c_kv8_attention; the formula is stated in include/h2cuda.h).
 //
-// Few queries: k_att_rows (kv8_rows.cuh). Many queries: k_att_prompt (kv8_prompt.cuh). Here: the kernel that joins the parts of spans, and the entry.
+// Few queries: k_att_rows (kv8_rows.cuh). Many queries: k_att_prompt (kv8_prompt.cuh). Here: the kernel that joins the parts of
+// spans, and the entry.
 #include "kv8_rows.cuh"
 
 #include <algorithm>

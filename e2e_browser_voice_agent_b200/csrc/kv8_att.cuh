@@ -1,4 +1,4 @@
-// Attention over the paged 8-bit cache: what the kernels of kv8_att.cu share.
+// Attention over the paged 8-bit cache: what the kernels of kv8_att.cu and kv8_prefix.cu share.
 #pragma once
 #include "ops.cuh"
 

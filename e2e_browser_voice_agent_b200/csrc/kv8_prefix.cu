@@ -7,6 +7,10 @@
 // the workspace, and k_prefix_join adds up what belongs to a row: the softmax over all its positions. The kernels are launched one
 // behind the other without waiting for each other's end (programmatic dependent launch), those with tensor memory first; the
 // single tokens' CTAs take the SMs that they leave.
+// Bound, 28 heads over 4 of 128, bfloat16: 256 single tokens with 16-2,000 positions of their own behind 16,385: 137 us, of which the own
+// positions alone take 65 and the rest is k_att_prompt's rate on the prefix (74 us for 28 row tiles of 257 tiles of keys, see there);
+// turns of 63 tokens of 26 requests in three groups, float16, 201 us: that rate alone. 4 single tokens behind a prefix: 9 us, two launches and the latency of a span.
+// Without the sharing, kv8.attention over tables that name the prefix reads its keys for each request: 256 times.
 #include "kv8_rows.cuh"
 
 namespace h2 {
@@ -18,7 +22,8 @@ struct Pass {
   int rows, prompt;  // whether k_att_rows, k_att_prompt take part
 };
 
-// k_att_rows of both passes in one launch: the groups, then the requests.
+// k_att_rows of both passes in one launch: the groups, then the requests (4 sessions 9.1 us, 9.8 in two launches; 8 long requests 42 and
+// 48; on one grid of both passes' largest axes, whose CTAs without work cost more than the launch, 54).
 struct BothRows {
   RowArgsOf<SharedArgs> ra[2];
   unsigned across[2], first_own;  // CTAs that a request's rows take; the requests' first CTA
@@ -92,7 +97,8 @@ __device__ __forceinline__ Owner owner_of(const Pass& p, int blocks, int t) {
   return o;
 }
 
-// The parts of row t of q, which `o` has, and head h of kv head `head`'s group. row_blocks: blocks of k_att_rows' spans. (Beyond what was computed only with starts of requests without sense.)
+// The parts of row t of q, which `o` has, and head h of kv head `head`'s group. row_blocks: blocks of k_att_rows' spans. (None where starts
+// of requests without sense would lead beyond what was computed.)
 template <int HD>
 __device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_blocks, const Owner& o, int t, int head, int h) {
   if (o.r < 0) return {nullptr, nullptr, 0, 0, 0};
@@ -339,10 +345,11 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
     auto most = [&](const WorkPlan& p) {  // spans of a row
       return std::max(p.rows ? p.splits : 0, p.prompt ? p.p_units / (p.shape.tiles * g->own.kv_heads) : 0);
     };
-    // eight warps a head where spans are many and rows few; else a warp a head, and no more CTAs than the SMs hold at a time
-    const long long all = (long long)g->own.rows * g->own.heads;
-    const bool many = most(plan.own) + most(plan.prefix) > JOIN_WARP_SPANS && all <= 148 * 8;
-    const int heads = many ? 1 : all <= JOIN_CTAS * JOIN_WARPS * JOIN_TOKENS ? std::min(JOIN_WARPS, g->own.heads) : g->own.heads;
+    // Eight warps a head where spans are many and rows few (28 heads over 4 of 128: 8 requests of up to 30,000 of their own behind 2,000
+    // 42 us, 64 by a warp a head; 2 behind 300 10.2 and 11.5); else a warp a head, and no more CTAs than the SMs hold at a time (256
+    // single tokens behind 16,385: 137 us, 140 with a CTA for each token's eight heads).
+    const bool many = most(plan.own) + most(plan.prefix) > JOIN_WARP_SPANS && (long long)g->own.rows * g->own.heads <= 148 * 8;
+    const int heads = many ? 1 : std::min(JOIN_WARPS, g->own.heads);
     const long long ctas = (long long)g->own.rows * ((g->own.heads + heads - 1) / heads);
     const int tokens = many ? 1 : (int)std::min<long long>(JOIN_TOKENS, (ctas + JOIN_CTAS - 1) / JOIN_CTAS);
     cfg.gridDim = dim3((g->own.rows + tokens - 1) / tokens, (g->own.heads + heads - 1) / heads);

@@ -1,8 +1,7 @@
 // Attention over the paged 8-bit cache for few queries (single tokens, short continuations): k_att_rows, and the division of a call's work
 // between it and k_att_prompt. Included by kv8_att.cu and kv8_prefix.cu.
 //
-// A CTA takes 8 rows (query, head of the kv head's
-// group) of one request and kv head and one span of its keys; 4 warps take blocks of 16 keys in turn, each with its own
+// A CTA takes 8 rows (query, head of the kv head's group) of one request and kv head and one span of its keys; 4 warps take blocks of 16 keys in turn, each with its own
 // running maximum, sum and output, joined at the end; up to 8 spans are joined by their cluster, more by a second kernel.
 // * Tensor cores (mma.sync m16n8k16, float16 in, float32 sums): codes are integers up to 127 and exact in float16. The
 //   16 rows of an operand tile hold 8 rows twice: a float16 term in rows 0-7 and the remainder in rows 8-15, for the
@@ -494,7 +493,9 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
     // 60,000-131,072 175, 176 and 164; 32 of 4,000-16,000 89, 81 and 75). Up to 8 are one cluster, whose join costs little: spans of 128 keys (2
     // blocks per warp) or more. More of them, for few rows over long histories, leave their parts in the workspace for a
     // second kernel: spans of 256 keys or more, below which a span's start-up costs more than it shares out
-    // (a warp's spans, where they are joined in any case: four waves of 12 warps an SM, of 128 keys or more, or of 64 where those are few)
+    // A warp's spans, where they are joined in any case: four waves of 12 warps an SM (256 single tokens of 16-2,000 keys 66 us, 72 with
+    // two waves), of 128 keys or more (32 requests behind 4,096: 30 us, 39 with 64), or of 64 where those are few (4 sessions 10.4,
+    // 12.7 with 128).
     const long long groups = (long long)g->n_req * g->kv_heads * p.tiles, want = ((parts ? 7104 : 888) + groups - 1) / groups;
     const int n_blocks = (int)((keys + RW_BLK - 1) / RW_BLK) + (g->window > 0 ? 1 : 0);
     p.cluster = !parts && groups * RW_CLUSTER <= 444 && n_blocks / 16 <= RW_CLUSTER;

@@ -1,4 +1,4 @@
-// What the stand-alone 8-bit serving operators (kv8.cu, kv8_att.cu, i8mm.cu) share: error reporting at the C entries,
+// What the stand-alone serving operators (kv8*.cu, i8mm.cu, i8norm.cu, rope.cu, logits.cu) share: error reporting at the C entries,
 // once-per-device kernel attributes, the record of expired waits, and loads and stores of activations of any type.
 #pragma once
 #include <cuda_bf16.h>
