@@ -37,12 +37,11 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_prefix_row
   att_rows<T, HD>(both.ra[own], at - rz * across, rz % n, rz / n);
 }
 
-// Where the spans of a row lie: span s has its sums at part + s * part_step and its (m, l) at ml + s * ml_step.
+// Where the spans of a row lie: span s is row `first` + s * (rows of a tile) of the sums and of the (m, l) of one of a pass's two kernels.
 struct Parts {
-  const float* part;
-  const float2* ml;
-  unsigned part_step, ml_step;
-  int used;  // 0: the row is in no request (group)
+  long long first;
+  int used;     // spans; 0: the row is in no request (group)
+  bool prompt;  // k_att_prompt's
 };
 
 // Quotients of numbers below 2^31 by multiplication: the joining kernel would spend most of its instructions on divisions else.
@@ -57,7 +56,7 @@ struct Divisor {
   __device__ __forceinline__ int rounded_up(int n) const { return quotient(n + (int)d - 1); }
 };
 
-// The request (group) that has row t of q, and k_att_prompt's spans before its own, `blocks` tiles of keys each. By whole warps.
+// The request (group) that has a row of q, and k_att_prompt's spans before its own, `blocks` tiles of keys each.
 struct Owner {
   int r, n_all;      // r = -1: no request has it
   long long before;
@@ -65,43 +64,44 @@ struct Owner {
   int tiles, spans;  // its row tiles in k_att_prompt, if it takes them, the spans of each and the tiles of keys of a span
   Divisor blocks;
 };
-__device__ __forceinline__ Owner owner_of(const Pass& p, int blocks, int t) {
+// Those of rows t0 + i, for i = i0, i0 + step and so on below nt, to to[2 * i]. By whole warps, in one pass over the requests.
+__device__ __forceinline__ void owners_of(const Pass& p, int t0, int i0, int step, int nt, Owner* to) {
   const SharedArgs& a = p.ra.a;
-  const int lane = threadIdx.x & 31;
-  Owner o{-1, 0, 0, {0, 0, 0}, 0, 1, Divisor(1)};
-  for (int base = 0; base < a.n_req; base += 32) {
+  const int lane = threadIdx.x & 31, blocks = p.prompt ? blocks_of_call(p.pa) : 1;
+  for (int i = i0 + lane * step; i < nt; i += 32 * step) to[2 * i].r = -1;
+  __syncwarp();
+  long long before = 0;
+  unsigned left = 0;  // rows to be found: bit m for i0 + m * step (JOIN_TOKENS at most)
+  for (int i = i0, m = 0; i < nt; i += step, m++) left |= 1u << m;
+  for (int base = 0; base < a.n_req && left; base += 32) {
     const int r = base + lane;
-    int n = 0, n_all = 0;
+    int n = 0, n_all = 0, tiles = 0, spans = 1;
     Request R{0, 0, 0};
     if (r < a.n_req) {
       R = request_of(a, r, &n_all);
-      if (p.prompt) n = units_of(p.pa, row_tiles_of(p.pa, R), spans_of_len(p.pa, R.len, blocks));
-    }
-    const unsigned in = __ballot_sync(0xffffffffu, t >= R.first && t - R.first < R.n_q);
-    const int l = in ? __ffs(in) - 1 : 32;  // (of several, the first)
-    o.before += __reduce_add_sync(0xffffffffu, lane < l ? n : 0);
-    if (in) {
-      o.r = base + l;
-      o.n_all = __shfl_sync(0xffffffffu, n_all, l);
-      o.R.first = __shfl_sync(0xffffffffu, R.first, l);
-      o.R.n_q = __shfl_sync(0xffffffffu, R.n_q, l);
-      o.R.len = __shfl_sync(0xffffffffu, R.len, l);
       if (p.prompt) {
-        o.tiles = row_tiles_of(p.pa, o.R);
-        o.spans = spans_of_len(p.pa, o.R.len, blocks);
-        o.blocks = Divisor(even_blocks(p.pa, o.R.len, o.spans));
+        tiles = row_tiles_of(p.pa, R);
+        spans = spans_of_len(p.pa, R.len, blocks);
+        n = units_of(p.pa, tiles, spans);
       }
-      break;
     }
+    for (unsigned todo = left; todo; todo &= todo - 1) {
+      const int m = __ffs(todo) - 1, i = i0 + m * step, t = t0 + i;
+      const unsigned in = __ballot_sync(0xffffffffu, t >= R.first && t - R.first < R.n_q);
+      if (!in) continue;
+      const int l = __ffs(in) - 1;  // (of several, the first)
+      const long long at = before + __reduce_add_sync(0xffffffffu, lane < l ? n : 0);
+      if (lane == l) to[2 * i] = {r, n_all, at, R, tiles, spans, Divisor(tiles ? even_blocks(p.pa, R.len, spans) : 1)};
+      left &= ~(1u << m);
+    }
+    before += __reduce_add_sync(0xffffffffu, n);
   }
-  return o;
 }
 
 // The parts of row t of q, which `o` has, and head h of kv head `head`'s group. row_blocks: blocks of k_att_rows' spans. (None where starts
 // of requests without sense would lead beyond what was computed.)
-template <int HD>
 __device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_blocks, const Owner& o, int t, int head, int h) {
-  if (o.r < 0) return {nullptr, nullptr, 0, 0, 0};
+  if (o.r < 0) return {0, 0, false};
   const SharedArgs& a = p.ra.a;
   const Divisor group(a.group, a.group_magic);
   const int row = (t - o.R.first) * a.group + h;
@@ -110,21 +110,25 @@ __device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_bloc
   if (o.tiles) {
     const int tile = row / PR_ROWS, n_blocks = (max(0, end_of(tile * PR_ROWS + PR_ROWS - 1)) + PR_KEYS - 1) / PR_KEYS;
     const long long unit = o.before + ((o.tiles - 1LL - tile) * a.kv_heads + head) * o.spans;
-    if (unit + o.spans > p.pa.cap) return {nullptr, nullptr, 0, 0, 0};
-    const size_t u = (size_t)unit * PR_ROWS + (row - tile * PR_ROWS);
-    return {p.pa.part + u * HD, p.pa.ml + u, PR_ROWS * HD, PR_ROWS, max(1, min(o.spans, o.blocks.rounded_up(n_blocks)))};
+    if (unit + o.spans > p.pa.cap) return {0, 0, false};
+    return {unit * PR_ROWS + (row - tile * PR_ROWS), max(1, min(o.spans, o.blocks.rounded_up(n_blocks))), true};
   }
   const int tile = row / RW_ROWS, n_blocks = (max(0, end_of(tile * RW_ROWS + RW_ROWS - 1)) + RW_BLK - 1) / RW_BLK;
-  if (tile >= p.ra.tiles) return {nullptr, nullptr, 0, 0, 0};
-  const size_t u = (((size_t)o.r * a.kv_heads + head) * p.ra.tiles + tile) * p.ra.splits * RW_ROWS + (row - tile * RW_ROWS);
-  return {p.ra.part + u * HD, p.ra.ml + u, RW_ROWS * HD, RW_ROWS, max(1, min(p.ra.splits, row_blocks.rounded_up(n_blocks)))};
+  if (tile >= p.ra.tiles) return {0, 0, false};
+  const long long unit = (((long long)o.r * a.kv_heads + head) * p.ra.tiles + tile) * p.ra.splits;
+  return {unit * RW_ROWS + (row - tile * RW_ROWS), max(1, min(p.ra.splits, row_blocks.rounded_up(n_blocks))), false};
+}
+// The same for all lanes as lane j has them.
+__device__ __forceinline__ Parts of_lane(const Parts& p, int j) {
+  return {__shfl_sync(0xffffffffu, p.first, j), __shfl_sync(0xffffffffu, p.used, j), __shfl_sync(0xffffffffu, (int)p.prompt, j) != 0};
 }
 
-// A CTA takes `heads` heads of `tokens` (at most JOIN_TOKENS) rows of q, NW warps (1, or JOIN_WARPS for one row) a head. What it looks up
-// needs nothing of the passes and goes on while they end; the host makes no more CTAs than the SMs hold where it can.
-constexpr int JOIN_TOKENS = JOIN_WARPS / 2, JOIN_CTAS = 148 * 3;
+// A CTA takes `heads` heads (at most JOIN_WARPS) of `tokens` (at most JOIN_TOKENS) rows of q, NW warps (1, or JOIN_WARPS for one row) a
+// head. What it looks up, whose row and request are shared by all warps and whose places by a warp's lanes, needs nothing of the
+// passes and goes on while they end; the host makes no more CTAs than the SMs hold where it can.
+constexpr int JOIN_TOKENS = 32, JOIN_PER_SM = 3, JOIN_CTAS = 148 * JOIN_PER_SM;
 template <class T, int HD, int NW>
-__global__ void __launch_bounds__(32 * JOIN_WARPS, 3) k_prefix_join(const Pass prefix, const Pass own, int tokens, int heads) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(const Pass prefix, const Pass own, int tokens, int heads) {
   constexpr int V = HD / 32, UN = 6;
   __shared__ float acc[NW][HD];
   __shared__ float2 acc_ml[NW];
@@ -132,21 +136,29 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, 3) k_prefix_join(const Pass p
   Owner(*owner)[2] = reinterpret_cast<Owner(*)[2]>(owner_s);
   const AttArgs& a = own.ra.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = NW > 1 ? warp : 0, t0 = blockIdx.x * tokens;
-  const int h0 = blockIdx.y * heads, nh = min(heads, a.heads - h0), n = min(tokens, a.rows - t0) * nh;
-  if (warp < 2 * tokens) {  // two warps a token: its prefix's group, its request
-    const Pass& p = warp & 1 ? own : prefix;
-    const int blocks = p.prompt ? blocks_of_call(p.pa) : 1;
-    const Owner o = owner_of(p, blocks, t0 + (warp >> 1));
-    if (lane == 0) owner[warp >> 1][warp & 1] = o;
-  }
+  const int h0 = blockIdx.y * heads, nh = min(heads, a.heads - h0), nt = min(tokens, a.rows - t0), n = nt * nh;
+  // (every second warp the rows' requests, the others their prefixes' groups)
+  owners_of(warp & 1 ? own : prefix, t0, warp >> 1, JOIN_WARPS / 2, nt, &owner[0][warp & 1]);
   __syncthreads();
   const Divisor by_heads(nh), by_group(a.group, a.group_magic), prefix_row_blocks(max(1, prefix.ra.blocks)), own_row_blocks(max(1, own.ra.blocks));
+  // lane j: of the warp's j-th row and head
+  Parts o_of{0, 0, false}, p_of{0, 0, false};
+  const int mine = NW > 1 ? lane : warp + lane * JOIN_WARPS;
+  if (mine < n) {
+    const int k_t = by_heads.quotient(mine), t = t0 + k_t, hq = h0 + mine - k_t * nh, head = by_group.quotient(hq), h = hq - head * a.group;
+    o_of = parts_of(own, own_row_blocks, owner[k_t][1], t, head, h);
+    p_of = parts_of(prefix, prefix_row_blocks, owner[k_t][0], t, head, h);
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int i = NW > 1 ? 0 : warp; i < n; i += NW > 1 ? 1 : JOIN_WARPS) {
-    const int k_t = by_heads.quotient(i), t = t0 + k_t, hq = h0 + i - k_t * nh, head = by_group.quotient(hq), h = hq - head * a.group;
-    const Parts o = parts_of<HD>(own, own_row_blocks, owner[k_t][1], t, head, h);
+  for (int j = 0, i = NW > 1 ? 0 : warp; i < n; j++, i += NW > 1 ? 1 : JOIN_WARPS) {
+    const Parts o = of_lane(o_of, j), p = of_lane(p_of, j);
     if (o.used == 0) continue;  // (a row of no request is not touched)
-    const Parts p = parts_of<HD>(prefix, prefix_row_blocks, owner[k_t][0], t, head, h);
+    const int k_t = by_heads.quotient(i), t = t0 + k_t, hq = h0 + i - k_t * nh;
+    const float* o_part = (o.prompt ? own.pa.part : own.ra.part) + o.first * HD + V * lane;
+    const float2* o_ml = (o.prompt ? own.pa.ml : own.ra.ml) + o.first;
+    const float* p_part = (p.prompt ? prefix.pa.part : prefix.ra.part) + p.first * HD + V * lane;
+    const float2* p_ml = (p.prompt ? prefix.pa.ml : prefix.ra.ml) + p.first;
+    const unsigned o_step = o.prompt ? PR_ROWS : RW_ROWS, p_step = p.prompt ? PR_ROWS : RW_ROWS;
     const int all = p.used + o.used;
     // UN spans at a time, everything of them on its way at once; the sums are relative to the largest maximum so far
     float m = -INFINITY, v[V], l = 0.f;
@@ -163,9 +175,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, 3) k_prefix_join(const Pass p
         for (int j = 0; j < V; j++) x[k][j] = 0.f;
         if (s < all) {
           const bool shared = s < p.used;
-          const unsigned n = shared ? s : s - p.used;
-          const float* src = (shared ? p.part : o.part) + (size_t)n * (shared ? p.part_step : o.part_step) + V * lane;
-          ml[k] = (shared ? p.ml : o.ml)[(size_t)n * (shared ? p.ml_step : o.ml_step)];
+          const size_t at = shared ? (size_t)s * p_step : (size_t)(s - p.used) * o_step;
+          const float* src = (shared ? p_part : o_part) + at * HD;
+          ml[k] = (shared ? p_ml : o_ml)[at];
           if (V == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(src);
           else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(src);
         }
