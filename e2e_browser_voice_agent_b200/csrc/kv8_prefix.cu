@@ -7,9 +7,11 @@
 // the workspace, and k_prefix_join adds up what belongs to a row: the softmax over all its positions. The kernels are launched one
 // behind the other without waiting for each other's end (programmatic dependent launch), those with tensor memory first; the
 // single tokens' CTAs take the SMs that they leave.
-// Bound, 28 heads over 4 of 128, bfloat16: 256 single tokens with 16-2,000 positions of their own behind 16,385: 137 us, of which the own
-// positions alone take 65 and the rest is k_att_prompt's rate on the prefix (74 us for 28 row tiles of 257 tiles of keys, see there);
-// turns of 63 tokens of 26 requests in three groups, float16, 201 us: that rate alone. 4 single tokens behind a prefix: 9 us, two launches and the latency of a span.
+// Bound, 28 heads over 4 of 128, bfloat16: 256 single tokens with 16-2,000 positions of their own behind 16,385: 135 us, of which 86 are
+// k_att_prompt's rate on the prefix (28 row tiles of 257 tiles of keys, see there); the own positions would take 61 alone, and 42 behind
+// the prefix, as their first CTAs fill the SMs that it leaves. Turns of 63 tokens of 26 requests in three groups, float16, 193 us: 168
+// that rate with the starts of some 600 CTAs of 8-17 tiles of keys, 25 the join of 70 MB (2.8 TB/s). 4 single tokens behind a prefix: 8.6
+// us, two launches and the latency of a span.
 // Without the sharing, kv8.attention over tables that name the prefix reads its keys for each request: 256 times.
 #include "kv8_rows.cuh"
 
@@ -23,7 +25,7 @@ struct Pass {
 };
 
 // k_att_rows of both passes in one launch: the groups, then the requests (4 sessions 9.1 us, 9.8 in two launches; 8 long requests 42 and
-// 48; on one grid of both passes' largest axes, whose CTAs without work cost more than the launch, 54).
+// 48; with a grid of both passes' largest axes, whose CTAs without work cost more than the launch, 54).
 struct BothRows {
   RowArgsOf<SharedArgs> ra[2];
   unsigned across[2], first_own;  // CTAs that a request's rows take; the requests' first CTA
@@ -358,8 +360,8 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
       return std::max(p.rows ? p.splits : 0, p.prompt ? p.p_units / (p.shape.tiles * g->own.kv_heads) : 0);
     };
     // Eight warps a head where spans are many and rows few (28 heads over 4 of 128: 8 requests of up to 30,000 of their own behind 2,000
-    // 42 us, 64 by a warp a head; 2 behind 300 10.2 and 11.5); else a warp a head, and no more CTAs than the SMs hold at a time (256
-    // single tokens behind 16,385: 137 us, 140 with a CTA for each token's eight heads).
+    // 42 us, 64 by a warp a head; 2 behind 300 10.2 and 11.5); else a warp a head, and no more CTAs than the SMs hold at a time, so that
+    // all look up their places while the passes end (256 single tokens behind 16,385: 137 us, 140 with a CTA for each token's eight heads).
     const bool many = most(plan.own) + most(plan.prefix) > JOIN_WARP_SPANS && (long long)g->own.rows * g->own.heads <= 148 * 8;
     const int heads = many ? 1 : std::min(JOIN_WARPS, g->own.heads);
     const long long ctas = (long long)g->own.rows * ((g->own.heads + heads - 1) / heads);

@@ -493,10 +493,10 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
     // 60,000-131,072 175, 176 and 164; 32 of 4,000-16,000 89, 81 and 75). Up to 8 are one cluster, whose join costs little: spans of 128 keys (2
     // blocks per warp) or more. More of them, for few rows over long histories, leave their parts in the workspace for a
     // second kernel: spans of 256 keys or more, below which a span's start-up costs more than it shares out
-    // A warp's spans, where they are joined in any case: four waves of 12 warps an SM (256 single tokens of 16-2,000 keys 66 us, 72 with
-    // two waves), of 128 keys or more (32 requests behind 4,096: 30 us, 39 with 64), or of 64 where those are few (4 sessions 10.4,
-    // 12.7 with 128).
-    const long long groups = (long long)g->n_req * g->kv_heads * p.tiles, want = ((parts ? 7104 : 888) + groups - 1) / groups;
+    // A warp's spans, where they are joined in any case: three waves of 12 warps an SM (256 single tokens of 16-2,000 keys 61 us, 64 with four
+    // and 68 with eight; with two 9% more than with four), of 128 keys or more (32 requests behind 4,096: 27 us, 38 with 64), or of 64
+    // where those are few (4 sessions 10.4, 12.7 with 128).
+    const long long groups = (long long)g->n_req * g->kv_heads * p.tiles, want = ((parts ? 5328 : 888) + groups - 1) / groups;
     const int n_blocks = (int)((keys + RW_BLK - 1) / RW_BLK) + (g->window > 0 ? 1 : 0);
     p.cluster = !parts && groups * RW_CLUSTER <= 444 && n_blocks / 16 <= RW_CLUSTER;
     const int least = !parts ? 16 : groups * (n_blocks / 4) <= 888 && n_blocks <= 256 ? 4 : 8;
