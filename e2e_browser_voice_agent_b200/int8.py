@@ -128,7 +128,7 @@ def norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Opt
             raise TypeError(f"residual: {x.dtype} or float32 is wanted, not {residual.dtype}")
         r_type = _TYPES[residual.dtype]
         if out is None:
-            out = residual.new_empty((rows, k))
+            out = residual.new_empty(rows, k)
             po, o_row = out.data_ptr(), k
         else:
             if out.shape != x.shape:
@@ -139,8 +139,8 @@ def norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Opt
     elif out is not None:
         raise ValueError("out: there is no residual, so no sum")
     k_pad = (k + 15) // 16 * 16
-    q = x.new_empty((rows, k_pad), dtype=torch.int8)
-    scale = weight.new_empty((rows,), dtype=torch.float32)
+    q = x.new_empty(rows, k_pad, dtype=torch.int8)
+    scale = weight.new_empty(rows, dtype=torch.float32)
     _call(index, _lib.load().h2c_i8_norm, _TYPES[x.dtype], px, x.stride(0), r_type, pr, r_row, po, o_row,
           _want("weight", weight, torch.float32, index, (k,)), eps, rows, k, q.data_ptr(), k_pad, scale.data_ptr())
     return Norm(q, scale, out)
@@ -159,7 +159,7 @@ def values(codes: torch.Tensor, scale: torch.Tensor, k: Optional[int] = None, dt
     k = codes.shape[1] if k is None else k
     if not 0 < k <= codes.shape[1]:
         raise ValueError(f"k: 1 to {codes.shape[1]} is wanted, not {k}")
-    y = codes.new_empty((rows, k), dtype=dtype)
+    y = codes.new_empty(rows, k, dtype=dtype)
     _call(index, _lib.load().h2c_i8_values, pq, codes.stride(0), _want("scale", scale, torch.float32, index, (rows,)), rows, k,
           _TYPES[dtype], y.data_ptr())
     return y

@@ -195,13 +195,13 @@ def _attention_args(q, kv, kv_scale, block_table, q_start, kv_len, max_q, max_kv
     _int32("heads, max_q, max_kv, window, columns", heads, max_q, max_kv, window, block_table.shape[1])
     i32 = torch.int32
     if out is None:
-        out = q.new_empty((rows, heads, hd))
+        out = q.new_empty(rows, heads, hd)
         po, o_row, o_head = out.data_ptr(), heads * hd, hd
     else:
         po, to, o_row, o_head = _rows("out", out, index, heads, hd)
         if to != tq or out.shape[0] != rows:
             raise ValueError("out must have q's rows and type")
-    lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
+    lse = q.new_empty(rows, heads, dtype=torch.float32) if return_lse else None
     a = _lib.Kv8AttentionArgs(pq, q_row, q_head, po, o_row, o_head, lse.data_ptr() if return_lse else None, pkv, ps, n_pages,
                               page, kvh, hd, heads, tq, _want("block_table", block_table, i32, index), block_table.shape[1], n,
                               _want("q_start", q_start, i32, index, (n + 1,)), _want("kv_len", kv_len, i32, index, (n,)), rows,
@@ -221,7 +221,7 @@ def attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, block_t
     L = _lib.load()
     need = L.h2c_kv8_attention_workspace(a)
     if need:
-        work = kv.new_empty((need,), dtype=torch.uint8)
+        work = kv.new_empty(need, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = work.data_ptr(), need
     _call(index, L.h2c_kv8_attention, a)
     return (out, lse) if return_lse else out
@@ -245,7 +245,7 @@ def prefix_attention(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor, 
     L = _lib.load()
     need = L.h2c_kv8_prefix_attention_workspace(a)
     if need:
-        work = kv.new_empty((need,), dtype=torch.uint8)
+        work = kv.new_empty(need, dtype=torch.uint8)
         a.own.workspace, a.own.workspace_bytes = work.data_ptr(), need
     _call(index, L.h2c_kv8_prefix_attention, a)
     return (out, lse) if return_lse else out

@@ -50,7 +50,7 @@ def adjust(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, length: 
     rows, vocab = logits.shape
     p_in, in_row = _lines("logits", logits, logits.dtype, index, rows)
     if out is None:
-        out = logits.new_empty((rows, vocab))
+        out = logits.new_empty(rows, vocab)
         p_out, out_row = out.data_ptr(), vocab
     else:
         p_out, out_row = _lines("out", out, logits.dtype, index, rows, vocab)

@@ -91,7 +91,7 @@ def rotate(q: torch.Tensor, position: torch.Tensor, frequency: torch.Tensor, k: 
         if k_tokens != tokens or k_dim != head_dim:
             raise ValueError(f"k: [{tokens}, heads, {head_dim}] is wanted, not {tuple(k.shape)}")
         if k_out is None:
-            k_out = k.new_empty((tokens, k_heads, head_dim))
+            k_out = k.new_empty(tokens, k_heads, head_dim)
             pko, ko_row, ko_head = k_out.data_ptr(), k_heads * head_dim, head_dim
         else:
             if k_out.shape != k.shape:
@@ -100,7 +100,7 @@ def rotate(q: torch.Tensor, position: torch.Tensor, frequency: torch.Tensor, k: 
     elif k_out is not None:
         raise ValueError("k_out: there is no k")
     if out is None:
-        out = q.new_empty((tokens, heads, head_dim))
+        out = q.new_empty(tokens, heads, head_dim)
         po, o_row, o_head = out.data_ptr(), heads * head_dim, head_dim
     else:
         if out.shape != shape:
