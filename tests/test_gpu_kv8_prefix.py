@@ -173,6 +173,26 @@ def test_strides_in_place_and_rows_of_nobody(dtype, n, p, n_q):
         assert float((got[~last].double() - want[~last].double()).abs().max()) <= 2.0**-7 * float(want.double().abs().max())
 
 
+@pytest.mark.parametrize("n,p,n_q", [(5, 900, 1), (4, 1500, 70)])
+def test_pages_and_rows_more_than_32_bits_apart(n, p, n_q):
+    """The same pages at the far end of a large cache, the same rows far apart: the same bits."""
+    kv_len = [n_q + 50 * i for i in range(n)]
+    q, kv, sc, ptable, table, q_start = inputs(torch.bfloat16, 128, 28, 4, 128, [p], kv_len, [n_q] * n)
+    want, want_lse = call(q, kv, sc, ptable, [p], [0, n], table, q_start, kv_len)
+    off = 2**32 // kv[0].numel()
+    big = torch.empty((off + len(kv),) + kv.shape[1:], dtype=torch.int8, device=DEV)
+    far_sc = torch.full((off + len(kv),) + sc.shape[1:], math.nan, device=DEV)
+    big[off:], far_sc[off:] = kv, sc
+    shift = lambda t: torch.where(t >= 0, t + off, t)
+    rest = [shift(ptable), [p], [0, n], shift(table), q_start, kv_len]
+    got, lse = call(q, big, far_sc, *rest)
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    row = 2**31 // (len(q) - 1) + 64
+    far = torch.empty(row * len(q), dtype=torch.bfloat16, device=DEV).as_strided(q.shape, (row, 128, 1))
+    far.copy_(q)
+    call(far, big, far_sc, *rest, out=far)
+    assert torch.equal(far, want)
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_the_same_as_attention_over_tables_that_name_the_prefix(dtype):
     """A prefix that ends with its page can also stand in every request's table. Two computations of the tolerance each."""

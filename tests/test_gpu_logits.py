@@ -151,6 +151,19 @@ def test_strides_and_starts(dtype):
     same(adjust(**one), formula(a["logits"], **{k: v for k, v in one.items() if k != "logits"}))
 
 
+def test_rows_more_than_32_bits_apart():
+    far = 2**31 + 64
+    a = inputs(2, 5000, 40, torch.bfloat16, 6, 0)
+    want = adjust(**a)
+    buf = torch.empty(far + 10048, dtype=torch.bfloat16, device=DEV)
+    for at in (0, 1):
+        x, y = buf[at:].as_strided((2, 5000), (far, 1)), buf[5024:].as_strided((2, 5000), (far, 1))
+        x.copy_(a["logits"])
+        adjust(**{**a, "logits": x}, out=y)
+        same(y, want)
+        adjust(**{**a, "logits": x}, out=x)
+        same(x, want)
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_lengths_and_tokens_without_sense(dtype):
     a = inputs(6, 400, 30, dtype)

@@ -110,6 +110,20 @@ def test_strides_places_and_in_place(dtype):
     check(int8().norm(long, w, 1e-6, residual=r, out=r), want, 40000)   # rows longer than the registers hold, in place
 
 
+@pytest.mark.parametrize("k", [3584, 3585])
+def test_rows_more_than_32_bits_apart(k):
+    far = 2**31 + 64
+    x, w = stream(2, k, torch.bfloat16)
+    r, _ = stream(2, k, torch.bfloat16, 1)
+    buf = torch.empty(far + 3 * k + 64, dtype=torch.bfloat16, device=DEV)
+    a, b, c = (buf[at:].as_strided((2, k), (far, 1)) for at in (0, k + 15 & ~15, 2 * k + 31 & ~15))
+    a.copy_(x)
+    b.copy_(r)
+    want = formula(x, w, 1e-6, r)
+    check(int8().norm(a, w, 1e-6, residual=b, out=c), want, k)
+    check(int8().norm(a, w, 1e-6, residual=b, out=b), want, k)
+    assert torch.equal(a, x) and torch.equal(b, want[2]) and torch.equal(c, want[2])
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_extreme_rows(dtype):
     big = torch.finfo(dtype).max

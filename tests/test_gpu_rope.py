@@ -109,6 +109,20 @@ def test_slices_of_a_product(dtype, interleaved):
         assert torch.equal(got, wq)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_tokens_and_heads_more_than_32_bits_apart(interleaved):
+    far = 2**31 + 64
+    q, _, position = case(2, 3, 1, 64, torch.bfloat16)
+    f = rope().frequencies(64)
+    want = rope().rotate(q, position, f, interleaved=interleaved)
+    buf = torch.empty(2 * far + 1024, dtype=torch.bfloat16, device=DEV)
+    for shape, strides in (((2, 3, 64), (far, 64, 1)), ((2, 3, 64), (64, far, 1))):
+        x = buf.as_strided(shape, strides)
+        x.copy_(q)
+        assert torch.equal(rope().rotate(x, position, f, interleaved=interleaved), want)
+        rope().rotate(x, position, f, interleaved=interleaved, out=x)
+        assert torch.equal(x, want)
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_far_positions(dtype):
     q, k, _ = case(6, 2, 1, 128, dtype)
