@@ -108,7 +108,10 @@ __device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_bloc
   const Divisor group(a.group, a.group_magic);
   const int row = (t - o.R.first) * a.group + h;
   // the keys before the end of what the tile's last row sees
-  auto end_of = [&](int last_row) { return min(position_of(a, o.R, o.n_all, group.quotient(min(last_row, o.R.n_q * a.group - 1))) + 1, o.R.len); };
+  auto end_of = [&](int last_row) {
+    const int last = group.quotient(min(last_row, o.R.n_q * a.group - 1));
+    return min(position_of(a, o.R, o.n_all, last) + 1, o.R.len);
+  };
   if (o.tiles) {
     const int tile = row / PR_ROWS, n_blocks = (max(0, end_of(tile * PR_ROWS + PR_ROWS - 1)) + PR_KEYS - 1) / PR_KEYS;
     const long long unit = o.before + ((o.tiles - 1LL - tile) * a.kv_heads + head) * o.spans;
@@ -142,7 +145,8 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
   // (every second warp the rows' requests, the others their prefixes' groups)
   owners_of(warp & 1 ? own : prefix, t0, warp >> 1, JOIN_WARPS / 2, nt, &owner[0][warp & 1]);
   __syncthreads();
-  const Divisor by_heads(nh), by_group(a.group, a.group_magic), prefix_row_blocks(max(1, prefix.ra.blocks)), own_row_blocks(max(1, own.ra.blocks));
+  const Divisor by_heads(nh), by_group(a.group, a.group_magic);
+  const Divisor prefix_row_blocks(max(1, prefix.ra.blocks)), own_row_blocks(max(1, own.ra.blocks));
   // lane j: of the warp's j-th row and head
   Parts o_of{0, 0, false}, p_of{0, 0, false};
   const int mine = NW > 1 ? lane : warp + lane * JOIN_WARPS;
@@ -270,7 +274,8 @@ PrefixPlan plan_prefix(const h2c_kv8_prefix_args* g) {
 }
 // Whether a pass's counts fit their types: CTAs and rows of the workspace.
 bool fits(const WorkPlan& p, long long kv_heads, long long requests) {
-  return (long long)p.splits * p.tiles * RW_ROWS * kv_heads <= INT_MAX && (p.tiles * kv_heads / RW_WARPS + 1) * requests * p.splits <= INT_MAX / 2 &&
+  return (long long)p.splits * p.tiles * RW_ROWS * kv_heads <= INT_MAX &&
+         (p.tiles * kv_heads / RW_WARPS + 1) * requests * p.splits <= INT_MAX / 2 &&
          spans_at_most((long long)p.shape.tiles * kv_heads, p.p_keys) * PR_ROWS <= INT_MAX;
 }
 

@@ -1,8 +1,9 @@
 // Attention over the paged 8-bit cache for few queries (single tokens, short continuations): k_att_rows, and the division of a call's work
 // between it and k_att_prompt. Included by kv8_att.cu and kv8_prefix.cu.
 //
-// A CTA takes 8 rows (query, head of the kv head's group) of one request and kv head and one span of its keys; 4 warps take blocks of 16 keys in turn, each with its own
-// running maximum, sum and output, joined at the end; up to 8 spans are joined by their cluster, more by a second kernel.
+// A CTA takes 8 rows (query, head of the kv head's group) of one request and kv head and one span of its keys; 4 warps take blocks
+// of 16 keys in turn, each with its own running maximum, sum and output, joined at the end; up to 8 spans are joined by their
+// cluster, more by a second kernel. (Behind shared prefixes each warp takes a span of its own.)
 // * Tensor cores (mma.sync m16n8k16, float16 in, float32 sums): codes are integers up to 127 and exact in float16. The
 //   16 rows of an operand tile hold 8 rows twice: a float16 term in rows 0-7 and the remainder in rows 8-15, for the
 //   queries (scaled by a power of two per row) and for the softmax weights, so the products carry 22 bits, whatever the
@@ -85,8 +86,8 @@ __device__ __forceinline__ void att_rows(const RowArgsOf<A>& ra, const int x, co
   const A& a = ra.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   // Where parts are left to a joining kernel in any case, a warp takes a span for itself: no warp waits for another, and four times as
-  // many spans are on their way (256 single tokens of 16-2,000 keys, 28 heads over 4 of 128). Spans are the grid's slowest axis and the
-  // last go first: only long requests have them, and the CTAs without one are over before the work begins.
+  // many spans are on their way. Spans are the grid's slowest axis and the last go first: only long requests have them, and the CTAs
+  // without one are over before the work begins.
   constexpr bool ALONE = PARTS_ONLY<A>;
   const int split = ALONE ? ra.splits - 1 - z : x % ra.splits, th = ALONE ? x * RW_WARPS + warp : x / ra.splits;
   const int head = th % a.kv_heads, tile = th / a.kv_heads;

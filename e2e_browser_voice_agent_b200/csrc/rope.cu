@@ -118,8 +118,9 @@ __device__ __forceinline__ void turn_unit(Piece<T, N>& p, Piece<T, W>& q, const 
 
 // One unit of work is W neighbouring values and, in the half layout, the W that are their partners; of the part that is not turned, W
 // values: W is what 16 bytes hold, or 1 where a pointer, a stride or a head's parts are not multiples of 16 bytes (2,050 tokens of
-// 36 heads of 128: 9.3 us, and 31 with 62 of the 128 values turned, which have to go one by one). FEW: a head has at most 32 units, so a lane has one of them, of several heads at a time, and keeps its cosines and sines; else
-// the lanes go through a head's units together.
+// 36 heads of 128: 9.3 us, and 31 with 62 of the 128 values turned, which have to go one by one). FEW: a head has at most 32 units, so
+// a lane has one of them, of several heads at a time, and keeps its cosines and sines; else the lanes go through a head's units
+// together.
 template <class T, int W, bool INTER, bool FEW>
 __global__ void __launch_bounds__(32 * ROPE_WARPS, 3) k_rope(const RopeArgs a) {
   extern __shared__ __align__(16) float2 turn[];  // [warp][pair]: cosine and sine, times the magnitude
