@@ -9,8 +9,8 @@
 // single tokens' CTAs take the SMs that they leave.
 // Bound, 28 heads over 4 of 128, bfloat16: 256 single tokens with 16-2,000 positions of their own behind 16,385: 135 us, of which 86 are
 // k_att_prompt's rate on the prefix (28 row tiles of 257 tiles of keys, see there); the own positions would take 61 alone, and 42 behind
-// the prefix, as their first CTAs fill the SMs that it leaves. Turns of 63 tokens of 26 requests in three groups, float16, 193 us: 168
-// that rate with the starts of some 600 CTAs of 8-17 tiles of keys, 25 the join of 70 MB (2.8 TB/s). 4 single tokens behind a prefix: 8.6
+// the prefix, as their first CTAs fill the SMs that it leaves. Turns of 63 tokens of 26 requests in three groups, float16, 184 us: 160
+// that rate with the starts of some 540 CTAs of up to 22 tiles of keys, 24 the join of 65 MB (2.7 TB/s). 4 single tokens behind a prefix: 8.6
 // us, two launches and the latency of a span.
 // Without the sharing, kv8.attention over tables that name the prefix reads its keys for each request: 256 times.
 #include "kv8_rows.cuh"

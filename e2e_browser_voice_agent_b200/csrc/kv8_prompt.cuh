@@ -181,10 +181,11 @@ __device__ __forceinline__ Work work_of(const PromptArgsOf<AttArgs>& pa) {
 // `blocks` tiles of keys, as many as its request's length needs. With u tiles of keys an SM in all, spans of B cost about
 // u + u / B c + B / 2, where c = SPAN_COST tiles is what a span's start and end take and B / 2 what the last ones leave idle: least at
 // B = sqrt(2 u c). (One request: what fills the SMs once, known to the host.) Row tiles for SPAN_TILES CTAs and more are not cut.
-// Turns of three groups, c = 3, 5, 10 and 20: 206, 201, 200 and 210 us. Spans of SPAN_LEAST tiles or more: 44 single tokens in two groups
+// Turns of 63 tokens of 26 requests in three groups behind 814-4,099, 28 heads over 4 of 128, c = 3, 5, 8 and 10: float16 195, 193, 184
+// and 191 us, bfloat16 176, 167, 159 and 157; behind 4,000-16,000 553, 528, 499 and 520. Spans of SPAN_LEAST tiles or more: 44 single tokens in two groups
 // 48 us, 57 with 16. One request's spans for 148 CTAs: 256 single tokens behind 16,385 positions 138 us, for 112 and 84, which leave
 // SMs to the single tokens, 151 and 175.
-constexpr int SPAN_COST = 5, SPAN_LEAST = 8, SPAN_TILES = 148 * 4;
+constexpr int SPAN_COST = 8, SPAN_LEAST = 8, SPAN_TILES = 148 * 4;
 __host__ __device__ inline long long spans_at_most(long long ctas, long long key_tiles) {  // of `ctas` uncut row tiles
   const double cut = (double)(ctas < SPAN_TILES ? ctas : SPAN_TILES) * (double)key_tiles;
   return ctas + (long long)sqrt(cut * 148 / (2 * SPAN_COST)) + 2;
