@@ -7,11 +7,11 @@
 // the workspace, and k_prefix_join adds up what belongs to a row: the softmax over all its positions. The kernels are launched one
 // behind the other without waiting for each other's end (programmatic dependent launch), those with tensor memory first; the
 // single tokens' CTAs take the SMs that they leave.
-// Bound, 28 heads over 4 of 128, bfloat16: 256 single tokens with 16-2,000 positions of their own behind 16,385: 135 us, of which 86 are
+// Bound, 28 heads over 4 of 128, bfloat16: 256 single tokens with 16-2,000 positions of their own behind 16,385: 134 us, of which 86 are
 // k_att_prompt's rate on the prefix (28 row tiles of 257 tiles of keys, see there); the own positions would take 61 alone, and 42 behind
-// the prefix, as their first CTAs fill the SMs that it leaves. Turns of 63 tokens of 26 requests in three groups, float16, 184 us: 160
-// that rate with the starts of some 540 CTAs of up to 22 tiles of keys, 24 the join of 65 MB (2.7 TB/s). 4 single tokens behind a prefix: 8.6
-// us, two launches and the latency of a span.
+// the prefix, as their first CTAs fill the SMs that it leaves. Turns of 63 tokens of 26 requests in three groups, float16, 180 us: 160
+// that rate with the starts of some 540 CTAs of up to 22 tiles of keys, 20 the join of 65 MB (3.3 TB/s). 4 single tokens behind a
+// prefix: 8.6 us, two launches and the latency of a span.
 // Without the sharing, kv8.attention over tables that name the prefix reads its keys for each request: 256 times.
 #include "kv8_rows.cuh"
 
@@ -128,19 +128,19 @@ __device__ __forceinline__ Parts of_lane(const Parts& p, int j) {
   return {__shfl_sync(0xffffffffu, p.first, j), __shfl_sync(0xffffffffu, p.used, j), __shfl_sync(0xffffffffu, (int)p.prompt, j) != 0};
 }
 
-// A CTA takes `heads` heads (at most JOIN_WARPS) of `tokens` (at most JOIN_TOKENS) rows of q, NW warps (1, or JOIN_WARPS for one row) a
-// head. What it looks up, whose row and request are shared by all warps and whose places by a warp's lanes, needs nothing of the
-// passes and goes on while they end; the host makes no more CTAs than the SMs hold where it can.
+// A CTA takes `heads` heads (at most JOIN_WARPS) of `tokens` (at most JOIN_TOKENS) rows of q, L lanes (or NW = JOIN_WARPS warps, for one
+// row) a head. What it looks up, whose row and request are shared by all warps and whose places by a warp's lanes, needs nothing of
+// the passes and goes on while they end; the host makes no more CTAs than the SMs hold where it can.
 constexpr int JOIN_TOKENS = 32, JOIN_PER_SM = 3, JOIN_CTAS = 148 * JOIN_PER_SM;
-template <class T, int HD, int NW>
+template <class T, int HD, int NW, int L>
 __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(const Pass prefix, const Pass own, int tokens, int heads) {
-  constexpr int V = HD / 32, UN = 6;
+  constexpr int V = HD / L, UN = V > 4 ? 4 : 6;
   __shared__ float acc[NW][HD];
   __shared__ float2 acc_ml[NW];
   __shared__ __align__(16) uint8_t owner_s[JOIN_TOKENS * 2 * sizeof(Owner)];
   Owner(*owner)[2] = reinterpret_cast<Owner(*)[2]>(owner_s);
   const AttArgs& a = own.ra.a;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = NW > 1 ? warp : 0, t0 = blockIdx.x * tokens;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = NW > 1 ? warp : 0, t0 = blockIdx.x * tokens, ln = lane % L;
   const int h0 = blockIdx.y * heads, nh = min(heads, a.heads - h0), nt = min(tokens, a.rows - t0), n = nt * nh;
   // (every second warp the rows' requests, the others their prefixes' groups)
   owners_of(warp & 1 ? own : prefix, t0, warp >> 1, JOIN_WARPS / 2, nt, &owner[0][warp & 1]);
@@ -156,13 +156,14 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
     p_of = parts_of(prefix, prefix_row_blocks, owner[k_t][0], t, head, h);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int j = 0, i = NW > 1 ? 0 : warp; i < n; j++, i += NW > 1 ? 1 : JOIN_WARPS) {
+  for (int j0 = 0; (NW > 1 ? j0 : warp + j0 * JOIN_WARPS) < n; j0 += 32 / L) {
+    const int j = j0 + lane / L, i = NW > 1 ? j : warp + j * JOIN_WARPS;
     const Parts o = of_lane(o_of, j), p = of_lane(p_of, j);
-    if (o.used == 0) continue;  // (a row of no request is not touched)
+    if (o.used == 0) continue;  // (a row of no request is not touched; nor is what lies past the warp's last)
     const int k_t = by_heads.quotient(i), t = t0 + k_t, hq = h0 + i - k_t * nh;
-    const float* o_part = (o.prompt ? own.pa.part : own.ra.part) + o.first * HD + V * lane;
+    const float* o_part = (o.prompt ? own.pa.part : own.ra.part) + o.first * HD + V * ln;
     const float2* o_ml = (o.prompt ? own.pa.ml : own.ra.ml) + o.first;
-    const float* p_part = (p.prompt ? prefix.pa.part : prefix.ra.part) + p.first * HD + V * lane;
+    const float* p_part = (p.prompt ? prefix.pa.part : prefix.ra.part) + p.first * HD + V * ln;
     const float2* p_ml = (p.prompt ? prefix.pa.ml : prefix.ra.ml) + p.first;
     const unsigned o_step = o.prompt ? PR_ROWS : RW_ROWS, p_step = p.prompt ? PR_ROWS : RW_ROWS;
     const int all = p.used + o.used;
@@ -184,8 +185,12 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
           const size_t at = shared ? (size_t)s * p_step : (size_t)(s - p.used) * o_step;
           const float* src = (shared ? p_part : o_part) + at * HD;
           ml[k] = (shared ? p_ml : o_ml)[at];
-          if (V == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(src);
-          else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(src);
+          if (V == 2) {
+            *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(src);
+          } else {
+#pragma unroll
+            for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(x[k] + j) = *reinterpret_cast<const float4*>(src + j);
+          }
         }
       }
       float top = m;
@@ -206,7 +211,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
     }
     if (NW > 1) {
 #pragma unroll
-      for (int k = 0; k < V; k++) acc[w][V * lane + k] = v[k];
+      for (int k = 0; k < V; k++) acc[w][V * ln + k] = v[k];
       if (lane == 0) acc_ml[w] = make_float2(m, l);
       __syncthreads();
       if (w == 0) {
@@ -218,23 +223,24 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
           const float f = acc_ml[n].x == -INFINITY ? 0.f : exp2_fast(acc_ml[n].x - m);
           l = fmaf(f, acc_ml[n].y, l);
 #pragma unroll
-          for (int k = 0; k < V; k++) v[k] = fmaf(f, acc[n][V * lane + k], v[k]);
+          for (int k = 0; k < V; k++) v[k] = fmaf(f, acc[n][V * ln + k], v[k]);
         }
       }
       __syncthreads();
     }
     if (w == 0) {
       const float inv = l != 0.f ? 1.f / l : 1.f;
-      T* dst = static_cast<T*>(a.out) + (long long)t * a.out_row + hq * a.out_head + V * lane;
+      T* dst = static_cast<T*>(a.out) + (long long)t * a.out_row + hq * a.out_head + V * ln;
 #pragma unroll
       for (int k = 0; k < V; k++) v[k] *= inv;
-      if (V == 4) {
-        store4(dst, v, a.out_vec);
-      } else {
+      if (V == 2) {
 #pragma unroll
         for (int k = 0; k < V; k++) dst[k] = from_f<T>(v[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) store4(dst + k, v + k, a.out_vec);
       }
-      if (lane == 0 && a.lse)
+      if (ln == 0 && a.lse)
         a.lse[(size_t)t * a.heads + hq] = l == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l) + m - P_SHIFT);
     }
   }
@@ -374,8 +380,13 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
     cfg.gridDim = dim3((g->own.rows + tokens - 1) / tokens, (g->own.heads + heads - 1) / heads);
     cfg.blockDim = dim3(32 * JOIN_WARPS);
     cfg.dynamicSmemBytes = 0;
-    c = many ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, JOIN_WARPS>, pass[0], pass[1], tokens, heads)
-             : cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, 1>, pass[0], pass[1], tokens, heads);
+    // Where a warp has more than four rows and heads, two at a time: most instructions are then for both, and twice as much is on its way
+    // (turns of 63 tokens of 26 requests 180 us, 184 one by one, of 200 484 and 511; 256 single tokens, two of whose rows and heads a
+    // warp has, 135.5 and 134).
+    const bool two = (long long)g->own.rows * g->own.heads > JOIN_CTAS * JOIN_WARPS * 4;
+    c = many  ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, JOIN_WARPS, 32>, pass[0], pass[1], tokens, heads)
+        : two ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, 1, 16>, pass[0], pass[1], tokens, heads)
+              : cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, 1, 32>, pass[0], pass[1], tokens, heads);
   }
   if (c == cudaSuccess) return H2C_OK;
   cudaGetLastError();

@@ -135,6 +135,21 @@ def test_prompts_behind_a_prefix(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,kvh,hd,plen,gs,kv_len,n_q", [
+    (28, 4, 128, [500, 90], [0, 2, 3], [300, 129, 260, 9, 0], [300, 129, 131, 1, 0]),
+    (14, 2, 64, [700], [0, 3], [600, 500, 77], [600, 401, 77]),
+    (9, 3, 64, [33, 2000], [1, 2, 4], [900, 5, 700, 31], [900, 7, 700, 31])])
+def test_turns_of_many_rows(dtype, H, kvh, hd, plen, gs, kv_len, n_q):
+    """So many rows that the join takes two at a time; in place, and rows past the last request's stay."""
+    q, kv, sc, ptable, table, q_start = inputs(dtype, 16, H, kvh, hd, plen, kv_len, n_q)
+    buf = torch.full((len(q) + 37, H, hd), 9.0, dtype=dtype, device=DEV)
+    buf[:len(q)] = q
+    rest = [ptable, plen, gs, table, q_start, kv_len]
+    o, lse = call(buf, kv, sc, *rest, out=buf)
+    assert (o[len(q):] == 9).all()
+    t.close(o[:len(q)], lse[:len(q)], reference(q, kv, sc, *rest, hd ** -0.5), dtype, dtype != torch.float32)
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_more_queries_than_own_positions(dtype):
     """Queries before the first own position see the prefix alone, and nothing where there is none."""
     o, lse = run_case(dtype, 16, 14, 2, 64, [40], [0, 2], [5, 0, 3], [9, 3, 6])
