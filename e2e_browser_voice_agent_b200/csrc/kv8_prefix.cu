@@ -327,7 +327,7 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
   }
 
   static unsigned char done[OP_MAX_DEVICES];
-  constexpr int p_smem = PromptCfg<T, HD>::SMEM, r_smem = RowSmem<HD>::BYTES;
+  constexpr int p_smem = PromptCfg<T, HD, true>::SMEM, r_smem = RowSmem<HD>::BYTES;
   if (int rc = op_once(who, done, [] {
         const cudaError_t c = cudaFuncSetAttribute(k_att_prompt<T, HD, SharedArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, p_smem);
         return c != cudaSuccess ? c : cudaFuncSetAttribute(k_prefix_rows<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, r_smem);

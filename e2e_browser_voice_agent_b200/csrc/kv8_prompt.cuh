@@ -15,7 +15,8 @@
 // * A page's scale of K multiplies its scores; its scale of V joins the exponent (see split_scale), so a row's weights
 //   are powers of two relative to one running maximum, which moves only when a score passes it by M_SLACK: only then is
 //   O rescaled (by the softmax warps, in TMEM).
-// * float32 queries and float32 and float16 rows' weights are two float16 terms each (22 bits), one tcgen05.mma per term.
+// * float32 queries, and the weights but for those of bfloat16 rows in h2c_kv8_attention, are two float16 terms each (22 bits), one
+//   tcgen05.mma per term.
 // * The tensor cores' sums are added up outside them every few tiles of keys (see FOLD).
 // * V lies in shared memory as its rows come, [key][dimension]: the second product's B operand in MN-major form.
 // * The softmaxes of the two row tiles take turns at the exponentials, so that one's wait for its scores falls into the
@@ -363,13 +364,16 @@ __device__ __forceinline__ bool wait_two(uint64_t* b0, unsigned p0, uint64_t* b1
 // a 128-byte-swizzled tile of 64-element (128-byte) rows: byte address of the 16-byte piece c of row r
 __device__ __forceinline__ uint32_t sw128(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-template <class T, int HD>
+// PARTS: of h2c_kv8_prefix_attention.
+template <class T, int HD, bool PARTS = false>
 struct PromptCfg {
   static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   static constexpr int Q_TERMS = sizeof(T) == 4 ? 2 : 1;  // float16 terms of queries
-  // ... and of weights. One where the output is bfloat16: 2^-12 of each weight, an eighth of that rounding. With float16 outputs one
-  // term's error would be as large as theirs (some 1.2 times the error in all; 445 us for the prompts below, 543 with two).
-  static constexpr int P_TERMS = BF16 ? 1 : 2;
+  // ... and of weights. One where h2c_kv8_attention's output is bfloat16: 2^-12 of each weight, an eighth of that rounding. With float16
+  // outputs one term's error would be as large as theirs (some 1.2 times the error in all; 445 us for the prompts below, 543 with two).
+  // Behind shared prefixes two throughout: with one, 6% of bfloat16 outputs are not the rounding of a float32 computation's but a step
+  // beside it (256 single tokens behind 16,385 positions: 134 us, 160 with two).
+  static constexpr int P_TERMS = BF16 && !PARTS ? 1 : 2;
   static constexpr int BLKS = HD / 64;                   // 64-dimension blocks of a row
   static constexpr int Q_TILE = 128 * HD * 2;            // one row tile, one term
   static constexpr int KV_TILE = PR_KEYS * HD * 2;
@@ -384,7 +388,7 @@ struct PromptCfg {
   // us for 53, prompts of 2,064-4,099 797 for 650: the places' way to L2. 4 tiles: 63 and 830 us, 4e-7 and 1.4e-6; CTAs of one row
   // tile, whose sum fits into the other's TMEM: 78 and 1,071). 16-bit types 1.2e-5 and less, a twentieth of float16's rounding: chunks
   // on 32,000 and more keys take 2-3% longer.
-  static constexpr int FOLD = sizeof(T) == 4 ? (HD == 64 ? 4 : 8) : HD == 64 ? 32 : BF16 ? 128 : 64;
+  static constexpr int FOLD = sizeof(T) == 4 ? (HD == 64 ? 4 : 8) : HD == 64 ? 32 : P_TERMS == 1 ? 128 : 64;
   static constexpr bool SPILL = HD == 128;
   static constexpr int OFF_K = 2 * Q_AREA;
   static constexpr int STAGES = Q_TERMS * HD > 128 ? 2 : 3;   // K and V tiles each
@@ -679,7 +683,7 @@ __device__ __forceinline__ float tile_max(const float* s, const KeyInfo* in, int
 template <class T, int HD, class A>
 __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgsOf<A> pa) {
   const EndAfterTheOthers<PARTS_ONLY<A>> end;
-  using C = PromptCfg<T, HD>;
+  using C = PromptCfg<T, HD, PARTS_ONLY<A>>;
   constexpr int STG = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u);

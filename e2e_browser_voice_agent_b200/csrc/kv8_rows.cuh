@@ -470,11 +470,12 @@ struct WorkPlan {
   size_t bytes;
 };
 // Tiles of keys after which k_att_prompt's sums go to the workspace.
-int spill_after(int type, int head_dim) {
+int spill_after(int type, int head_dim, bool parts) {
   if (head_dim == 64) return INT_MAX;
   return type == H2C_TYPE_F32 ? PromptCfg<float, 128>::FOLD
          : type == H2C_TYPE_F16 ? PromptCfg<__half, 128>::FOLD
-                                : PromptCfg<__nv_bfloat16, 128>::FOLD;
+         : parts ? PromptCfg<__nv_bfloat16, 128, true>::FOLD
+                 : PromptCfg<__nv_bfloat16, 128>::FOLD;
 }
 // parts: all that the kernels compute stays in the workspace for a joining kernel of the caller's.
 WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
@@ -539,7 +540,7 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
   // whether a row tile can have more tiles of keys than a sum may take, whatever max_kv says
   const long long room = (long long)g->table_cols * g->page_size;
   const long long most_keys = g->window > 0 ? std::min(room, (long long)g->window + PR_ROWS + 16) : room;
-  p.spill = p.prompt && (most_keys + PR_KEYS - 1) / PR_KEYS + 1 > spill_after(g->type, g->head_dim);
+  p.spill = p.prompt && (most_keys + PR_KEYS - 1) / PR_KEYS + 1 > spill_after(g->type, g->head_dim, parts);
   p.bytes = (p.units * RW_ROWS + (size_t)p.p_units * PR_ROWS) * ((size_t)g->head_dim * 4 + 8) +
             (p.spill ? (size_t)PR_SLOTS * PR_ROWS * g->head_dim * 4 : 0);
   return p;
