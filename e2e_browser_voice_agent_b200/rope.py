@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from .kv8 import _TYPES, _call, _want
 
-SCALINGS = ("none", "linear", "ntk", "yarn")
+SCALINGS = ("none", "linear", "ntk", "yarn", "turns")
 
 
 def frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 0,
@@ -25,8 +25,10 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", f
       linear  all divided by factor
       ntk     the base raised by factor ** (rotary_dim / (rotary_dim - 2)): the slowest is divided by factor, the fastest stays
       yarn    pairs that turn more than `fast` times within `original` positions stay, those that turn less than `slow` times are
-              divided by factor, and between them the share of both goes linearly with the turns (YaRN, Peng et al. 2023; the
-              attention temperature that belongs to it is yarn_magnitude(factor), an argument of rotate).
+              divided by factor, and between them (from the pair at or before the one to the pair at or after the other) the share of both goes
+              linearly with the pair's number, as models with YaRN (Peng et al. 2023) are trained and run; the attention
+              temperature that belongs to it is yarn_magnitude(factor), an argument of rotate
+      turns   the same, but that the share goes linearly with the turns
     A model whose frequencies are made otherwise brings its own tensor."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim: an even number is wanted, not {rotary_dim}")
@@ -42,11 +44,17 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", f
     f = [base ** (-2 * j / rotary_dim) for j in range(half)]
     if scaling == "linear":
         f = [x / factor for x in f]
-    if scaling == "yarn":
+    if scaling in ("yarn", "turns"):
         if original < 1 or not fast > slow > 0:
-            raise ValueError(f"scaling yarn: original ({original}) positions and fast ({fast}) above slow ({slow}) are wanted")
+            raise ValueError(f"scaling {scaling}: original ({original}) positions and fast ({fast}) above slow ({slow}) are wanted")
+        at = lambda turns: rotary_dim * math.log(original / (2 * math.pi * turns)) / (2 * math.log(base))  # the pair that turns so often
+        low, high = max(0, math.floor(at(fast))), min(rotary_dim - 1, math.ceil(at(slow)))
         for j in range(half):
-            kept = min(1.0, max(0.0, (f[j] * original / (2 * math.pi) - slow) / (fast - slow)))
+            if scaling == "yarn":
+                kept = 1 - (j - low) / max(high - low, 0.001)
+            else:
+                kept = (f[j] * original / (2 * math.pi) - slow) / (fast - slow)
+            kept = min(1.0, max(0.0, kept))
             f[j] *= kept + (1 - kept) / factor
     return torch.tensor(f, dtype=torch.float64, device=device)
 
