@@ -428,8 +428,8 @@ int h2c_i8_values(const void* q, int64_t q_row, const float* scale, int32_t rows
  * to 1024) and of k_heads keys (likewise; either may be 0) go to q_out and k_out with the first rotary_dim (even) values turned and
  * the others as they are. Pair j < rotary_dim / 2 is (x[j], x[j + rotary_dim / 2]), or with `interleaved` (x[2j], x[2j + 1]):
  *   (a, b) -> (a c - b s, b c + a s),  c = magnitude * cos(u), s = magnitude * sin(u),  u = position[t] * frequency[j]
- * frequency: float64 [rotary_dim / 2], radians per position. The angle's whole turns are dropped in 64 bits, so it is as exact far
- * out as near 0; the rest is float32, rounded once. A token whose position is negative (h2c_kv8_plan's beyond the last) is not turned,
+ * frequency: float64 [rotary_dim / 2], radians per position. The angle's whole turns are dropped from a product that keeps its
+ * remainder, so it is as exact far out as near 0; c and s are taken in 64 bits and rounded to float32 once, the rest is float32. A token whose position is negative (h2c_kv8_plan's beyond the last) is not turned,
  * magnitude included. q_out may be q itself (same address and strides), k_out k; beside that what is written shares no memory with
  * another argument, nor do two vectors of it (refused). */
 int h2c_rope(int32_t type, const void* q, int64_t q_row, int64_t q_head, void* q_out, int64_t q_out_row, int64_t q_out_head,
