@@ -39,11 +39,11 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_prefix_row
   att_rows<T, HD>(both.ra[own], at - rz * across, rz % n, rz / n);
 }
 
-// Where the spans of a row lie: span s is row `first` + s * (rows of a tile) of the sums and of the (m, l) of one of a pass's two kernels.
+// Where the spans of a row lie: span s is row `first` + s * `step` of the sums and of the (m, l) of one of a pass's two kernels.
 struct Parts {
   long long first;
-  int used;     // spans; 0: the row is in no request (group)
-  bool prompt;  // k_att_prompt's
+  int used, step;  // spans; 0: the row is in no request (group)
+  bool prompt;     // k_att_prompt's
 };
 
 // Quotients of numbers below 2^31 by multiplication: the joining kernel would spend most of its instructions on divisions else.
@@ -58,10 +58,10 @@ struct Divisor {
   __device__ __forceinline__ int rounded_up(int n) const { return quotient(n + (int)d - 1); }
 };
 
-// The request (group) that has a row of q, and k_att_prompt's spans before its own, `blocks` tiles of keys each.
+// The request (group) that has a row of q, and k_att_prompt's spans and rows of parts before its own, `blocks` tiles of keys each.
 struct Owner {
   int r, n_all;      // r = -1: no request has it
-  long long before;
+  long long before, part;  // (part: its first row there)
   Request R;
   int tiles, spans;  // its row tiles in k_att_prompt, if it takes them, the spans of each and the tiles of keys of a span
   Divisor blocks;
@@ -72,12 +72,13 @@ __device__ __forceinline__ void owners_of(const Pass& p, int t0, int i0, int ste
   const int lane = threadIdx.x & 31, blocks = p.prompt ? blocks_of_call(p.pa) : 1;
   for (int i = i0 + lane * step; i < nt; i += 32 * step) to[2 * i].r = -1;
   __syncwarp();
-  long long before = 0;
+  long long before = 0, rows_before = 0;  // spans; rows of this lane's requests
   unsigned left = 0;  // rows to be found: bit m for i0 + m * step (JOIN_TOKENS at most)
   for (int i = i0, m = 0; i < nt; i += step, m++) left |= 1u << m;
   for (int base = 0; base < a.n_req && left; base += 32) {
     const int r = base + lane;
     int n = 0, n_all = 0, tiles = 0, spans = 1;
+    long long rows = 0;
     Request R{0, 0, 0};
     if (r < a.n_req) {
       R = request_of(a, r, &n_all);
@@ -85,6 +86,7 @@ __device__ __forceinline__ void owners_of(const Pass& p, int t0, int i0, int ste
         tiles = row_tiles_of(p.pa, R);
         spans = spans_of_len(p.pa, R.len, blocks);
         n = units_of(p.pa, tiles, spans);
+        rows = part_rows_of(p.pa, R, tiles, spans);
       }
     }
     for (unsigned todo = left; todo; todo &= todo - 1) {
@@ -93,17 +95,21 @@ __device__ __forceinline__ void owners_of(const Pass& p, int t0, int i0, int ste
       if (!in) continue;
       const int l = __ffs(in) - 1;  // (of several, the first)
       const long long at = before + __reduce_add_sync(0xffffffffu, lane < l ? n : 0);
-      if (lane == l) to[2 * i] = {r, n_all, at, R, tiles, spans, Divisor(tiles ? even_blocks(p.pa, R.len, spans) : 1)};
+      const long long part = p.prompt ? sum_of_warp(rows_before + (lane < l ? rows : 0)) : 0;
+      // (without room for its parts nothing of it was computed)
+      if (lane == l && (!tiles || part + rows <= p.pa.part_rows))
+        to[2 * i] = {r, n_all, at, part, R, tiles, spans, Divisor(tiles ? even_blocks(p.pa, R.len, spans) : 1)};
       left &= ~(1u << m);
     }
     before += __reduce_add_sync(0xffffffffu, n);
+    rows_before += rows;
   }
 }
 
 // The parts of row t of q, which `o` has, and head h of kv head `head`'s group. row_blocks: blocks of k_att_rows' spans. (None where starts
 // of requests without sense would lead beyond what was computed.)
 __device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_blocks, const Owner& o, int t, int head, int h) {
-  if (o.r < 0) return {0, 0, false};
+  if (o.r < 0) return {0, 0, 0, false};
   const SharedArgs& a = p.ra.a;
   const Divisor group(a.group, a.group_magic);
   const int row = (t - o.R.first) * a.group + h;
@@ -115,17 +121,19 @@ __device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_bloc
   if (o.tiles) {
     const int tile = row / PR_ROWS, n_blocks = (max(0, end_of(tile * PR_ROWS + PR_ROWS - 1)) + PR_KEYS - 1) / PR_KEYS;
     const long long unit = o.before + ((o.tiles - 1LL - tile) * a.kv_heads + head) * o.spans;
-    if (unit + o.spans > p.pa.cap) return {0, 0, false};
-    return {unit * PR_ROWS + (row - tile * PR_ROWS), max(1, min(o.spans, o.blocks.rounded_up(n_blocks))), true};
+    if (unit + o.spans > p.pa.cap) return {0, 0, 0, false};
+    const int n_rows = o.R.n_q * a.group;
+    return {o.part + (long long)head * o.spans * n_rows + row, max(1, min(o.spans, o.blocks.rounded_up(n_blocks))), n_rows, true};
   }
   const int tile = row / RW_ROWS, n_blocks = (max(0, end_of(tile * RW_ROWS + RW_ROWS - 1)) + RW_BLK - 1) / RW_BLK;
-  if (tile >= p.ra.tiles) return {0, 0, false};
+  if (tile >= p.ra.tiles) return {0, 0, 0, false};
   const long long unit = (((long long)o.r * a.kv_heads + head) * p.ra.tiles + tile) * p.ra.splits;
-  return {unit * RW_ROWS + (row - tile * RW_ROWS), max(1, min(p.ra.splits, row_blocks.rounded_up(n_blocks))), false};
+  return {unit * RW_ROWS + (row - tile * RW_ROWS), max(1, min(p.ra.splits, row_blocks.rounded_up(n_blocks))), RW_ROWS, false};
 }
 // The same for all lanes as lane j has them.
 __device__ __forceinline__ Parts of_lane(const Parts& p, int j) {
-  return {__shfl_sync(0xffffffffu, p.first, j), __shfl_sync(0xffffffffu, p.used, j), __shfl_sync(0xffffffffu, (int)p.prompt, j) != 0};
+  return {__shfl_sync(0xffffffffu, p.first, j), __shfl_sync(0xffffffffu, p.used, j), __shfl_sync(0xffffffffu, p.step, j),
+          __shfl_sync(0xffffffffu, (int)p.prompt, j) != 0};
 }
 
 // A CTA takes `heads` heads (at most JOIN_WARPS) of `tokens` (at most JOIN_TOKENS) rows of q, L lanes (or NW = JOIN_WARPS warps, for one
@@ -148,7 +156,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
   const Divisor by_heads(nh), by_group(a.group, a.group_magic);
   const Divisor prefix_row_blocks(max(1, prefix.ra.blocks)), own_row_blocks(max(1, own.ra.blocks));
   // lane j: of the warp's j-th row and head
-  Parts o_of{0, 0, false}, p_of{0, 0, false};
+  Parts o_of{0, 0, 0, false}, p_of{0, 0, 0, false};
   const int mine = NW > 1 ? lane : warp + lane * JOIN_WARPS;
   if (mine < n) {
     const int k_t = by_heads.quotient(mine), t = t0 + k_t, hq = h0 + mine - k_t * nh, head = by_group.quotient(hq), h = hq - head * a.group;
@@ -165,7 +173,6 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
     const float2* o_ml = (o.prompt ? own.pa.ml : own.ra.ml) + o.first;
     const float* p_part = (p.prompt ? prefix.pa.part : prefix.ra.part) + p.first * HD + V * ln;
     const float2* p_ml = (p.prompt ? prefix.pa.ml : prefix.ra.ml) + p.first;
-    const unsigned o_step = o.prompt ? PR_ROWS : RW_ROWS, p_step = p.prompt ? PR_ROWS : RW_ROWS;
     const int all = p.used + o.used;
     // UN spans at a time, everything of them on its way at once; the sums are relative to the largest maximum so far
     float m = -INFINITY, v[V], l = 0.f;
@@ -182,7 +189,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
         for (int j = 0; j < V; j++) x[k][j] = 0.f;
         if (s < all) {
           const bool shared = s < p.used;
-          const size_t at = shared ? (size_t)s * p_step : (size_t)(s - p.used) * o_step;
+          const size_t at = shared ? (size_t)s * p.step : (size_t)(s - p.used) * o.step;
           const float* src = (shared ? p_part : o_part) + at * HD;
           ml[k] = (shared ? p_ml : o_ml)[at];
           if (V == 2) {
@@ -312,18 +319,18 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
       if (!plan.shared) a.n_req = 0;
     }
     float* part = take(p.units, RW_ROWS);
-    float* p_part = take(p.p_units, PR_ROWS);
+    float* p_part = take(p.p_rows, 1);
     pass[i].rows = p.rows;
     pass[i].prompt = p.prompt;
     pass[i].ra = {a, p.splits, p.blocks, p.tiles, p.max_rows, 0, part, nullptr};
-    pass[i].pa = {a, p.min_rows, p.shape, p.p_keys, p.counted, p_part, nullptr, p.spill ? sums : nullptr, err, p.p_units};
+    pass[i].pa = {a, p.min_rows, p.shape, p.p_keys, p.counted, p_part, nullptr, p.spill ? sums : nullptr, err, p.p_units, p.p_rows};
   }
   for (int i = 0; i < 2; i++) {
     const WorkPlan& p = i ? plan.own : plan.prefix;
     pass[i].ra.ml = reinterpret_cast<float2*>(at);
     at += p.units * RW_ROWS * 2;
     pass[i].pa.ml = reinterpret_cast<float2*>(at);
-    at += (size_t)p.p_units * PR_ROWS * 2;
+    at += (size_t)p.p_rows * 2;
   }
 
   static unsigned char done[OP_MAX_DEVICES];

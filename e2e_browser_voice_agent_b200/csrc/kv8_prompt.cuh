@@ -83,7 +83,8 @@ struct PromptArgsOf {
   float2* ml;
   float* sums;        // (PromptCfg::SPILL) PR_SLOTS places of 256 rows' sums; nullptr where no row tile has more than FOLD tiles of keys
   int* err;
-  int cap;            // (SharedArgs) CTAs, and spans that the workspace has room for
+  int cap;            // (SharedArgs) CTAs, one for each span of a row tile
+  long long part_rows;  // (SharedArgs) rows of part and ml
 };
 using PromptArgs = PromptArgsOf<AttArgs>;
 
@@ -157,11 +158,11 @@ __device__ __forceinline__ TileAt tile_at(const PromptArgsOf<A>& pa, int idx) {
 }
 
 // What a CTA does: span `split` of the at most `splits` spans of `blocks` tiles of keys that the row tile `at` of a kv head is cut into
-// (r = -1: nothing), and the number of that span in the workspace.
+// (r = -1: nothing), and where the tile's first row lies in part and ml.
 struct Work {
   TileAt at;
   int head, split, splits, blocks;
-  size_t unit;
+  size_t part;
 };
 __device__ __forceinline__ Work work_of(const PromptArgsOf<AttArgs>& pa) {
   const AttArgs& a = pa.a;
@@ -174,7 +175,7 @@ __device__ __forceinline__ Work work_of(const PromptArgsOf<AttArgs>& pa) {
   const int idx = shape.tiles - 1 - (int)blockIdx.x / (shape.splits * a.kv_heads);
   if (idx < 0) return w;
   w.at = tile_at(pa, idx);
-  w.unit = ((size_t)idx * a.kv_heads + w.head) * shape.splits + w.split;
+  w.part = (((size_t)idx * a.kv_heads + w.head) * shape.splits + w.split) * PR_ROWS;
   return w;
 }
 
@@ -207,6 +208,16 @@ __device__ __forceinline__ int even_blocks(const PromptArgsOf<SharedArgs>& pa, i
 __device__ __forceinline__ int units_of(const PromptArgsOf<SharedArgs>& pa, int tiles, int spans) {
   return (int)min((long long)tiles * pa.a.kv_heads * spans, pa.cap + 1LL);
 }
+// Its rows in part and ml: [kv head][span][row], each request's behind those of the one before it (spans of whole tiles would take up to 256 / 17
+// times as much where requests have few rows); counted as one too many where there is no room for them.
+__device__ __forceinline__ long long part_rows_of(const PromptArgsOf<SharedArgs>& pa, const Request& R, int tiles, int spans) {
+  return tiles ? min((long long)R.n_q * pa.a.group * pa.a.kv_heads * spans, pa.part_rows + 1) : 0;
+}
+__device__ __forceinline__ long long sum_of_warp(long long x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
 // Tiles of keys a span. By whole warps.
 __device__ __forceinline__ int blocks_of_call(const PromptArgsOf<SharedArgs>& pa) {
   if (!pa.units) return pa.shape.blocks;
@@ -234,8 +245,8 @@ __device__ __forceinline__ Work work_of(const PromptArgsOf<SharedArgs>& pa) {
   Work w{};
   w.at.r = -1;
   const int blocks = blocks_of_call(pa);
-  w.unit = unit;
   int before = 0;
+  long long rows_before = 0;  // of this lane's requests
   for (int base = 0; base < a.n_req; base += 32) {
     const int r = base + lane;
     int n = 0, n_all = 0, spans = 1, tiles = 0;
@@ -268,8 +279,13 @@ __device__ __forceinline__ Work work_of(const PromptArgsOf<SharedArgs>& pa) {
       w.split = i - th * w.splits;
       w.head = th % a.kv_heads;
       w.at.row0 = (tiles - 1 - th / a.kv_heads) * PR_ROWS;  // (the last tiles of a causal prompt first)
+      const int rows = w.at.R.n_q * a.group;
+      const long long first = sum_of_warp(rows_before + (lane < l ? part_rows_of(pa, R, n ? 1 : 0, spans) : 0));
+      if (first + part_rows_of(pa, w.at.R, 1, w.splits) > pa.part_rows) w.at.r = -1;  // (starts without sense)
+      w.part = first + ((size_t)w.head * w.splits + w.split) * rows + w.at.row0;
       return w;
     }
+    rows_before += part_rows_of(pa, R, tiles, spans);
     before = min(before + __shfl_sync(0xffffffffu, sum, 31), pa.cap + 1);  // (32 of them fit)
   }
   return w;
@@ -1037,7 +1053,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgsOf
     if (ok) {
       const bool whole = !PARTS_ONLY<A> && sp.used == 1;
       const float inv = whole && l_run != 0.f ? 1.f / l_run : 1.f;
-      const size_t unit = wk.unit;
+      const size_t part_row = wk.part + q * 128 + trow;
       uint8_t* stage = sm + q * C::Q_AREA + trow * C::OUT_LD;
       const bool folded = n_tiles > fold;
       const uint32_t sum_at = folded && !C::SPILL ? to + HD : 0;
@@ -1052,7 +1068,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgsOf
           copy_row<T, NC>(dst + c, stage, live, a.out_vec16);
         }
       } else {
-        float* dst = pa.part + (unit * PR_ROWS + q * 128 + trow) * HD;
+        float* dst = pa.part + part_row * HD;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 64) {
           stage_row<float, 64>(stage, to + c, n_tiles > 0, 1.f, sum_at ? sum_at + c : 0, spilled, trow, c, f_sum);
@@ -1060,7 +1076,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) k_att_prompt(const PromptArgsOf
         }
       }
       if (live) {
-        if (!whole) pa.ml[unit * PR_ROWS + q * 128 + trow] = make_float2(m_run, l_run);
+        if (!whole) pa.ml[part_row] = make_float2(m_run, l_run);
         else if (a.lse)
           a.lse[(size_t)(R.first + tok) * a.heads + hq] =
               l_run == 0.f ? -INFINITY : 0.69314718055994531f * (log2f(l_run) + m_run - P_SHIFT);

@@ -463,6 +463,7 @@ struct WorkPlan {
   bool rows, prompt, cluster, counted;
   int max_rows, splits, blocks, tiles;         // k_att_rows
   int min_rows, p_keys, p_units;               // k_att_prompt (see PromptArgs; p_units also without counting)
+  long long p_rows;                            // rows of its parts in the workspace
   PromptShape shape;
   unsigned p_join;                             // CTAs of its joining kernel, 0 without one
   size_t units;                                // row tiles x spans in the workspace
@@ -512,8 +513,11 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
   }
   if (p.prompt) {
     p.min_rows = p.rows ? few + 1 : 0;
+    const long long all_rows = g->rows * group;  // (of which a request has min_rows or more)
     const int tiles = (int)std::min<long long>({(long long)g->n_req * ((most_rows + PR_ROWS - 1) / PR_ROWS),
-                                                (long long)g->rows * group / PR_ROWS + g->n_req, (long long)INT_MAX / g->kv_heads});
+                                                all_rows / PR_ROWS + (parts && p.min_rows ? std::min<long long>(g->n_req, all_rows / p.min_rows)
+                                                                                          : g->n_req),
+                                                (long long)INT_MAX / g->kv_heads});
     p.p_keys = (int)((keys + PR_KEYS - 1) / PR_KEYS) + (g->window > 0 ? 1 : 0);
     p.shape = prompt_shape(tiles, g->kv_heads, p.p_keys, g->n_req == 1 ? 148 : 0, 4);
     if (g->n_req == 1) {
@@ -536,12 +540,20 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
     p.counted = g->n_req > 1;
     p.p_units = (int)std::min<long long>(INT_MAX / PR_ROWS, p.counted ? spans_at_most(ctas, p.p_keys) : ctas * p.shape.splits);
     p.p_join = 0;
+    // (a request of n rows and t tiles of keys has n rows for each kv head and span; t / B + 1 spans at most, and 256 times what
+    // spans_at_most has beside the uncut tiles is a bound of the sum of n t / B)
+    const long long once = std::min((long long)g->rows * group, g->n_req * most_rows) * g->kv_heads;
+    p.p_rows = !p.counted ? once * p.shape.splits
+                          : std::min(once + (spans_at_most(ctas, p.p_keys) - ctas) * PR_ROWS,
+                                     once * std::max(1, (p.p_keys + SPAN_LEAST - 1) / SPAN_LEAST));
+  } else {
+    p.p_rows = (long long)p.p_units * PR_ROWS;
   }
   // whether a row tile can have more tiles of keys than a sum may take, whatever max_kv says
   const long long room = (long long)g->table_cols * g->page_size;
   const long long most_keys = g->window > 0 ? std::min(room, (long long)g->window + PR_ROWS + 16) : room;
   p.spill = p.prompt && (most_keys + PR_KEYS - 1) / PR_KEYS + 1 > spill_after(g->type, g->head_dim, parts);
-  p.bytes = (p.units * RW_ROWS + (size_t)p.p_units * PR_ROWS) * ((size_t)g->head_dim * 4 + 8) +
+  p.bytes = (p.units * RW_ROWS + (size_t)p.p_rows) * ((size_t)g->head_dim * 4 + 8) +
             (p.spill ? (size_t)PR_SLOTS * PR_ROWS * g->head_dim * 4 : 0);
   return p;
 }
