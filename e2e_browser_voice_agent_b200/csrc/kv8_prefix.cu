@@ -278,7 +278,7 @@ PrefixPlan plan_prefix(const h2c_kv8_prefix_args* g) {
   p.shared = g->n_groups > 0 && g->prefix_cols > 0;
   if (p.shared) {
     const h2c_kv8_attention_args groups = groups_of(g);
-    p.prefix = plan_work(&groups, true);
+    p.prefix = plan_work(&groups, true, true);
   }
   // (a CTA holds its place of spilled sums alone, whichever kernel it is of: one set of them)
   const size_t sums = (size_t)PR_SLOTS * PR_ROWS * g->own.head_dim * 4;

@@ -459,6 +459,12 @@ inline unsigned join_ctas(long long rows, int splits) {
 // (1,024,000) 67 and 38. float32: 70 rows of one 21 and 26, 126 rows 31 and 28. 64 wide, 14 over 2, bfloat16 and float32: one of
 // 4,000 keys, 504 rows (504,000) 23, 22 and 27, 1,008 rows (1,008,000) 36, 27 and 32; of 16,000, 126 rows (512,000) 24, 18 and 22;
 // 8 of 4,000 keys, 63 rows (512,000) 23, 28 and 34, 126 rows (1,024,000) 35, 29 and 35.
+// Groups behind their prefixes share all rows out among them, so the visits are those of the row tiles that there can be, not of as many for each
+// group; us so, and with n_req times as many, which are k_att_prompt's earlier: 8 groups of 4 single tokens behind 640 positions, 28 heads over 4
+// of 128, bfloat16, 20 and 37, 2 of 3 behind 4,096 20 and 27; 8 of 6 behind 2,000, 14 over 2 of 64, float32, 23 and 30. Not where a
+// group's average is up to 16 (32) rows, which k_att_rows takes in either case, but with two (four) row tiles a group on its grid instead of all:
+// 16 groups of 2 behind 640 25 and 22; nor where the row tiles of all groups together would be more than 3,200 units: 24 of 3 behind 1,280,
+// 16 heads over 1 of 64 (3,456 units) 35 and 32, 32 of 3 behind 300, 8 over 1 of 128 18 and 28.
 struct WorkPlan {
   bool rows, prompt, cluster, counted;
   int max_rows, splits, blocks, tiles;         // k_att_rows
@@ -478,14 +484,17 @@ int spill_after(int type, int head_dim, bool parts) {
          : parts ? PromptCfg<__nv_bfloat16, 128, true>::FOLD
                  : PromptCfg<__nv_bfloat16, 128>::FOLD;
 }
-// parts: all that the kernels compute stays in the workspace for a joining kernel of the caller's.
-WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
+// parts: all that the kernels compute stays in the workspace for a joining kernel of the caller's. groups: the requests are groups that share
+// all rows out among them (max_q = rows), so that there are far fewer row tiles than n_req * max_q has.
+WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false, bool groups = false) {
   WorkPlan p = {};
   const long long group = g->heads / g->kv_heads, most_rows = g->max_q * group;
   long long keys = g->max_kv;
   if (g->window > 0) keys = std::min(keys, (long long)g->window + g->max_q);
-  const long long visits = (most_rows + RW_ROWS - 1) / RW_ROWS * g->n_req * g->kv_heads * std::max(keys, 256LL);
+  const long long per_request = (most_rows + RW_ROWS - 1) / RW_ROWS, row_tiles = per_request * g->n_req;
   const int few = g->head_dim == 64 ? 32 : 16;
+  const bool shared_out = groups && most_rows > (long long)few * g->n_req && row_tiles * g->kv_heads <= 3200;
+  const long long visits = (shared_out ? std::min(row_tiles, most_rows / RW_ROWS + g->n_req) : row_tiles) * g->kv_heads * std::max(keys, 256LL);
   p.prompt = most_rows > few && visits > (g->head_dim == 64 ? 1 << 19 : 1 << 17);
   p.rows = !p.prompt || g->n_req > 1;
   if (p.rows) {
@@ -499,17 +508,17 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false) {
     // A warp's spans, where they are joined in any case: three waves of 12 warps an SM (256 single tokens of 16-2,000 keys 61 us, 64 with four
     // and 68 with eight; with two 9% more than with four), of 128 keys or more (32 requests behind 4,096: 27 us, 38 with 64), or of 64
     // where those are few (4 sessions 10.4, 12.7 with 128).
-    const long long groups = (long long)g->n_req * g->kv_heads * p.tiles, want = ((parts ? 5328 : 888) + groups - 1) / groups;
+    const long long units = (long long)g->n_req * g->kv_heads * p.tiles, want = ((parts ? 5328 : 888) + units - 1) / units;
     const int n_blocks = (int)((keys + RW_BLK - 1) / RW_BLK) + (g->window > 0 ? 1 : 0);
-    p.cluster = !parts && groups * RW_CLUSTER <= 444 && n_blocks / 16 <= RW_CLUSTER;
-    const int least = !parts ? 16 : groups * (n_blocks / 4) <= 888 && n_blocks <= 256 ? 4 : 8;
+    p.cluster = !parts && units * RW_CLUSTER <= 444 && n_blocks / 16 <= RW_CLUSTER;
+    const int least = !parts ? 16 : units * (n_blocks / 4) <= 888 && n_blocks <= 256 ? 4 : 8;
     p.splits = (int)std::max(1LL, p.cluster ? std::min<long long>({(long long)RW_CLUSTER, want, (n_blocks + 7LL) / 8})
                                             : std::min<long long>(want, n_blocks / least));
     const int step = parts ? 1 : RW_WARPS;  // blocks of a span: a multiple of the warps that share it
     p.blocks = std::max(step, ((n_blocks + p.splits - 1) / p.splits + step - 1) / step * step);
     p.splits = std::max(1, (n_blocks + p.blocks - 1) / p.blocks);
     p.cluster = p.cluster && p.splits > 1;
-    p.units = parts || (p.splits > 1 && !p.cluster) ? (size_t)groups * p.splits : 0;
+    p.units = parts || (p.splits > 1 && !p.cluster) ? (size_t)units * p.splits : 0;
   }
   if (p.prompt) {
     p.min_rows = p.rows ? few + 1 : 0;

@@ -51,3 +51,14 @@ def test_starts_that_name_rows_many_times(dtype):
     got, _ = p.call(q, kv, sc, ptable, [P] * n, list(range(n + 1)), table, q_start, kv_len)
     assert torch.equal(got, want)
     t.kv8()._lib.check_ops()
+
+
+@pytest.mark.parametrize("dtype", p.TYPES)
+@pytest.mark.parametrize("H,kvh,hd", [(14, 2, 64), (28, 4, 128), (8, 1, 128)])
+@pytest.mark.parametrize("groups,n,P", [(8, 4, 640), (2, 3, 4096), (12, 3, 640), (3, 5, 1283)])
+def test_groups_of_few_rows(dtype, H, kvh, hd, groups, n, P):
+    kv_len = [1 + (23 * i) % 150 for i in range(groups * n)]
+    plen = [P - 7 * g for g in range(groups)]
+    p.run_case(dtype, 16, H, kvh, hd, plen, list(range(0, groups * n + 1, n)), kv_len, [1] * (groups * n))
+    gs = [0, 1] + [n * g for g in range(2, groups)] + [groups * n]   # uneven: the first group has one, the second the others of two
+    p.run_case(dtype, 32, H, kvh, hd, plen, gs, kv_len, [1] * (groups * n), seed=1)
