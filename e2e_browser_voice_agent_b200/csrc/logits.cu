@@ -1,10 +1,9 @@
 // Penalties for repeated tokens, biases and masks of allowed tokens on a step's logits (h2c_logits_adjust; the formula is
 // stated in include/h2cuda.h).
 //
-// A CTA takes a chunk of one row's vocabulary, whose logits are on their way to registers (all of them but of the longest chunks) while it
-// counts the row's earlier tokens that fall there in shared memory (whole numbers, so the order does not matter) and its first
-// warp looks for the biased tokens among them and adds the biases of each up in the list's order. Then it changes, masks and writes
-// the logits, and at last the few biased ones.
+// A CTA takes a chunk of one row's vocabulary, whose logits are on their way to registers while it counts the row's earlier tokens that
+// fall there in shared memory (whole numbers, so the order does not matter) and its first warp looks for the biased tokens among
+// them and adds the biases of each up in the list's order. Then it changes, masks and writes the logits, and at last the few biased ones.
 // Bound: bandwidth for many rows, and the instructions of the pass: a token that was said is found in nearly every warp's 256 logits, so
 // its division is one of five multiplications where it can be. Each chunk goes through the row's history (from L2), so chunks are long.
 // 32 rows of 151,936 float32: 15.3 us (2.6 TB/s); 256 rows behind up to 16,384 tokens, bfloat16: 58 us; one row: 3.6 us.
@@ -26,7 +25,7 @@ struct LogitArgs {
   const void* in;
   void* out;
   long long in_row, out_row, tokens_row, bias_row, allowed_row;
-  int vocab, chunk, chunks, columns, n_bias;
+  int vocab, chunk, chunks, columns, n_bias;  // chunk: at most LG_UNITS units
   const int *tokens, *length;
   const float *repetition, *presence, *frequency;
   const int* bias_id;
@@ -106,17 +105,14 @@ __global__ void __launch_bounds__(LG_THREADS, LG_PER_SM) k_logits(const LogitArg
   T* out = static_cast<T*>(a.out) + row * a.out_row + c0;
   const unsigned* allowed = a.allowed ? a.allowed + row * a.allowed_row + (c0 >> 5) : nullptr;
   auto is_allowed = [&](int i) { return !allowed || (allowed[i >> 5] >> (i & 31) & 1u); };
-  // the first units of V logits are on their way while the history is counted
+  // the units of V logits are on their way while the history is counted
   const int units = VEC ? n / V : 0;
   uint4 raw[UN];
-  auto fetch = [&](int u0) {
 #pragma unroll
-    for (int k = 0; k < UN; k++) {
-      const int u = u0 + k * LG_THREADS;
-      if (u < units) raw[k] = reinterpret_cast<const uint4*>(in)[u];
-    }
-  };
-  fetch(tid);
+  for (int k = 0; k < UN; k++) {
+    const int u = tid + k * LG_THREADS;
+    if (u < units) raw[k] = reinterpret_cast<const uint4*>(in)[u];
+  }
   const Strength s = strength_of(a, row);
   auto count_of = [&](unsigned i) { return CPW == 1 ? counts[i] : counts[i >> 1] >> (16 * (i & 1)) & 0xffffu; };
   if (a.tokens) {
@@ -182,44 +178,41 @@ __global__ void __launch_bounds__(LG_THREADS, LG_PER_SM) k_logits(const LogitArg
   __syncthreads();
   // (most units hold no token that was said: their counts are looked at together)
   constexpr int CW = V * (int)sizeof(C) / 4, PER = 4 / (int)sizeof(T);  // words of a unit's counts; logits of a word
-  for (int u0 = tid; u0 < units; u0 += UN * LG_THREADS) {
-    if (u0 != tid) fetch(u0);
 #pragma unroll
-    for (int k = 0; k < UN; k++) {
-      const int u = u0 + k * LG_THREADS;
-      if (u >= units) break;
-      uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-      if (a.tokens) {
-        uint32_t c[CW], any = 0;
+  for (int k = 0; k < UN; k++) {
+    const int u = tid + k * LG_THREADS;
+    if (u >= units) break;
+    uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+    if (a.tokens) {
+      uint32_t c[CW], any = 0;
 #pragma unroll
-        for (int i = 0; i < CW; i += 2) {
-          const uint2 x = *reinterpret_cast<const uint2*>(counts + u * CW + i);
-          c[i] = x.x, c[i + 1] = x.y;
-          any |= x.x | x.y;
-        }
-        if (any) {
+      for (int i = 0; i < CW; i += 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(counts + u * CW + i);
+        c[i] = x.x, c[i + 1] = x.y;
+        any |= x.x | x.y;
+      }
+      if (any) {
 #pragma unroll
-          for (int i = 0; i < V; i++) {
-            const unsigned said = CPW == 1 ? c[i / CPW] : i % CPW ? c[i / CPW] >> 16 : c[i / CPW] & 0xffffu;
-            if (said) {
-              const T x = from_f<T>(penalized(value_of<T>(w[i / PER], i % PER), said, s));
-              put_value<T>(&w[i / PER], i % PER, x);
-            }
+        for (int i = 0; i < V; i++) {
+          const unsigned said = CPW == 1 ? c[i / CPW] : i % CPW ? c[i / CPW] >> 16 : c[i / CPW] & 0xffffu;
+          if (said) {
+            const T x = from_f<T>(penalized(value_of<T>(w[i / PER], i % PER), said, s));
+            put_value<T>(&w[i / PER], i % PER, x);
           }
         }
       }
-      if (allowed) {
-        const unsigned bits = ~(allowed[u * V >> 5] >> (u * V & 31));  // of those that may not come
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          uint32_t m;
-          if (sizeof(T) == 4) m = bits >> i & 1u ? ~0u : 0u;
-          else m = (bits >> (2 * i) & 1u ? 0xffffu : 0u) | (bits >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
-          w[i] = (w[i] & ~m) | (MINUS_INF<T> & m);
-        }
-      }
-      reinterpret_cast<uint4*>(out)[u] = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    if (allowed) {
+      const unsigned bits = ~(allowed[u * V >> 5] >> (u * V & 31));  // of those that may not come
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t m;
+        if (sizeof(T) == 4) m = bits >> i & 1u ? ~0u : 0u;
+        else m = (bits >> (2 * i) & 1u ? 0xffffu : 0u) | (bits >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+        w[i] = (w[i] & ~m) | (MINUS_INF<T> & m);
+      }
+    }
+    reinterpret_cast<uint4*>(out)[u] = make_uint4(w[0], w[1], w[2], w[3]);
   }
   for (int i = units * V + tid; i < n; i += LG_THREADS) {
     const unsigned said = a.tokens ? count_of(i) : 0u;
