@@ -62,3 +62,49 @@ def test_groups_of_few_rows(dtype, H, kvh, hd, groups, n, P):
     p.run_case(dtype, 16, H, kvh, hd, plen, list(range(0, groups * n + 1, n)), kv_len, [1] * (groups * n))
     gs = [0, 1] + [n * g for g in range(2, groups)] + [groups * n]   # uneven: the first group has one, the second the others of two
     p.run_case(dtype, 32, H, kvh, hd, plen, gs, kv_len, [1] * (groups * n), seed=1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,kvh,hd", [(14, 2, 64), (28, 4, 128)])
+def test_a_replayed_graph_follows_lengths_groups_and_starts(dtype, H, kvh, hd):
+    """Captured once with generous bounds; then own lengths, prefix lengths, groups, starts, tables and queries change in place between replays, so
+    that rows go from one kernel to the other and from one group to another. Each replay has the bits of a fresh call with the same bounds."""
+    n, rows, max_q, max_kv, max_prefix = 60, 420, 200, 400, 1600
+    steps = [  # prefix lengths, groups, queries, own lengths
+        ([1600, 300, 0], [0, 40, 50, 60], [7] * 60, [7 + 5 * i for i in range(60)]),
+        ([1500, 1600, 70], [0, 5, 58, 60], [1] * 30 + [200] + [1] * 20 + [90] + [0] * 8, [1 + 3 * i for i in range(30)] + [400] + [60] * 20 + [95] + [4] * 8),
+        ([16, 1, 1599], [10, 10, 11, 59], [3] * 20 + [0, 17, 130] + [2] * 37, [9 + (31 * i) % 300 for i in range(20)] + [0, 20, 390] + [5] * 37),
+        ([0, 0, 0], [0, 0, 0, 0], [1] * 60, [1 + 6 * i for i in range(60)]),
+        ([1600, 1600, 1600], [0, 20, 40, 60], [1] * 60, [0] * 60)]
+    gen = torch.Generator(device=p.DEV)
+    gen.manual_seed(hd)
+    kv, sc, both = t.make_cache(gen, [max_prefix] * 3 + [max_kv] * n, 16, kvh, hd)
+    ptable, table = both[:3].contiguous(), both[3:, :max_kv // 16].contiguous()
+    q = torch.empty(rows, H, hd, dtype=dtype, device=p.DEV)
+    plen, gs, start, lens = (torch.zeros(k, dtype=torch.int32, device=p.DEV) for k in (3, 4, n + 1, n))
+    out = torch.zeros(rows, H, hd, dtype=dtype, device=p.DEV)
+    go = lambda o: t.kv8().prefix_attention(q, kv, sc, ptable, plen, gs, table, start, lens, max_q, max_kv, max_prefix, out=o, return_lse=True)
+    graph = torch.cuda.CUDAGraph()
+    q.zero_()
+    go(out)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        _, lse = go(out)
+    for i, (a, b, c, d) in enumerate(steps + steps[::-1]):
+        assert sum(c) <= rows and max(c) <= max_q and max(d) <= max_kv and max(a) <= max_prefix
+        starts = [0] + np.cumsum(c).tolist()
+        q.copy_(torch.randn(q.shape, generator=gen, device=p.DEV))
+        for x, y in ((plen, a), (gs, b), (start, starts), (lens, d)):
+            x.copy_(p.i32(y))
+        if i == len(steps):  # other pages of the same pool
+            ptable.copy_(ptable.flip(0))
+            table.copy_(table.flip(0))
+        out.fill_(9.0)
+        graph.replay()
+        fresh = torch.full_like(out, 9.0)
+        _, fresh_lse = go(fresh)
+        used = starts[-1]
+        assert torch.equal(out, fresh) and torch.equal(lse[:used], fresh_lse[:used]) and (out[used:] == 9).all()
+        ref = p.reference(q, kv, sc, ptable, a, b, table, starts, d, hd ** -0.5)
+        t.close(out[:used], lse[:used], [x[:used] for x in ref[:2]] + list(ref[2:]), dtype, dtype != torch.float32)
+    t.kv8()._lib.check_ops()
