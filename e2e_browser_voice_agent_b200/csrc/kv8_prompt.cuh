@@ -230,7 +230,8 @@ __device__ __forceinline__ int blocks_of_call(const PromptArgsOf<SharedArgs>& pa
     const Request R = request_of(a, r, &n_all);
     const int tiles = row_tiles_of(pa, R);
     n += tiles;
-    all += (float)tiles * (float)min((R.len + PR_KEYS - 1) / PR_KEYS, pa.key_tiles);
+    // (one rounding in every kernel that this is part of, which must all find the same spans)
+    all = __fmaf_rn((float)tiles, (float)min((R.len + PR_KEYS - 1) / PR_KEYS, pa.key_tiles), all);
   }
   n = __reduce_add_sync(0xffffffffu, n);
 #pragma unroll
