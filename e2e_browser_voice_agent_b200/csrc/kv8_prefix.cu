@@ -39,11 +39,11 @@ __global__ void __launch_bounds__(RW_WARPS * 32, HD == 128 ? 3 : 5) k_prefix_row
   att_rows<T, HD>(both.ra[own], at - rz * across, rz % n, rz / n);
 }
 
-// Where the spans of a row lie: span s is row `first` + s * `step` of the sums and of the (m, l) of one of a pass's two kernels.
+// Where the spans of a row lie: span s is row `first` + s * |`step`| of the sums and of the (m, l) of one of a pass's two kernels: of
+// k_att_prompt where step is negative.
 struct Parts {
   long long first;
   int used, step;  // spans; 0: the row is in no request (group)
-  bool prompt;     // k_att_prompt's
 };
 
 // Quotients of numbers below 2^31 by multiplication: the joining kernel would spend most of its instructions on divisions else.
@@ -109,7 +109,7 @@ __device__ __forceinline__ void owners_of(const Pass& p, int t0, int i0, int ste
 // The parts of row t of q, which `o` has, and head h of kv head `head`'s group. row_blocks: blocks of k_att_rows' spans. (None where starts
 // of requests without sense would lead beyond what was computed.)
 __device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_blocks, const Owner& o, int t, int head, int h) {
-  if (o.r < 0) return {0, 0, 0, false};
+  if (o.r < 0) return {0, 0, 0};
   const SharedArgs& a = p.ra.a;
   const Divisor group(a.group, a.group_magic);
   const int row = (t - o.R.first) * a.group + h;
@@ -121,19 +121,18 @@ __device__ __forceinline__ Parts parts_of(const Pass& p, const Divisor& row_bloc
   if (o.tiles) {
     const int tile = row / PR_ROWS, n_blocks = (max(0, end_of(tile * PR_ROWS + PR_ROWS - 1)) + PR_KEYS - 1) / PR_KEYS;
     const long long unit = o.before + ((o.tiles - 1LL - tile) * a.kv_heads + head) * o.spans;
-    if (unit + o.spans > p.pa.cap) return {0, 0, 0, false};
+    if (unit + o.spans > p.pa.cap) return {0, 0, 0};
     const int n_rows = o.R.n_q * a.group;
-    return {o.part + (long long)head * o.spans * n_rows + row, max(1, min(o.spans, o.blocks.rounded_up(n_blocks))), n_rows, true};
+    return {o.part + (long long)head * o.spans * n_rows + row, max(1, min(o.spans, o.blocks.rounded_up(n_blocks))), -n_rows};
   }
   const int tile = row / RW_ROWS, n_blocks = (max(0, end_of(tile * RW_ROWS + RW_ROWS - 1)) + RW_BLK - 1) / RW_BLK;
-  if (tile >= p.ra.tiles) return {0, 0, 0, false};
+  if (tile >= p.ra.tiles) return {0, 0, 0};
   const long long unit = (((long long)o.r * a.kv_heads + head) * p.ra.tiles + tile) * p.ra.splits;
-  return {unit * RW_ROWS + (row - tile * RW_ROWS), max(1, min(p.ra.splits, row_blocks.rounded_up(n_blocks))), RW_ROWS, false};
+  return {unit * RW_ROWS + (row - tile * RW_ROWS), max(1, min(p.ra.splits, row_blocks.rounded_up(n_blocks))), RW_ROWS};
 }
 // The same for all lanes as lane j has them.
 __device__ __forceinline__ Parts of_lane(const Parts& p, int j) {
-  return {__shfl_sync(0xffffffffu, p.first, j), __shfl_sync(0xffffffffu, p.used, j), __shfl_sync(0xffffffffu, p.step, j),
-          __shfl_sync(0xffffffffu, (int)p.prompt, j) != 0};
+  return {__shfl_sync(0xffffffffu, p.first, j), __shfl_sync(0xffffffffu, p.used, j), __shfl_sync(0xffffffffu, p.step, j)};
 }
 
 // A CTA takes `heads` heads (at most JOIN_WARPS) of `tokens` (at most JOIN_TOKENS) rows of q, L lanes (or NW = JOIN_WARPS warps, for one
@@ -156,7 +155,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
   const Divisor by_heads(nh), by_group(a.group, a.group_magic);
   const Divisor prefix_row_blocks(max(1, prefix.ra.blocks)), own_row_blocks(max(1, own.ra.blocks));
   // lane j: of the warp's j-th row and head
-  Parts o_of{0, 0, 0, false}, p_of{0, 0, 0, false};
+  Parts o_of{0, 0, 0}, p_of{0, 0, 0};
   const int mine = NW > 1 ? lane : warp + lane * JOIN_WARPS;
   if (mine < n) {
     const int k_t = by_heads.quotient(mine), t = t0 + k_t, hq = h0 + mine - k_t * nh, head = by_group.quotient(hq), h = hq - head * a.group;
@@ -169,10 +168,11 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
     const Parts o = of_lane(o_of, j), p = of_lane(p_of, j);
     if (o.used == 0) continue;  // (a row of no request is not touched; nor is what lies past the warp's last)
     const int k_t = by_heads.quotient(i), t = t0 + k_t, hq = h0 + i - k_t * nh;
-    const float* o_part = (o.prompt ? own.pa.part : own.ra.part) + o.first * HD + V * ln;
-    const float2* o_ml = (o.prompt ? own.pa.ml : own.ra.ml) + o.first;
-    const float* p_part = (p.prompt ? prefix.pa.part : prefix.ra.part) + p.first * HD + V * ln;
-    const float2* p_ml = (p.prompt ? prefix.pa.ml : prefix.ra.ml) + p.first;
+    const float* o_part = (o.step < 0 ? own.pa.part : own.ra.part) + o.first * HD + V * ln;
+    const float2* o_ml = (o.step < 0 ? own.pa.ml : own.ra.ml) + o.first;
+    const float* p_part = (p.step < 0 ? prefix.pa.part : prefix.ra.part) + p.first * HD + V * ln;
+    const float2* p_ml = (p.step < 0 ? prefix.pa.ml : prefix.ra.ml) + p.first;
+    const unsigned o_step = abs(o.step), p_step = abs(p.step);
     const int all = p.used + o.used;
     // UN spans at a time, everything of them on its way at once; the sums are relative to the largest maximum so far
     float m = -INFINITY, v[V], l = 0.f;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM) k_prefix_join(co
         for (int j = 0; j < V; j++) x[k][j] = 0.f;
         if (s < all) {
           const bool shared = s < p.used;
-          const size_t at = shared ? (size_t)s * p.step : (size_t)(s - p.used) * o.step;
+          const size_t at = shared ? (size_t)s * p_step : (size_t)(s - p.used) * o_step;
           const float* src = (shared ? p_part : o_part) + at * HD;
           ml[k] = (shared ? p_ml : o_ml)[at];
           if (V == 2) {
