@@ -20,8 +20,11 @@ namespace {
 // bound it (16,392 x 3,584 bfloat16 with a float32 residual: 146 us; now 97, 6.7 TB/s). Few rows: two units a thread, four times
 // the warps, as latency is what counts (k_i8_norm's launch below). Other rows (k_i8_norm_any): a CTA each, whose values that do not fit
 // its registers are read again.
-// Bound: bandwidth for many rows (16,392 x 3,584 with a bfloat16 residual 63 us, 6.5 TB/s; float32 x 896 31 us, 6.1 TB/s); rows without a
-// residual have the fewest bytes for the same sums in 64 bits and are bound by those (47 us, 3.7 TB/s). One row: 2.3 us, a launch.
+// Bound: bandwidth for many rows (16,392 x 3,584 with a bfloat16 residual 63 us, 6.5 TB/s; float32 x 896 31 us, 6.1 TB/s). Rows without a
+// residual have half the bytes on their way for each thread and are bound by latency: 47 us (3.7 TB/s) with 5 CTAs an SM, for which the compiler
+// spills 8-16 bytes a thread, 86 with one. One row: 2.3 us, a launch.
+// k_i8_norm_any, a CTA of 1,024 threads a row however short, is far from that: 16,392 rows of 10 or 100 bfloat16 values 190 us, of 1,001
+// 200 (250 with a residual), of 3,586 275 (310), whose bytes would take 0.1, 0.8, 8 and 27; 4,000 rows of 40,000 380 (560), 73 by bytes.
 constexpr int NORM_V = 4;        // values of a unit: 16 bytes of float32, so that a warp's accesses are whole lines
 constexpr int NORM_WARPS = 8;    // of a CTA whose rows take fewer
 constexpr int NORM_MOST = 32768; // values of a row that registers hold
@@ -77,7 +80,8 @@ __device__ __forceinline__ float max_mag(float m, float x, float y) {
   return m;
 }
 
-// 1 / sqrt(x) as float32: float32's, made exact to 2^-80 by two of Newton's steps in 64 bits, so that the rounding is that of the value.
+// 1 / sqrt(x) as float32: float32's, made exact to 2^-51 by two of Newton's steps in 64 bits, so that the rounding is that of the value but
+// where that lies as near to a border between two float32 numbers.
 __device__ __forceinline__ float inverse_root(double x) {
   if (!(x > 1e-30 && x < 1e30)) return (float)rsqrt(x);
   double y = rsqrtf((float)x);

@@ -6,13 +6,18 @@
 // Each request attends to its own positions as in h2c_kv8_attention. Both passes leave (sum, maximum, weight) of each span of keys in
 // the workspace, and k_prefix_join adds up what belongs to a row: the softmax over all its positions. The kernels are launched one
 // behind the other without waiting for each other's end (programmatic dependent launch), those with tensor memory first; the
-// single tokens' CTAs take the SMs that they leave.
-// Bound, 28 heads over 4 of 128, bfloat16: 256 single tokens with 16-2,000 positions of their own behind 16,385: 134 us, of which 86 are
-// k_att_prompt's rate on the prefix (28 row tiles of 257 tiles of keys, see there); the own positions would take 61 alone, and 42 behind
-// the prefix, as their first CTAs fill the SMs that it leaves. Turns of 63 tokens of 26 requests in three groups, float16, 180 us: 160
-// that rate with the starts of some 540 CTAs of up to 22 tiles of keys, 20 the join of 65 MB (3.3 TB/s). 4 single tokens behind a
-// prefix: 8.6 us, two launches and the latency of a span.
-// Without the sharing, kv8.attention over tables that name the prefix reads its keys for each request: 256 times.
+// single tokens' first CTAs take the SMs that they leave, and keep them until the kernel before is over (EndAfterTheOthers).
+// Bound, 28 heads over 4 of 128, bfloat16: 256 single tokens with 16-2,000 positions of their own behind 16,385: 154 us, of which some 105 are
+// k_att_prompt's rate on the prefix (28 row tiles of 257 tiles of keys, see there; with weights of one term 86); the own positions would take
+// 54 alone, and 43 behind the prefix. Turns of 63 tokens of 26 requests in three groups, float16, 182 us: 160 that rate with the starts of
+// some 540 CTAs of up to 22 tiles of keys, 20 the join of 65 MB (3.3 TB/s). 4 single tokens behind a prefix: 8.8 us, two launches and the
+// latency of a span.
+// Without the sharing, kv8.attention over tables that name the prefix reads its keys for each request (256 of 20-200 positions of their own
+// behind 16,384: 731 us, 117 so), in one launch where there are few: it is the faster until the keys that it reads again are some 32 MB (32
+// behind 640 18 us, 16 so; 8 behind 640 10 and 12).
+// Where k_att_prompt takes part, its grid is a bound of the spans that its rows can have; CTAs without one look through the requests and end.
+// With hundreds of groups of few rows these are thousands (1,024 groups of two single tokens behind 320 positions each: 660 us, 254 by
+// kv8.attention over whole tables).
 #include "kv8_rows.cuh"
 
 namespace h2 {
@@ -379,7 +384,8 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
     };
     // Eight warps a head where spans are many and rows few (28 heads over 4 of 128: 8 requests of up to 30,000 of their own behind 2,000
     // 42 us, 64 by a warp a head; 2 behind 300 10.2 and 11.5); else a warp a head, and no more CTAs than the SMs hold at a time, so that
-    // all look up their places while the passes end (256 single tokens behind 16,385: 137 us, 140 with a CTA for each token's eight heads).
+    // all look up their places while the passes end (256 single tokens behind 16,385, weights of one term: 137 us, 140 with a CTA for each
+    // token's eight heads).
     const bool many = most(plan.own) + most(plan.prefix) > JOIN_WARP_SPANS && (long long)g->own.rows * g->own.heads <= 148 * 8;
     const int heads = many ? 1 : std::min(JOIN_WARPS, g->own.heads);
     const long long ctas = (long long)g->own.rows * ((g->own.heads + heads - 1) / heads);
@@ -389,7 +395,7 @@ int launch(const char* who, const PrefixPlan& plan, const h2c_kv8_prefix_args* g
     cfg.dynamicSmemBytes = 0;
     // Where a warp has more than four rows and heads, two at a time: most instructions are then for both, and twice as much is on its way
     // (turns of 63 tokens of 26 requests 180 us, 184 one by one, of 200 484 and 511; 256 single tokens, two of whose rows and heads a
-    // warp has, 135.5 and 134).
+    // warp has, 135.5 and 134, when their weights had one term).
     const bool two = (long long)g->own.rows * g->own.heads > JOIN_CTAS * JOIN_WARPS * 4;
     c = many  ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, JOIN_WARPS, 32>, pass[0], pass[1], tokens, heads)
         : two ? cudaLaunchKernelEx(&cfg, k_prefix_join<T, HD, 1, 16>, pass[0], pass[1], tokens, heads)

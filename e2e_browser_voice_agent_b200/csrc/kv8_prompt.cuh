@@ -44,7 +44,7 @@ constexpr bool PARTS_ONLY = std::is_same<A, SharedArgs>::value;
 
 // A kernel that was launched to start while the one before it on the stream still runs (programmatic dependent launch), and uses nothing
 // of it, ends after it, so that what follows on the stream finds both done. (Such kernels start when all CTAs of the kernel before
-// have started, so none waits for a CTA that needs its place.)
+// have started, so none waits for a CTA that needs its place; each of its CTAs keeps its own until then, those without work, too.)
 template <bool DO>
 struct EndAfterTheOthers {
   __device__ __forceinline__ ~EndAfterTheOthers() {
@@ -184,9 +184,9 @@ __device__ __forceinline__ Work work_of(const PromptArgsOf<AttArgs>& pa) {
 // u + u / B c + B / 2, where c = SPAN_COST tiles is what a span's start and end take and B / 2 what the last ones leave idle: least at
 // B = sqrt(2 u c). (One request: what fills the SMs once, known to the host.) Row tiles for SPAN_TILES CTAs and more are not cut.
 // Turns of 63 tokens of 26 requests in three groups behind 814-4,099, 28 heads over 4 of 128, c = 3, 5, 8 and 10: float16 195, 193, 184
-// and 191 us, bfloat16 176, 167, 159 and 157; behind 4,000-16,000 553, 528, 499 and 520. Spans of SPAN_LEAST tiles or more: 44 single tokens in two groups
-// 48 us, 57 with 16. One request's spans for 148 CTAs: 256 single tokens behind 16,385 positions 138 us, for 112 and 84, which leave
-// SMs to the single tokens, 151 and 175.
+// and 191 us; bfloat16 (c = 5, 8 and 10) 194, 184 and 186; float16 behind 4,000-16,000 553, 528, 499 and 520. Spans of SPAN_LEAST tiles or
+// more: 44 single tokens in two groups 48 us, 57 with 16. One request's spans for 148 CTAs: 256 single tokens behind 16,385 positions 155
+// us, for 112 and 84, which leave SMs to the single tokens, 174 and 203.
 constexpr int SPAN_COST = 8, SPAN_LEAST = 8, SPAN_TILES = 148 * 4;
 __host__ __device__ inline long long spans_at_most(long long ctas, long long key_tiles) {  // of `ctas` uncut row tiles
   const double cut = (double)(ctas < SPAN_TILES ? ctas : SPAN_TILES) * (double)key_tiles;
@@ -389,7 +389,7 @@ struct PromptCfg {
   // ... and of weights. One where h2c_kv8_attention's output is bfloat16: 2^-12 of each weight, an eighth of that rounding. With float16
   // outputs one term's error would be as large as theirs (some 1.2 times the error in all; 445 us for the prompts below, 543 with two).
   // Behind shared prefixes two throughout: with one, 6% of bfloat16 outputs are not the rounding of a float32 computation's but a step
-  // beside it (256 single tokens behind 16,385 positions: 134 us, 160 with two).
+  // beside it (256 single tokens behind 16,385 positions: 135 us, 154 with two; turns of 26 requests in three groups 155 and 183).
   static constexpr int P_TERMS = BF16 && !PARTS ? 1 : 2;
   static constexpr int BLKS = HD / 64;                   // 64-dimension blocks of a row
   static constexpr int Q_TILE = 128 * HD * 2;            // one row tile, one term

@@ -87,7 +87,7 @@ __device__ __forceinline__ void att_rows(const RowArgsOf<A>& ra, const int x, co
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   // Where parts are left to a joining kernel in any case, a warp takes a span for itself: no warp waits for another, and four times as
   // many spans are on their way. Spans are the grid's slowest axis and the last go first: only long requests have them, and the CTAs
-  // without one are over before the work begins.
+  // without one are over before the work begins (where no k_att_prompt comes before, whose end they would wait for).
   constexpr bool ALONE = PARTS_ONLY<A>;
   const int split = ALONE ? ra.splits - 1 - z : x % ra.splits, th = ALONE ? x * RW_WARPS + warp : x / ra.splits;
   const int head = th % a.kv_heads, tile = th / a.kv_heads;
@@ -505,7 +505,7 @@ WorkPlan plan_work(const h2c_kv8_attention_args* g, bool parts = false, bool gro
     // 60,000-131,072 175, 176 and 164; 32 of 4,000-16,000 89, 81 and 75). Up to 8 are one cluster, whose join costs little: spans of 128 keys (2
     // blocks per warp) or more. More of them, for few rows over long histories, leave their parts in the workspace for a
     // second kernel: spans of 256 keys or more, below which a span's start-up costs more than it shares out
-    // A warp's spans, where they are joined in any case: three waves of 12 warps an SM (256 single tokens of 16-2,000 keys 61 us, 64 with four
+    // A warp's spans, where they are joined in any case: three waves of 12 warps an SM (256 single tokens of 16-2,000 keys 61 us with their join, 64 with four
     // and 68 with eight; with two 9% more than with four), of 128 keys or more (32 requests behind 4,096: 27 us, 38 with 64), or of 64
     // where those are few (4 sessions 10.4, 12.7 with 128).
     const long long units = (long long)g->n_req * g->kv_heads * p.tiles, want = ((parts ? 5328 : 888) + units - 1) / units;

@@ -6,7 +6,9 @@
 // them and adds the biases of each up in the list's order. Then it changes, masks and writes the logits, and at last the few biased ones.
 // Bound: bandwidth for many rows, and the instructions of the pass: a token that was said is found in nearly every warp's 256 logits, so
 // its division is one of five multiplications where it can be. Each chunk goes through the row's history (from L2), so chunks are long.
-// 32 rows of 151,936 float32: 15.3 us (2.6 TB/s); 256 rows behind up to 16,384 tokens, bfloat16: 58 us; one row: 3.6 us.
+// 32 rows of 151,936 float32: 15.3 us (2.6 TB/s); 256 rows behind up to 16,384 tokens, bfloat16: 57 us; one row: 3.6 us.
+// A chunk's biased tokens are compared with each other, which counts where many fall into one chunk: 1,024 biases on 151,936 float32
+// tokens take 12 us a row (32 rows 45), on 4,096 tokens 150, on 2,048 490; 128 biases 4, 10 and 17; 16 biases 3-4 everywhere.
 #include "ops.cuh"
 
 #include <algorithm>

@@ -4,10 +4,10 @@
 // heads, and hand them around through shared memory. A lane then has the same few pairs of every head that it turns, so it keeps their
 // cosines and sines, and goes from head to head with loads and stores of 16 bytes where the layout has them.
 // Bound: bandwidth for many tokens (16,392 of 32 heads of 128, bfloat16: 44 us, 6.0 TB/s), the launch and the 64-bit angles of a warp for
-// few (one token 2.4 us).
+// few (one token 2.5 us).
 // The angle is formed in turns: position * frequency / 2 pi, of which the product's remainder and the factor's are kept, too, so that what
 // is left without the whole turns is exact to 2^-52 at any position. Its cosine and sine are taken in 64 bits and rounded once, times the
-// magnitude (angles and functions in 32 bits: 0.93 x 2^-24 of a vector for 0.62, and the same times).
+// magnitude (angles and functions in 32 bits: 0.93 x 2^-24 of a vector for 0.62, and 0.1-0.2 us less).
 #include "ops.cuh"
 
 #include <algorithm>
@@ -129,9 +129,9 @@ __device__ __forceinline__ void turn_unit(Piece<T, N>& p, Piece<T, W>& q, const 
 
 // One unit of work is W neighbouring values and, in the half layout, the W that are their partners; of the part that is not turned, W
 // values: W is what 16 bytes hold, or 1 where a pointer, a stride or a head's parts are not multiples of 16 bytes (2,050 tokens of
-// 36 heads of 128: 9.3 us, and 31 with 62 of the 128 values turned, which have to go one by one). FEW: a head has at most 32 units, so
-// a lane has one of them, of several heads at a time, and keeps its cosines and sines; else the lanes go through a head's units
-// together.
+// 36 heads of 128, bfloat16: 7.2 us, and 39 with 62 of the 128 values turned, which have to go one by one; interleaved 8.0 and 58).
+// FEW: a head has at most 32 units, so a lane has one of them, of several heads at a time, and keeps its cosines and sines; else the
+// lanes go through a head's units together.
 template <class T, int W, bool INTER, bool FEW>
 __global__ void __launch_bounds__(32 * ROPE_WARPS, 3) k_rope(const RopeArgs a) {
   extern __shared__ __align__(16) float2 turn[];  // [warp][pair]: cosine and sine, times the magnitude

@@ -365,8 +365,9 @@ int h2c_kv8_attention(const h2c_kv8_attention_args* args, void* stream);
  * i of n its own positions 0 .. kv_len[r] - n + i. The softmax is over both, and a prefix's keys are read once for all of a group's
  * rows of a kv head, or for every 256 of them. A query that sees nothing gives zeros and lse = -infinity.
  * own.window must be 0. What is rounded where is as in h2c_kv8_attention, where a group's rows count as one prompt for the prefix, but
- * that the softmax's weights have 22 bits in bfloat16 prompts, too; the parts are joined in float32. group_start is clamped to 0 .. own.n_req and should not decrease (a row in two groups has the first's
- * prefix). The workspace is h2c_kv8_prefix_attention_workspace bytes. */
+ * that the softmax's weights have 22 bits in bfloat16 prompts, too; the parts are joined in float32. group_start is clamped to
+ * 0 .. own.n_req and must not decrease: where groups overlap, a row has the prefix of one of its groups or, when their rows are more
+ * than the call's, of none. The workspace is h2c_kv8_prefix_attention_workspace bytes. */
 typedef struct h2c_kv8_prefix_args {
   h2c_kv8_attention_args own;
   const int32_t* prefix_table; /* [n_groups][prefix_cols] */
